@@ -154,6 +154,24 @@ int nxd_flash_attn_bwd_tc(const void* q, const void* k, const void* v, const voi
                           void* dq, void* dk, void* dv, const long long* strides, int B, int Hq, int Hkv, int Sq,
                           int Sk, int D, float scale, int causal, void* stream);
 
+/* ---- attention over packed sequences (rows cu[s] .. cu[s + 1] of a row of T tokens each attend to themselves) ------------
+ * nxd_packed_plan makes the tile list from the boundaries on the device (int32, or int64 with `wide`): room for
+ * nxd_packed_plan_entries tiles of 16 bytes, `seqs` 16 bytes per sequence; nxd_packed_plan_columns is the row length of
+ * the per-row scratch.  strides = {head, row} in elements: {q, k, v, o} forward, {q, k, v, o, dout, dq, dk, dv} backward, multiples of 8.
+ * lse [Hq, columns] (NULL: not wanted), delta the same; dq_accum: ZEROED [Hq, D, columns]; dkv_accum: NULL, or ZEROED
+ * [2, Hkv, T, D] where nxd_packed_attn_bwd_splits is above 1.  Rows outside every sequence come out as zeros. */
+int nxd_packed_plan_entries(long long T, int N);
+long long nxd_packed_plan_columns(long long T, int N);
+int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, void* tiles, void* seqs, void* stream);
+int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const long long* strides,
+                        const void* tiles, int entries, long long columns, long long T, int Hq, int Hkv, int D, float scale,
+                        int causal, void* stream);
+int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv);
+int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+                        float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
+                        const long long* strides, const void* tiles, int entries, long long columns, long long T, int N,
+                        int Hq, int Hkv, int D, float scale, int causal, void* stream);
+
 /* ---- symmetric (peer-mapped) memory over CUDA IPC + fused compute/collective kernels ---------------------------
  * No counterpart in the reference (its collectives are XLA ops).  One process per GPU: every rank allocates a
  * region, exchanges the 64-byte handles out of band (torch.distributed), opens the peers' handles and passes the

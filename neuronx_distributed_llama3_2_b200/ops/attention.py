@@ -5,6 +5,8 @@
   (``src/neuronx_distributed/kernels/flash_attn.py:151-191``; tensors ``[B, H, S, D]``), without its
   ``S % 2048`` restriction and without ``repeat_kv`` (the reference expands KV heads first,
   ``examples/training/llama/modeling_llama_nxd.py:409-410``).
+* ``flash_attn_packed_func`` / ``rope_flash_attn_packed_func`` -- the same over sequences of different lengths laid
+  end to end in one row (``PackedSequences``), each attending to itself.
 * ``decode_attention`` / ``kv_cache_update`` -- token generation over a contiguous or paged cache.
 
 Backends for ``flash_attn_func`` (``ops.backend.set_backends(attn=...)``, default from ``NXD_ATTN_BACKEND``):
@@ -18,12 +20,13 @@ from __future__ import annotations
 import ctypes as _c
 import math
 import os
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 import torch.nn.functional as F
 
 from . import _lib, backend
+from .packed_attention import PackedSequences, as_packed, packed_attn_nxd, rope_packed_attn
 
 
 def attention_ref(q, k, v, causal=True, softmax_scale=None, dropout_p=0.0, seed=0):
@@ -98,6 +101,54 @@ def rope_flash_attn_func(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor
     x = apply_rope(qkv.reshape(S * B, heads, D), cos, sin, n_q + n_kv, pos_div=B, pos_mod=S).reshape(S, B, heads, D)
     q, k, v = (x[:, :, a:b].permute(1, 2, 0, 3) for a, b in ((0, n_q), (n_q, n_q + n_kv), (n_q + n_kv, heads)))  # views
     return flash_attn_func(q, k, v, causal=True)
+
+
+def flash_attn_packed_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           cu_seqlens: Union[torch.Tensor, "PackedSequences"], softmax_scale: Optional[float] = None,
+                           causal: bool = True) -> torch.Tensor:
+    """Attention of every sequence of a packed row to itself: q ``[T, Hq, D]``, k / v ``[T, Hkv, D]`` (``Hq`` a multiple of ``Hkv``)
+    -> ``[T, Hq, D]``.  ``cu_seqlens [N + 1]`` (int32 or int64, on the tensors' device): sequence ``s`` is rows ``cu_seqlens[s] ..
+    cu_seqlens[s + 1]``, or a ``PackedSequences`` that several calls share.  ``causal``: a token sees its sequence up to itself,
+    else all of it.  Rows outside every sequence give zeros and get zero gradients.
+
+    Backends as ``flash_attn_func``; other types and head sizes than the kernel's run that function on one sequence after the
+    other (the lengths are read on the host then)."""
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"packed attention of q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if not k.shape[1] or not q.shape[1] or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{q.shape[1]} query heads over {k.shape[1]} key heads")
+    if q.dtype != k.dtype or q.dtype != v.dtype or q.device != k.device or q.device != v.device:
+        raise ValueError("packed attention needs q, k and v of one type on one device")
+    packed = as_packed(cu_seqlens, q.shape[0], q.device)
+    if _backend(q) == "nxd":
+        return packed_attn_nxd(q, k, v, packed, softmax_scale, causal)
+    parts, rows = [], 0
+    for s in packed.slices():
+        if s.start > rows:
+            parts.append(q.new_zeros((s.start - rows,) + tuple(q.shape[1:])))
+        rows = max(rows, s.stop)
+        if s.stop > s.start:
+            o = flash_attn_func(*(x[s].transpose(0, 1).unsqueeze(0) for x in (q, k, v)), softmax_scale=softmax_scale, causal=causal)
+            parts.append(o[0].transpose(0, 1))
+    parts.append(q.new_zeros((q.shape[0] - rows,) + tuple(q.shape[1:])))
+    parts.append(q[:0] + k[:0].sum() + v[:0].sum())          # no rows: a batch without sequences has (zero) gradients too
+    return torch.cat(parts)
+
+
+def rope_flash_attn_packed_func(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_q: int, n_kv: int,
+                                cu_seqlens: Union[torch.Tensor, "PackedSequences"]) -> torch.Tensor:
+    """Causal attention inside the sequences of a packed projection ``qkv [T, n_q + 2 n_kv, D]`` (q | k | v heads) whose queries and
+    keys are first rotated at their position in their own sequence -> ``[T, n_q, D]``.  The tables need as many rows as the
+    longest sequence has tokens."""
+    if qkv.dim() != 3 or qkv.shape[1] != n_q + 2 * n_kv:
+        raise ValueError(f"a projection of {n_q} + 2 x {n_kv} heads, not {tuple(qkv.shape)}")
+    packed = as_packed(cu_seqlens, qkv.shape[0], qkv.device)
+    if qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.shape[-1] in (64, 128) and _backend(qkv) == "nxd":
+        return rope_packed_attn(qkv, cos, sin, n_q, n_kv, packed)
+    from .rope import apply_rope
+
+    x = apply_rope(qkv, cos, sin, n_q + n_kv, positions=packed.positions())
+    return flash_attn_packed_func(x[:, :n_q], x[:, n_q:n_q + n_kv], x[:, n_q + n_kv:], packed)
 
 
 # ---------------------------------------------------------------------------------------------

@@ -1,0 +1,202 @@
+"""Attention over packed sequences: the samples of a batch laid end to end in one row instead of padded to the longest.
+
+``PackedSequences`` holds where the sequences of a step begin and the tile list that the kernels walk (``csrc/packed_plan.cu``);
+it is made on the device from ``cu_seqlens`` without a copy to the host and serves every layer of the step, forward and
+backward.  The kernels are the packed instantiations of the tcgen05 attention (``csrc/flash_attn_tc.cu``,
+``csrc/flash_attn_bwd_tc.cu``).  ``ops.attention`` has the public functions."""
+from __future__ import annotations
+
+import ctypes as _c
+import math
+from typing import List, Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+from .rope import _aligned as _rope_aligned, _launch as _rope_launch
+
+
+class PackedSequences:
+    """The sequences of a packed row of ``total`` tokens: sequence ``s`` takes rows ``cu_seqlens[s] .. cu_seqlens[s + 1]``.
+
+    ``cu_seqlens [N + 1]``: int32 or int64, rising (equal neighbours are an empty sequence), inside ``[0, total]``; rows ahead of the
+    first boundary or behind the last belong to no sequence, attend to nothing and give zeros.  On the CPU this is checked; on
+    the GPU, where a check would wait for the device, a boundary that falls or leaves the row is taken as the nearest one
+    that does not.  What is made of the boundaries (tile lists, positions) is made once, on the stream of the first call that needs it:
+    lengths that change want a new object.  One that is made while a CUDA graph is captured reads ``cu_seqlens`` again in
+    every replay, and is of use inside that graph only."""
+
+    def __init__(self, cu_seqlens: torch.Tensor, total: int):
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"cu_seqlens: N + 1 boundaries as int32 or int64, not {tuple(cu_seqlens.shape)} {cu_seqlens.dtype}")
+        if not 0 < total < 2 ** 31 - 256:
+            raise ValueError(f"a packed row of {total} tokens")
+        self.cu_seqlens, self.total, self.count = cu_seqlens.contiguous(), int(total), cu_seqlens.numel() - 1
+        self._plans: dict = {}
+        self._positions: Optional[torch.Tensor] = None
+        if not cu_seqlens.is_cuda:
+            ends = cu_seqlens.tolist()
+            if any(b < a for a, b in zip(ends, ends[1:])) or ends[0] < 0 or ends[-1] > total:
+                raise ValueError(f"cu_seqlens have to rise inside [0, {total}]: {ends[:8]} ...")
+
+    @property
+    def device(self) -> torch.device:
+        return self.cu_seqlens.device
+
+    def plan(self, causal: bool) -> Tuple[torch.Tensor, int, int]:
+        """``(tile list, its entries, columns of the per-row scratch)`` for the kernels, made on first use."""
+        if causal not in self._plans:
+            lib = _lib.lib()
+            lib.nxd_packed_plan_columns.restype = _c.c_longlong
+            entries = lib.nxd_packed_plan_entries(_c.c_longlong(self.total), _c.c_int(self.count))
+            columns = lib.nxd_packed_plan_columns(_c.c_longlong(self.total), _c.c_int(self.count))
+            lists = torch.empty((entries + self.count, 4), dtype=torch.int32, device=self.device)
+            rc = lib.nxd_packed_plan(_lib.ptr(self.cu_seqlens), _c.c_int(self.cu_seqlens.dtype == torch.int64), _c.c_int(self.count),
+                                     _c.c_longlong(self.total), _c.c_int(causal), _lib.ptr(lists),
+                                     _c.c_void_p(lists.data_ptr() + 16 * entries), _lib.stream_ptr())
+            _lib.check(rc, "nxd_packed_plan")
+            self._plans[causal] = (lists, entries, columns)
+        return self._plans[causal]
+
+    def positions(self) -> torch.Tensor:
+        """int32 ``[total]``: every token's position in its own sequence (0 outside of them), for the rotation."""
+        if self._positions is None:
+            cu = self.cu_seqlens.long().clamp(0, self.total).cummax(0).values
+            rows = torch.arange(self.total, device=self.device)
+            s = torch.searchsorted(cu, rows, right=True) - 1
+            inside = (s >= 0) & (s < self.count)
+            pos = torch.where(inside, rows - cu[s.clamp(0, self.count)], 0)
+            self._positions = pos.to(torch.int32)
+        return self._positions
+
+    def last_tokens(self) -> torch.Tensor:
+        """bool ``[total]``: the last token of a sequence (it has no next token to predict), and every row outside of them."""
+        cu = self.cu_seqlens.long().clamp(0, self.total).cummax(0).values
+        mask = torch.zeros(self.total + 1, dtype=torch.bool, device=self.device)
+        mask[cu] = True
+        return mask[1:] | ~self.inside()
+
+    def inside(self) -> torch.Tensor:
+        """bool ``[total]``: the tokens that belong to a sequence."""
+        rows = torch.arange(self.total, device=self.device)
+        cu = self.cu_seqlens
+        return (rows >= cu[0]) & (rows < cu.max())
+
+    def slices(self) -> List[slice]:
+        """The sequences' rows, on the host (waits for the device)."""
+        ends = self.cu_seqlens.long().clamp(0, self.total).cummax(0).values.tolist()
+        return [slice(a, b) for a, b in zip(ends, ends[1:])]
+
+
+def as_packed(sequences: Union[torch.Tensor, PackedSequences], total: int, device: torch.device) -> PackedSequences:
+    packed = sequences if isinstance(sequences, PackedSequences) else PackedSequences(sequences, total)
+    if packed.total != total:
+        raise ValueError(f"sequences packed in {packed.total} rows, tensors of {total}")
+    if packed.device != device:
+        raise ValueError(f"cu_seqlens on {packed.device}, tensors on {device}")
+    return packed
+
+
+def _fix(t: torch.Tensor) -> torch.Tensor:
+    """Unit stride on the head dimension, the others multiples of 8 elements that do not overlap, 16-byte aligned."""
+    T, H, D = t.shape
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0
+    ok = ok and (H == 1 or t.stride(1) % 8 == 0 and t.stride(1) >= D) and (T == 1 or t.stride(0) % 8 == 0 and t.stride(0) >= D)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(*ts: torch.Tensor):
+    """(head, row) strides; a dimension of one has any."""
+    vals = [s for t in ts for s in (t.stride(1) if t.shape[1] > 1 else t.shape[2], t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2])]
+    return (_c.c_longlong * len(vals))(*vals)
+
+
+def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, want_lse: bool):
+    T, Hq, D = q.shape
+    tiles, entries, columns = packed.plan(causal)
+    o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((Hq, columns), dtype=torch.float32, device=q.device) if want_lse else None
+    rc = _lib.lib().nxd_packed_attn_fwd(
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(lse), _strides(q, k, v, o), _lib.ptr(tiles), _c.c_int(entries),
+        _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(Hq), _c.c_int(k.shape[1]), _c.c_int(D), _c.c_float(scale), _c.c_int(causal),
+        _lib.stream_ptr())
+    _lib.check(rc, "nxd_packed_attn_fwd")
+    return o, lse
+
+
+def _backward(q, k, v, o, lse, do, dq, dk, dv, packed: PackedSequences, scale: float, causal: bool) -> None:
+    """Every element of ``dq / dk / dv`` is written."""
+    do = _fix(do)
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    tiles, entries, columns = packed.plan(causal)
+    delta = torch.empty_like(lse)
+    acc = torch.zeros((Hq, D, columns), dtype=torch.float32, device=q.device)
+    splits = _lib.lib().nxd_packed_attn_bwd_splits(_c.c_longlong(T), _c.c_int(packed.count), _c.c_int(Hq), _c.c_int(Hkv))
+    kv_acc = torch.zeros((2, Hkv, T, D), dtype=torch.float32, device=q.device) if splits > 1 else None
+    rc = _lib.lib().nxd_packed_attn_bwd(
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(do), _lib.ptr(lse), _lib.ptr(delta), _lib.ptr(acc), _lib.ptr(kv_acc),
+        _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _strides(q, k, v, o, do, dq, dk, dv), _lib.ptr(tiles), _c.c_int(entries),
+        _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(packed.count), _c.c_int(Hq), _c.c_int(Hkv), _c.c_int(D), _c.c_float(scale),
+        _c.c_int(causal), _lib.stream_ptr())
+    _lib.check(rc, "nxd_packed_attn_bwd")
+
+
+class _PackedAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, packed, scale, causal):
+        q, k, v = _fix(q), _fix(k), _fix(v)
+        grad = any(ctx.needs_input_grad[:3])
+        with torch.cuda.device(q.device):
+            o, lse = _forward(q, k, v, packed, scale, causal, grad)
+        if grad:
+            ctx.save_for_backward(q, k, v, o, lse)
+            ctx.args = (packed, scale, causal)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        with torch.cuda.device(q.device):
+            _backward(q, k, v, o, lse, do, dq, dk, dv, *ctx.args)
+        return dq, dk, dv, None, None, None
+
+
+class _RopePackedAttnFn(torch.autograd.Function):
+    """Rotation (positions that start again with every sequence) and causal attention of one projection output as one node: the
+    three gradients are written side by side into one buffer and rotated back there, as in ``flash_attn.rope_flash_attn``."""
+
+    @staticmethod
+    def forward(ctx, qkv, cos, sin, n_q, n_kv, packed, scale):
+        T, heads, D = qkv.shape
+        with torch.cuda.device(qkv.device):
+            qkv = _rope_aligned(qkv)
+            rot = torch.empty_like(qkv)
+            positions = packed.positions()
+            _rope_launch(qkv, cos, sin, n_q + n_kv, 1, 1 << 30, positions, False, rot)
+            o, lse = _forward(rot[:, :n_q], rot[:, n_q:n_q + n_kv], rot[:, n_q + n_kv:], packed, scale, True, ctx.needs_input_grad[0])
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(rot, o, lse, cos, sin, positions)
+            ctx.args = (n_q, n_kv, packed, scale)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        rot, o, lse, cos, sin, positions = ctx.saved_tensors
+        n_q, n_kv, packed, scale = ctx.args
+        parts = lambda x: (x[:, :n_q], x[:, n_q:n_q + n_kv], x[:, n_q + n_kv:])     # noqa: E731
+        with torch.cuda.device(rot.device):
+            d = torch.empty_like(rot)
+            _backward(*parts(rot), o, lse, do, *parts(d), packed, scale, True)
+            _rope_launch(d, cos, sin, n_q + n_kv, 1, 1 << 30, positions, True)
+        return d, None, None, None, None, None, None
+
+
+def packed_attn_nxd(q, k, v, packed: PackedSequences, softmax_scale: Optional[float], causal: bool) -> torch.Tensor:
+    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    return _PackedAttnFn.apply(q, k, v, packed, float(scale), bool(causal))
+
+
+def rope_packed_attn(qkv, cos, sin, n_q: int, n_kv: int, packed: PackedSequences) -> torch.Tensor:
+    return _RopePackedAttnFn.apply(qkv, cos, sin, n_q, n_kv, packed, 1.0 / math.sqrt(qkv.shape[-1]))

@@ -1,0 +1,224 @@
+"""Attention over packed sequences on the tensor cores against float64, with bounds that count the roundings."""
+import pytest
+import torch
+
+from packed_oracle import check, packed
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(T, H, G, D, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed + T)
+    qkv = torch.randn(T, H + 2 * G, D, generator=g, device="cuda").mul_(scale).bfloat16()
+    do = torch.randn(T, H, D, generator=g, device="cuda").bfloat16()
+    return qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:], do
+
+
+def _run(q, k, v, do, ends, causal, dtype=torch.int32, scale=None):
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    cu = ends if isinstance(ends, torch.Tensor) else torch.tensor(ends, dtype=dtype, device="cuda")
+    o = flash_attn_packed_func(q, k, v, cu, softmax_scale=scale, causal=causal)
+    return dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, (q, k, v), do)), o=o.detach())
+
+
+def _ends(lens, first=0):
+    out = [first]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+# boundaries on and beside the tiles of 64 and 128 rows, one token, empty sequences, rows ahead of the first and behind the last
+BATCHES = [([1], 0, 1), ([1, 1, 1], 0, 3), ([64], 0, 64), ([65, 63, 128], 0, 256), ([127, 1, 0, 129, 300, 0], 0, 557), ([256, 384], 0, 700),
+           ([5, 200, 33], 7, 400), ([], 0, 130), ([0, 0], 3, 5), ([1000, 37, 2, 513], 129, 1700)]
+
+
+def test_plan_lists_every_tile_once():
+    from neuronx_distributed_llama3_2_b200.ops.packed_attention import PackedSequences
+
+    g = torch.Generator().manual_seed(0)
+    long = torch.randint(0, 3, (5000,), generator=g).tolist()
+    for lens, first, T in BATCHES + [(long, 0, sum(long) + 200), ([600000, 70], 0, 600200)]:
+        for dtype in (torch.int32, torch.int64):
+            for causal in (True, False):
+                ends = _ends(lens, first)
+                lists, entries, columns = PackedSequences(torch.tensor(ends, dtype=dtype, device="cuda"), T).plan(causal)
+                rows = lists[:entries].tolist()
+                want, pad = set(), 0
+                for a, b in zip(ends, ends[1:]):
+                    want |= {(a, b - a, t, pad) for t in range((b - a + 127) // 128)}
+                    pad += (b - a + 3) // 4 * 4
+                tiles = [tuple(r) for r in rows if r[1]]
+                assert set(tiles) == want and len(tiles) == len(want) and pad + 64 <= columns
+                assert all(r[1] for r in rows[:len(tiles)])
+                weight = [min(t[2] + 1 if causal else (t[1] + 127) // 128, 4096) for t in tiles]
+                assert weight == sorted(weight, reverse=True)
+                outside = [r for a, n, t, _ in rows if not n for r in range(a, a + t)]
+                assert sorted(outside) == [r for r in range(T) if r < first or r >= ends[-1]]
+
+
+def test_plan_brings_wrong_boundaries_back():
+    from neuronx_distributed_llama3_2_b200.ops.packed_attention import PackedSequences
+
+    cu = torch.tensor([-5, 40, 30, 2 ** 31 + 10, 90], dtype=torch.int64, device="cuda")
+    lists, entries, _ = PackedSequences(cu, 100).plan(True)
+    tiles = sorted(tuple(r) for r in lists[:entries].tolist() if r[1])
+    assert tiles == [(0, 40, 0, 0), (40, 60, 0, 40)]
+
+
+@pytest.mark.parametrize("H,G,D", [(4, 2, 64), (2, 2, 128), (6, 1, 64), (3, 1, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,first,T", BATCHES)
+def test_matches_float64(lens, first, T, causal, H, G, D):
+    q, k, v, do = _inputs(T, H, G, D)
+    ends = _ends(lens, first)
+    got = _run(q, k, v, do, ends, causal, torch.int64 if T % 2 else torch.int32)
+    want = packed(q, k, v, ends, causal, do)
+    for name in ("o", "dq", "dk", "dv"):
+        check(got[name], want, name)
+    outside = [r for r in range(T) if r < first or r >= ends[-1]]
+    assert all(got[n][outside].eq(0).all() for n in got)
+
+
+# one K/V block per CTA and several CTAs per block, long walks, many query heads over one key head
+@pytest.mark.parametrize("lens,H,G,D,causal", [([2500, 1200], 4, 1, 128, True), ([4100], 2, 1, 64, True), ([700] * 40, 8, 8, 64, False),
+                                               ([1, 2, 3] * 200, 4, 4, 128, True), ([129] * 90 + [2048], 8, 2, 128, True)])
+def test_long_and_many(lens, H, G, D, causal):
+    T = sum(lens) + 11
+    q, k, v, do = _inputs(T, H, G, D)
+    got, want = _run(q, k, v, do, _ends(lens), causal), packed(q, k, v, _ends(lens), causal, do)
+    for name in got:
+        check(got[name], want, name)
+
+
+# scores that rise along the keys (the running maximum moves in every tile) and scores that leave one weight
+@pytest.mark.parametrize("scale", [0.01, 1.0, None])
+def test_scales(scale):
+    q, k, v, do = _inputs(777, 4, 2, 64, scale=2.0)
+    k = (k.float() * torch.linspace(0.1, 3.0, 777, device="cuda")[:, None, None]).bfloat16()
+    ends = [0, 300, 777]
+    got, want = _run(q, k, v, do, ends, True, scale=scale), packed(q, k, v, ends, True, do, scale)
+    check(got["o"], want, "o")
+    # scores are up to 1000 here, so their fp32 error is up to 2^-14 and more of a weight: gradients by norm, four roundings
+    for n in ("dq", "dk", "dv"):
+        assert (got[n].double() - want[n][0]).norm() <= 4 * 2.0 ** -8 * want[n][0].norm()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_sequences_do_not_touch(causal, D):
+    """What one sequence holds, infinities and NaN among it, leaves every other sequence's results as they are, bit by bit where
+    nothing is summed in an order that is not fixed."""
+    lens, T = [100, 130, 70, 1, 250], 600
+    q, k, v, do = (x.contiguous() for x in _inputs(T, 4, 2, D))
+    ends = _ends(lens)
+    clean = _run(q, k, v, do, ends, causal)
+    for bad, fill in ((1, float("nan")), (2, float("inf")), (3, float("nan")), (5, float("nan"))):
+        rows = slice(ends[bad], ends[bad + 1] if bad < 5 else T)
+        dirty = [x.clone() for x in (q, k, v, do)]
+        for x in dirty:
+            x[rows] = fill
+        got = _run(*dirty, ends, causal)
+        keep = torch.ones(T, dtype=torch.bool, device="cuda")
+        if bad < 5:
+            keep[rows] = False
+        assert torch.equal(got["o"][keep], clean["o"][keep])
+        for n in ("dq", "dk", "dv"):
+            assert got[n][keep].isfinite().all()
+            # the same sums in another order: at most one step of bf16
+            assert ((got[n] - clean[n])[keep].abs() <= 2 * 2.0 ** -8 * clean[n][keep].abs() + 1e-6).all()
+
+
+def test_strides_and_a_second_stream():
+    T, H, G, D = 333, 4, 2, 128
+    q, k, v, do = _inputs(T, H, G, D)
+    ends = [0, 50, 333]
+    want = packed(q, k, v, ends, True, do)
+    head_first = q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    odd = torch.empty(T * G * D + 1, dtype=torch.bfloat16, device="cuda")[1:].view(T, G, D).copy_(k)          # 2 bytes off a boundary
+    wide = torch.empty(T, G, 2 * D, dtype=torch.bfloat16, device="cuda")[..., ::2].copy_(v)                    # no unit stride
+    late = do.transpose(0, 1).contiguous().transpose(0, 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(head_first, odd, wide, late, ends, True)
+    torch.cuda.current_stream().wait_stream(side)
+    for name in got:
+        check(got[name], want, name)
+    grad = torch.ones((), dtype=torch.bfloat16, device="cuda").expand(T, H, D)                     # a sum's gradient has no strides
+    got, want = _run(q, k, v, grad, ends, True), packed(q, k, v, ends, True, grad)
+    for name in got:
+        check(got[name], want, name)
+
+
+def test_one_list_for_several_calls_and_no_gradients():
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+    from neuronx_distributed_llama3_2_b200.ops.packed_attention import PackedSequences
+
+    ends = [0, 90, 400]
+    p = PackedSequences(torch.tensor(ends, device="cuda"), 400)
+    for seed in (0, 1):
+        q, k, v, _ = _inputs(400, 4, 2, 64, seed)
+        for causal in (True, False):
+            with torch.no_grad():
+                o = flash_attn_packed_func(q, k, v, p, causal=causal)
+            check(o, packed(q, k, v, ends, causal), "o")
+            check(flash_attn_packed_func(q, k, v, p, causal=causal), packed(q, k, v, ends, causal), "o")
+
+
+def test_captured_step_follows_new_lengths():
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+
+    T = 640
+    q, k, v, do = (x.contiguous() for x in _inputs(T, 4, 2, 64))
+    cu = torch.tensor([0, 100, 640], dtype=torch.int32, device="cuda")
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+
+    def step():
+        o = flash_attn_packed_func(*leaves, cu)
+        return (o, *torch.autograd.grad(o, leaves, do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for ends in ([0, 100, 640], [0, 333, 334], [7, 7, 600]):
+        cu.copy_(torch.tensor(ends))
+        graph.replay()
+        want = packed(q, k, v, ends, True, do)
+        for name, x in zip(("o", "dq", "dk", "dv"), out):
+            check(x, want, name)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rotation_and_attention(D):
+    from neuronx_distributed_llama3_2_b200.ops import attention, rope
+
+    T, H, G, ends = 500, 4, 2, [0, 1, 200, 470]
+    g = torch.Generator(device="cuda").manual_seed(D)
+    qkv = torch.randn(T, H + 2 * G, D, generator=g, device="cuda").bfloat16().requires_grad_()
+    do = torch.randn(T, H, D, generator=g, device="cuda").bfloat16()
+    cos, sin = rope.build_rope_cache(T, D, 10000.0, None, device="cuda")
+    o = attention.rope_flash_attn_packed_func(qkv, cos, sin, H, G, torch.tensor(ends, device="cuda"))
+    (grad,) = torch.autograd.grad(o, qkv, do)
+    for a, b in zip(ends, ends[1:]):          # every sequence as the dense path computes it: the same roundings, sums in another order
+        x = qkv[a:b, None].detach().requires_grad_()
+        alone = attention.rope_flash_attn_func(x, cos, sin, H, G)
+        (ref,) = torch.autograd.grad(alone, x, do[a:b, None].permute(1, 2, 0, 3))
+        assert torch.equal(o[a:b], alone[0].transpose(0, 1))
+        assert (grad[a:b].float() - ref[:, 0].float()).norm() <= 2 * 2.0 ** -8 * ref.float().norm()
+    assert not o[470:].any() and not grad[470:].any()
+
+
+def test_other_types_take_one_sequence_after_the_other():
+    q, k, v, do = (x.float() for x in _inputs(130, 4, 2, 64))
+    ends = [0, 60, 120]
+    got, want = _run(q, k, v, do, ends, True), packed(q, k, v, ends, True, do)
+    for name in got:          # at most 60 products, 2^-24 each, numbers below 8
+        assert (got[name].double() - want[name][0]).abs().max() <= 2.0 ** -24 * 60 * 64
