@@ -1,0 +1,367 @@
+// Load-balancing loss of a mixture's routers with its per-expert counts, and its gradient (reference:
+// src/neuronx_distributed/modules/moe/loss_function.py:5-48).
+//
+//   p_r = softmax(x_r) over E experts, S_r = the k largest logits of row r (ties: the lowest expert; NaN counts as largest),
+//   f_e = #{r : e in S_r} / n,  P_e = sum_r p_re / n,  loss = E / k sum_e f_e P_e     over the n rows that the mask leaves
+//   d loss / d x_re = E / (k n) p_re (f_e - sum_j p_rj f_j)
+//
+// The rows are those of up to 128 tensors (the layers' routers), read where they are.  L lanes share a row and hold V neighbouring experts
+// each, so a row is read in 16-byte pieces and the softmax is L-lane shuffles; a thread keeps its experts' sums and counts in
+// registers over all its rows.  Sums of a block go to global memory in a fixed order and a second kernel adds the blocks' in
+// double precision: no atomics, the loss does not depend on the schedule.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int kMaxLayers = 128;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+struct Layers {
+    const void* x[kMaxLayers];
+    long long ld[kMaxLayers];            // elements between rows
+    long long first[kMaxLayers + 1];     // rows of the layers before
+};
+struct RouterArgs {
+    const unsigned char* mask;           // [rows of a layer] or NULL: 0 leaves the row out
+    int E, k, vec;                       // vec: whole 16-byte pieces
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ void from_float(float v, float& o) { o = v; }
+__device__ __forceinline__ void from_float(float v, bf16& o) { o = __float2bfloat16(v); }
+__device__ __forceinline__ void from_float(float v, __half& o) { o = __float2half(v); }
+
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, float (&x)[V]) {
+    constexpr int N = 16 / sizeof(T) < V ? 16 / sizeof(T) : V;
+    if (vec && e0 + V <= E) {
+#pragma unroll
+        for (int i = 0; i < V; i += N) {
+            struct alignas(N * sizeof(T)) Piece { T v[N]; };
+            const Piece p = *reinterpret_cast<const Piece*>(row + e0 + i);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[i + j] = to_float(p.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = e0 + i < E ? to_float(row[e0 + i]) : -INFINITY;
+    }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* row, int e0, int E, bool vec, const float (&x)[V]) {
+    constexpr int N = 16 / sizeof(T) < V ? 16 / sizeof(T) : V;
+    if (vec && e0 + V <= E) {
+#pragma unroll
+        for (int i = 0; i < V; i += N) {
+            struct alignas(N * sizeof(T)) Piece { T v[N]; } p;
+#pragma unroll
+            for (int j = 0; j < N; ++j) from_float(x[i + j], p.v[j]);
+            *reinterpret_cast<Piece*>(row + e0 + i) = p;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (e0 + i < E) from_float(x[i], row[e0 + i]);
+    }
+}
+
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// x <- softmax of the row.  A NaN, or a maximum that is infinite, makes the whole row NaN, as exp(x - max) / sum does.
+template <int L, int V>
+__device__ __forceinline__ void softmax_row(float (&x)[V]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
+    m = group_max<L>(m);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += x[i] = expf(x[i] - m);
+    const float inv = 1.f / group_sum<L>(s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] *= inv;
+}
+
+// larger numbers have larger keys, +0 and -0 the same one, NaN the largest; 0 is below every number's
+__device__ __forceinline__ uint32_t order_key(float v) {
+    if (v != v) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(v + 0.f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// grid (blocks of a layer, layers).  part_p / part_c: [blocks][E] sums of probabilities and counts.
+template <typename T, int L, int V>
+__global__ void __launch_bounds__(kThreads) balance_fwd_kernel(const __grid_constant__ Layers layers, const RouterArgs a,
+                                                               float* __restrict__ part_p, int* __restrict__ part_c) {
+    constexpr int R = kThreads / L;      // rows of a block at a time
+    pdl_trigger();
+    pdl_wait();
+    const int layer = blockIdx.y, l = threadIdx.x % L, e0 = l * V;
+    const T* x0 = reinterpret_cast<const T*>(layers.x[layer]);
+    const long long ld = layers.ld[layer], rows = layers.first[layer + 1] - layers.first[layer];
+    float sum[V];
+    int count[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f, count[i] = 0;
+    // all lanes of a warp go through the same iterations: the shuffles want every one
+    for (long long r0 = (long long)blockIdx.x * R; r0 < rows; r0 += (long long)gridDim.x * R) {
+        const long long r = r0 + threadIdx.x / L;
+        const bool valid = r < rows && (a.mask == nullptr || a.mask[r] != 0);
+        float x[V];
+        load_row<T, V>(x0 + min(r, rows - 1) * ld, e0, a.E, a.vec, x);
+        uint32_t key[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = e0 + i < a.E ? order_key(x[i]) : 0u;
+        softmax_row<L, V>(x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += valid ? x[i] : 0.f;
+        for (int j = 0; j < a.k; ++j) {
+            uint32_t best = key[0];
+            int at = e0;
+#pragma unroll
+            for (int i = 1; i < V; ++i)
+                if (key[i] > best) best = key[i], at = e0 + i;
+            unsigned long long top = (unsigned long long)best << 32 | (uint32_t)~at;
+#pragma unroll
+            for (int o = 1; o < L; o <<= 1) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, top, o);
+                top = other > top ? other : top;
+            }
+            at = (int)~(uint32_t)top;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (at == e0 + i) key[i] = 0u, count[i] += valid;
+        }
+    }
+    // lanes that hold the same experts, then the warps, in one array for either
+    __shared__ uint32_t s_warp[kWarps][L * V];
+    const long long base = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * a.E;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int o = L; o < 32; o <<= 1) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+            count[i] += __shfl_xor_sync(0xffffffffu, count[i], o);
+        }
+        if ((threadIdx.x & 31) < L) s_warp[threadIdx.x >> 5][e0 + i] = __float_as_uint(sum[i]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += kThreads) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) s += __uint_as_float(s_warp[w][e]);
+        part_p[base + e] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if ((threadIdx.x & 31) < L) s_warp[threadIdx.x >> 5][e0 + i] = (uint32_t)count[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += kThreads) {
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) c += (int)s_warp[w][e];
+        part_c[base + e] = c;
+    }
+}
+
+// One block: sums over the blocks of the first kernel, the loss, the counts, and for the gradient f_e E / (k n).
+constexpr int kFinalThreads = 1024;
+__global__ void __launch_bounds__(kFinalThreads) balance_final_kernel(const float* __restrict__ part_p, const int* __restrict__ part_c,
+                                                                      int blocks, int E, int k, float* loss, long long* counts,
+                                                                      float* share) {
+    __shared__ double s_p[kFinalThreads];
+    __shared__ long long s_c[kFinalThreads];
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x;
+    int W = 1;                            // threads of one expert group
+    while (W < E) W <<= 1;                // at most 1024
+    const int e = tid % W, g = tid / W, G = kFinalThreads / W;
+    double p = 0.0;
+    long long c = 0;
+    if (e < E)
+        for (int b = g; b < blocks; b += G) {
+            p += (double)part_p[(long long)b * E + e];
+            c += part_c[(long long)b * E + e];
+        }
+    s_p[tid] = p;
+    s_c[tid] = c;
+    __syncthreads();
+    for (int h = kFinalThreads / 2; h >= W; h >>= 1) {
+        if (tid < h) s_p[tid] += s_p[tid + h], s_c[tid] += s_c[tid + h];
+        __syncthreads();
+    }
+    if (tid < W) p = s_p[tid], c = s_c[tid];
+    __syncthreads();
+    // over the experts: sum of f_e P_e and of the counts, which are k for every row
+    if (tid < W) s_p[tid] = (double)c * p;
+    __syncthreads();
+    for (int h = W / 2; h > 0; h >>= 1) {
+        if (tid < h) s_p[tid] += s_p[tid + h], s_c[tid] += s_c[tid + h];
+        __syncthreads();
+    }
+    const double n = (double)(s_c[0] / k), factor = n > 0.0 ? (double)E / ((double)k * n * n) : 0.0;
+    if (tid == 0) *loss = n > 0.0 ? (float)(s_p[0] * factor) : 0.f;
+    if (tid < E) {
+        counts[tid] = c;
+        share[tid] = (float)((double)c * factor);
+    }
+}
+
+template <typename T, int L, int V>
+__global__ void __launch_bounds__(kThreads) balance_bwd_kernel(const __grid_constant__ Layers layers, const RouterArgs a,
+                                                               const float* __restrict__ share, const float* __restrict__ grad,
+                                                               T* __restrict__ dx) {
+    constexpr int R = kThreads / L;
+    pdl_trigger();
+    pdl_wait();
+    const int layer = blockIdx.y, l = threadIdx.x % L, e0 = l * V;
+    const T* x0 = reinterpret_cast<const T*>(layers.x[layer]);
+    const long long ld = layers.ld[layer], first = layers.first[layer], rows = layers.first[layer + 1] - first;
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = e0 + i < a.E ? share[e0 + i] : 0.f;
+    const float g = *grad;
+    for (long long r0 = (long long)blockIdx.x * R; r0 < rows; r0 += (long long)gridDim.x * R) {
+        const long long r = r0 + threadIdx.x / L;
+        const bool valid = r < rows && (a.mask == nullptr || a.mask[r] != 0);
+        float x[V];
+        load_row<T, V>(x0 + min(r, rows - 1) * ld, e0, a.E, a.vec, x);
+        softmax_row<L, V>(x);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) s = fmaf(x[i], e0 + i < a.E ? f[i] : 0.f, s);
+        s = group_sum<L>(s);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = valid ? x[i] * (f[i] - s) * g : 0.f;
+        if (r < rows) store_row<T, V>(dx + (first + r) * a.E, e0, a.E, a.vec, x);
+    }
+}
+
+struct Plan {
+    Layers layers;
+    RouterArgs args;
+    int blocks_x, n;
+};
+
+// blocks of a layer: enough of all layers together to fill the chip, no more than there are rows for
+int blocks_of(long long most_rows, int layers, int lanes) {
+    const long long want = (most_rows + kThreads / lanes - 1) / (kThreads / lanes);
+    const long long fill = (6ll * 148 + layers - 1) / layers;
+    return (int)(want < fill ? want : fill);
+}
+int lanes_of(int E) {
+    int l = 1;
+    while (l < 32 && l * 8 < E) l <<= 1;
+    return l;
+}
+
+int make_plan(Plan* p, const void* const* x, const long long* ld, const long long* rows, int n, int elem, const void* mask, int E, int k,
+              const void* dx) {
+    NXD_REQUIRE(n > 0 && n <= kMaxLayers && E > 0 && E <= 1024 && k > 0 && k <= E, "balance_loss: %d tensors, %d of %d experts", n, k, E);
+    long long most = 0, total = 0;
+    bool vec = (long long)E * elem % 16 == 0 && ((uintptr_t)dx & 15) == 0;
+    for (int i = 0; i < n; ++i) {
+        NXD_REQUIRE(rows[i] >= 0, "balance_loss: %lld rows", rows[i]);
+        p->layers.x[i] = x[i];
+        p->layers.ld[i] = ld[i];
+        p->layers.first[i] = total;
+        total += rows[i];
+        most = rows[i] > most ? rows[i] : most;
+        vec = vec && ((uintptr_t)x[i] & 15) == 0 && ld[i] * elem % 16 == 0;
+    }
+    p->layers.first[n] = total;
+    NXD_REQUIRE(total < (1ll << 31) && total * k < (1ll << 40), "balance_loss: %lld rows", total);
+    p->args = RouterArgs{(const unsigned char*)mask, E, k, vec};
+    p->n = n;
+    p->blocks_x = blocks_of(most, n, lanes_of(E));
+    if (p->blocks_x < 1) p->blocks_x = 1;
+    return 0;
+}
+
+template <typename T, int L, int V>
+int run(const Plan& p, float* part_p, int* part_c, const float* share, const float* grad, void* dx, cudaStream_t st) {
+    const dim3 grid(p.blocks_x, p.n);
+    if (dx == nullptr)
+        NXD_CHECK_CUDA((nxd_launch_pdl(balance_fwd_kernel<T, L, V>, grid, dim3(kThreads), 0, st, p.layers, p.args, part_p, part_c)));
+    else
+        NXD_CHECK_CUDA((nxd_launch_pdl(balance_bwd_kernel<T, L, V>, grid, dim3(kThreads), 0, st, p.layers, p.args, share, grad, (T*)dx)));
+    NXD_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T>
+int run_sized(const Plan& p, float* part_p, int* part_c, const float* share, const float* grad, void* dx, cudaStream_t st) {
+    const int E = p.args.E;
+    if (E <= 8) return run<T, 1, 8>(p, part_p, part_c, share, grad, dx, st);
+    if (E <= 16) return run<T, 2, 8>(p, part_p, part_c, share, grad, dx, st);
+    if (E <= 32) return run<T, 4, 8>(p, part_p, part_c, share, grad, dx, st);
+    if (E <= 64) return run<T, 8, 8>(p, part_p, part_c, share, grad, dx, st);
+    if (E <= 128) return run<T, 16, 8>(p, part_p, part_c, share, grad, dx, st);
+    if (E <= 256) return run<T, 32, 8>(p, part_p, part_c, share, grad, dx, st);
+    if (E <= 512) return run<T, 32, 16>(p, part_p, part_c, share, grad, dx, st);
+    return run<T, 32, 32>(p, part_p, part_c, share, grad, dx, st);
+}
+
+int run_typed(const Plan& p, int dtype, float* part_p, int* part_c, const float* share, const float* grad, void* dx, cudaStream_t st) {
+    if (dtype == 0) return run_sized<float>(p, part_p, part_c, share, grad, dx, st);
+    if (dtype == 1) return run_sized<bf16>(p, part_p, part_c, share, grad, dx, st);
+    return run_sized<__half>(p, part_p, part_c, share, grad, dx, st);
+}
+
+}  // namespace
+
+// Blocks of the first kernel: its scratch is that many times E floats and as many ints.
+NXD_API int nxd_balance_loss_num_blocks(long long most_rows, int layers, int E) {
+    const int b = blocks_of(most_rows, layers, lanes_of(E));
+    return (b < 1 ? 1 : b) * layers;
+}
+
+// x, ld, rows: HOST arrays of `layers` device pointers, row strides (elements; unit stride along the experts) and row counts;
+// dtype 0 fp32, 1 bf16, 2 fp16; mask: NULL, or a byte per row that every layer shares.  loss: 1 float, counts: E int64, share: E floats
+// for the backward call, scratch: nxd_balance_loss_num_blocks * E * 8 bytes.
+NXD_API int nxd_balance_loss_fwd(const void* const* x, const long long* ld, const long long* rows, int layers, int dtype,
+                                 const void* mask, int E, int k, float* loss, long long* counts, float* share, void* scratch,
+                                 void* stream) {
+    NXD_REQUIRE(dtype >= 0 && dtype <= 2, "balance_loss: dtype %d", dtype);
+    Plan p;
+    int rc = make_plan(&p, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, nullptr);
+    if (rc) return rc;
+    const int blocks = p.blocks_x * layers;
+    float* part_p = (float*)scratch;
+    int* part_c = (int*)(part_p + (long long)blocks * E);
+    cudaStream_t st = (cudaStream_t)stream;
+    if ((rc = run_typed(p, dtype, part_p, part_c, nullptr, nullptr, nullptr, st))) return rc;
+    NXD_CHECK_CUDA(nxd_launch_pdl(balance_final_kernel, dim3(1), dim3(kFinalThreads), 0, st, (const float*)part_p, (const int*)part_c, blocks,
+                                  E, k, loss, counts, share));
+    NXD_LAUNCH_CHECK();
+    return 0;
+}
+
+// dx: [all rows, E] in x's type, the layers one after the other; grad: the loss's gradient, 1 float on the device.
+NXD_API int nxd_balance_loss_bwd(const void* const* x, const long long* ld, const long long* rows, int layers, int dtype,
+                                 const void* mask, int E, int k, const float* share, const float* grad, void* dx, void* stream) {
+    NXD_REQUIRE(dtype >= 0 && dtype <= 2 && dx != nullptr, "balance_loss: dtype %d", dtype);
+    Plan p;
+    int rc = make_plan(&p, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, dx);
+    if (rc) return rc;
+    return run_typed(p, dtype, nullptr, nullptr, share, grad, dx, (cudaStream_t)stream);
+}

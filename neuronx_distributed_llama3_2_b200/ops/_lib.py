@@ -85,7 +85,7 @@ GROUPS["state_space_serving"] = ["window_attention.cu", "state_space.cu", "strea
 
 # sources whose fp32 state is carried over thousands of steps: no approximate exp / tanh / division
 PRECISE_SOURCES = {"mlstm.cu", "delta_rule.cu", "delta_chunks.cu", "retention.cu", "retention_tc.cu", "hyper_connection.cu", "stream_norm.cu",
-                   "state_space.cu"}
+                   "state_space.cu", "balance_loss.cu"}
 
 _lib: Optional[ctypes.CDLL] = None
 _group_libs = {}

@@ -11,6 +11,7 @@ import math
 from typing import List, Optional, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rope import _aligned as _rope_aligned, _launch as _rope_launch
@@ -155,6 +156,7 @@ class _PackedAttnFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -182,6 +184,7 @@ class _RopePackedAttnFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         rot, o, lse, cos, sin, positions = ctx.saved_tensors
         n_q, n_kv, packed, scale = ctx.args

@@ -1,0 +1,169 @@
+"""The load-balancing loss, its counts and its gradient against float64."""
+import math
+
+import pytest
+import torch
+
+from neuronx_distributed_llama3_2_b200.modules.moe import load_balancing_loss_func
+
+BF16, FP16, FP32 = 2.0 ** -8, 2.0 ** -11, 2.0 ** -24
+
+
+def oracle(logits, E, k, mask=None, coef=1.0):
+    x = torch.cat([t.detach().reshape(-1, E) for t in logits]).double()
+    keep = torch.ones(x.shape[0], dtype=torch.bool, device=x.device) if mask is None else mask.reshape(-1).bool().repeat(len(logits))
+    p = torch.softmax(x, -1)[keep]
+    counts = torch.zeros(E, dtype=torch.int64, device=x.device)
+    left = torch.where(torch.isnan(x), math.inf, x)[keep]
+    for _ in range(k):
+        best = (left == left.amax(-1, keepdim=True)).int().argmax(-1)
+        counts += torch.bincount(best, minlength=E)
+        left = left.scatter(1, best[:, None], float("-inf"))
+    n = max(1, int(keep.sum()))
+    f, P = counts.double() / n, p.sum(0) / n
+    dx = torch.zeros_like(x)
+    dx[keep] = coef * E / (k * n) * p * (f - (p * f).sum(-1, keepdim=True))
+    return E / k * (f * P).sum(), counts, dx
+
+
+def _logits(layers, rows, E, dtype, device, seed=0):
+    g = torch.Generator(device=device).manual_seed(seed + E)
+    lean = torch.randn(E, generator=g, device=device)
+    return [(1.5 * torch.randn(rows, E, generator=g, device=device) + lean).to(dtype) for _ in range(layers)]
+
+
+def _check(logits, E, k, mask, coef=1.0):
+    leaves = [t.detach().requires_grad_() for t in logits]
+    loss, counts = load_balancing_loss_func(leaves, E, k, mask=mask, return_counts=True)
+    assert loss.dtype == torch.float32 and counts.dtype == torch.int64 and not counts.requires_grad
+    grads = torch.autograd.grad(loss, leaves, torch.full((), coef, device=loss.device))
+    want_loss, want_counts, want = oracle(logits, E, k, mask, coef)
+    assert torch.equal(counts, want_counts)
+    # probabilities: an exponential, a sum of E terms and a product, 2^-24 each; the loss also sums over the rows in fp32, a few hundred
+    # a thread
+    assert abs(loss.double() - want_loss) <= FP32 * (8 + E / 8 + 256) * want_loss
+    got = torch.cat([x.reshape(-1, E) for x in grads]).double()
+    step = {torch.float32: 0.0, torch.bfloat16: BF16, torch.float16: FP16}[logits[0].dtype]
+    # f - sum p f loses what the two have in common: relative to the larger of them, not to their difference
+    top = want_counts.max().double() / max(1, int(want_counts.sum()) // k)
+    x = torch.cat([t.reshape(-1, E) for t in logits]).double()
+    scale = abs(coef) * E / k / max(1, int(want_counts.sum()) // k) * torch.softmax(x, -1) * top
+    tiny = 2.0 ** -25 if logits[0].dtype == torch.float16 else 1e-38          # half of fp16's smallest step
+    assert ((got - want).abs() <= step * want.abs() + FP32 * (24 + E / 4) * scale * 4 + tiny).all()
+    return loss, counts, grads
+
+
+@pytest.mark.parametrize("E,k", [(1, 1), (2, 1), (5, 5), (8, 2), (16, 4)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_torch_path(E, k, masked):
+    logits = _logits(3, 17, E, torch.float32, "cpu")
+    mask = (torch.arange(17) % 3 > 0) if masked else None
+    _check(logits, E, k, mask)
+
+
+def test_gradient_is_a_difference():
+    logits = [t.double() for t in _logits(2, 7, 5, torch.float64, "cpu")]
+    g = torch.Generator().manual_seed(3)
+    mask = torch.tensor([1, 1, 0, 1, 0, 1, 1])
+    d = [torch.randn(7, 5, generator=g, dtype=torch.float64) for _ in logits]
+    _, counts, dx = oracle(logits, 5, 2, mask)
+    ahead, back = ([t + s * 1e-6 * e for t, e in zip(logits, d)] for s in (1, -1))
+    assert torch.equal(oracle(ahead, 5, 2, mask)[1], counts) and torch.equal(oracle(back, 5, 2, mask)[1], counts)
+    slope = (oracle(ahead, 5, 2, mask)[0] - oracle(back, 5, 2, mask)[0]) / 2e-6
+    assert abs(slope - (dx * torch.cat(d)).sum()) <= 1e-8          # central difference: 1e-12, and 1e-16 / 1e-6 of rounding
+
+
+def test_no_rows_and_refusals():
+    x = torch.randn(4, 8, requires_grad=True)
+    loss, counts = load_balancing_loss_func([x, None], 8, 2, mask=torch.zeros(4), return_counts=True)
+    assert loss.item() == 0.0 and not counts.any() and not torch.autograd.grad(loss, x)[0].any()
+    for bad in (dict(router_logits=[], num_experts=8, top_k=2), dict(router_logits=x, num_experts=8, top_k=9),
+                dict(router_logits=x, num_experts=8, top_k=0), dict(router_logits=x, num_experts=5, top_k=2),
+                dict(router_logits=[x, x[:3]], num_experts=8, top_k=2, mask=torch.ones(4))):
+        with pytest.raises(ValueError):
+            load_balancing_loss_func(**bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,k", [(1, 1), (2, 1), (3, 2), (8, 2), (8, 8), (9, 3), (16, 4), (31, 6), (64, 8), (100, 7), (128, 8), (129, 2),
+                                 (256, 8), (300, 4), (512, 10), (1000, 3), (1024, 16)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_kernel(E, k, dtype):
+    for layers, rows, masked in ((1, 1, False), (3, 130, True), (2, 1037, False)):
+        logits = _logits(layers, rows, E, dtype, "cuda", seed=rows)
+        mask = (torch.rand(rows, generator=torch.Generator().manual_seed(E)) < 0.7).cuda() if masked else None
+        _check(logits, E, k, mask, coef=0.02 * layers * rows)
+
+
+@pytest.mark.gpu
+def test_kernel_of_many_layers_and_rows():
+    _check(_logits(100, 77, 8, torch.bfloat16, "cuda"), 8, 2, None)
+    _check(_logits(129, 5, 8, torch.float32, "cuda"), 8, 2, None)          # more tensors than one launch takes: torch
+    _check(_logits(1, 300001, 16, torch.float32, "cuda"), 16, 4, torch.arange(300001, device="cuda") < 299990)
+    uneven = [t for n in (0, 3, 1000, 1) for t in _logits(1, n, 8, torch.float32, "cuda")]
+    _check(uneven, 8, 2, None)
+
+
+@pytest.mark.gpu
+def test_kernel_reads_views():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    wide = torch.randn(50, 3, 24, generator=g, device="cuda")
+    odd = torch.randn(50 * 3 * 8 + 1, generator=g, device="cuda")[1:].view(50, 3, 8)
+    for x in (wide[..., 8:16], wide[..., ::3], odd, wide[:1, :, :8].expand(50, 3, 8), wide[:, :1, :8].expand(50, 3, 8)):
+        _check([x], 8, 2, None)
+        _check([x, odd], 8, 2, torch.arange(300, device="cuda")[::2] % 4 < 3)
+
+
+@pytest.mark.gpu
+def test_ties_and_special_values():
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[0.0, -0.0, 0.0, 0.0], [-inf, -inf, 1.0, -inf], [2.0, 2.0, 1.0, 2.0], [-1.0, -1.0, -inf, -1.0], [1e-40, 0.0, -1e-40, 0.0]])
+    _, counts = load_balancing_loss_func(x.cuda(), 4, 2, return_counts=True)
+    # row 2 has one finite logit: the second is the lowest expert of the infinite ones
+    assert counts.tolist() == [5, 4, 1, 0] and counts.tolist() == load_balancing_loss_func(x, 4, 2, return_counts=True)[1].tolist()
+    for row in ([0.0, nan, 1.0, 2.0], [inf, 0.0, 1.0, 2.0], [-inf] * 4):
+        y = torch.cat([x, torch.tensor([row])])
+        for mask in (None, torch.tensor([1, 1, 1, 1, 1, 0])):
+            got = load_balancing_loss_func(y.cuda(), 4, 2, mask=None if mask is None else mask.cuda(), return_counts=True)
+            want = load_balancing_loss_func(y, 4, 2, mask=mask, return_counts=True)
+            assert torch.equal(got[1].cpu(), want[1]) and got[0].isnan().item() == want[0].isnan().item() == (mask is None)
+    leaf = torch.cat([x, torch.full((1, 4), nan)]).cuda().requires_grad_()
+    loss = load_balancing_loss_func(leaf, 4, 2, mask=torch.tensor([1, 1, 1, 1, 1, 0], device="cuda"))
+    (grad,) = torch.autograd.grad(loss, leaf)
+    assert grad.isfinite().all() and not grad[5].any()
+
+
+@pytest.mark.gpu
+def test_same_bits_twice_captured_and_on_another_stream():
+    logits = [t.requires_grad_() for t in _logits(4, 3000, 8, torch.float32, "cuda")]
+
+    def step():
+        loss, counts = load_balancing_loss_func(logits, 8, 2, return_counts=True)
+        return [loss.detach(), counts, *torch.autograd.grad(loss, logits)]
+
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        third = step()
+    graph.replay()
+    for a, b, c in zip(first, second, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    with torch.no_grad():
+        logits[2].mul_(-1.0)
+    graph.replay()
+    for a, c in zip(step(), third):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_part_of_the_layers_needs_gradients():
+    a, b = _logits(2, 40, 8, torch.float32, "cuda")
+    a.requires_grad_()
+    loss = load_balancing_loss_func([b, a], 8, 2)
+    loss.backward()
+    assert (a.grad.double() - oracle([b, a], 8, 2)[2][40:]).abs().max() <= 1e-7
