@@ -28,7 +28,7 @@ def load_balancing_loss_func(router_logits: Union[torch.Tensor, Sequence[torch.T
         raise ValueError("no router logits")
     if not 0 < top_k <= num_experts:
         raise ValueError(f"Invalid top_k={top_k} for num_experts={num_experts}")
-    if any(t.numel() % num_experts for t in logits):
+    if any(t.shape[-1:] != (num_experts,) and t.numel() % num_experts for t in logits):
         raise ValueError(f"router logits {[tuple(t.shape) for t in logits]} are no rows of {num_experts}")
     if mask is not None:
         mask = mask.reshape(-1).bool().contiguous()

@@ -83,9 +83,10 @@ GROUPS["state_space_serving"] = ["window_attention.cu", "state_space.cu", "strea
                                  "runtime.cu", "gemm_tcgen05.cu", "gemm_smallm.cu", "fused_gemm_ar.cu", "tma_host.cu",
                                  "flash_attn_tc.cu", "attn_tc_host.cu"]
 
-# sources whose fp32 state is carried over thousands of steps: no approximate exp / tanh / division
+# sources whose fp32 state is carried over thousands of steps, or whose fp32 results are exact to a rounding: no approximate exp /
+# tanh / division, no flushed subnormals
 PRECISE_SOURCES = {"mlstm.cu", "delta_rule.cu", "delta_chunks.cu", "retention.cu", "retention_tc.cu", "hyper_connection.cu", "stream_norm.cu",
-                   "state_space.cu", "balance_loss.cu"}
+                   "state_space.cu", "balance_loss.cu", "dropout.cu"}
 
 _lib: Optional[ctypes.CDLL] = None
 _group_libs = {}
@@ -270,6 +271,25 @@ def kernel_launches() -> int:
 def stream_ptr() -> ctypes.c_void_p:
     """The current stream of the current device, without a ``Stream`` object in between (5 us of every launch)."""
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+
+
+class _Here:
+    """A device guard that has nothing to do."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (launches go to its current stream); free of charge where it is already."""
+    index = t.get_device()
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def check(code: int, what: str, handle: Optional[ctypes.CDLL] = None) -> None:

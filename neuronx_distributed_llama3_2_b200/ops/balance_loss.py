@@ -16,54 +16,57 @@ MAX_LAYERS, MAX_EXPERTS = 128, 1024
 
 def _rows(t: torch.Tensor, E: int) -> torch.Tensor:
     """``[rows, E]`` with unit stride along the experts."""
-    t = t.reshape(-1, E)
-    return t if E == 1 or t.stride(1) == 1 else t.contiguous()
+    if t.dim() != 2 or t.shape[1] != E:
+        t = t.reshape(-1, E)
+    return t if t.stride(1) == 1 or E == 1 else t.contiguous()
 
 
 def qualifies(logits: List[torch.Tensor], E: int) -> bool:
     x = logits[0]
-    return (x.is_cuda and x.dtype in _DTYPES and len(logits) <= MAX_LAYERS and E <= MAX_EXPERTS
-            and all(t.dtype == x.dtype and t.device == x.device for t in logits) and _lib.available())
-
-
-def _table(rows: List[torch.Tensor]):
-    n = len(rows)
-    return ((_c.c_void_p * n)(*[t.data_ptr() for t in rows]), (_c.c_longlong * n)(*[t.stride(0) for t in rows]),
-            (_c.c_longlong * n)(*[t.shape[0] for t in rows]), _c.c_int(n), _c.c_int(_DTYPES[rows[0].dtype]))
+    dtype, device = x.dtype, x.get_device()
+    return (x.is_cuda and dtype in _DTYPES and len(logits) <= MAX_LAYERS and E <= MAX_EXPERTS
+            and all(t.dtype is dtype and t.get_device() == device for t in logits) and _lib.available())
 
 
 class _BalanceLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, E, top_k, mask, *logits):
         rows = [_rows(t, E) for t in logits]
-        dev = rows[0].device
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        counts = torch.empty(E, dtype=torch.int64, device=dev)
+        sizes = [t.shape[0] for t in rows]
+        n, x = len(rows), rows[0]
+        # pointers, row strides, rows: built once, the backward call reads the same tensors
+        table = ((_c.c_void_p * n)(*[t.data_ptr() for t in rows]), (_c.c_longlong * n)(*[t.stride(0) for t in rows]),
+                 (_c.c_longlong * n)(*sizes), _c.c_int(n), _c.c_int(_DTYPES[x.dtype]), _lib.ptr(mask), _c.c_int(E), _c.c_int(top_k))
         lib = _lib.lib()
-        blocks = lib.nxd_balance_loss_num_blocks(_c.c_longlong(max(t.shape[0] for t in rows)), _c.c_int(len(rows)), _c.c_int(E))
-        share = torch.empty(E + 2 * blocks * E, dtype=torch.float32, device=dev)          # the shares, then the call's scratch
-        with torch.cuda.device(dev):
-            rc = lib.nxd_balance_loss_fwd(*_table(rows), _lib.ptr(mask), _c.c_int(E), _c.c_int(top_k), _lib.ptr(loss), _lib.ptr(counts),
-                                          _lib.ptr(share), _c.c_void_p(share.data_ptr() + 4 * E), _lib.stream_ptr())
+        blocks = lib.nxd_balance_loss_num_blocks(_c.c_longlong(max(sizes)), _c.c_int(n), _c.c_int(E))
+        loss = torch.empty((), dtype=torch.float32, device=x.device)
+        counts = torch.empty(E, dtype=torch.int64, device=x.device)
+        share = torch.empty(E + 2 * blocks * E, dtype=torch.float32, device=x.device)     # the shares, then the call's scratch
+        with _lib.on_device_of(x):
+            rc = lib.nxd_balance_loss_fwd(*table, _lib.ptr(loss), _lib.ptr(counts), _lib.ptr(share),
+                                          _c.c_void_p(share.data_ptr() + 4 * E), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_fwd")
         ctx.mark_non_differentiable(counts)
         ctx.save_for_backward(share, mask, *rows)
-        ctx.args = (E, top_k, [t.shape for t in logits])
+        ctx.args = (table, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
         return loss, counts
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _):
-        share, mask, *rows = ctx.saved_tensors
-        E, top_k, shapes = ctx.args
-        sizes = [t.shape[0] for t in rows]
-        dx = torch.empty((sum(sizes), E), dtype=rows[0].dtype, device=rows[0].device)
+        saved = ctx.saved_tensors          # all of them: none may have been written since
+        share, x = saved[0], saved[2]
+        table, sizes, shapes = ctx.args
+        dx = torch.empty((sum(sizes), x.shape[1]), dtype=x.dtype, device=x.device)
         grad = grad.float()
-        with torch.cuda.device(dx.device):
-            rc = _lib.lib().nxd_balance_loss_bwd(*_table(rows), _lib.ptr(mask), _c.c_int(E), _c.c_int(top_k), _lib.ptr(share),
-                                                 _lib.ptr(grad), _lib.ptr(dx), _lib.stream_ptr())
+        with _lib.on_device_of(x):
+            rc = _lib.lib().nxd_balance_loss_bwd(*table, _lib.ptr(share), _lib.ptr(grad), _lib.ptr(dx), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_bwd")
-        grads = [g.view(s) if need else None for g, s, need in zip(dx.split(sizes), shapes, ctx.needs_input_grad[3:])]
+        grads = dx.split(sizes)
+        if any(s is not None for s in shapes):
+            grads = [g if s is None else g.view(s) for g, s in zip(grads, shapes)]
+        if not all(ctx.needs_input_grad[3:]):
+            grads = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[3:])]
         return (None, None, None, *grads)
 
 

@@ -40,8 +40,8 @@ def dropout_keep(shape, p: float, seed: int, offset: int = 0, device=None) -> to
 
 
 def _launch(x, residual, p, seed, offset, state, used):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
+    y = torch.empty_like(x)
+    with _lib.on_device_of(x):
         rc = _lib.lib().nxd_dropout(
             _lib.ptr(x), _lib.ptr(residual), _lib.ptr(y), _c.c_longlong(x.numel()), _c.c_int(_DTYPES[x.dtype]), _c.c_double(p),
             _c.c_ulonglong(seed), _c.c_ulonglong(offset), _lib.ptr(state), _c.c_int(0 if state is None else state.numel()),
@@ -101,7 +101,9 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: Seed = None, offset: int = 0,
             raise RuntimeError("a captured dropout would drop the same elements in every replay: pass its seed as a tensor")
         seed = int(torch.randint(0, 2 ** 62, (1,)).item())
     if x.is_cuda and x.dtype in _DTYPES and _lib.available():
-        return _DropoutFn.apply(x, residual, p, seed & _M64, offset & _M64, state)
+        if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
+            return _DropoutFn.apply(x, residual, p, seed & _M64, offset & _M64, state)
+        return _launch(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed & _M64, offset & _M64, state, None)
     if state is not None:
         numbers = state.view(-1).tolist()
         seed, offset = numbers[0], offset + (numbers[1] if len(numbers) > 1 else 0)

@@ -47,12 +47,11 @@ class PackedSequences:
     def plan(self, causal: bool) -> Tuple[torch.Tensor, int, int]:
         """``(tile list, its entries, columns of the per-row scratch)`` for the kernels, made on first use."""
         if causal not in self._plans:
-            lib = _lib.lib()
-            lib.nxd_packed_plan_columns.restype = _c.c_longlong
-            entries = lib.nxd_packed_plan_entries(_c.c_longlong(self.total), _c.c_int(self.count))
-            columns = lib.nxd_packed_plan_columns(_c.c_longlong(self.total), _c.c_int(self.count))
+            most = min(self.count, self.total)
+            entries = self.total // 128 + most + 2                          # nxd_packed_plan_entries
+            columns = (self.total + 3 * most + 3 & ~3) + 64                 # nxd_packed_plan_columns
             lists = torch.empty((entries + self.count, 4), dtype=torch.int32, device=self.device)
-            rc = lib.nxd_packed_plan(_lib.ptr(self.cu_seqlens), _c.c_int(self.cu_seqlens.dtype == torch.int64), _c.c_int(self.count),
+            rc = _lib.lib().nxd_packed_plan(_lib.ptr(self.cu_seqlens), _c.c_int(self.cu_seqlens.dtype == torch.int64), _c.c_int(self.count),
                                      _c.c_longlong(self.total), _c.c_int(causal), _lib.ptr(lists),
                                      _c.c_void_p(lists.data_ptr() + 16 * entries), _lib.stream_ptr())
             _lib.check(rc, "nxd_packed_plan")
@@ -101,14 +100,19 @@ def as_packed(sequences: Union[torch.Tensor, PackedSequences], total: int, devic
 def _fix(t: torch.Tensor) -> torch.Tensor:
     """Unit stride on the head dimension, the others multiples of 8 elements that do not overlap, 16-byte aligned."""
     T, H, D = t.shape
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0
-    ok = ok and (H == 1 or t.stride(1) % 8 == 0 and t.stride(1) >= D) and (T == 1 or t.stride(0) % 8 == 0 and t.stride(0) >= D)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    row, head, unit = t.stride()
+    if unit == 1 and t.data_ptr() % 16 == 0 and (H == 1 or head % 8 == 0 and head >= D) and (T == 1 or row % 8 == 0 and row >= D):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(*ts: torch.Tensor):
     """(head, row) strides; a dimension of one has any."""
-    vals = [s for t in ts for s in (t.stride(1) if t.shape[1] > 1 else t.shape[2], t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2])]
+    vals = []
+    for t in ts:
+        T, H, D = t.shape
+        row, head, _ = t.stride()
+        vals += (head if H > 1 else D, row if T > 1 else H * D)
     return (_c.c_longlong * len(vals))(*vals)
 
 
@@ -148,7 +152,7 @@ class _PackedAttnFn(torch.autograd.Function):
     def forward(ctx, q, k, v, packed, scale, causal):
         q, k, v = _fix(q), _fix(k), _fix(v)
         grad = any(ctx.needs_input_grad[:3])
-        with torch.cuda.device(q.device):
+        with _lib.on_device_of(q):
             o, lse = _forward(q, k, v, packed, scale, causal, grad)
         if grad:
             ctx.save_for_backward(q, k, v, o, lse)
@@ -160,7 +164,7 @@ class _PackedAttnFn(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, o, lse = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        with torch.cuda.device(q.device):
+        with _lib.on_device_of(q):
             _backward(q, k, v, o, lse, do, dq, dk, dv, *ctx.args)
         return dq, dk, dv, None, None, None
 
@@ -172,7 +176,7 @@ class _RopePackedAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, cos, sin, n_q, n_kv, packed, scale):
         T, heads, D = qkv.shape
-        with torch.cuda.device(qkv.device):
+        with _lib.on_device_of(qkv):
             qkv = _rope_aligned(qkv)
             rot = torch.empty_like(qkv)
             positions = packed.positions()
@@ -189,7 +193,7 @@ class _RopePackedAttnFn(torch.autograd.Function):
         rot, o, lse, cos, sin, positions = ctx.saved_tensors
         n_q, n_kv, packed, scale = ctx.args
         parts = lambda x: (x[:, :n_q], x[:, n_q:n_q + n_kv], x[:, n_q + n_kv:])     # noqa: E731
-        with torch.cuda.device(rot.device):
+        with _lib.on_device_of(rot):
             d = torch.empty_like(rot)
             _backward(*parts(rot), o, lse, do, *parts(d), packed, scale, True)
             _rope_launch(d, cos, sin, n_q + n_kv, 1, 1 << 30, positions, True)
@@ -198,6 +202,9 @@ class _RopePackedAttnFn(torch.autograd.Function):
 
 def packed_attn_nxd(q, k, v, packed: PackedSequences, softmax_scale: Optional[float], causal: bool) -> torch.Tensor:
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or v.requires_grad):
+        with _lib.on_device_of(q):
+            return _forward(_fix(q), _fix(k), _fix(v), packed, float(scale), bool(causal), False)[0]
     return _PackedAttnFn.apply(q, k, v, packed, float(scale), bool(causal))
 
 
