@@ -13,11 +13,14 @@
 
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kMaxLayers = 128;
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;            // forward: few blocks, so that there is little to add up
 constexpr int kWarps = kThreads / 32;
+constexpr int kBwdThreads = 256;
 
 struct Layers {
     const void* x[kMaxLayers];
@@ -84,6 +87,14 @@ __device__ __forceinline__ float group_max(float v) {
     return v;
 }
 
+// 2^x by the hardware instruction: within 2 units in the last place, and the rounding of its argument (x - max) log2 e adds 2^-24 of
+// that argument, so a probability of 2^-10 is off by 6e-7 of itself at most.
+__device__ __forceinline__ float exp_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
 // x <- softmax of the row.  A NaN, or a maximum that is infinite, makes the whole row NaN, as exp(x - max) / sum does.
 template <int L, int V>
 __device__ __forceinline__ void softmax_row(float (&x)[V]) {
@@ -93,17 +104,59 @@ __device__ __forceinline__ void softmax_row(float (&x)[V]) {
     m = group_max<L>(m);
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) s += x[i] = expf(x[i] - m);
-    const float inv = 1.f / group_sum<L>(s);
+    for (int i = 0; i < V; ++i) s += x[i] = exp_of(x[i] - m);
+    const float inv = __fdividef(1.f, group_sum<L>(s));          // 1 <= sum <= E: the approximate reciprocal is off by 2^-23
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] *= inv;
 }
 
-// larger numbers have larger keys, +0 and -0 the same one, NaN the largest; 0 is below every number's
-__device__ __forceinline__ uint32_t order_key(float v) {
-    if (v != v) return 0xffffffffu;
-    const uint32_t b = __float_as_uint(v + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+// Larger numbers have larger keys, +0 and -0 the same one, NaN the largest; 0 is below every number's.  Numbers of 16 bits leave room
+// for the expert, so that no two keys of a row are equal and the lower of two equal logits has the larger one.
+template <typename T>
+__device__ __forceinline__ uint32_t order_key(float v, int e) {
+    v += 0.f;          // -0 becomes +0, and every NaN the one whose bits are 0x7fffffff
+    uint32_t b = __float_as_uint(v);
+    if (std::is_same<T, __half>::value) b = (uint32_t)__half_as_ushort(__float2half_rn(v)) << 16;          // the bits that were read
+    const uint32_t k = b ^ (uint32_t)((int)b >> 31 | (int)0x80000000);
+    return sizeof(T) == 4 ? k : (k & 0xffff0000u) | (uint32_t)(0xffff - e);
+}
+
+// the eight largest of the keys, largest first
+template <int N>
+__device__ __forceinline__ void order2(uint32_t (&h)[N], int i, int j) {
+    const uint32_t a = max(h[i], h[j]), b = min(h[i], h[j]);
+    h[i] = a;
+    h[j] = b;
+}
+// Batcher's odd-even merge sort of eight, 19 exchanges
+__device__ __forceinline__ void sort8(uint32_t (&h)[8]) {
+    order2(h, 0, 1), order2(h, 2, 3), order2(h, 4, 5), order2(h, 6, 7);
+    order2(h, 0, 2), order2(h, 1, 3), order2(h, 4, 6), order2(h, 5, 7);
+    order2(h, 1, 2), order2(h, 5, 6);
+    order2(h, 0, 4), order2(h, 1, 5), order2(h, 2, 6), order2(h, 3, 7);
+    order2(h, 2, 4), order2(h, 3, 5);
+    order2(h, 1, 2), order2(h, 3, 4), order2(h, 5, 6);
+}
+template <int V>
+__device__ __forceinline__ void top8(const uint32_t (&key)[V], uint32_t (&h)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = key[i];
+    sort8(h);
+#pragma unroll
+    for (int g = 8; g < V; g += 8) {
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = key[g + i];
+        sort8(o);
+        // the larger halves of two sorted lists are a bitonic list
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = max(h[i], o[7 - i]);
+#pragma unroll
+        for (int d = 4; d > 0; d >>= 1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!(i & d)) order2(h, i, i + d);
+    }
 }
 
 // grid (blocks of a layer, layers).  part_p / part_c: [blocks][E] sums of probabilities and counts.
@@ -120,6 +173,8 @@ __global__ void __launch_bounds__(kThreads) balance_fwd_kernel(const __grid_cons
     int count[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f, count[i] = 0;
+    const int lane = threadIdx.x & 31;
+    const unsigned lanes_below = ((1u << lane) - 1u) & (0xffffffffu << (lane & ~(L - 1)));          // of this row's lanes
     // all lanes of a warp go through the same iterations: the shuffles want every one
     for (long long r0 = (long long)blockIdx.x * R; r0 < rows; r0 += (long long)gridDim.x * R) {
         const long long r = r0 + threadIdx.x / L;
@@ -128,56 +183,105 @@ __global__ void __launch_bounds__(kThreads) balance_fwd_kernel(const __grid_cons
         load_row<T, V>(x0 + min(r, rows - 1) * ld, e0, a.E, a.vec, x);
         uint32_t key[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = e0 + i < a.E ? order_key(x[i]) : 0u;
+        for (int i = 0; i < V; ++i) key[i] = e0 + i < a.E ? order_key<T>(x[i], e0 + i) : 0u;
         softmax_row<L, V>(x);
 #pragma unroll
         for (int i = 0; i < V; ++i) sum[i] += valid ? x[i] : 0.f;
-        for (int j = 0; j < a.k; ++j) {
-            uint32_t best = key[0];
-            int at = e0;
+        // The k-th largest key: every lane's largest ones in order, and k times the largest first one of the row's lanes leaves its list.
+        // Equal keys (fp32 only) would leave together: then more than k keys are as large as the last one, and the row's warp takes them
+        // one by one, the lowest expert first.
+        bool exact = a.k <= 8;
+        if (exact) {
+            uint32_t h[8], last = 0u;
+            top8<V>(key, h);
+            for (int j = 0; j < a.k; ++j) {
+                last = h[0];
 #pragma unroll
-            for (int i = 1; i < V; ++i)
-                if (key[i] > best) best = key[i], at = e0 + i;
-            unsigned long long top = (unsigned long long)best << 32 | (uint32_t)~at;
+                for (int o = 1; o < L; o <<= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+                const bool pop = h[0] == last;
 #pragma unroll
-            for (int o = 1; o < L; o <<= 1) {
-                const unsigned long long other = __shfl_xor_sync(0xffffffffu, top, o);
-                top = other > top ? other : top;
+                for (int i = 0; i < 7; ++i) h[i] = pop ? h[i + 1] : h[i];
+                h[7] = pop ? 0u : h[7];
             }
-            at = (int)~(uint32_t)top;
+            int chosen = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (at == e0 + i) key[i] = 0u, count[i] += valid;
+            for (int i = 0; i < V; ++i) chosen += key[i] >= last;
+            if (sizeof(T) == 4) {
+                int all = chosen;
+#pragma unroll
+                for (int o = 1; o < L; o <<= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+                exact = __all_sync(0xffffffffu, all == a.k);
+            }
+            if (exact) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) count[i] += valid && key[i] >= last;
+            }
+        }
+        if (!exact) {
+            for (int j = 0; j < a.k; ++j) {
+                uint32_t best = key[0];
+#pragma unroll
+                for (int i = 1; i < V; ++i) best = max(best, key[i]);
+                uint32_t top = best;
+#pragma unroll
+                for (int o = 1; o < L; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                bool mine = true;
+                if (L > 1) mine = (__ballot_sync(0xffffffffu, best == top) & lanes_below) == 0u;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const bool hit = mine && key[i] == top;
+                    if (hit) key[i] = 0u;
+                    mine = mine && !hit;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) count[i] += valid && key[i] == 0u;          // those past E too: they are not stored
         }
     }
-    // lanes that hold the same experts, then the warps, in one array for either
-    __shared__ uint32_t s_warp[kWarps][L * V];
+    // lanes that hold the same experts, then the warps in a fixed order, in one array for sums and counts
+    __shared__ uint32_t s_warp[kWarps / 2][L * V];
     const long long base = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * a.E;
+    const int warp = threadIdx.x >> 5, slot = warp % (kWarps / 2);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int o = L; o < 32; o <<= 1) {
             sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
             count[i] += __shfl_xor_sync(0xffffffffu, count[i], o);
         }
-        if ((threadIdx.x & 31) < L) s_warp[threadIdx.x >> 5][e0 + i] = __float_as_uint(sum[i]);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        if (warp / (kWarps / 2) == half && lane < L) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                uint32_t* at = &s_warp[slot][e0 + i];
+                *at = __float_as_uint(half ? __uint_as_float(*at) + sum[i] : sum[i]);
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += kThreads) {
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += __uint_as_float(s_warp[w][e]);
+        for (int w = 0; w < kWarps / 2; ++w) s += __uint_as_float(s_warp[w][e]);
         part_p[base + e] = s;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if ((threadIdx.x & 31) < L) s_warp[threadIdx.x >> 5][e0 + i] = (uint32_t)count[i];
-    __syncthreads();
+    for (int half = 0; half < 2; ++half) {
+        if (warp / (kWarps / 2) == half && lane < L) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                uint32_t* at = &s_warp[slot][e0 + i];
+                *at = half ? *at + (uint32_t)count[i] : (uint32_t)count[i];
+            }
+        }
+        __syncthreads();
+    }
     for (int e = threadIdx.x; e < a.E; e += kThreads) {
         int c = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) c += (int)s_warp[w][e];
+        for (int w = 0; w < kWarps / 2; ++w) c += (int)s_warp[w][e];
         part_c[base + e] = c;
     }
 }
@@ -198,6 +302,7 @@ __global__ void __launch_bounds__(kFinalThreads) balance_final_kernel(const floa
     double p = 0.0;
     long long c = 0;
     if (e < E)
+#pragma unroll 8
         for (int b = g; b < blocks; b += G) {
             p += (double)part_p[(long long)b * E + e];
             c += part_c[(long long)b * E + e];
@@ -227,10 +332,10 @@ __global__ void __launch_bounds__(kFinalThreads) balance_final_kernel(const floa
 }
 
 template <typename T, int L, int V>
-__global__ void __launch_bounds__(kThreads) balance_bwd_kernel(const __grid_constant__ Layers layers, const RouterArgs a,
+__global__ void __launch_bounds__(kBwdThreads) balance_bwd_kernel(const __grid_constant__ Layers layers, const RouterArgs a,
                                                                const float* __restrict__ share, const float* __restrict__ grad,
                                                                T* __restrict__ dx) {
-    constexpr int R = kThreads / L;
+    constexpr int R = kBwdThreads / L;
     pdl_trigger();
     pdl_wait();
     const int layer = blockIdx.y, l = threadIdx.x % L, e0 = l * V;
@@ -263,10 +368,11 @@ struct Plan {
 };
 
 // blocks of a layer: enough of all layers together to fill the chip, no more than there are rows for
-int blocks_of(long long most_rows, int layers, int lanes) {
-    const long long want = (most_rows + kThreads / lanes - 1) / (kThreads / lanes);
-    const long long fill = (6ll * 148 + layers - 1) / layers;
-    return (int)(want < fill ? want : fill);
+int blocks_of(long long most_rows, int layers, int lanes, bool backward) {
+    const int threads = backward ? kBwdThreads : kThreads;
+    const long long want = (most_rows + threads / lanes - 1) / (threads / lanes);
+    const long long fill = ((backward ? 8ll : 3ll) * 148 + layers - 1) / layers, n = want < fill ? want : fill;
+    return n < 1 ? 1 : (int)n;
 }
 int lanes_of(int E) {
     int l = 1;
@@ -292,8 +398,7 @@ int make_plan(Plan* p, const void* const* x, const long long* ld, const long lon
     NXD_REQUIRE(total < (1ll << 31) && total * k < (1ll << 40), "balance_loss: %lld rows", total);
     p->args = RouterArgs{(const unsigned char*)mask, E, k, vec};
     p->n = n;
-    p->blocks_x = blocks_of(most, n, lanes_of(E));
-    if (p->blocks_x < 1) p->blocks_x = 1;
+    p->blocks_x = blocks_of(most, n, lanes_of(E), dx != nullptr);
     return 0;
 }
 
@@ -303,7 +408,7 @@ int run(const Plan& p, float* part_p, int* part_c, const float* share, const flo
     if (dx == nullptr)
         NXD_CHECK_CUDA((nxd_launch_pdl(balance_fwd_kernel<T, L, V>, grid, dim3(kThreads), 0, st, p.layers, p.args, part_p, part_c)));
     else
-        NXD_CHECK_CUDA((nxd_launch_pdl(balance_bwd_kernel<T, L, V>, grid, dim3(kThreads), 0, st, p.layers, p.args, share, grad, (T*)dx)));
+        NXD_CHECK_CUDA((nxd_launch_pdl(balance_bwd_kernel<T, L, V>, grid, dim3(kBwdThreads), 0, st, p.layers, p.args, share, grad, (T*)dx)));
     NXD_LAUNCH_CHECK();
     return 0;
 }
@@ -331,8 +436,7 @@ int run_typed(const Plan& p, int dtype, float* part_p, int* part_c, const float*
 
 // Blocks of the first kernel: its scratch is that many times E floats and as many ints.
 NXD_API int nxd_balance_loss_num_blocks(long long most_rows, int layers, int E) {
-    const int b = blocks_of(most_rows, layers, lanes_of(E));
-    return (b < 1 ? 1 : b) * layers;
+    return blocks_of(most_rows, layers, lanes_of(E), false) * layers;
 }
 
 // x, ld, rows: HOST arrays of `layers` device pointers, row strides (elements; unit stride along the experts) and row counts;

@@ -127,6 +127,9 @@ def test_ties_and_special_values():
             got = load_balancing_loss_func(y.cuda(), 4, 2, mask=None if mask is None else mask.cuda(), return_counts=True)
             want = load_balancing_loss_func(y, 4, 2, mask=mask, return_counts=True)
             assert torch.equal(got[1].cpu(), want[1]) and got[0].isnan().item() == want[0].isnan().item() == (mask is None)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):          # a NaN of either sign is the largest
+        row = torch.tensor([1.0, nan, 2.0, -nan]).copysign(torch.tensor([1.0, 1.0, 1.0, -1.0])).to(dtype)
+        assert load_balancing_loss_func(row[None].cuda(), 4, 2, return_counts=True)[1].tolist() == [0, 1, 0, 1]
     leaf = torch.cat([x, torch.full((1, 4), nan)]).cuda().requires_grad_()
     loss = load_balancing_loss_func(leaf, 4, 2, mask=torch.tensor([1, 1, 1, 1, 1, 0], device="cuda"))
     (grad,) = torch.autograd.grad(loss, leaf)
