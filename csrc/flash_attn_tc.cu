@@ -53,11 +53,6 @@ struct TcParams {
     int page_size, table_cols, cache_rows;      // cache_rows: rows of a line (of a page)
     const bf16* v;               // values, for the last tile's rows (see the producer)
     long long v_line, v_head, v_row;
-    // PACKED instantiation only: one entry per CTA row, the row stride of the per-row scratch and the output
-    const PackedTile* tiles;
-    long long lse_row;
-    bf16* o;
-    long long o_head, o_row;
 };
 
 template <int D>
@@ -89,10 +84,7 @@ struct TcSmem {
 // Bound by the softmax like the other instantiations; portion of 2048 after 2048 tokens, 2 rows, 32 heads of 128 over 8,
 // window 2048 (138 GF): 168 us (820 TF) against 587 us on the mma.sync kernel over the cache (window_attention.cu).  A tile takes its
 // softmax warp 2400 clocks: 1050 exponentials, 460 bias, 430 waiting for scores; without bias 530 more for the accumulator.
-// PACKED: sequences of different lengths laid end to end, [rows, heads, D].  A CTA takes one entry of the batch's tile list and stays
-// inside its sequence: key tiles start at the sequence's first row, the V tile that crosses its end is copied like CACHE's, and the
-// rows of a 32-row store box that belong to the next sequence are left alone by storing the others one by one.
-template <int D, bool CAUSAL, bool DROP, bool WIN = false, int SCORE = 0, bool CACHE = false, bool PACKED = false>
+template <int D, bool CAUSAL, bool DROP, bool WIN = false, int SCORE = 0, bool CACHE = false>
 __global__ void __launch_bounds__(kThreadsTc, 2)
 fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                  const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o,
@@ -114,25 +106,17 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(pv_done + 1);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    if (CACHE || PACKED) pdl_wait();
-    PackedTile pt{};
-    if (PACKED) {
-        pt = packed_tile(p.tiles, blockIdx.x / p.Hq);
-        if (pt.len == 0) {
-            block_zero_rows<D>(p.o + (long long)pt.start * p.o_row + (blockIdx.x % p.Hq) * p.o_head, p.o_row, pt.t, threadIdx.x, kThreadsTc);
-            return;
-        }
-    }
+    if (CACHE) pdl_wait();
     // grid = (q heads, batch, q blocks): the q block is the slowest launch dimension and counted from the end, so the
     // long causal rows of EVERY head are scheduled before any short one (longest-first list scheduling)
-    const int mb = PACKED ? pt.t : gridDim.z - 1 - blockIdx.z;
-    const int hq = PACKED ? blockIdx.x % p.Hq : blockIdx.x, b = PACKED ? 0 : blockIdx.y;
+    const int mb = gridDim.z - 1 - blockIdx.z;
+    const int hq = blockIdx.x, b = blockIdx.y;
     const int hkv = hq / (p.Hq / p.Hkv);
     const int m0 = mb * kBM;
-    const int n_real = PACKED ? pt.len : !CACHE ? p.Sq : (p.n_new != nullptr ? min(p.n_new[b], p.Sq) : p.Sq);
+    const int n_real = !CACHE ? p.Sq : (p.n_new != nullptr ? min(p.n_new[b], p.Sq) : p.Sq);
     const int line = CACHE && p.seq_ids != nullptr ? p.seq_ids[b] : b;
-    const int offset = CACHE ? p.q_start[b] : PACKED ? 0 : p.Sk - p.Sq;      // position of query row 0
-    const int sk = PACKED ? pt.len : CACHE ? offset + n_real : p.Sk;
+    const int offset = CACHE ? p.q_start[b] : p.Sk - p.Sq;      // position of query row 0
+    const int sk = CACHE ? offset + n_real : p.Sk;
     int n_tiles = m0 < n_real ? (sk + kBN - 1) / kBN : 0;
     if (CAUSAL) n_tiles = min(n_tiles, max((m0 + kBM + offset + kBN - 1) / kBN, 0));
     int n_sink = 0, t_win = 0;
@@ -166,7 +150,7 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         ptx::fence_barrier_init();
     }
     if (warp == 1) ptx::tmem_alloc<1>(tmem_ptr_smem, L::kTmemCols);
-    if (!CACHE && !PACKED) pdl_wait();
+    if (!CACHE) pdl_wait();
     float* dtab = reinterpret_cast<float*>(sP);          // bias table (SCORE): the P staging area is free, P lives in TMEM
     constexpr float kL2e = score::kLog2e;                // r1 ln(.) in log2 units is r1 log2(.)
     constexpr float kSign = SCORE == 2 ? -1.f : 1.f;     // sigmoid weights are computed from the negative score
@@ -191,14 +175,14 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 
     if (warp == 0) {
         // ============================ TMA producer ============================
-        if ((CACHE || PACKED || lane == 0) && n_tiles > 0) {
+        if ((CACHE || lane == 0) && n_tiles > 0) {
             int c[4];
             if (lane == 0) {
                 ptx::mbar_arrive_expect_tx(q_full, L::kQBytes);
 #pragma unroll
                 for (int g = 0; g < D / 64; ++g) {
                     c[0] = g * 64;
-                    coords(p.pos_q, (PACKED ? pt.start : 0) + m0, hq, b, c);
+                    coords(p.pos_q, m0, hq, b, c);
                     tma_load_4d(&tmap_q, q_full, sQ + g * (kBM * 128), c[0], c[1], c[2], c[3]);
                 }
             }
@@ -212,15 +196,6 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     row = row0 % p.page_size;
                 }
                 ptx::mbar_wait(&slot_empty[slot], ph ^ 1u);
-                if (PACKED) row += pt.start;
-                if (PACKED && map == &tmap_v && row0 + kBN > sk) {
-                    warp_load_tile<D>(sRing + slot * L::kSlotBytes, p.v + hkv * p.v_head + row * p.v_row, p.v_row, kBN, sk - row0, lane);
-                    ptx::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&slot_full[slot]);
-                    ++it;
-                    return;
-                }
                 if (CACHE && map == &tmap_v && row0 + kBN > sk) {        // the last tile: zeros behind the end
                     const bf16* src = p.v + at * p.v_line + hkv * p.v_head + row * p.v_row;
                     const int rows = min(sk - row0, p.cache_rows - row);
@@ -237,7 +212,7 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     ++it;
                     return;
                 }
-                if ((CACHE || PACKED) && lane != 0) {
+                if (CACHE && lane != 0) {
                     ++it;
                     return;
                 }
@@ -523,9 +498,7 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         if (WIN && SCORE != 2 && p.sinks != nullptr && m_run != -INFINITY) l_run += ex2_approx(p.sinks[hq] * kL2e - m_run);
         float inv = l_run > 0.f ? 1.f / l_run : 0.f;
         if (WIN && grow < p.Sq) inv *= score::out_gate<bf16>(p.mod, (long long)b * p.Sq + grow, hq);
-        if (PACKED && p.lse && grow < n_real)
-            p.lse[hq * p.lse_row + pt.pad + grow] = l_run > 0.f ? m_run * sc + log2f(l_run) : INFINITY;
-        if (!PACKED && p.lse && grow < p.Sq)
+        if (p.lse && grow < p.Sq)
             p.lse[((long long)b * p.Hq + hq) * p.Sq + grow] = l_run > 0.f ? m_run * sc + log2f(l_run) : INFINITY;
         // every MMA that read Q has completed: reuse the Q tile as staging (warp q owns rows [32q, 32q+32) of
         // each 64-column group: 32 rows x 128 bytes = one TMA store box)
@@ -563,23 +536,12 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 }
                 st_shared_v4(dst + ((c ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
-            if (PACKED && m0 + q * 32 + 32 > n_real) {           // the rows behind the end are the next sequence's
-                __syncwarp();
-                const uint8_t* src = sQ + g * (kBM * 128) + q * 32 * 128;
-                for (int i = lane; i < 32 * 8; i += 32) {
-                    const int r = i >> 3, ch = i & 7;
-                    if (m0 + q * 32 + r < n_real)
-                        *reinterpret_cast<uint4*>(p.o + hq * p.o_head + (long long)(pt.start + m0 + q * 32 + r) * p.o_row + g * 64 + ch * 8) =
-                            *reinterpret_cast<const uint4*>(src + r * 128 + ((ch ^ (r & 7)) << 4));
-                }
-                continue;
-            }
             ptx::fence_proxy_async();
             __syncwarp();
-            if (lane == 0 && (PACKED || m0 + q * 32 < p.Sq)) {
+            if (lane == 0 && m0 + q * 32 < p.Sq) {
                 int c[4];
                 c[0] = g * 64;
-                coords(p.pos_o, (PACKED ? pt.start : 0) + m0 + q * 32, hq, b, c);
+                coords(p.pos_o, m0 + q * 32, hq, b, c);
                 tma_store_4d(&tmap_o, sQ + g * (kBM * 128) + q * 32 * 128, c[0], c[1], c[2], c[3]);
                 ptx::bulk_commit();
             }
@@ -625,53 +587,7 @@ int launch_fwd_tc_win(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
     return 0;
 }
 
-template <int D, bool CAUSAL>
-int launch_fwd_tc_packed(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const TcParams& p,
-                         int entries, cudaStream_t st) {
-    using L = TcSmem<D>;
-    constexpr auto kern = fa_fwd_tc_kernel<D, CAUSAL, false, false, 0, false, true>;
-    NXD_CHECK_CUDA(nxd_allow_smem<kern>(L::kBytes));
-    NXD_CHECK_CUDA(nxd_launch_pdl(kern, dim3((unsigned)entries * p.Hq), dim3(kThreadsTc), L::kBytes, st, tq, tk, tv, to, p));
-    NXD_LAUNCH_CHECK();
-    return 0;
-}
-
 }  // namespace
-
-// Attention inside each sequence of a packed batch: q [T, Hq, D], k and v [T, Hkv, D], o [T, Hq, D], strides {q_h, q_row, k_h,
-// k_row, v_h, v_row, o_h, o_row} in elements (multiples of 8), 16-byte aligned bases; tiles: the `entries` tiles that
-// nxd_packed_plan has made; lse NULL or [Hq, lse_row] floats, log2 units, written at the plan's padded columns.  Rows
-// outside every sequence get zeros.
-NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const long long* strides,
-                                const void* tiles, int entries, long long lse_row, long long T, int Hq, int Hkv, int D, float scale,
-                                int causal, void* stream) {
-    NXD_REQUIRE(D == 64 || D == 128, "packed_attn: head dim %d not supported (64 or 128)", D);
-    NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && (long long)entries * Hq < (1ll << 31),
-                "packed_attn: bad problem");
-    for (int i = 0; i < 8; ++i)
-        NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
-    NXD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)tiles) & 15) == 0,
-                "packed_attn: tensors must be 16-byte aligned");
-    TcParams p{};
-    p.lse = lse; p.lse_row = lse_row;
-    p.B = 1; p.Hq = Hq; p.Hkv = Hkv; p.Sq = p.Sk = (int)T;
-    p.scale_log2 = scale * 1.4426950408889634f;
-    p.drop.inv_keep = 1.f;
-    p.tiles = (const PackedTile*)tiles;
-    p.v = (const bf16*)v; p.v_head = strides[4]; p.v_row = strides[5];
-    p.o = (bf16*)o; p.o_head = strides[6]; p.o_row = strides[7];
-    CUtensorMap tq, tk, tv, to;
-    int rc;
-    if ((rc = make_tmap_bhsd(&tq, q, D, T, Hq, 1, strides[1], strides[0], 0, kBM, p.pos_q))) return rc;
-    if ((rc = make_tmap_bhsd(&tk, k, D, T, Hkv, 1, strides[3], strides[2], 0, kBN, p.pos_k))) return rc;
-    if ((rc = make_tmap_bhsd(&tv, v, D, T, Hkv, 1, strides[5], strides[4], 0, kBN, p.pos_v))) return rc;
-    if ((rc = make_tmap_bhsd(&to, o, D, T, Hq, 1, strides[7], strides[6], 0, 32, p.pos_o))) return rc;
-    cudaStream_t st = (cudaStream_t)stream;
-    if (D == 64) return causal ? launch_fwd_tc_packed<64, true>(tq, tk, tv, to, p, entries, st)
-                               : launch_fwd_tc_packed<64, false>(tq, tk, tv, to, p, entries, st);
-    return causal ? launch_fwd_tc_packed<128, true>(tq, tk, tv, to, p, entries, st)
-                  : launch_fwd_tc_packed<128, false>(tq, tk, tv, to, p, entries, st);
-}
 
 // Same arguments as nxd_flash_attn_fwd.  Extra requirement: 16-byte aligned base pointers.
 static int fwd_tc_impl(const void* q, const void* k, const void* v, void* o, float* lse, const long long* strides, int B,

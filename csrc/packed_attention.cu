@@ -1,0 +1,652 @@
+// Attention over packed sequences, forward, on 5th-gen tensor cores (tcgen05 + TMEM + TMA), sm_100a.
+//
+// q [T, Hq, D], k and v [T, Hkv, D]: the sequences of a batch laid end to end, each attending to itself (tile list: packed_plan.cu).
+//   S = scale Q K^T, P = exp2(S - m), O = P V / sum P over the keys of the row's sequence (up to the row itself if causal)
+//
+// One CTA per SM stays for the whole call and walks over items of two query tiles of 128 rows that read the same keys and values: two
+// heads of one key head, or (where the heads of a key head are odd in number) two neighbouring tiles of one head.  Sequences of
+// fine-tuning are a few hundred tokens, so an item is a few key tiles long: with a CTA per item its start (barriers, tensor memory,
+// the first loads) and end were most of its time.  Here the loads of the next item and its first scores run under the last softmax and
+// the stores of this one.
+//   warps 0-3, 4-7   softmax of query tile 0 / 1, a thread per row; the accumulator stays in tensor memory and is rescaled where a row's
+//                    maximum has moved by more than 2^8; at the end of an item they divide and store their rows
+//   warp 8           MMA: S_s = Q_s K^T (128 x 128), O_s += P_s V with P_s from tensor memory, s = 0, 1 in turn
+//   warp 9           TMA: Q_s of an item, key and value tiles of 128 rows in the order of their use through one ring
+// D = 128: two accumulators and two score tiles fill the tensor memory, so P_s lies in the columns of S_s, and S_s of the next tile follows
+// P_s V (the tensor core works in issue order).  D = 64: P_s has columns of its own, and S_s of the next tile is computed as soon as the
+// scores are in registers, so the softmax warps, which bound this size (128 exponentials a row for half the products), never wait.
+#include "attn_tc_common.cuh"
+#include "gemm_tcgen05.cuh"
+#include "ptx.cuh"
+
+namespace {
+using namespace nxd_attn;
+
+constexpr int kBM = 128, kBN = 128;
+constexpr int kThreads = 384;                     // 8 softmax warps, MMA, TMA, two without work (registers move by groups of four warps)
+constexpr float kRescale = 8.0f;                  // log2 units
+constexpr long long kWaitClocks = 4000000000ll;   // a wait that takes two seconds is given up: the CTA's results are NaN then
+
+struct FwdParams {
+    const PackedTile* tiles;
+    float* lse;
+    bf16* o;
+    const bf16* v;
+    long long lse_row, o_head, o_row, v_head, v_row;
+    int entries, Hq, group, pairs;                // pairs: items of one tile-list entry
+    int pos_q[3], pos_k[3], pos_v[3];
+    float scale_log2;
+};
+
+template <int D>
+struct FwdSmem {
+    static constexpr int kTileBytes = 128 * D * 2;
+    static constexpr int kSlots = D == 64 ? 8 : 5;
+    static constexpr int kQOff = 0;
+    static constexpr int kRingOff = 2 * kTileBytes;
+    static constexpr int kBarOff = kRingOff + kSlots * kTileBytes;
+    static constexpr int kNumBars = 4 + 2 * kSlots + 10 + 8;
+    static constexpr int kBytes = kBarOff + kNumBars * 8 + 16 + 1024;
+    static constexpr uint32_t kPolyOf8 = D == 64 ? 0x52 : 0x44;          // of eight pairs of weights, those by the polynomial
+    // tensor memory: O_0 O_1 | S_0 S_1 | P_0 P_1 (D = 64; else P_s = the first columns of S_s)
+    static constexpr bool kAlias = D == 128;
+    static constexpr uint32_t kColS = 2 * D, kColP = kAlias ? kColS : kColS + 256, kPStep = kAlias ? 128 : 64;
+};
+static_assert(FwdSmem<128>::kBytes <= 232448 && FwdSmem<64>::kBytes > 116 * 1024, "one CTA per SM");
+
+// A wait with an end: after kWaitClocks the CTA is marked, and no wait of its lasts any more.
+__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, volatile int* dead) {
+    if (ptx::mbar_try_wait(bar, parity)) return;
+    const long long start = clock64();
+    for (int i = 1;; ++i) {
+        if (ptx::mbar_try_wait(bar, parity) || *dead) return;
+        if ((i & 63) == 0 && clock64() - start > kWaitClocks) *dead = 1;
+    }
+}
+
+// The items of this CTA: every gridDim.x-th of the list, which is sorted by weight, forwards and backwards in turn so that nobody gets
+// the longest of every round.  The TMA warp, which is ahead of the others, reads them and hands them on through shared memory.
+struct alignas(16) Item {
+    int kind, start, len, pad;           // kind: 0 end of the list, 1 an item, above: that many rows from `start` are of no sequence
+    int t0, t1, n0, n1;                  // query tiles and the key tiles that they meet (0: there is no second one)
+    int h0, h1, hkv, unused;
+    __device__ __forceinline__ int t(int s) const { return s ? t1 : t0; }
+    __device__ __forceinline__ int n(int s) const { return s ? n1 : n0; }
+    __device__ __forceinline__ int h(int s) const { return s ? h1 : h0; }
+};
+constexpr int kRowsOfNone = 1;           // added to the rows of such an entry, to tell them from an item
+
+template <bool CAUSAL, bool HEADS>
+__device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
+    const int G = gridDim.x;
+    const long long at = (long long)round * G + (round & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
+    Item it{};
+    if (at >= (long long)p.entries * p.pairs) return it;
+    const int pr = (int)(at % p.pairs);
+    const PackedTile pt = packed_tile(p.tiles, (int)(at / p.pairs));
+    it.start = pt.start, it.len = pt.len, it.pad = pt.pad;
+    it.h0 = HEADS ? 2 * pr : pr;
+    it.h1 = HEADS ? it.h0 + 1 : it.h0;
+    if (pt.len == 0) {                   // an entry without anything: all that follow are like it
+        it.kind = pt.t > 0 ? pt.t + kRowsOfNone : 0;
+        return it;
+    }
+    const int all = (pt.len + kBN - 1) / kBN;
+    it.kind = 1;
+    it.hkv = it.h0 / p.group;
+    it.t0 = HEADS ? pt.t : 2 * pt.t;     // entries are of 128 rows, or of 256 where an item is two tiles of one head
+    it.t1 = HEADS ? pt.t : 2 * pt.t + 1;
+    it.n0 = CAUSAL ? it.t0 + 1 : all;
+    it.n1 = it.t1 < all ? (CAUSAL ? it.t1 + 1 : all) : 0;
+    return it;
+}
+
+constexpr int kItems = 4;                // of the ring in shared memory
+constexpr int kItemReaders = 9;          // the MMA thread and a lane of each softmax warp
+
+// the next item of the ring, for a whole warp or (WARP = false) one thread
+template <bool WARP>
+__device__ __forceinline__ Item next_item(const Item* ring, uint64_t* full, uint64_t* empty, int& count, volatile int* dead) {
+    const int i = count % kItems;
+    wait_for(&full[i], (uint32_t)(count / kItems) & 1u, dead);
+    ++count;
+    Item it{};
+    if (!*dead) {
+        const int4* src = reinterpret_cast<const int4*>(&ring[i]);
+        int4* dst = reinterpret_cast<int4*>(&it);
+#pragma unroll
+        for (int w = 0; w < 3; ++w) dst[w] = src[w];
+    }
+    if (WARP) __syncwarp();
+    if (!WARP || (threadIdx.x & 31) == 0) ptx::mbar_arrive(&empty[i]);
+    return it;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {          // NaN if one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^z of two numbers up to 2^7 by the FMA pipe, beside the 16 exponentials a clock of the special function unit: 2^z = 2^n 2^f with n the
+// nearest whole number, f in [-1/2, 1/2], and 2^f by the cubic of least relative error there (7.5e-5, fitted by linear
+// programming; a weight is rounded to 2^-8 anyway).  Numbers below -126 count as that.
+__device__ __forceinline__ void exp2_poly(uint64_t z, float& p0, float& p1) {
+    const float lo = fmaxf(f2_lo(z), -126.f), hi = fmaxf(f2_hi(z), -126.f);
+    const uint64_t x = f2_pack(lo, hi), magic = f2_pack(12582912.f, 12582912.f), neg_magic = f2_pack(-12582912.f, -12582912.f);
+    const uint64_t t = f2_add(x, magic);                                   // n in the low bits
+    const uint64_t f = f2_fma(f2_add(t, neg_magic), f2_pack(-1.f, -1.f), x);
+    uint64_t h = f2_fma(f, f2_pack(0.0551716685f, 0.0551716685f), f2_pack(0.2426111400f, 0.2426111400f));
+    h = f2_fma(f, h, f2_pack(0.6932609677f, 0.6932609677f));
+    h = f2_fma(f, h, f2_pack(0.9999280572f, 0.9999280572f));
+    p0 = __uint_as_float((uint32_t)h + ((uint32_t)t << 23));
+    p1 = __uint_as_float((uint32_t)(h >> 32) + ((uint32_t)(t >> 32) << 23));
+}
+
+template <int D, bool CAUSAL, bool HEADS>
+__global__ void __launch_bounds__(kThreads, 1)
+packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ FwdParams p) {
+    using L = FwdSmem<D>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ int dead_word;
+    __shared__ Item item_ring[kItems];
+    uint8_t* smem = ptx::align_smem_1024(smem_raw);
+    uint8_t* sQ = smem + L::kQOff;
+    uint8_t* sRing = smem + L::kRingOff;
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* kv_full = q_empty + 2;
+    uint64_t* kv_empty = kv_full + L::kSlots;
+    uint64_t* s_full = kv_empty + L::kSlots;
+    uint64_t* s_empty = s_full + 2;
+    uint64_t* p_half = s_empty + 2;
+    uint64_t* p_full = p_half + 2;
+    uint64_t* pv_done = p_full + 2;
+    uint64_t* item_full = pv_done + 2;
+    uint64_t* item_empty = item_full + kItems;
+    uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(item_empty + kItems);
+    volatile int* dead = &dead_word;
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        dead_word = 0;
+        for (int s = 0; s < 2; ++s) {
+            ptx::mbar_init(&q_full[s], 1);
+            ptx::mbar_init(&q_empty[s], 1);
+            ptx::mbar_init(&s_full[s], 1);
+            ptx::mbar_init(&s_empty[s], 128);
+            ptx::mbar_init(&p_half[s], 128);
+            ptx::mbar_init(&p_full[s], 128);
+            ptx::mbar_init(&pv_done[s], 1);
+        }
+        for (int i = 0; i < L::kSlots; ++i) {
+            ptx::mbar_init(&kv_full[i], 1);
+            ptx::mbar_init(&kv_empty[i], 1);
+        }
+        for (int i = 0; i < kItems; ++i) {
+            ptx::mbar_init(&item_full[i], 1);
+            ptx::mbar_init(&item_empty[i], kItemReaders);
+        }
+        ptx::fence_barrier_init();
+    }
+    if (warp == 9 && lane == 0) {
+        ptx::prefetch_tensormap(&tmap_q);
+        ptx::prefetch_tensormap(&tmap_k);
+        ptx::prefetch_tensormap(&tmap_v);
+    }
+    if (warp == 8) ptx::tmem_alloc<1>(tmem_ptr_smem, 512);
+    pdl_wait();
+    ptx::tcgen05_fence_before();
+    __syncthreads();
+    ptx::tcgen05_fence_after();
+    pdl_trigger();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr_smem, 0);
+
+    // 168 registers a thread at launch: 208 for the scores of a row, 88 for the others (256 x 208 + 128 x 88 = 384 x 168)
+    if (warp == 9) {
+        // ============================ TMA ============================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        int it = 0, loads[2] = {0, 0}, round = 0, published = 0;
+        // the item whose keys come next and its next key tile; the same of the values, which are one tile behind at most
+        Item ki, vi;
+        int kj = 0, vj = 0;
+        auto publish = [&]() {               // reads on to the next item with scores
+            do {
+                ki = fetch_item<CAUSAL, HEADS>(p, round++);
+                const int i = published % kItems;
+                wait_for(&item_empty[i], ((uint32_t)(published / kItems) & 1u) ^ 1u, dead);
+                ++published;
+                if (lane == 0) {
+                    const int4* src = reinterpret_cast<const int4*>(&ki);
+                    int4* dst = reinterpret_cast<int4*>(&item_ring[i]);
+#pragma unroll
+                    for (int w = 0; w < 3; ++w) dst[w] = src[w];
+                    ptx::mbar_arrive(&item_full[i]);
+                }
+            } while (ki.kind > 1);
+            kj = 0;
+        };
+        auto load = [&](const CUtensorMap* map, const int* pos, uint64_t* bar, uint8_t* dst, int row, int h) {
+            ptx::mbar_arrive_expect_tx(bar, L::kTileBytes);
+            int c[4];
+#pragma unroll
+            for (int g = 0; g < D / 64; ++g) {
+                c[0] = g * 64;
+                coords(pos, row, h, 0, c);
+                tma_load_4d(map, bar, dst + g * (128 * 128), c[0], c[1], c[2], c[3]);
+            }
+        };
+        auto key_tile = [&]() {
+            if (kj == 0) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (ki.n(s) == 0) continue;
+                    wait_for(&q_empty[s], ((uint32_t)loads[s] & 1u) ^ 1u, dead);
+                    ++loads[s];
+                    if (lane == 0) load(&tmap_q, p.pos_q, &q_full[s], sQ + s * L::kTileBytes, ki.start + ki.t(s) * kBM, ki.h(s));
+                }
+            }
+            const int slot = it % L::kSlots;
+            wait_for(&kv_empty[slot], ((uint32_t)(it / L::kSlots) & 1u) ^ 1u, dead);
+            if (lane == 0) load(&tmap_k, p.pos_k, &kv_full[slot], sRing + slot * L::kTileBytes, ki.start + kj * kBN, ki.hkv);
+            ++it;
+            ++kj;
+        };
+        auto value_tile = [&]() {
+            const int slot = it % L::kSlots;
+            wait_for(&kv_empty[slot], ((uint32_t)(it / L::kSlots) & 1u) ^ 1u, dead);
+            const int left = vi.len - vj * kBN, row = vi.start + vj * kBN;
+            if (left < kBN) {                 // behind the end is the next sequence, and 0 * NaN is NaN
+                warp_load_tile<D>(sRing + slot * L::kTileBytes, p.v + vi.hkv * p.v_head + row * p.v_row, p.v_row, kBN, left, lane);
+                ptx::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&kv_full[slot]);
+            } else if (lane == 0) {
+                load(&tmap_v, p.pos_v, &kv_full[slot], sRing + slot * L::kTileBytes, row, vi.hkv);
+            }
+            ++it;
+            ++vj;
+        };
+        publish();
+        if (ki.kind == 1) key_tile();
+        while (ki.kind == 1) {                // the order in which the MMA warp uses them
+            vi = ki;
+            vj = 0;
+            const int n = max(vi.n0, vi.n1);
+            for (; vj + 1 < n;) {
+                if (L::kAlias) value_tile(), key_tile();
+                else key_tile(), value_tile();
+            }
+            publish();
+            value_tile();
+            if (ki.kind == 1) key_tile();
+        }
+    } else if (warp == 8) {
+        // ============================ MMA ============================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (ptx::elect_one()) {
+            constexpr uint32_t idesc_s = ptx::make_idesc_bf16(kBM, kBN, 0, 0);
+            constexpr uint32_t idesc_o = ptx::make_idesc_bf16(kBM, D, 0, 1);
+            const uint32_t q_addr = ptx::smem_u32(sQ), ring = ptx::smem_u32(sRing);
+            int it = 0, items = 0, loads[2] = {0, 0}, tiles[2] = {0, 0}, done[2] = {0, 0};
+            uint32_t k_slot = 0, v_slot = 0;
+            int n0 = 0, n1 = 0;               // key tiles of the item whose scores come next
+            auto next = [&]() {
+                Item x;
+                do x = next_item<false>(item_ring, item_full, item_empty, items, dead);
+                while (x.kind > 1);
+                n0 = x.kind == 1 ? x.n0 : 0;
+                n1 = x.kind == 1 ? x.n1 : 0;
+            };
+            auto slot = [&](uint32_t& at) {
+                at = it % L::kSlots;
+                wait_for(&kv_full[at], (uint32_t)(it / L::kSlots) & 1u, dead);
+                ++it;
+            };
+            auto scores = [&](int s, int j) {          // of key tile j, if query tile s meets it
+                const int n = s ? n1 : n0;
+                if (j >= n) return;
+                if (j == 0) wait_for(&q_full[s], (uint32_t)(loads[s]++) & 1u, dead);
+                if (!L::kAlias) wait_for(&s_empty[s], ((uint32_t)tiles[s] & 1u) ^ 1u, dead);
+                ++tiles[s];
+                ptx::tcgen05_fence_after();
+                const uint32_t qb = q_addr + s * L::kTileBytes, kb = ring + k_slot * L::kTileBytes;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
+                    ptx::umma_bf16<1>(tmem + L::kColS + s * 128, ptx::make_smem_desc(qb + off, 16, 1024),
+                                      ptx::make_smem_desc(kb + off, 16, 1024), idesc_s, kk != 0 ? 1u : 0u);
+                }
+                ptx::umma_commit(&s_full[s]);
+                if (j + 1 == n) ptx::umma_commit(&q_empty[s]);
+            };
+            auto weigh = [&](int s, int j, int n) {    // O_s += P_s V of key tile j
+                if (j >= n) return;
+                const uint32_t vb = ring + v_slot * L::kTileBytes;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    wait_for(half ? &p_full[s] : &p_half[s], (uint32_t)done[s] & 1u, dead);
+                    ptx::tcgen05_fence_after();
+#pragma unroll
+                    for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                        ptx::umma_bf16_ts(tmem + s * D, tmem + L::kColP + s * L::kPStep + kk * 8,
+                                          ptx::make_smem_desc(vb + kk * 2048, kBN * 128, 1024), idesc_o, (j | kk) != 0 ? 1u : 0u);
+                }
+                ++done[s];
+                ptx::umma_commit(&pv_done[s]);
+            };
+            next();
+            if (n0) {
+                slot(k_slot);
+                scores(0, 0);
+                scores(1, 0);
+                ptx::umma_commit(&kv_empty[k_slot]);
+            }
+            while (n0) {
+                const int m0 = n0, m1 = n1, n = max(n0, n1);
+                for (int j = 0; j < n; ++j) {
+                    const bool last = j + 1 == n;
+                    if (!L::kAlias && !last) {
+                        slot(k_slot);
+                        scores(0, j + 1);
+                        scores(1, j + 1);
+                        ptx::umma_commit(&kv_empty[k_slot]);
+                        slot(v_slot);
+                        weigh(0, j, m0);
+                        weigh(1, j, m1);
+                        ptx::umma_commit(&kv_empty[v_slot]);
+                    } else {
+                        if (last) next();
+                        const int jn = last ? 0 : j + 1;
+                        slot(v_slot);
+                        weigh(0, j, m0);
+                        if (n0) {
+                            slot(k_slot);
+                            scores(0, jn);
+                        }
+                        weigh(1, j, m1);
+                        ptx::umma_commit(&kv_empty[v_slot]);
+                        if (n0) {
+                            scores(1, jn);
+                            ptx::umma_commit(&kv_empty[k_slot]);
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp < 8) {
+        // ============================ softmax and results ============================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int s = warp >> 2, q = warp & 3;
+        const int row = q * 32 + lane;                   // of the query tile == TMEM lane
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const uint32_t t_o = tmem + s * D + lanes, t_s = tmem + L::kColS + s * 128 + lanes, t_p = tmem + L::kColP + s * L::kPStep + lanes;
+        const float sc = p.scale_log2;
+        const uint64_t sc2 = f2_pack(sc, sc);
+        int tiles = 0, items = 0;
+        float m = -INFINITY, l = 0.f;                    // running maximum in units of the raw score, and sum
+        // rescales what has been summed so far where the maximum has moved far; the exponent's offset
+        auto follow_max = [&](float mx, int j) {
+            float alpha = 1.f;
+            bool rescale = false;
+            if (!(mx < INFINITY)) l = NAN;               // a score that is NaN, or infinite: the row has no softmax
+            if ((mx - m) * sc > kRescale || m == -INFINITY) {
+                const float now = fmaxf(m, mx);
+                if (now != -INFINITY) {
+                    alpha = ex2_approx((m - now) * sc);
+                    rescale = j > 0 && m != -INFINITY;
+                    m = now;
+                    l *= alpha;
+                }
+            }
+            if (__any_sync(0xffffffffu, rescale)) {
+                if (!L::kAlias) {                        // O has the weights of the tile before
+                    wait_for(&pv_done[s], (uint32_t)(tiles - 1) & 1u, dead);
+                    ptx::tcgen05_fence_after();
+                }
+                const float f = rescale ? alpha : 1.f;
+                const uint64_t f2 = f2_pack(f, f);
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t o[16];
+                    ptx::tmem_ld_32x32b_x16(t_o + c * 16, o);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const uint64_t z = f2_mul(f2_pack(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), f2);
+                        o[e] = (uint32_t)z;
+                        o[e + 1] = (uint32_t)(z >> 32);
+                    }
+                    tmem_st_32x32b_x16(t_o + c * 16, o);
+                }
+            }
+            return m == -INFINITY ? 0.f : -m * sc;
+        };
+        auto weights_free = [&](int j) {                 // D = 64: the weights of the tile before have been used
+            if (!L::kAlias && j > 0) {
+                wait_for(&pv_done[s], (uint32_t)(tiles - 1) & 1u, dead);
+                ptx::tcgen05_fence_after();
+            }
+        };
+        auto scores_read = [&]() {
+            ptx::tmem_ld_wait();
+            if (!L::kAlias) {
+                ptx::tcgen05_fence_before();
+                ptx::mbar_arrive(&s_empty[s]);
+            }
+        };
+        for (;;) {
+            const Item it = next_item<true>(item_ring, item_full, item_empty, items, dead);
+            if (it.kind == 0) break;
+            const int head = it.h(s);
+            if (it.kind > 1) {                           // rows of no sequence; once a head
+                if (HEADS || s == 0)
+                    for (int i = threadIdx.x & 127; i < (it.kind - kRowsOfNone) * (D / 8); i += 128)
+                        *reinterpret_cast<uint4*>(p.o + head * p.o_head + (long long)(it.start + i / (D / 8)) * p.o_row + (i % (D / 8)) * 8) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                continue;
+            }
+            const int n = it.n(s), t = it.t(s);
+            if (n == 0) continue;
+            m = -INFINITY, l = 0.f;
+            for (int j = 0; j < n; ++j, ++tiles) {
+                // columns that the warp's last row sees
+                int seen = min(it.len - j * kBN, kBN);
+                if (CAUSAL && j == t) seen = min(seen, q * 32 + 32);
+                wait_for(&s_full[s], (uint32_t)tiles & 1u, dead);
+                ptx::tcgen05_fence_after();
+                uint32_t x[kBN];
+                uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+                if (seen == kBN && !(CAUSAL && j == t)) {
+                    // every row sees the whole tile
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(t_s + c * 32, x + c * 32);
+                    scores_read();
+                    float a[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) a[i] = max3(__uint_as_float(x[i]), __uint_as_float(x[8 + i]), __uint_as_float(x[16 + i]));
+#pragma unroll
+                    for (int e = 24; e < 120; e += 16)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) a[i] = max3(a[i], __uint_as_float(x[e + i]), __uint_as_float(x[e + 8 + i]));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) a[i] = max2(a[i], __uint_as_float(x[120 + i]));
+                    const float neg = follow_max(max3(max3(a[0], a[1], a[2]), max3(a[3], a[4], a[5]), max2(a[6], a[7])), j);
+                    const uint64_t neg2 = f2_pack(neg, neg);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                        for (int e = 0; e < 64; e += 2) {
+                            const int i = half * 64 + e;
+                            const uint64_t z = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, neg2);
+                            float p0, p1;
+                            if ((L::kPolyOf8 >> ((e >> 1) & 7)) & 1) {
+                                exp2_poly(z, p0, p1);
+                            } else {
+                                p0 = ex2_approx(f2_lo(z));
+                                p1 = ex2_approx(f2_hi(z));
+                            }
+                            sum[(e >> 1) & 3] = f2_add(sum[(e >> 1) & 3], f2_pack(p0, p1));
+                            x[i >> 1] = pack_bf16x2(p0, p1);
+                        }
+                        if (half == 0) weights_free(j);
+                        tmem_st_32x32b_x32(t_p + half * 32, x + half * 32);
+                        tmem_st_wait();
+                        ptx::tcgen05_fence_before();
+                        ptx::mbar_arrive(half ? &p_full[s] : &p_half[s]);
+                    }
+                } else {
+                    // the diagonal, or the end of the sequence: chunks of 32 columns, those behind `seen` without weight for any row of
+                    // the warp, the last of the others cut where this row's keys end
+                    const int chunks = (seen + 31) >> 5, mine = CAUSAL && j == t ? min(seen, row + 1) : seen;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (c < chunks) ptx::tmem_ld_32x32b_x32(t_s + c * 32, x + c * 32);
+                    scores_read();
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (c >= chunks) break;
+                        uint32_t* y = x + c * 32;
+                        if (c + 1 == chunks) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) y[e] = c * 32 + e < mine ? y[e] : 0xff800000u;          // -inf
+                        }
+                        float a[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) a[i] = max2(__uint_as_float(y[i]), __uint_as_float(y[4 + i]));
+#pragma unroll
+                        for (int e = 8; e < 32; e += 8)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) a[i] = max3(a[i], __uint_as_float(y[e + i]), __uint_as_float(y[e + 4 + i]));
+                        mx = max3(mx, max2(a[0], a[1]), max2(a[2], a[3]));
+                    }
+                    const float neg = follow_max(mx, j);
+                    const uint64_t neg2 = f2_pack(neg, neg);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (c < chunks) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const int i = c * 32 + e;
+                                const uint64_t z = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, neg2);
+                                const float p0 = ex2_approx(f2_lo(z)), p1 = ex2_approx(f2_hi(z));
+                                sum[(e >> 1) & 3] = f2_add(sum[(e >> 1) & 3], f2_pack(p0, p1));
+                                x[i >> 1] = pack_bf16x2(p0, p1);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[c * 16 + e] = 0u;
+                        }
+                    }
+                    weights_free(j);
+                    tmem_st_32x32b_x32(t_p, x);
+                    tmem_st_32x32b_x32(t_p + 32, x + 32);
+                    tmem_st_wait();
+                    ptx::tcgen05_fence_before();
+                    ptx::mbar_arrive(&p_half[s]);
+                    ptx::mbar_arrive(&p_full[s]);
+                }
+                const uint64_t all = f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3]));
+                l += f2_lo(all) + f2_hi(all);
+            }
+            // O / l, one row a thread, nothing behind the sequence's end.  A row without a finite score has no softmax.
+            wait_for(&pv_done[s], (uint32_t)(tiles - 1) & 1u, dead);
+            ptx::tcgen05_fence_after();
+            const int at = t * kBM + row;
+            const bool real = at < it.len;
+            if (m == -INFINITY || *dead) l = NAN;
+            const float inv = 1.f / l;
+            if (p.lse != nullptr && real) p.lse[head * p.lse_row + it.pad + at] = m * sc + log2f(l);
+            bf16* to = p.o + head * p.o_head + (long long)(it.start + at) * p.o_row;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                ptx::tmem_ld_32x32b_x32(t_o + c * 32, o);
+                ptx::tmem_ld_wait();
+                if (!real) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = pack_bf16x2(__uint_as_float(o[e + 2 * i]) * inv, __uint_as_float(o[e + 2 * i + 1]) * inv);
+                    *reinterpret_cast<uint4*>(to + c * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            ptx::tcgen05_fence_before();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    }
+    ptx::tcgen05_fence_before();
+    __syncthreads();
+    if (dead_word) {          // copies may still be on their way into this CTA's memory
+        const long long start = clock64();
+        while (clock64() - start < kWaitClocks / 100) {
+        }
+    }
+    if (warp == 8) ptx::tmem_dealloc<1>(tmem, 512);
+}
+
+template <int D, bool CAUSAL, bool HEADS>
+int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, cudaStream_t st) {
+    using L = FwdSmem<D>;
+    constexpr auto kern = packed_fwd_kernel<D, CAUSAL, HEADS>;
+    NXD_CHECK_CUDA(nxd_allow_smem<kern>(L::kBytes));
+    const long long items = (long long)p.entries * p.pairs;
+    const unsigned grid = (unsigned)(items < nxd_num_sms() ? items : nxd_num_sms());
+    NXD_CHECK_CUDA(nxd_launch_pdl(kern, dim3(grid), dim3(kThreads), L::kBytes, st, tq, tk, tv, p));
+    NXD_LAUNCH_CHECK();
+    return 0;
+}
+
+template <int D>
+int launch_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, int causal, cudaStream_t st) {
+    if (p.group % 2 == 0) return causal ? launch<D, true, true>(tq, tk, tv, p, st) : launch<D, false, true>(tq, tk, tv, p, st);
+    return causal ? launch<D, true, false>(tq, tk, tv, p, st) : launch<D, false, false>(tq, tk, tv, p, st);
+}
+
+}  // namespace
+
+// Attention inside each sequence of a packed batch: q [T, Hq, D], k and v [T, Hkv, D], o [T, Hq, D], strides {q_h, q_row, k_h,
+// k_row, v_h, v_row, o_h, o_row} in elements (multiples of 8), 16-byte aligned bases; tiles: the `entries` tiles that
+// nxd_packed_plan has made; lse NULL or [Hq, lse_row] floats, log2 units, written at the plan's padded columns.  Rows
+// outside every sequence get zeros.
+NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const long long* strides,
+                                const void* tiles, int entries, long long lse_row, long long T, int Hq, int Hkv, int D, float scale,
+                                int causal, void* stream) {
+    NXD_REQUIRE(D == 64 || D == 128, "packed_attn: head dim %d not supported (64 or 128)", D);
+    NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && (long long)entries * Hq < (1ll << 31),
+                "packed_attn: bad problem");
+    for (int i = 0; i < 8; ++i)
+        NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
+    NXD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)tiles) & 15) == 0,
+                "packed_attn: tensors must be 16-byte aligned");
+    FwdParams p{};
+    p.tiles = (const PackedTile*)tiles;
+    p.entries = entries;
+    p.lse = lse; p.lse_row = lse_row;
+    p.Hq = Hq; p.group = Hq / Hkv;
+    p.pairs = p.group % 2 == 0 ? Hq / 2 : Hq;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.v = (const bf16*)v; p.v_head = strides[4]; p.v_row = strides[5];
+    p.o = (bf16*)o; p.o_head = strides[6]; p.o_row = strides[7];
+    CUtensorMap tq, tk, tv;
+    int rc;
+    if ((rc = make_tmap_bhsd(&tq, q, D, T, Hq, 1, strides[1], strides[0], 0, kBM, p.pos_q))) return rc;
+    if ((rc = make_tmap_bhsd(&tk, k, D, T, Hkv, 1, strides[3], strides[2], 0, kBN, p.pos_k))) return rc;
+    if ((rc = make_tmap_bhsd(&tv, v, D, T, Hkv, 1, strides[5], strides[4], 0, kBN, p.pos_v))) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    return D == 64 ? launch_as<64>(tq, tk, tv, p, causal, st) : launch_as<128>(tq, tk, tv, p, causal, st);
+}

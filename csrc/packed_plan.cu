@@ -1,8 +1,8 @@
 // The tile list of a packed batch: sequences of different lengths laid end to end in `T` rows, bounded by cu[0 .. N], for the
-// attention kernels that take one 128-row tile of one sequence per CTA (flash_attn_tc.cu, flash_attn_bwd_tc.cu).
+// attention kernels, which work by tiles of 128 (flash_attn_bwd_tc.cu, packed_attention.cu) or 256 rows (the latter) of one sequence.
 //
 // The lengths stay on the device, so that a step needs no copy to the host and can be captured: the list has room for
-// T / 128 + N + 2 tiles whatever the lengths are, and CTAs without a tile end at once.  Boundaries that fall or leave [0, T] are
+// T / 128 + N + 2 tiles whatever the lengths are, and entries without a tile cost nothing.  Boundaries that fall or leave [0, T] are
 // brought back (running maximum, clamped), so no list can lead a kernel out of its tensors.
 //
 // Order: longest first.  A query tile t of a causal sequence meets t + 1 tiles of keys, so with c(w) = the number of sequences of
@@ -17,7 +17,6 @@ namespace {
 using nxd_attn::PackedTile;
 
 constexpr int kThreads = 1024;
-constexpr int kTile = 128;
 constexpr int kBins = 4096;          // weights above (half a million rows) share the last bin
 constexpr int kOwn = 2;              // tiles of a sequence that its thread places itself
 
@@ -56,7 +55,7 @@ __device__ int block_scan(int v, int* warps, int& total) {
 }
 
 template <typename Index>
-__global__ void __launch_bounds__(kThreads) packed_plan_kernel(const Index* __restrict__ cu, int N, int T, int causal, PackedTile* tiles,
+__global__ void __launch_bounds__(kThreads) packed_plan_kernel(const Index* __restrict__ cu, int N, int T, int causal, int rows, PackedTile* tiles,
                                                               int entries, int4* seqs) {
     __shared__ int bins[kBins + 2], warps[32];
     const int tid = threadIdx.x, lane = tid & 31;
@@ -81,7 +80,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const Index* __re
         __syncthreads();
         if (lane == 0) start = tid ? warps[(tid >> 5) - 1] : high;
         __syncthreads();
-        const int len = i < N ? end - start : 0, n = (len + kTile - 1) / kTile;
+        const int len = i < N ? end - start : 0, n = (len + rows - 1) / rows;
         const int before = block_scan<ScanSum>((len + 3) & ~3, warps, total) - ((len + 3) & ~3);
         if (i < N) seqs[i] = make_int4(start, len, pad + before, n);
         pad += total;
@@ -141,21 +140,21 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const Index* __re
         }
     }
     // rows before the first and behind the last sequence, then entries without work
-    const int gap0 = (first + kTile - 1) / kTile, gap1 = (T - high + kTile - 1) / kTile;
+    const int gap0 = (first + rows - 1) / rows, gap1 = (T - high + rows - 1) / rows;
     for (int i = n_tiles + tid; i < entries; i += kThreads) {
         const int j = i - n_tiles;
-        int from = 0, rows = 0;
-        if (j < gap0) from = j * kTile, rows = min(kTile, first - from);
-        else if (j < gap0 + gap1) from = high + (j - gap0) * kTile, rows = min(kTile, T - from);
-        reinterpret_cast<int4*>(tiles)[i] = make_int4(from, 0, rows, 0);
+        int from = 0, here = 0;
+        if (j < gap0) from = j * rows, here = min(rows, first - from);
+        else if (j < gap0 + gap1) from = high + (j - gap0) * rows, here = min(rows, T - from);
+        reinterpret_cast<int4*>(tiles)[i] = make_int4(from, 0, here, 0);
     }
 }
 
 }  // namespace
 
 // Tiles that the list has room for.
-NXD_API int nxd_packed_plan_entries(long long T, int N) {
-    const long long n = T / kTile + (N < T ? N : T) + 2;
+NXD_API int nxd_packed_plan_entries(long long T, int N, int rows) {
+    const long long n = T / rows + (N < T ? N : T) + 2;
     return n < (1ll << 31) ? (int)n : -1;
 }
 
@@ -165,18 +164,19 @@ NXD_API long long nxd_packed_plan_columns(long long T, int N) {
     return ((T + 3 * (N < T ? (long long)N : T) + 3) & ~3ll) + 64;
 }
 
-// cu: N + 1 boundaries, int32 or (wide) int64; tiles: nxd_packed_plan_entries(T, N) entries of 16 bytes; seqs: 16 bytes of scratch
+// cu: N + 1 boundaries, int32 or (wide) int64; rows of a tile: 128 or 256; tiles: nxd_packed_plan_entries entries of 16 bytes; seqs: 16 bytes of scratch
 // per sequence, afterwards {first row, rows, first padded column, tiles} of each.
-NXD_API int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, void* tiles, void* seqs, void* stream) {
-    const int entries = nxd_packed_plan_entries(T, N);
+NXD_API int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, int rows, void* tiles, void* seqs, void* stream) {
+    NXD_REQUIRE(rows == 128 || rows == 256, "packed_plan: tiles of %d rows", rows);
+    const int entries = nxd_packed_plan_entries(T, N, rows);
     NXD_REQUIRE(N >= 0 && T > 0 && T < (1ll << 31) - 256 && entries > 0, "packed_plan: %d sequences in %lld rows", N, T);
     NXD_REQUIRE((((uintptr_t)tiles | (uintptr_t)seqs) & 15) == 0, "packed_plan: the lists must be %s", "16-byte aligned");
     cudaStream_t st = (cudaStream_t)stream;
     if (wide)
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_plan_kernel<long long>, dim3(1), dim3(kThreads), 0, st, (const long long*)cu, N, (int)T, causal,
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_plan_kernel<long long>, dim3(1), dim3(kThreads), 0, st, (const long long*)cu, N, (int)T, causal, rows,
             (PackedTile*)tiles, entries, (int4*)seqs)));
     else
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_plan_kernel<int>, dim3(1), dim3(kThreads), 0, st, (const int*)cu, N, (int)T, causal,
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_plan_kernel<int>, dim3(1), dim3(kThreads), 0, st, (const int*)cu, N, (int)T, causal, rows,
             (PackedTile*)tiles, entries, (int4*)seqs)));
     NXD_LAUNCH_CHECK();
     return 0;

@@ -2,8 +2,7 @@
 
 ``PackedSequences`` holds where the sequences of a step begin and the tile list that the kernels walk (``csrc/packed_plan.cu``);
 it is made on the device from ``cu_seqlens`` without a copy to the host and serves every layer of the step, forward and
-backward.  The kernels are the packed instantiations of the tcgen05 attention (``csrc/flash_attn_tc.cu``,
-``csrc/flash_attn_bwd_tc.cu``).  ``ops.attention`` has the public functions."""
+backward.  The kernels are ``csrc/packed_attention.cu`` and the packed instantiation of ``csrc/flash_attn_bwd_tc.cu``.  ``ops.attention`` has the public functions."""
 from __future__ import annotations
 
 import ctypes as _c
@@ -44,19 +43,20 @@ class PackedSequences:
     def device(self) -> torch.device:
         return self.cu_seqlens.device
 
-    def plan(self, causal: bool) -> Tuple[torch.Tensor, int, int]:
-        """``(tile list, its entries, columns of the per-row scratch)`` for the kernels, made on first use."""
-        if causal not in self._plans:
+    def plan(self, causal: bool, rows: int = 128) -> Tuple[torch.Tensor, int, int]:
+        """``(list of tiles of that many rows, its entries, columns of the per-row scratch)`` for the kernels, made on first use."""
+        key = (causal, rows)
+        if key not in self._plans:
             most = min(self.count, self.total)
-            entries = self.total // 128 + most + 2                          # nxd_packed_plan_entries
+            entries = self.total // rows + most + 2                         # nxd_packed_plan_entries
             columns = (self.total + 3 * most + 3 & ~3) + 64                 # nxd_packed_plan_columns
             lists = torch.empty((entries + self.count, 4), dtype=torch.int32, device=self.device)
             rc = _lib.lib().nxd_packed_plan(_lib.ptr(self.cu_seqlens), _c.c_int(self.cu_seqlens.dtype == torch.int64), _c.c_int(self.count),
-                                     _c.c_longlong(self.total), _c.c_int(causal), _lib.ptr(lists),
-                                     _c.c_void_p(lists.data_ptr() + 16 * entries), _lib.stream_ptr())
+                                            _c.c_longlong(self.total), _c.c_int(causal), _c.c_int(rows), _lib.ptr(lists),
+                                            _c.c_void_p(lists.data_ptr() + 16 * entries), _lib.stream_ptr())
             _lib.check(rc, "nxd_packed_plan")
-            self._plans[causal] = (lists, entries, columns)
-        return self._plans[causal]
+            self._plans[key] = (lists, entries, columns)
+        return self._plans[key]
 
     def positions(self) -> torch.Tensor:
         """int32 ``[total]``: every token's position in its own sequence (0 outside of them), for the rotation."""
@@ -118,7 +118,8 @@ def _strides(*ts: torch.Tensor):
 
 def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, want_lse: bool):
     T, Hq, D = q.shape
-    tiles, entries, columns = packed.plan(causal)
+    # an odd number of heads to a key head: two neighbouring tiles of one head are worked on together (csrc/packed_attention.cu)
+    tiles, entries, columns = packed.plan(causal, 128 if Hq // k.shape[1] % 2 == 0 else 256)
     o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((Hq, columns), dtype=torch.float32, device=q.device) if want_lse else None
     rc = _lib.lib().nxd_packed_attn_fwd(

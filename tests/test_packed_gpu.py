@@ -44,16 +44,17 @@ def test_plan_lists_every_tile_once():
         for dtype in (torch.int32, torch.int64):
             for causal in (True, False):
                 ends = _ends(lens, first)
-                lists, entries, columns = PackedSequences(torch.tensor(ends, dtype=dtype, device="cuda"), T).plan(causal)
+                size = 256 if causal == (dtype is torch.int32) else 128
+                lists, entries, columns = PackedSequences(torch.tensor(ends, dtype=dtype, device="cuda"), T).plan(causal, size)
                 rows = lists[:entries].tolist()
                 want, pad = set(), 0
                 for a, b in zip(ends, ends[1:]):
-                    want |= {(a, b - a, t, pad) for t in range((b - a + 127) // 128)}
+                    want |= {(a, b - a, t, pad) for t in range(-(-(b - a) // size))}
                     pad += (b - a + 3) // 4 * 4
                 tiles = [tuple(r) for r in rows if r[1]]
                 assert set(tiles) == want and len(tiles) == len(want) and pad + 64 <= columns
                 assert all(r[1] for r in rows[:len(tiles)])
-                weight = [min(t[2] + 1 if causal else (t[1] + 127) // 128, 4096) for t in tiles]
+                weight = [min(t[2] + 1 if causal else -(-t[1] // size), 4096) for t in tiles]
                 assert weight == sorted(weight, reverse=True)
                 outside = [r for a, n, t, _ in rows if not n for r in range(a, a + t)]
                 assert sorted(outside) == [r for r in range(T) if r < first or r >= ends[-1]]
@@ -207,12 +208,15 @@ def test_rotation_and_attention(D):
     cos, sin = rope.build_rope_cache(T, D, 10000.0, None, device="cuda")
     o = attention.rope_flash_attn_packed_func(qkv, cos, sin, H, G, torch.tensor(ends, device="cuda"))
     (grad,) = torch.autograd.grad(o, qkv, do)
-    for a, b in zip(ends, ends[1:]):          # every sequence as the dense path computes it: the same roundings, sums in another order
-        x = qkv[a:b, None].detach().requires_grad_()
-        alone = attention.rope_flash_attn_func(x, cos, sin, H, G)
-        (ref,) = torch.autograd.grad(alone, x, do[a:b, None].permute(1, 2, 0, 3))
-        assert torch.equal(o[a:b], alone[0].transpose(0, 1))
-        assert (grad[a:b].float() - ref[:, 0].float()).norm() <= 2 * 2.0 ** -8 * ref.float().norm()
+    positions = torch.cat([torch.arange(b - a, device="cuda") for a, b in zip([0] + ends, ends + [T])])
+    turn = lambda x, back: rope.rope_ref(x, cos.double(), sin.double(), H + G, 1, 1, positions, inverse=back)     # noqa: E731
+    r = turn(qkv.detach().double(), False)
+    want = packed(r[:, :H], r[:, H:H + G], r[:, H + G:], ends, True, do)
+    back = turn(torch.cat([want[n][0] for n in ("dq", "dk", "dv")], 1), True)
+    # roundings to bf16, 2^-8 of a value each: forward the rotated heads, the weights and the result; backward also the score gradients,
+    # the three gradients, and their rotation back
+    assert (o.double() - want["o"][0]).norm() <= 3 * 2.0 ** -8 * want["o"][0].norm()
+    assert (grad.double() - back).norm() <= 6 * 2.0 ** -8 * back.norm()
     assert not o[470:].any() and not grad[470:].any()
 
 
