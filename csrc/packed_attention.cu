@@ -10,8 +10,10 @@
 // the stores of this one.
 //   warps 0-3, 4-7   softmax of query tile 0 / 1, a thread per row; the accumulator stays in tensor memory and is rescaled where a row's
 //                    maximum has moved by more than 2^8; at the end of an item they divide and store their rows
-//   warp 8           MMA: S_s = Q_s K^T (128 x 128), O_s += P_s V with P_s from tensor memory, s = 0, 1 in turn
+//   warps 8, 11      MMA of query tile s = 0 / 1: S_s = Q_s K^T (128 x 128), O_s += P_s V with P_s from tensor memory; one thread for
+//                    both would hold one tile up where it waits for the other
 //   warp 9           TMA: Q_s of an item, key and value tiles of 128 rows in the order of their use through one ring
+//   warp 10          zeros behind the end of a sequence in its last value tile
 // D = 128: two accumulators and two score tiles fill the tensor memory, so P_s lies in the columns of S_s, and S_s of the next tile follows
 // P_s V (the tensor core works in issue order).  D = 64: P_s has columns of its own, and S_s of the next tile is computed as soon as the
 // scores are in registers, so the softmax warps, which bound this size (128 exponentials a row for half the products), never wait.
@@ -19,11 +21,13 @@
 #include "gemm_tcgen05.cuh"
 #include "ptx.cuh"
 
+#include <type_traits>
+
 namespace {
 using namespace nxd_attn;
 
 constexpr int kBM = 128, kBN = 128;
-constexpr int kThreads = 384;                     // 8 softmax warps, MMA, TMA, two without work (registers move by groups of four warps)
+constexpr int kThreads = 384;                     // 8 softmax warps, MMA, TMA, ends of sequences, MMA (registers move by groups of four warps)
 constexpr float kRescale = 8.0f;                  // log2 units
 constexpr long long kWaitClocks = 4000000000ll;   // a wait that takes two seconds is given up: the CTA's results are NaN then
 
@@ -34,18 +38,19 @@ struct FwdParams {
     const bf16* v;
     long long lse_row, o_head, o_row, v_head, v_row;
     int entries, Hq, group, pairs;                // pairs: items of one tile-list entry
-    int pos_q[3], pos_k[3], pos_v[3];
+    int pos_q[3], pos_k[3], pos_v[3], pos_o[3];
     float scale_log2;
 };
 
 template <int D>
 struct FwdSmem {
     static constexpr int kTileBytes = 128 * D * 2;
-    static constexpr int kSlots = D == 64 ? 8 : 5;
+    static constexpr int kSlots = D == 64 ? 6 : 4;
     static constexpr int kQOff = 0;
     static constexpr int kRingOff = 2 * kTileBytes;
-    static constexpr int kBarOff = kRingOff + kSlots * kTileBytes;
-    static constexpr int kNumBars = 4 + 2 * kSlots + 10 + 8;
+    static constexpr int kOutOff = kRingOff + kSlots * kTileBytes;       // 32 rows x 64 columns of each softmax warp
+    static constexpr int kBarOff = kOutOff + 8 * 4096;
+    static constexpr int kNumBars = 4 + 3 * kSlots + 10 + 8;
     static constexpr int kBytes = kBarOff + kNumBars * 8 + 16 + 1024;
     static constexpr uint32_t kPolyOf8 = D == 64 ? 0x52 : 0x44;          // of eight pairs of weights, those by the polynomial
     // tensor memory: O_0 O_1 | S_0 S_1 | P_0 P_1 (D = 64; else P_s = the first columns of S_s)
@@ -78,12 +83,12 @@ constexpr int kRowsOfNone = 1;           // added to the rows of such an entry, 
 
 template <bool CAUSAL, bool HEADS>
 __device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
-    const int G = gridDim.x;
-    const long long at = (long long)round * G + (round & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
+    const unsigned G = gridDim.x, at = round * G + (round & 1 ? G - 1 - blockIdx.x : blockIdx.x);          // below 2^31 + 148
     Item it{};
-    if (at >= (long long)p.entries * p.pairs) return it;
-    const int pr = (int)(at % p.pairs);
-    const PackedTile pt = packed_tile(p.tiles, (int)(at / p.pairs));
+    if (at >= (unsigned)p.entries * p.pairs) return it;
+    const unsigned e = at / (unsigned)p.pairs;
+    const int pr = (int)(at - e * p.pairs);
+    const PackedTile pt = packed_tile(p.tiles, (int)e);
     it.start = pt.start, it.len = pt.len, it.pad = pt.pad;
     it.h0 = HEADS ? 2 * pr : pr;
     it.h1 = HEADS ? it.h0 + 1 : it.h0;
@@ -102,7 +107,7 @@ __device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
 }
 
 constexpr int kItems = 4;                // of the ring in shared memory
-constexpr int kItemReaders = 9;          // the MMA thread and a lane of each softmax warp
+constexpr int kItemReaders = 11;         // the two MMA threads and a lane of each softmax warp and of the one that cuts value tiles
 
 // the next item of the ring, for a whole warp or (WARP = false) one thread
 template <bool WARP>
@@ -155,7 +160,8 @@ __device__ __forceinline__ void exp2_poly(uint64_t z, float& p0, float& p1) {
 template <int D, bool CAUSAL, bool HEADS>
 __global__ void __launch_bounds__(kThreads, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                  const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ FwdParams p) {
+                  const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o,
+                  const __grid_constant__ FwdParams p) {
     using L = FwdSmem<D>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ int dead_word;
@@ -167,7 +173,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     uint64_t* q_empty = q_full + 2;
     uint64_t* kv_full = q_empty + 2;
     uint64_t* kv_empty = kv_full + L::kSlots;
-    uint64_t* s_full = kv_empty + L::kSlots;
+    uint64_t* kv_cut = kv_empty + L::kSlots;
+    uint64_t* s_full = kv_cut + L::kSlots;
     uint64_t* s_empty = s_full + 2;
     uint64_t* p_half = s_empty + 2;
     uint64_t* p_full = p_half + 2;
@@ -191,7 +198,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
         for (int i = 0; i < L::kSlots; ++i) {
             ptx::mbar_init(&kv_full[i], 1);
-            ptx::mbar_init(&kv_empty[i], 1);
+            ptx::mbar_init(&kv_empty[i], 2);          // both MMA warps
+            ptx::mbar_init(&kv_cut[i], 1);
         }
         for (int i = 0; i < kItems; ++i) {
             ptx::mbar_init(&item_full[i], 1);
@@ -203,6 +211,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         ptx::prefetch_tensormap(&tmap_q);
         ptx::prefetch_tensormap(&tmap_k);
         ptx::prefetch_tensormap(&tmap_v);
+        ptx::prefetch_tensormap(&tmap_o);
     }
     if (warp == 8) ptx::tmem_alloc<1>(tmem_ptr_smem, 512);
     pdl_wait();
@@ -218,11 +227,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         int it = 0, loads[2] = {0, 0}, round = 0, published = 0;
         // the item whose keys come next and its next key tile; the same of the values, which are one tile behind at most
-        Item ki, vi;
+        Item ki, vi, ahead = fetch_item<CAUSAL, HEADS>(p, round++);
         int kj = 0, vj = 0;
-        auto publish = [&]() {               // reads on to the next item with scores
+        auto publish = [&]() {               // goes on to the next item with scores; the one behind it is read meanwhile
             do {
-                ki = fetch_item<CAUSAL, HEADS>(p, round++);
+                ki = ahead;
+                if (ki.kind) ahead = fetch_item<CAUSAL, HEADS>(p, round++);
                 const int i = published % kItems;
                 wait_for(&item_empty[i], ((uint32_t)(published / kItems) & 1u) ^ 1u, dead);
                 ++published;
@@ -265,15 +275,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         auto value_tile = [&]() {
             const int slot = it % L::kSlots;
             wait_for(&kv_empty[slot], ((uint32_t)(it / L::kSlots) & 1u) ^ 1u, dead);
-            const int left = vi.len - vj * kBN, row = vi.start + vj * kBN;
-            if (left < kBN) {                 // behind the end is the next sequence, and 0 * NaN is NaN
-                warp_load_tile<D>(sRing + slot * L::kTileBytes, p.v + vi.hkv * p.v_head + row * p.v_row, p.v_row, kBN, left, lane);
-                ptx::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&kv_full[slot]);
-            } else if (lane == 0) {
-                load(&tmap_v, p.pos_v, &kv_full[slot], sRing + slot * L::kTileBytes, row, vi.hkv);
-            }
+            // the tile that crosses the sequence's end goes through warp 10
+            if (lane == 0)
+                load(&tmap_v, p.pos_v, vi.len - vj * kBN < kBN ? &kv_cut[slot] : &kv_full[slot], sRing + slot * L::kTileBytes,
+                     vi.start + vj * kBN, vi.hkv);
             ++it;
             ++vj;
         };
@@ -291,97 +296,83 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             value_tile();
             if (ki.kind == 1) key_tile();
         }
-    } else if (warp == 8) {
+    } else if (warp == 8 || warp == 11) {
         // ============================ MMA ============================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (ptx::elect_one()) {
             constexpr uint32_t idesc_s = ptx::make_idesc_bf16(kBM, kBN, 0, 0);
             constexpr uint32_t idesc_o = ptx::make_idesc_bf16(kBM, D, 0, 1);
-            const uint32_t q_addr = ptx::smem_u32(sQ), ring = ptx::smem_u32(sRing);
-            int it = 0, items = 0, loads[2] = {0, 0}, tiles[2] = {0, 0}, done[2] = {0, 0};
-            uint32_t k_slot = 0, v_slot = 0;
-            int n0 = 0, n1 = 0;               // key tiles of the item whose scores come next
+            const int s = warp == 8 ? 0 : 1;
+            const uint32_t q_addr = ptx::smem_u32(sQ) + s * L::kTileBytes, ring = ptx::smem_u32(sRing);
+            const uint32_t t_o = tmem + s * D, t_s = tmem + L::kColS + s * 128, t_p = tmem + L::kColP + s * L::kPStep;
+            int it = 0, items = 0, loads = 0, tiles = 0, done = 0;
+            int n = 0, steps = 0;             // key tiles that query tile s meets in the item whose scores come next, and those of the item
             auto next = [&]() {
                 Item x;
                 do x = next_item<false>(item_ring, item_full, item_empty, items, dead);
                 while (x.kind > 1);
-                n0 = x.kind == 1 ? x.n0 : 0;
-                n1 = x.kind == 1 ? x.n1 : 0;
+                n = x.kind == 1 ? x.n(s) : 0;
+                steps = x.kind == 1 ? max(x.n0, x.n1) : 0;
             };
-            auto slot = [&](uint32_t& at) {
-                at = it % L::kSlots;
+            auto slot = [&]() {
+                const int at = it % L::kSlots;
                 wait_for(&kv_full[at], (uint32_t)(it / L::kSlots) & 1u, dead);
                 ++it;
+                return at;
             };
-            auto scores = [&](int s, int j) {          // of key tile j, if query tile s meets it
-                const int n = s ? n1 : n0;
-                if (j >= n) return;
-                if (j == 0) wait_for(&q_full[s], (uint32_t)(loads[s]++) & 1u, dead);
-                if (!L::kAlias) wait_for(&s_empty[s], ((uint32_t)tiles[s] & 1u) ^ 1u, dead);
-                ++tiles[s];
+            auto scores = [&](int j) {                 // S = Q K^T of key tile j
+                const int at = slot();
+                if (j >= n) {                          // the other query tile alone meets it
+                    ptx::mbar_arrive(&kv_empty[at]);
+                    return;
+                }
+                if (j == 0) wait_for(&q_full[s], (uint32_t)(loads++) & 1u, dead);
+                if (!L::kAlias) wait_for(&s_empty[s], ((uint32_t)tiles & 1u) ^ 1u, dead);
+                ++tiles;
                 ptx::tcgen05_fence_after();
-                const uint32_t qb = q_addr + s * L::kTileBytes, kb = ring + k_slot * L::kTileBytes;
+                const uint32_t kb = ring + at * L::kTileBytes;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-                    ptx::umma_bf16<1>(tmem + L::kColS + s * 128, ptx::make_smem_desc(qb + off, 16, 1024),
-                                      ptx::make_smem_desc(kb + off, 16, 1024), idesc_s, kk != 0 ? 1u : 0u);
+                    ptx::umma_bf16<1>(t_s, ptx::make_smem_desc(q_addr + off, 16, 1024), ptx::make_smem_desc(kb + off, 16, 1024), idesc_s,
+                                      kk != 0 ? 1u : 0u);
                 }
                 ptx::umma_commit(&s_full[s]);
+                ptx::umma_commit(&kv_empty[at]);
                 if (j + 1 == n) ptx::umma_commit(&q_empty[s]);
             };
-            auto weigh = [&](int s, int j, int n) {    // O_s += P_s V of key tile j
-                if (j >= n) return;
-                const uint32_t vb = ring + v_slot * L::kTileBytes;
+            auto weigh = [&](int j, int meets) {       // O += P V of key tile j
+                const int at = slot();
+                if (j >= meets) {
+                    ptx::mbar_arrive(&kv_empty[at]);
+                    return;
+                }
+                const uint32_t vb = ring + at * L::kTileBytes;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    wait_for(half ? &p_full[s] : &p_half[s], (uint32_t)done[s] & 1u, dead);
+                    wait_for(half ? &p_full[s] : &p_half[s], (uint32_t)done & 1u, dead);
                     ptx::tcgen05_fence_after();
 #pragma unroll
                     for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                        ptx::umma_bf16_ts(tmem + s * D, tmem + L::kColP + s * L::kPStep + kk * 8,
-                                          ptx::make_smem_desc(vb + kk * 2048, kBN * 128, 1024), idesc_o, (j | kk) != 0 ? 1u : 0u);
+                        ptx::umma_bf16_ts(t_o, t_p + kk * 8, ptx::make_smem_desc(vb + kk * 2048, kBN * 128, 1024), idesc_o,
+                                          (j | kk) != 0 ? 1u : 0u);
                 }
-                ++done[s];
+                ++done;
                 ptx::umma_commit(&pv_done[s]);
+                ptx::umma_commit(&kv_empty[at]);
             };
             next();
-            if (n0) {
-                slot(k_slot);
-                scores(0, 0);
-                scores(1, 0);
-                ptx::umma_commit(&kv_empty[k_slot]);
-            }
-            while (n0) {
-                const int m0 = n0, m1 = n1, n = max(n0, n1);
-                for (int j = 0; j < n; ++j) {
-                    const bool last = j + 1 == n;
-                    if (!L::kAlias && !last) {
-                        slot(k_slot);
-                        scores(0, j + 1);
-                        scores(1, j + 1);
-                        ptx::umma_commit(&kv_empty[k_slot]);
-                        slot(v_slot);
-                        weigh(0, j, m0);
-                        weigh(1, j, m1);
-                        ptx::umma_commit(&kv_empty[v_slot]);
-                    } else {
-                        if (last) next();
-                        const int jn = last ? 0 : j + 1;
-                        slot(v_slot);
-                        weigh(0, j, m0);
-                        if (n0) {
-                            slot(k_slot);
-                            scores(0, jn);
-                        }
-                        weigh(1, j, m1);
-                        ptx::umma_commit(&kv_empty[v_slot]);
-                        if (n0) {
-                            scores(1, jn);
-                            ptx::umma_commit(&kv_empty[k_slot]);
-                        }
-                    }
+            if (steps) scores(0);
+            while (steps) {
+                const int meets = n, last = steps - 1;
+                for (int j = 0; j < last; ++j) {
+                    if (!L::kAlias) scores(j + 1);
+                    weigh(j, meets);
+                    if (L::kAlias) scores(j + 1);
                 }
+                next();
+                weigh(last, meets);
+                if (steps) scores(0);
             }
         }
     } else if (warp < 8) {
@@ -445,149 +436,171 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 ptx::mbar_arrive(&s_empty[s]);
             }
         };
-        for (;;) {
-            const Item it = next_item<true>(item_ring, item_full, item_empty, items, dead);
-            if (it.kind == 0) break;
-            const int head = it.h(s);
+        // One tile: weights of its 128 columns, the row's maximum and sum.  CUT: `mine` of them count for this row and `seen` for any of the
+        // warp (the diagonal, the end of the sequence); those tiles take all exponentials from the special function unit, whose
+        // 2^-inf is 0.
+        auto tile_weights = [&](auto cut, int j, int seen, int mine) {
+            constexpr bool CUT = decltype(cut)::value;
+            uint32_t x[kBN];
+            uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(t_s + c * 32, x + c * 32);
+            scores_read();
+            if (CUT) {
+                const int whole = CAUSAL ? min(seen, q * 32 + 1) : seen;          // columns that every row of the warp sees, at least
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c * 32 + 32 > whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[c * 32 + e] = c * 32 + e < mine ? x[c * 32 + e] : 0xff800000u;          // -inf
+                    }
+            }
+            float a[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = max3(__uint_as_float(x[i]), __uint_as_float(x[8 + i]), __uint_as_float(x[16 + i]));
+#pragma unroll
+            for (int e = 24; e < 120; e += 16)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = max3(a[i], __uint_as_float(x[e + i]), __uint_as_float(x[e + 8 + i]));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = max2(a[i], __uint_as_float(x[120 + i]));
+            const float neg = follow_max(max3(max3(a[0], a[1], a[2]), max3(a[3], a[4], a[5]), max2(a[6], a[7])), j);
+            const uint64_t neg2 = f2_pack(neg, neg);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (CUT && half && seen <= 64) {                 // no row of the warp sees the second half
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[32 + e] = 0u;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) {
+                        const int i = half * 64 + e;
+                        const uint64_t z = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, neg2);
+                        float p0, p1;
+                        if (!CUT && ((L::kPolyOf8 >> ((e >> 1) & 7)) & 1)) {
+                            exp2_poly(z, p0, p1);
+                        } else {
+                            p0 = ex2_approx(f2_lo(z));
+                            p1 = ex2_approx(f2_hi(z));
+                        }
+                        sum[(e >> 1) & 3] = f2_add(sum[(e >> 1) & 3], f2_pack(p0, p1));
+                        x[i >> 1] = pack_bf16x2(p0, p1);
+                    }
+                }
+                if (half == 0) weights_free(j);
+                tmem_st_32x32b_x32(t_p + half * 32, x + half * 32);
+                tmem_st_wait();
+                ptx::tcgen05_fence_before();
+                ptx::mbar_arrive(half ? &p_full[s] : &p_half[s]);
+            }
+            const uint64_t all = f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3]));
+            l += f2_lo(all) + f2_hi(all);
+        };
+        Item it = next_item<true>(item_ring, item_full, item_empty, items, dead);
+        for (; it.kind != 0;) {
+            const int head = it.h(s), n = it.n(s), t = it.t(s);
             if (it.kind > 1) {                           // rows of no sequence; once a head
                 if (HEADS || s == 0)
                     for (int i = threadIdx.x & 127; i < (it.kind - kRowsOfNone) * (D / 8); i += 128)
                         *reinterpret_cast<uint4*>(p.o + head * p.o_head + (long long)(it.start + i / (D / 8)) * p.o_row + (i % (D / 8)) * 8) =
                             make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (it.kind > 1 || n == 0) {
+                it = next_item<true>(item_ring, item_full, item_empty, items, dead);
                 continue;
             }
-            const int n = it.n(s), t = it.t(s);
-            if (n == 0) continue;
             m = -INFINITY, l = 0.f;
             for (int j = 0; j < n; ++j, ++tiles) {
-                // columns that the warp's last row sees
                 int seen = min(it.len - j * kBN, kBN);
-                if (CAUSAL && j == t) seen = min(seen, q * 32 + 32);
+                const bool diagonal = CAUSAL && j == t;
+                const int mine = diagonal ? min(seen, row + 1) : seen;
+                if (diagonal) seen = min(seen, q * 32 + 32);
                 wait_for(&s_full[s], (uint32_t)tiles & 1u, dead);
                 ptx::tcgen05_fence_after();
-                uint32_t x[kBN];
-                uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
-                if (seen == kBN && !(CAUSAL && j == t)) {
-                    // every row sees the whole tile
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(t_s + c * 32, x + c * 32);
-                    scores_read();
-                    float a[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) a[i] = max3(__uint_as_float(x[i]), __uint_as_float(x[8 + i]), __uint_as_float(x[16 + i]));
-#pragma unroll
-                    for (int e = 24; e < 120; e += 16)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) a[i] = max3(a[i], __uint_as_float(x[e + i]), __uint_as_float(x[e + 8 + i]));
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) a[i] = max2(a[i], __uint_as_float(x[120 + i]));
-                    const float neg = follow_max(max3(max3(a[0], a[1], a[2]), max3(a[3], a[4], a[5]), max2(a[6], a[7])), j);
-                    const uint64_t neg2 = f2_pack(neg, neg);
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                        for (int e = 0; e < 64; e += 2) {
-                            const int i = half * 64 + e;
-                            const uint64_t z = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, neg2);
-                            float p0, p1;
-                            if ((L::kPolyOf8 >> ((e >> 1) & 7)) & 1) {
-                                exp2_poly(z, p0, p1);
-                            } else {
-                                p0 = ex2_approx(f2_lo(z));
-                                p1 = ex2_approx(f2_hi(z));
-                            }
-                            sum[(e >> 1) & 3] = f2_add(sum[(e >> 1) & 3], f2_pack(p0, p1));
-                            x[i >> 1] = pack_bf16x2(p0, p1);
-                        }
-                        if (half == 0) weights_free(j);
-                        tmem_st_32x32b_x32(t_p + half * 32, x + half * 32);
-                        tmem_st_wait();
-                        ptx::tcgen05_fence_before();
-                        ptx::mbar_arrive(half ? &p_full[s] : &p_half[s]);
-                    }
-                } else {
-                    // the diagonal, or the end of the sequence: chunks of 32 columns, those behind `seen` without weight for any row of
-                    // the warp, the last of the others cut where this row's keys end
-                    const int chunks = (seen + 31) >> 5, mine = CAUSAL && j == t ? min(seen, row + 1) : seen;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (c < chunks) ptx::tmem_ld_32x32b_x32(t_s + c * 32, x + c * 32);
-                    scores_read();
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c >= chunks) break;
-                        uint32_t* y = x + c * 32;
-                        if (c + 1 == chunks) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) y[e] = c * 32 + e < mine ? y[e] : 0xff800000u;          // -inf
-                        }
-                        float a[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) a[i] = max2(__uint_as_float(y[i]), __uint_as_float(y[4 + i]));
-#pragma unroll
-                        for (int e = 8; e < 32; e += 8)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) a[i] = max3(a[i], __uint_as_float(y[e + i]), __uint_as_float(y[e + 4 + i]));
-                        mx = max3(mx, max2(a[0], a[1]), max2(a[2], a[3]));
-                    }
-                    const float neg = follow_max(mx, j);
-                    const uint64_t neg2 = f2_pack(neg, neg);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c < chunks) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                const int i = c * 32 + e;
-                                const uint64_t z = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, neg2);
-                                const float p0 = ex2_approx(f2_lo(z)), p1 = ex2_approx(f2_hi(z));
-                                sum[(e >> 1) & 3] = f2_add(sum[(e >> 1) & 3], f2_pack(p0, p1));
-                                x[i >> 1] = pack_bf16x2(p0, p1);
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) x[c * 16 + e] = 0u;
-                        }
-                    }
-                    weights_free(j);
-                    tmem_st_32x32b_x32(t_p, x);
-                    tmem_st_32x32b_x32(t_p + 32, x + 32);
-                    tmem_st_wait();
-                    ptx::tcgen05_fence_before();
-                    ptx::mbar_arrive(&p_half[s]);
-                    ptx::mbar_arrive(&p_full[s]);
-                }
-                const uint64_t all = f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3]));
-                l += f2_lo(all) + f2_hi(all);
+                if (diagonal || seen < kBN) tile_weights(std::true_type{}, j, seen, mine);
+                else tile_weights(std::false_type{}, j, seen, mine);
             }
+            const Item done = it;                        // the next one is read while the last products run
+            it = next_item<true>(item_ring, item_full, item_empty, items, dead);
             // O / l, one row a thread, nothing behind the sequence's end.  A row without a finite score has no softmax.
             wait_for(&pv_done[s], (uint32_t)(tiles - 1) & 1u, dead);
             ptx::tcgen05_fence_after();
             const int at = t * kBM + row;
-            const bool real = at < it.len;
+            const bool real = at < done.len;
             if (m == -INFINITY || *dead) l = NAN;
             const float inv = 1.f / l;
-            if (p.lse != nullptr && real) p.lse[head * p.lse_row + it.pad + at] = m * sc + log2f(l);
-            bf16* to = p.o + head * p.o_head + (long long)(it.start + at) * p.o_row;
+            if (p.lse != nullptr && real) p.lse[head * p.lse_row + done.pad + at] = m * sc + log2f(l);
+            // through shared memory, 32 rows x 64 columns at a time: stored by rows from the registers, a warp's 16-byte pieces fall into
+            // 32 different lines, and the end of an item took 5000 clocks
+            const int first = t * kBM + q * 32;              // row of the warp in its sequence
+            uint8_t* stage = smem + L::kOutOff + warp * 4096;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                ptx::tmem_ld_32x32b_x32(t_o + c * 32, o);
+            for (int g = 0; g < D / 64; ++g) {
+                uint32_t o[64];
+                ptx::tmem_ld_32x32b_x32(t_o + g * 64, o);
+                ptx::tmem_ld_32x32b_x32(t_o + g * 64 + 32, o + 32);
                 ptx::tmem_ld_wait();
-                if (!real) continue;
+                if (lane == 0) ptx::bulk_wait_read<0>();     // what was stored from here before
+                __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
+                for (int c = 0; c < 8; ++c) {
                     uint32_t w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        w[i] = pack_bf16x2(__uint_as_float(o[e + 2 * i]) * inv, __uint_as_float(o[e + 2 * i + 1]) * inv);
-                    *reinterpret_cast<uint4*>(to + c * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        w[i] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * i]) * inv, __uint_as_float(o[8 * c + 2 * i + 1]) * inv);
+                    st_shared_v4(stage + lane * 128 + ((c ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                }
+                if (first + 32 <= done.len) {
+                    ptx::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        int c[4];
+                        c[0] = g * 64;
+                        coords(p.pos_o, done.start + first, head, 0, c);
+                        tma_store_4d(&tmap_o, stage, c[0], c[1], c[2], c[3]);
+                        ptx::bulk_commit();
+                    }
+                } else {                                     // the rows behind the end are the next sequence's
+                    __syncwarp();
+                    bf16* to = p.o + head * p.o_head + (long long)(done.start + first) * p.o_row + g * 64;
+                    for (int i = lane; i < 32 * 8; i += 32) {
+                        const int r = i >> 3, ch = i & 7;
+                        if (first + r < done.len)
+                            *reinterpret_cast<uint4*>(to + r * p.o_row + ch * 8) =
+                                *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+                    }
+                    __syncwarp();
                 }
             }
             ptx::tcgen05_fence_before();
         }
-    } else {
+        if (lane == 0) ptx::bulk_wait<0>();
+    } else if (warp == 10) {
+        // ============================ ends of sequences ============================
+        // Behind the end of a sequence a value tile holds the next one, and 0 * NaN is NaN: those rows become zeros once the tile is there.
+        // (Tiles that a warp copied with zeros instead were 4000 clocks late.)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        int it = 0, items = 0;
+        uint32_t phases = 0;
+        for (;;) {
+            const Item x = next_item<true>(item_ring, item_full, item_empty, items, dead);
+            if (x.kind == 0) break;
+            if (x.kind > 1) continue;
+            const int n = max(x.n0, x.n1), left = x.len - (n - 1) * kBN;
+            it += 2 * n;                       // keys and values of the item; its last values are the last of them
+            if (left >= kBN) continue;
+            const int slot = (it - 1) % L::kSlots;
+            wait_for(&kv_cut[slot], (phases >> slot) & 1u, dead);
+            phases ^= 1u << slot;
+            uint8_t* tile = sRing + slot * L::kTileBytes;
+            for (int i = lane; i < (kBN - left) * (D / 8); i += 32) {
+                const int r = left + i / (D / 8), ch = i % (D / 8);
+                st_shared_v4(tile + (ch >> 3) * (128 * 128) + r * 128 + ((ch & 7) << 4), 0u, 0u, 0u, 0u);
+            }
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&kv_full[slot]);
+        }
     }
     ptx::tcgen05_fence_before();
     __syncthreads();
@@ -600,21 +613,21 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 }
 
 template <int D, bool CAUSAL, bool HEADS>
-int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, cudaStream_t st) {
+int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const FwdParams& p, cudaStream_t st) {
     using L = FwdSmem<D>;
     constexpr auto kern = packed_fwd_kernel<D, CAUSAL, HEADS>;
     NXD_CHECK_CUDA(nxd_allow_smem<kern>(L::kBytes));
     const long long items = (long long)p.entries * p.pairs;
     const unsigned grid = (unsigned)(items < nxd_num_sms() ? items : nxd_num_sms());
-    NXD_CHECK_CUDA(nxd_launch_pdl(kern, dim3(grid), dim3(kThreads), L::kBytes, st, tq, tk, tv, p));
+    NXD_CHECK_CUDA(nxd_launch_pdl(kern, dim3(grid), dim3(kThreads), L::kBytes, st, tq, tk, tv, to, p));
     NXD_LAUNCH_CHECK();
     return 0;
 }
 
 template <int D>
-int launch_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, int causal, cudaStream_t st) {
-    if (p.group % 2 == 0) return causal ? launch<D, true, true>(tq, tk, tv, p, st) : launch<D, false, true>(tq, tk, tv, p, st);
-    return causal ? launch<D, true, false>(tq, tk, tv, p, st) : launch<D, false, false>(tq, tk, tv, p, st);
+int launch_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const FwdParams& p, int causal, cudaStream_t st) {
+    if (p.group % 2 == 0) return causal ? launch<D, true, true>(tq, tk, tv, to, p, st) : launch<D, false, true>(tq, tk, tv, to, p, st);
+    return causal ? launch<D, true, false>(tq, tk, tv, to, p, st) : launch<D, false, false>(tq, tk, tv, to, p, st);
 }
 
 }  // namespace
@@ -642,11 +655,12 @@ NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, voi
     p.scale_log2 = scale * 1.4426950408889634f;
     p.v = (const bf16*)v; p.v_head = strides[4]; p.v_row = strides[5];
     p.o = (bf16*)o; p.o_head = strides[6]; p.o_row = strides[7];
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq, tk, tv, to;
     int rc;
     if ((rc = make_tmap_bhsd(&tq, q, D, T, Hq, 1, strides[1], strides[0], 0, kBM, p.pos_q))) return rc;
     if ((rc = make_tmap_bhsd(&tk, k, D, T, Hkv, 1, strides[3], strides[2], 0, kBN, p.pos_k))) return rc;
     if ((rc = make_tmap_bhsd(&tv, v, D, T, Hkv, 1, strides[5], strides[4], 0, kBN, p.pos_v))) return rc;
+    if ((rc = make_tmap_bhsd(&to, o, D, T, Hq, 1, strides[7], strides[6], 0, 32, p.pos_o))) return rc;
     cudaStream_t st = (cudaStream_t)stream;
-    return D == 64 ? launch_as<64>(tq, tk, tv, p, causal, st) : launch_as<128>(tq, tk, tv, p, causal, st);
+    return D == 64 ? launch_as<64>(tq, tk, tv, to, p, causal, st) : launch_as<128>(tq, tk, tv, to, p, causal, st);
 }
