@@ -55,6 +55,7 @@ struct FwdSmem {
     static constexpr uint32_t kPolyOf8 = D == 64 ? 0x52 : 0x44;          // of eight pairs of weights, those by the polynomial
     // tensor memory: O_0 O_1 | S_0 S_1 | P_0 P_1 (D = 64; else P_s = the first columns of S_s)
     static constexpr bool kAlias = D == 128;
+    static constexpr int kMmaThreads = kAlias ? 1 : 2;
     static constexpr uint32_t kColS = 2 * D, kColP = kAlias ? kColS : kColS + 256, kPStep = kAlias ? 128 : 64;
 };
 static_assert(FwdSmem<128>::kBytes <= 232448 && FwdSmem<64>::kBytes > 116 * 1024, "one CTA per SM");
@@ -107,7 +108,7 @@ __device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
 }
 
 constexpr int kItems = 4;                // of the ring in shared memory
-constexpr int kItemReaders = 11;         // the two MMA threads and a lane of each softmax warp and of the one that cuts value tiles
+constexpr int kItemReaders = 9;          // besides the MMA threads: a lane of each softmax warp and of the one that cuts value tiles
 
 // the next item of the ring, for a whole warp or (WARP = false) one thread
 template <bool WARP>
@@ -198,12 +199,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
         for (int i = 0; i < L::kSlots; ++i) {
             ptx::mbar_init(&kv_full[i], 1);
-            ptx::mbar_init(&kv_empty[i], 2);          // both MMA warps
+            ptx::mbar_init(&kv_empty[i], L::kMmaThreads);
             ptx::mbar_init(&kv_cut[i], 1);
         }
         for (int i = 0; i < kItems; ++i) {
             ptx::mbar_init(&item_full[i], 1);
-            ptx::mbar_init(&item_empty[i], kItemReaders);
+            ptx::mbar_init(&item_empty[i], kItemReaders + L::kMmaThreads);
         }
         ptx::fence_barrier_init();
     }
@@ -299,19 +300,20 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     } else if (warp == 8 || warp == 11) {
         // ============================ MMA ============================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (ptx::elect_one()) {
+        if (warp == 8 || L::kMmaThreads == 2) if (ptx::elect_one()) {
             constexpr uint32_t idesc_s = ptx::make_idesc_bf16(kBM, kBN, 0, 0);
             constexpr uint32_t idesc_o = ptx::make_idesc_bf16(kBM, D, 0, 1);
-            const int s = warp == 8 ? 0 : 1;
-            const uint32_t q_addr = ptx::smem_u32(sQ) + s * L::kTileBytes, ring = ptx::smem_u32(sRing);
-            const uint32_t t_o = tmem + s * D, t_s = tmem + L::kColS + s * 128, t_p = tmem + L::kColP + s * L::kPStep;
-            int it = 0, items = 0, loads = 0, tiles = 0, done = 0;
-            int n = 0, steps = 0;             // key tiles that query tile s meets in the item whose scores come next, and those of the item
+            constexpr int kMine = 2 / L::kMmaThreads;          // query tiles of this thread, from s0
+            const int s0 = warp == 8 ? 0 : 1;
+            const uint32_t ring = ptx::smem_u32(sRing);
+            int it = 0, items = 0, loads[kMine] = {}, tiles[kMine] = {}, done[kMine] = {};
+            int n[kMine] = {}, steps = 0;     // key tiles that the query tiles meet in the item whose scores come next, and those of the item
             auto next = [&]() {
                 Item x;
                 do x = next_item<false>(item_ring, item_full, item_empty, items, dead);
                 while (x.kind > 1);
-                n = x.kind == 1 ? x.n(s) : 0;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) n[i] = x.kind == 1 ? x.n(s0 + i) : 0;
                 steps = x.kind == 1 ? max(x.n0, x.n1) : 0;
             };
             auto slot = [&]() {
@@ -320,59 +322,75 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 ++it;
                 return at;
             };
-            auto scores = [&](int j) {                 // S = Q K^T of key tile j
-                const int at = slot();
-                if (j >= n) {                          // the other query tile alone meets it
-                    ptx::mbar_arrive(&kv_empty[at]);
-                    return;
-                }
-                if (j == 0) wait_for(&q_full[s], (uint32_t)(loads++) & 1u, dead);
-                if (!L::kAlias) wait_for(&s_empty[s], ((uint32_t)tiles & 1u) ^ 1u, dead);
-                ++tiles;
+            auto scores = [&](int i, int j, int at) {          // S_s = Q_s K^T of key tile j, if query tile s meets it
+                const int s = s0 + i;
+                if (j >= n[i]) return;
+                if (j == 0) wait_for(&q_full[s], (uint32_t)(loads[i]++) & 1u, dead);
+                if (!L::kAlias) wait_for(&s_empty[s], ((uint32_t)tiles[i] & 1u) ^ 1u, dead);
+                ++tiles[i];
                 ptx::tcgen05_fence_after();
-                const uint32_t kb = ring + at * L::kTileBytes;
+                const uint32_t qb = ptx::smem_u32(sQ) + s * L::kTileBytes, kb = ring + at * L::kTileBytes;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-                    ptx::umma_bf16<1>(t_s, ptx::make_smem_desc(q_addr + off, 16, 1024), ptx::make_smem_desc(kb + off, 16, 1024), idesc_s,
-                                      kk != 0 ? 1u : 0u);
+                    ptx::umma_bf16<1>(tmem + L::kColS + s * 128, ptx::make_smem_desc(qb + off, 16, 1024),
+                                      ptx::make_smem_desc(kb + off, 16, 1024), idesc_s, kk != 0 ? 1u : 0u);
                 }
                 ptx::umma_commit(&s_full[s]);
-                ptx::umma_commit(&kv_empty[at]);
-                if (j + 1 == n) ptx::umma_commit(&q_empty[s]);
+                if (j + 1 == n[i]) ptx::umma_commit(&q_empty[s]);
             };
-            auto weigh = [&](int j, int meets) {       // O += P V of key tile j
-                const int at = slot();
-                if (j >= meets) {
-                    ptx::mbar_arrive(&kv_empty[at]);
-                    return;
-                }
+            auto weigh = [&](int i, int j, int meets, int at) {          // O_s += P_s V of key tile j
+                const int s = s0 + i;
+                if (j >= meets) return;
                 const uint32_t vb = ring + at * L::kTileBytes;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    wait_for(half ? &p_full[s] : &p_half[s], (uint32_t)done & 1u, dead);
+                    wait_for(half ? &p_full[s] : &p_half[s], (uint32_t)done[i] & 1u, dead);
                     ptx::tcgen05_fence_after();
 #pragma unroll
                     for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                        ptx::umma_bf16_ts(t_o, t_p + kk * 8, ptx::make_smem_desc(vb + kk * 2048, kBN * 128, 1024), idesc_o,
-                                          (j | kk) != 0 ? 1u : 0u);
+                        ptx::umma_bf16_ts(tmem + s * D, tmem + L::kColP + s * L::kPStep + kk * 8,
+                                          ptx::make_smem_desc(vb + kk * 2048, kBN * 128, 1024), idesc_o, (j | kk) != 0 ? 1u : 0u);
                 }
-                ++done;
+                ++done[i];
                 ptx::umma_commit(&pv_done[s]);
+            };
+            auto all_scores = [&](int j) {
+                const int at = slot();
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) scores(i, j, at);
                 ptx::umma_commit(&kv_empty[at]);
             };
             next();
-            if (steps) scores(0);
+            if (steps) all_scores(0);
             while (steps) {
-                const int meets = n, last = steps - 1;
+                int meets[kMine];
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) meets[i] = n[i];
+                const int last = steps - 1;
                 for (int j = 0; j < last; ++j) {
-                    if (!L::kAlias) scores(j + 1);
-                    weigh(j, meets);
-                    if (L::kAlias) scores(j + 1);
+                    if (L::kMmaThreads == 2) {
+                        all_scores(j + 1);
+                        const int at = slot();
+                        weigh(0, j, meets[0], at);
+                        ptx::umma_commit(&kv_empty[at]);
+                    } else {                           // the scores of one query tile while the softmax of the other runs
+                        const int at = slot();
+                        weigh(0, j, meets[0], at);
+                        const int key = slot();
+                        scores(0, j + 1, key);
+                        weigh(kMine - 1, j, meets[kMine - 1], at);
+                        ptx::umma_commit(&kv_empty[at]);
+                        scores(kMine - 1, j + 1, key);
+                        ptx::umma_commit(&kv_empty[key]);
+                    }
                 }
                 next();
-                weigh(last, meets);
-                if (steps) scores(0);
+                const int at = slot();
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) weigh(i, last, meets[i], at);
+                ptx::umma_commit(&kv_empty[at]);
+                if (steps) all_scores(0);
             }
         }
     } else if (warp < 8) {
