@@ -21,8 +21,6 @@
 #include "gemm_tcgen05.cuh"
 #include "ptx.cuh"
 
-#include <type_traits>
-
 namespace {
 using namespace nxd_attn;
 
@@ -52,7 +50,6 @@ struct FwdSmem {
     static constexpr int kBarOff = kOutOff + 8 * 4096;
     static constexpr int kNumBars = 4 + 3 * kSlots + 10 + 8;
     static constexpr int kBytes = kBarOff + kNumBars * 8 + 16 + 1024;
-    static constexpr uint32_t kPolyOf8 = D == 64 ? 0x52 : 0x44;          // of eight pairs of weights, those by the polynomial
     // tensor memory: O_0 O_1 | S_0 S_1 | P_0 P_1 (D = 64; else P_s = the first columns of S_s)
     static constexpr bool kAlias = D == 128;
     static constexpr int kMmaThreads = kAlias ? 1 : 2;
@@ -143,21 +140,6 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^z of two numbers up to 2^7 by the FMA pipe, beside the 16 exponentials a clock of the special function unit: 2^z = 2^n 2^f with n the
-// nearest whole number, f in [-1/2, 1/2], and 2^f by the cubic of least relative error there (7.5e-5, fitted by linear
-// programming; a weight is rounded to 2^-8 anyway).  Numbers below -126 count as that.
-__device__ __forceinline__ void exp2_poly(uint64_t z, float& p0, float& p1) {
-    const float lo = fmaxf(f2_lo(z), -126.f), hi = fmaxf(f2_hi(z), -126.f);
-    const uint64_t x = f2_pack(lo, hi), magic = f2_pack(12582912.f, 12582912.f), neg_magic = f2_pack(-12582912.f, -12582912.f);
-    const uint64_t t = f2_add(x, magic);                                   // n in the low bits
-    const uint64_t f = f2_fma(f2_add(t, neg_magic), f2_pack(-1.f, -1.f), x);
-    uint64_t h = f2_fma(f, f2_pack(0.0551716685f, 0.0551716685f), f2_pack(0.2426111400f, 0.2426111400f));
-    h = f2_fma(f, h, f2_pack(0.6932609677f, 0.6932609677f));
-    h = f2_fma(f, h, f2_pack(0.9999280572f, 0.9999280572f));
-    p0 = __uint_as_float((uint32_t)h + ((uint32_t)t << 23));
-    p1 = __uint_as_float((uint32_t)(h >> 32) + ((uint32_t)(t >> 32) << 23));
-}
-
 template <int D, bool CAUSAL, bool HEADS>
 __global__ void __launch_bounds__(kThreads, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -454,24 +436,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 ptx::mbar_arrive(&s_empty[s]);
             }
         };
-        // One tile: weights of its 128 columns, the row's maximum and sum.  CUT: `mine` of them count for this row and `seen` for any of the
-        // warp (the diagonal, the end of the sequence); those tiles take all exponentials from the special function unit, whose
-        // 2^-inf is 0.
-        auto tile_weights = [&](auto cut, int j, int seen, int mine) {
-            constexpr bool CUT = decltype(cut)::value;
+        // One tile: weights of its 128 columns, the row's maximum and sum; `mine` columns count for this row, `seen` for any of the warp.
+        // All of one path: a tile on the diagonal or at the end of a sequence takes the same instructions behind its mask (chunks of 32
+        // columns that were left out by branches made such a tile a half longer than a whole one).
+        auto tile_weights = [&](int j, int seen, int mine) {
             uint32_t x[kBN];
             uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(t_s + c * 32, x + c * 32);
             scores_read();
-            if (CUT) {
-                const int whole = CAUSAL ? min(seen, q * 32 + 1) : seen;          // columns that every row of the warp sees, at least
+            if (__any_sync(0xffffffffu, mine < kBN)) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c * 32 + 32 > whole) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) x[c * 32 + e] = c * 32 + e < mine ? x[c * 32 + e] : 0xff800000u;          // -inf
-                    }
+                for (int e = 0; e < kBN; ++e) x[e] = e < mine ? x[e] : 0xff800000u;          // -inf
             }
             float a[8];
 #pragma unroll
@@ -486,7 +462,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             const uint64_t neg2 = f2_pack(neg, neg);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                if (CUT && half && seen <= 64) {                 // no row of the warp sees the second half
+                if (half && seen <= 64) {                        // no row of the warp sees the second half
 #pragma unroll
                     for (int e = 0; e < 32; ++e) x[32 + e] = 0u;
                 } else {
@@ -494,13 +470,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                     for (int e = 0; e < 64; e += 2) {
                         const int i = half * 64 + e;
                         const uint64_t z = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, neg2);
-                        float p0, p1;
-                        if (!CUT && ((L::kPolyOf8 >> ((e >> 1) & 7)) & 1)) {
-                            exp2_poly(z, p0, p1);
-                        } else {
-                            p0 = ex2_approx(f2_lo(z));
-                            p1 = ex2_approx(f2_hi(z));
-                        }
+                        const float p0 = ex2_approx(f2_lo(z)), p1 = ex2_approx(f2_hi(z));
                         sum[(e >> 1) & 3] = f2_add(sum[(e >> 1) & 3], f2_pack(p0, p1));
                         x[i >> 1] = pack_bf16x2(p0, p1);
                     }
@@ -535,8 +505,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 if (diagonal) seen = min(seen, q * 32 + 32);
                 wait_for(&s_full[s], (uint32_t)tiles & 1u, dead);
                 ptx::tcgen05_fence_after();
-                if (diagonal || seen < kBN) tile_weights(std::true_type{}, j, seen, mine);
-                else tile_weights(std::false_type{}, j, seen, mine);
+                tile_weights(j, seen, mine);
             }
             const Item done = it;                        // the next one is read while the last products run
             it = next_item<true>(item_ring, item_full, item_empty, items, dead);
