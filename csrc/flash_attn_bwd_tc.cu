@@ -52,13 +52,6 @@ struct BwdParams {
     int pos_q[3], pos_do[3], pos_k[3], pos_v[3], pos_dk[3], pos_dv[3], pos_dq[3], pos_acc[3];
     float scale, scale_log2;
     DropParams drop;
-    // PACKED instantiation only: the tile list, the row stride of lse_pad / delta_pad, and the tensors that a tile which crosses the
-    // end of its sequence is copied from or stored to without TMA
-    const PackedTile* tiles;
-    long long lse_row;
-    const bf16 *q, *k, *v, *dout;
-    bf16 *dk, *dv;
-    long long q_head, q_row, k_head, k_row, v_head, v_row, do_head, do_row, dk_head, dk_row, dv_head, dv_row;
 };
 
 template <int kD>
@@ -81,11 +74,7 @@ struct BwdSmem {
 };
 static_assert(BwdSmem<128>::kBytes <= 232448, "shared memory budget exceeded");
 
-// PACKED: sequences of different lengths laid end to end.  A CTA takes an entry of the batch's tile list, mirrored: the list is sorted by
-// the key tiles that a query tile meets, and the K/V block as far from the end meets as many query rows.  Q, dO, K and V tiles that
-// cross the sequence's end are copied with zeros behind it (0 * NaN is NaN), query rows behind it have no weight, and what such a
-// tile would add to the rows of the next sequence is zero.
-template <int kD, bool CAUSAL, bool DROP, bool PACKED = false>
+template <int kD, bool CAUSAL, bool DROP>
 __global__ void __launch_bounds__(kThreadsBwd, 1)
 fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_do,
                  const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
@@ -122,27 +111,13 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     // grid = (kv heads x splits, batch, K/V blocks): the block index is the SLOWEST launch dimension, so with a causal mask
     // the CTAs are handed to the SMs longest first (K/V block 0 meets every query tile, the last one only two)
-    PackedTile pt{};
-    if (PACKED) {
-        pdl_wait();
-        pt = packed_tile(p.tiles, blockIdx.x / (p.Hkv * p.nsplit));
-    }
-    const int hs = PACKED ? blockIdx.x % (p.Hkv * p.nsplit) : blockIdx.x;
-    const int nbk = PACKED ? (pt.len + kBN - 1) / kBN - 1 - pt.t : blockIdx.z, hkv = hs / p.nsplit, split = hs % p.nsplit;
-    const int b = PACKED ? 0 : blockIdx.y;
-    if (PACKED && pt.len == 0) {       // with splits dK and dV come from accumulators that start as zeros
-        if (p.nsplit > 1) return;
-        block_zero_rows<kD>(p.dk + (long long)pt.start * p.dk_row + hkv * p.dk_head, p.dk_row, pt.t, threadIdx.x, kThreadsBwd);
-        block_zero_rows<kD>(p.dv + (long long)pt.start * p.dv_row + hkv * p.dv_head, p.dv_row, pt.t, threadIdx.x, kThreadsBwd);
-        return;
-    }
+    const int nbk = blockIdx.z, hkv = blockIdx.x / p.nsplit, split = blockIdx.x % p.nsplit, b = blockIdx.y;
     const int group = p.Hq / p.Hkv;
     const int n0 = nbk * kBN;
-    const int offset = PACKED ? 0 : p.Sk - p.Sq;
-    const int sq = PACKED ? pt.len : p.Sq, sk = PACKED ? pt.len : p.Sk, row_base = PACKED ? pt.start : 0;
+    const int offset = p.Sk - p.Sq;
     int mb_start = 0;
     if (CAUSAL) mb_start = max(0, (n0 - offset) / kBM);
-    const int mb_end = (sq + kBM - 1) / kBM;
+    const int mb_end = (p.Sq + kBM - 1) / kBM;
     const int tiles_per_head = max(mb_end - mb_start, 0);
     // (q head of the group, q tile) pairs of this K/V block, flattened; this CTA owns the slice [it0, it0 + total)
     const int all_tiles = tiles_per_head * group;
@@ -169,7 +144,7 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         ptx::mbar_init(dq_empty, kDrainThreads);
         ptx::fence_barrier_init();
     }
-    if (!PACKED) pdl_wait();         // ahead of the allocation: nothing that this grid waits for may be short of tensor memory
+    pdl_wait();         // ahead of the allocation: nothing that this grid waits for may be short of tensor memory
     if (warp == 1) ptx::tmem_alloc<1>(tmem_ptr_smem, 512);
     ptx::tcgen05_fence_before();
     __syncthreads();
@@ -178,24 +153,16 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 
     if (warp == 0) {
         // ============================ TMA producer ============================
-        if (PACKED || lane == 0) {
+        if (lane == 0) {
             int c[4];
-            if (PACKED && n0 + kBN > sk) {
-                warp_load_tile<kD>(sK, p.k + hkv * p.k_head + (long long)(row_base + n0) * p.k_row, p.k_row, kBN, sk - n0, lane);
-                warp_load_tile<kD>(sV, p.v + hkv * p.v_head + (long long)(row_base + n0) * p.v_row, p.v_row, kBN, sk - n0, lane);
-                ptx::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(kv_full);
-            } else if (lane == 0) {
-                ptx::mbar_arrive_expect_tx(kv_full, 2 * kBN * kD * 2);
+            ptx::mbar_arrive_expect_tx(kv_full, 2 * kBN * kD * 2);
 #pragma unroll
-                for (int g = 0; g < kD / 64; ++g) {
-                    c[0] = g * 64;
-                    coords(p.pos_k, row_base + n0, hkv, b, c);
-                    tma_load_4d(&tmap_k, kv_full, sK + g * (kBN * 128), c[0], c[1], c[2], c[3]);
-                    coords(p.pos_v, row_base + n0, hkv, b, c);
-                    tma_load_4d(&tmap_v, kv_full, sV + g * (kBN * 128), c[0], c[1], c[2], c[3]);
-                }
+            for (int g = 0; g < kD / 64; ++g) {
+                c[0] = g * 64;
+                coords(p.pos_k, n0, hkv, b, c);
+                tma_load_4d(&tmap_k, kv_full, sK + g * (kBN * 128), c[0], c[1], c[2], c[3]);
+                coords(p.pos_v, n0, hkv, b, c);
+                tma_load_4d(&tmap_v, kv_full, sV + g * (kBN * 128), c[0], c[1], c[2], c[3]);
             }
             int th = it0 % tiles_per_head, hq = hkv * group + it0 / tiles_per_head;   // (q tile, q head) walk
             for (int it = 0; it < total; ++it) {
@@ -203,31 +170,19 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 const uint32_t ph = (uint32_t)(it / kQStages) & 1u;
                 const int m0 = (mb_start + th) * kBM;
                 ptx::mbar_wait(&qdo_empty[st], ph ^ 1u);
-                const bool cut = PACKED && m0 + kBM > sq;
-                if (cut) {
-                    const long long row = row_base + m0;
-                    warp_load_tile<kD>(sQ + st * L::kStageBytes, p.q + hq * p.q_head + row * p.q_row, p.q_row, kBM, sq - m0, lane);
-                    warp_load_tile<kD>(sDO + st * L::kStageBytes, p.dout + hq * p.do_head + row * p.do_row, p.do_row, kBM, sq - m0, lane);
-                    ptx::fence_proxy_async();
-                    __syncwarp();
-                }
-                if (!PACKED || lane == 0) {
-                    ptx::mbar_arrive_expect_tx(&qdo_full[st], cut ? 2 * kBM * 4 : L::kTxPerStage);
-                    if (!cut) {
+                ptx::mbar_arrive_expect_tx(&qdo_full[st], L::kTxPerStage);
 #pragma unroll
-                        for (int g = 0; g < kD / 64; ++g) {
-                            c[0] = g * 64;
-                            coords(p.pos_q, row_base + m0, hq, b, c);
-                            tma_load_4d(&tmap_q, &qdo_full[st], sQ + st * L::kStageBytes + g * (kBM * 128), c[0], c[1], c[2], c[3]);
-                            coords(p.pos_do, row_base + m0, hq, b, c);
-                            tma_load_4d(&tmap_do, &qdo_full[st], sDO + st * L::kStageBytes + g * (kBM * 128), c[0], c[1], c[2],
-                                        c[3]);
-                        }
-                    }
-                    const long long row = PACKED ? hq * p.lse_row + pt.pad + m0 : ((long long)b * p.Hq + hq) * p.Sq_pad + m0;
-                    bulk_load_1d(sLD + st * 2 * kBM, p.lse_pad + row, kBM * 4, &qdo_full[st]);
-                    bulk_load_1d(sLD + st * 2 * kBM + kBM, p.delta_pad + row, kBM * 4, &qdo_full[st]);
+                for (int g = 0; g < kD / 64; ++g) {
+                    c[0] = g * 64;
+                    coords(p.pos_q, m0, hq, b, c);
+                    tma_load_4d(&tmap_q, &qdo_full[st], sQ + st * L::kStageBytes + g * (kBM * 128), c[0], c[1], c[2], c[3]);
+                    coords(p.pos_do, m0, hq, b, c);
+                    tma_load_4d(&tmap_do, &qdo_full[st], sDO + st * L::kStageBytes + g * (kBM * 128), c[0], c[1], c[2],
+                                c[3]);
                 }
+                const long long row = ((long long)b * p.Hq + hq) * p.Sq_pad + m0;
+                bulk_load_1d(sLD + st * 2 * kBM, p.lse_pad + row, kBM * 4, &qdo_full[st]);
+                bulk_load_1d(sLD + st * 2 * kBM + kBM, p.delta_pad + row, kBM * 4, &qdo_full[st]);
                 if (++th == tiles_per_head) { th = 0; ++hq; }
             }
         }
@@ -319,10 +274,6 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             }
             ptx::tcgen05_fence_before();
             ptx::mbar_arrive(dq_empty);
-            if (PACKED && m0 + kBM > sq) {       // those columns are the next sequence's: K may hold what 0 does not silence
-#pragma unroll
-                for (int e = 0; e < 64; ++e) v[e] = m0 + e < sq ? v[e] : 0u;
-            }
             if (has_rows) {
                 if (lane == 0) ptx::bulk_wait_read<0>();     // the previous reduce-adds have read the staging rows
                 __syncwarp();
@@ -342,8 +293,8 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                 if (lane == 0) {
                     int c[4];
                     coords(p.pos_dq, q4 * 32, hq, b, c);
-                    tma_reduce_add_4d(&tmap_dq, stage, pt.pad + m0, c[1], c[2], c[3]);
-                    if (!PACKED || m0 + 32 < sq) tma_reduce_add_4d(&tmap_dq, stage + 4096, pt.pad + m0 + 32, c[1], c[2], c[3]);
+                    tma_reduce_add_4d(&tmap_dq, stage, m0, c[1], c[2], c[3]);
+                    tma_reduce_add_4d(&tmap_dq, stage + 4096, m0 + 32, c[1], c[2], c[3]);
                     ptx::bulk_commit();
                 }
             }
@@ -365,10 +316,9 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             constexpr bool MASK = decltype(mask_tag)::value;
             // masked <=> krow >= Sk, or (causal) krow > m0 + c0h + c + offset  <=>  c < first_ok
             int first_ok = 0;
-            const int last_ok = sq - m0 - c0h;           // PACKED: query rows behind the end are masked too
             if (MASK) {
                 first_ok = CAUSAL ? krow - offset - m0 - c0h : 0;
-                if (krow >= sk) first_ok = 64;
+                if (krow >= p.Sk) first_ok = 64;
             }
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
@@ -393,7 +343,6 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     } else {
                         dsv[e] = pv[e] * (dpe - dv[e]);
                     }
-                    if (PACKED && MASK && (c + e < first_ok || c + e >= last_ok)) pv[e] = dsv[e] = 0.f;
                 }
                 pk[c >> 1] = pack_bf16x2(pv[0], pv[1]);
                 pk[(c >> 1) + 1] = pack_bf16x2(pv[2], pv[3]);
@@ -420,7 +369,7 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             const float* Ls = sLD + st * 2 * kBM;
             const float* Ds = Ls + kBM;
             // warp-uniform: does any (K/V row of this warp, query column of this warp) need masking?
-            const bool need_mask = (n0 + kBN > sk) || (PACKED && m0 + kBM > sq) || (CAUSAL && (n0 + q4 * 32 + 31 > m0 + c0h + offset));
+            const bool need_mask = (n0 + kBN > p.Sk) || (CAUSAL && (n0 + q4 * 32 + 31 > m0 + c0h + offset));
             uint32_t pk[16], dk_[16];
             if (need_mask) softmax_bwd(std::true_type{}, s, dp, Ls, Ds, m0, hq, pk, dk_);
             else softmax_bwd(std::false_type{}, s, dp, Ls, Ds, m0, hq, pk, dk_);
@@ -463,10 +412,6 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     uint32_t o[32];
                     ptx::tmem_ld_32x32b_x32(tmem_base + col + lane_off + g * 32, o);
                     ptx::tmem_ld_wait();
-                    if (PACKED && krow >= sk) {          // the next sequence's row
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0u;
-                    }
                     if (lane == 0) ptx::bulk_wait_read<1>();
                     __syncwarp();
                     uint8_t* dst = stg + buf * 4096 + lane * 128;
@@ -478,10 +423,10 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                     ptx::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        if (n0 + q4 * 32 < sk) {
+                        if (n0 + q4 * 32 < p.Sk) {
                             int c[4];
                             c[0] = g * 32;
-                            coords(p.pos_acc, row_base + n0 + q4 * 32, hkv, b, c);
+                            coords(p.pos_acc, n0 + q4 * 32, hkv, b, c);
                             tma_reduce_add_4d(which == 0 ? &tmap_dv_acc : &tmap_dk_acc, stg + buf * 4096, c[0], c[1], c[2],
                                               c[3]);
                         }
@@ -520,25 +465,12 @@ fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                         }
                         *reinterpret_cast<uint4*>(dst + ((c ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    if (PACKED && n0 + q4 * 32 + 32 > sk) {          // the rows behind the end are the next sequence's
-                        __syncwarp();
-                        bf16* to = which == 0 ? p.dv + hkv * p.dv_head : p.dk + hkv * p.dk_head;
-                        const long long ld = which == 0 ? p.dv_row : p.dk_row;
-                        const uint8_t* src = stage + g * (kBN * 128) + q4 * 32 * 128;
-                        for (int i = lane; i < 32 * 8; i += 32) {
-                            const int r = i >> 3, ch = i & 7;
-                            if (n0 + q4 * 32 + r < sk)
-                                *reinterpret_cast<uint4*>(to + (row_base + n0 + q4 * 32 + r) * ld + g * 64 + ch * 8) =
-                                    *reinterpret_cast<const uint4*>(src + r * 128 + ((ch ^ (r & 7)) << 4));
-                        }
-                        continue;
-                    }
                     ptx::fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0 && (PACKED || n0 + q4 * 32 < p.Sk)) {
+                    if (lane == 0 && n0 + q4 * 32 < p.Sk) {
                         int c[4];
                         c[0] = g * 64;
-                        coords(which == 0 ? p.pos_dv : p.pos_dk, row_base + n0 + q4 * 32, hkv, b, c);
+                        coords(which == 0 ? p.pos_dv : p.pos_dk, n0 + q4 * 32, hkv, b, c);
                         tma_store_4d(which == 0 ? &tmap_dv : &tmap_dk, stage + g * (kBN * 128) + q4 * 32 * 128, c[0], c[1],
                                      c[2], c[3]);
                         ptx::bulk_commit();
@@ -674,198 +606,7 @@ int launch_bwd_tc(dim3 grid, cudaStream_t st, const CUtensorMap& tq, const CUten
     return 0;
 }
 
-// Packed batch: Delta of one entry (up to 128 rows) of one head, at the plan's padded columns.  kD / 8 lanes own a row.
-template <int kD>
-__global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ dout, const PackedTile* tiles,
-                                                           float* __restrict__ delta, long long o_head, long long o_row,
-                                                           long long do_head, long long do_row, long long lse_row, int Hq) {
-    pdl_trigger();
-    pdl_wait();
-    constexpr int L = kD / 8, R = 256 / L;
-    const PackedTile pt = packed_tile(tiles, blockIdx.x / Hq);
-    const int h = blockIdx.x % Hq, l = threadIdx.x % L;
-    const int first = pt.t * kBN, rows = min(pt.len - first, kBN);        // negative where the entry is no tile
-    if (pt.len == 0) return;
-    bf16x8 a[kBN / R], g[kBN / R];
-#pragma unroll
-    for (int u = 0; u < kBN / R; ++u) {
-        const int r = u * R + threadIdx.x / L;
-        const long long row = pt.start + first + r;
-        if (r < rows) {
-            a[u] = reinterpret_cast<const bf16x8*>(o + h * o_head + row * o_row)[l];
-            g[u] = reinterpret_cast<const bf16x8*>(dout + h * do_head + row * do_row)[l];
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < kBN / R; ++u) {
-        const int r = u * R + threadIdx.x / L;
-        float acc = 0.f;
-        if (r < rows) {
-            float fa[8], fg[8];
-            unpack8(a[u], fa);
-            unpack8(g[u], fg);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fg[e], acc);
-        }
-#pragma unroll
-        for (int off = L / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-        if (l == 0 && r < rows) delta[h * lse_row + pt.pad + first + r] = acc;
-    }
-}
-
-// Packed batch: d-major fp32 accumulator [Hq, D, lse_row] -> dq, one entry of one head per block; rows of no sequence get zeros.
-template <int kD>
-__global__ void __launch_bounds__(256) packed_dq_kernel(const float* __restrict__ acc, bf16* __restrict__ dq, const PackedTile* tiles,
-                                                        long long head, long long row, long long lse_row, int Hq) {
-    pdl_trigger();
-    pdl_wait();
-    __shared__ float tile[kD][65];
-    const PackedTile pt = packed_tile(tiles, blockIdx.x / Hq);
-    const int h = blockIdx.x % Hq;
-    if (pt.len == 0) {
-        block_zero_rows<kD>(dq + (long long)pt.start * row + h * head, row, pt.t, threadIdx.x, 256);
-        return;
-    }
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int col = (threadIdx.x & 15) * 4, d0 = threadIdx.x >> 4;
-    for (int half = 0; half < 2; ++half) {
-        const int q0 = pt.t * kBN + half * 64;
-        if (q0 >= pt.len) return;
-        const float* src = acc + (long long)h * kD * lse_row + pt.pad + q0;
-        float4 v[kD / 16];
-#pragma unroll
-        for (int j = 0; j < kD / 16; ++j)        // columns in fours: those of a sequence are padded to a multiple of four
-            v[j] = q0 + col < pt.len ? *reinterpret_cast<const float4*>(src + (d0 + 16 * j) * lse_row + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (half) __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kD / 16; ++j) {
-            float* t = &tile[d0 + 16 * j][col];
-            t[0] = v[j].x, t[1] = v[j].y, t[2] = v[j].z, t[3] = v[j].w;
-        }
-        __syncthreads();
-        const int r = w * 8 + (lane >> 2);
-        if (q0 + r < pt.len) {
-            bf16* dst = dq + h * head + (long long)(pt.start + q0 + r) * row;
-#pragma unroll
-            for (int c = lane & 3; c < kD / 8; c += 4) {
-                float f[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = tile[c * 8 + e][r];
-                reinterpret_cast<bf16x8*>(dst)[c] = pack8(f);
-            }
-        }
-    }
-}
-
-template <int kD, bool CAUSAL>
-int launch_bwd_tc_packed(unsigned grid, cudaStream_t st, const CUtensorMap& tq, const CUtensorMap& tdo, const CUtensorMap& tk,
-                         const CUtensorMap& tv, const CUtensorMap& tdk, const CUtensorMap& tdv, const CUtensorMap& tdq,
-                         const CUtensorMap& tdka, const CUtensorMap& tdva, const BwdParams& p) {
-    constexpr auto kern = fa_bwd_tc_kernel<kD, CAUSAL, false, true>;
-    NXD_CHECK_CUDA(nxd_allow_smem<kern>(BwdSmem<kD>::kBytes));
-    NXD_CHECK_CUDA((nxd_launch_pdl(kern, dim3(grid), dim3(kThreadsBwd), BwdSmem<kD>::kBytes, st, tq, tdo, tk, tv, tdk, tdv, tdq, tdka,
-        tdva, p)));
-    NXD_LAUNCH_CHECK();
-    return 0;
-}
-
 }  // namespace
-
-// CTAs that share one K/V block of a packed batch: as nxd_flash_attn_bwd_tc_num_splits, for N sequences of average length.
-NXD_API int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv) {
-    const long long avg = (T + (N > 0 ? N : 1) - 1) / (N > 0 ? N : 1);
-    const long long blocks = (avg + kBN - 1) / kBN * (N > 0 ? N : 1);
-    const int B = (int)(blocks < 65536 ? blocks : 65536);
-    const int sms = nxd_num_sms();
-    const long long ctas = (long long)B * Hkv;
-    if (ctas >= 2LL * sms) return 1;
-    const long long iters = (avg + kBM - 1) / kBM * (Hq / (Hkv > 0 ? Hkv : 1));
-    long long n = (4LL * sms + ctas - 1) / ctas;
-    if (n > iters / 8) n = iters / 8;
-    if (n > 16) n = 16;
-    return n < 1 ? 1 : (int)n;
-}
-
-// Backward of nxd_packed_attn_fwd.  strides: {head, row} in elements of q, k, v, o, dout, dq, dk, dv (16 values, multiples of 8);
-// lse: what the forward pass wrote; delta: Hq * lse_row floats of scratch; dq_accum: ZEROED [Hq, D, lse_row] floats;
-// dkv_accum: NULL, or ZEROED [2, Hkv, T, D] floats where nxd_packed_attn_bwd_splits says more than one.
-// dQ (with splits dK and dV too) is summed in fp32 in an order that is not fixed.
-NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
-                                float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
-                                const long long* strides, const void* tiles, int entries, long long lse_row, long long T, int N, int Hq,
-                                int Hkv, int D, float scale, int causal, void* stream) {
-    NXD_REQUIRE(D == 64 || D == 128, "packed_attn_bwd: head dim %d not supported (64 or 128)", D);
-    NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && lse_row % 4 == 0 &&
-                (long long)entries * Hq * 16 < (1ll << 31), "packed_attn_bwd: bad problem");
-    for (int i = 0; i < 16; ++i)
-        NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn_bwd: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
-    const void* bases[] = {q, k, v, o, dout, lse, delta, dq_accum, dkv_accum, dq, dk, dv, tiles};
-    for (const void* x : bases) NXD_REQUIRE(((uintptr_t)x & 15) == 0, "packed_attn_bwd: tensors must be %s", "16-byte aligned");
-    cudaStream_t st = (cudaStream_t)stream;
-    const PackedTile* pt = (const PackedTile*)tiles;
-    BwdParams p{};
-    p.B = 1; p.Hq = Hq; p.Hkv = Hkv; p.Sq = p.Sk = (int)T;
-    p.lse_pad = lse; p.delta_pad = delta; p.lse_row = lse_row;
-    p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
-    p.drop.inv_keep = 1.f;
-    p.nsplit = dkv_accum ? nxd_packed_attn_bwd_splits(T, N, Hq, Hkv) : 1;
-    p.tiles = pt;
-    p.q = (const bf16*)q; p.q_head = strides[0]; p.q_row = strides[1];
-    p.k = (const bf16*)k; p.k_head = strides[2]; p.k_row = strides[3];
-    p.v = (const bf16*)v; p.v_head = strides[4]; p.v_row = strides[5];
-    p.dout = (const bf16*)dout; p.do_head = strides[8]; p.do_row = strides[9];
-    p.dk = (bf16*)dk; p.dk_head = strides[12]; p.dk_row = strides[13];
-    p.dv = (bf16*)dv; p.dv_head = strides[14]; p.dv_row = strides[15];
-    const unsigned per_head = (unsigned)entries * Hq;
-    if (D == 128)
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<128>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const bf16*)dout, pt,
-            delta, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
-    else
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<64>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const bf16*)dout, pt,
-            delta, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
-    NXD_LAUNCH_CHECK();
-    CUtensorMap tq, tdo, tk, tv, tdk, tdv, tdq, tdka, tdva;
-    int rc;
-    if ((rc = make_tmap_bhsd(&tq, q, D, T, Hq, 1, strides[1], strides[0], 0, kBM, p.pos_q))) return rc;
-    if ((rc = make_tmap_bhsd(&tk, k, D, T, Hkv, 1, strides[3], strides[2], 0, kBN, p.pos_k))) return rc;
-    if ((rc = make_tmap_bhsd(&tv, v, D, T, Hkv, 1, strides[5], strides[4], 0, kBN, p.pos_v))) return rc;
-    if ((rc = make_tmap_bhsd(&tdo, dout, D, T, Hq, 1, strides[9], strides[8], 0, kBM, p.pos_do))) return rc;
-    if ((rc = make_tmap_bhsd(&tdk, dk, D, T, Hkv, 1, strides[13], strides[12], 0, 32, p.pos_dk))) return rc;
-    if ((rc = make_tmap_bhsd(&tdv, dv, D, T, Hkv, 1, strides[15], strides[14], 0, 32, p.pos_dv))) return rc;
-    if ((rc = make_tmap_bhsd(&tdq, dq_accum, (int)lse_row, D, Hq, 1, lse_row, (long long)D * lse_row, 0, 32, p.pos_dq, 4))) return rc;
-    const long long kv_elems = (long long)Hkv * T * D;
-    float* dk_acc = dkv_accum;
-    float* dv_acc = dkv_accum + kv_elems;
-    tdka = tdva = tdq;             // unused maps still have to be valid
-    if (p.nsplit > 1) {
-        if ((rc = make_tmap_bhsd(&tdka, dk_acc, D, T, Hkv, 1, D, T * D, 0, 32, p.pos_acc, 4))) return rc;
-        if ((rc = make_tmap_bhsd(&tdva, dv_acc, D, T, Hkv, 1, D, T * D, 0, 32, p.pos_acc, 4))) return rc;
-    }
-    const unsigned grid = (unsigned)entries * Hkv * p.nsplit;
-    if (D == 128)
-        rc = causal ? launch_bwd_tc_packed<128, true>(grid, st, tq, tdo, tk, tv, tdk, tdv, tdq, tdka, tdva, p)
-                    : launch_bwd_tc_packed<128, false>(grid, st, tq, tdo, tk, tv, tdk, tdv, tdq, tdka, tdva, p);
-    else
-        rc = causal ? launch_bwd_tc_packed<64, true>(grid, st, tq, tdo, tk, tv, tdk, tdv, tdq, tdka, tdva, p)
-                    : launch_bwd_tc_packed<64, false>(grid, st, tq, tdo, tk, tv, tdk, tdv, tdq, tdka, tdva, p);
-    if (rc) return rc;
-    if (p.nsplit > 1) {
-        const long long n = kv_elems / 8;
-        NXD_CHECK_CUDA((nxd_launch_pdl(fa_bwd_tc_dq_convert_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (const float*)dk_acc,
-            (bf16*)dk, 0ll, strides[12], strides[13], 1, Hkv, (int)T, D)));
-        NXD_CHECK_CUDA((nxd_launch_pdl(fa_bwd_tc_dq_convert_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (const float*)dv_acc,
-            (bf16*)dv, 0ll, strides[14], strides[15], 1, Hkv, (int)T, D)));
-        NXD_LAUNCH_CHECK_N(2);
-    }
-    if (D == 128)
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<128>, dim3(per_head), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
-            strides[10], strides[11], lse_row, Hq)));
-    else
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<64>, dim3(per_head), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
-            strides[10], strides[11], lse_row, Hq)));
-    NXD_LAUNCH_CHECK();
-    return 0;
-}
 
 // Number of CTAs that should share one (K/V block, kv head) so that the grid fills the GPU: 1 = every CTA owns its
 // dK / dV tile (no accumulators needed), > 1 = pass `dkv_accum` to nxd_flash_attn_bwd_tc.

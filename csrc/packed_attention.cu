@@ -19,15 +19,16 @@
 // scores are in registers, so the softmax warps, which bound this size (128 exponentials a row for half the products), never wait.
 #include "attn_tc_common.cuh"
 #include "gemm_tcgen05.cuh"
+#include "packed_items.cuh"
 #include "ptx.cuh"
 
 namespace {
 using namespace nxd_attn;
+using namespace nxd_packed;
 
 constexpr int kBM = 128, kBN = 128;
 constexpr int kThreads = 384;                     // 8 softmax warps, MMA, TMA, ends of sequences, MMA (registers move by groups of four warps)
 constexpr float kRescale = 8.0f;                  // log2 units
-constexpr long long kWaitClocks = 4000000000ll;   // a wait that takes two seconds is given up: the CTA's results are NaN then
 
 struct FwdParams {
     const PackedTile* tiles;
@@ -57,31 +58,18 @@ struct FwdSmem {
 };
 static_assert(FwdSmem<128>::kBytes <= 232448 && FwdSmem<64>::kBytes > 116 * 1024, "one CTA per SM");
 
-// A wait with an end: after kWaitClocks the CTA is marked, and no wait of its lasts any more.
-__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    if (ptx::mbar_try_wait(bar, parity)) return;
-    const long long start = clock64();
-    for (int i = 1;; ++i) {
-        if (ptx::mbar_try_wait(bar, parity) || *dead) return;
-        if ((i & 63) == 0 && clock64() - start > kWaitClocks) *dead = 1;
-    }
-}
-
-// The items of this CTA: every gridDim.x-th of the list, which is sorted by weight, forwards and backwards in turn so that nobody gets
-// the longest of every round.  The TMA warp, which is ahead of the others, reads them and hands them on through shared memory.
 struct alignas(16) Item {
-    int kind, start, len, pad;           // kind: 0 end of the list, 1 an item, above: that many rows from `start` are of no sequence
+    int kind, start, len, pad;           // kind: 0 end of the list, 1 an item, above: that many (less kRowsOfNone) rows from `start` are of no sequence
     int t0, t1, n0, n1;                  // query tiles and the key tiles that they meet (0: there is no second one)
     int h0, h1, hkv, unused;
     __device__ __forceinline__ int t(int s) const { return s ? t1 : t0; }
     __device__ __forceinline__ int n(int s) const { return s ? n1 : n0; }
     __device__ __forceinline__ int h(int s) const { return s ? h1 : h0; }
 };
-constexpr int kRowsOfNone = 1;           // added to the rows of such an entry, to tell them from an item
 
 template <bool CAUSAL, bool HEADS>
 __device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
-    const unsigned G = gridDim.x, at = round * G + (round & 1 ? G - 1 - blockIdx.x : blockIdx.x);          // below 2^31 + 148
+    const unsigned at = item_of_round(round);
     Item it{};
     if (at >= (unsigned)p.entries * p.pairs) return it;
     const unsigned e = at / (unsigned)p.pairs;
@@ -104,26 +92,7 @@ __device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
     return it;
 }
 
-constexpr int kItems = 4;                // of the ring in shared memory
 constexpr int kItemReaders = 9;          // besides the MMA threads: a lane of each softmax warp and of the one that cuts value tiles
-
-// the next item of the ring, for a whole warp or (WARP = false) one thread
-template <bool WARP>
-__device__ __forceinline__ Item next_item(const Item* ring, uint64_t* full, uint64_t* empty, int& count, volatile int* dead) {
-    const int i = count % kItems;
-    wait_for(&full[i], (uint32_t)(count / kItems) & 1u, dead);
-    ++count;
-    Item it{};
-    if (!*dead) {
-        const int4* src = reinterpret_cast<const int4*>(&ring[i]);
-        int4* dst = reinterpret_cast<int4*>(&it);
-#pragma unroll
-        for (int w = 0; w < 3; ++w) dst[w] = src[w];
-    }
-    if (WARP) __syncwarp();
-    if (!WARP || (threadIdx.x & 31) == 0) ptx::mbar_arrive(&empty[i]);
-    return it;
-}
 
 __device__ __forceinline__ float max3(float a, float b, float c) {          // NaN if one of them is
     float r;
@@ -210,22 +179,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         int it = 0, loads[2] = {0, 0}, round = 0, published = 0;
         // the item whose keys come next and its next key tile; the same of the values, which are one tile behind at most
-        Item ki, vi, ahead = fetch_item<CAUSAL, HEADS>(p, round++);
+        Item ki{}, vi{}, ahead = fetch_item<CAUSAL, HEADS>(p, round++);
         int kj = 0, vj = 0;
         auto publish = [&]() {               // goes on to the next item with scores; the one behind it is read meanwhile
             do {
                 ki = ahead;
                 if (ki.kind) ahead = fetch_item<CAUSAL, HEADS>(p, round++);
-                const int i = published % kItems;
-                wait_for(&item_empty[i], ((uint32_t)(published / kItems) & 1u) ^ 1u, dead);
-                ++published;
-                if (lane == 0) {
-                    const int4* src = reinterpret_cast<const int4*>(&ki);
-                    int4* dst = reinterpret_cast<int4*>(&item_ring[i]);
-#pragma unroll
-                    for (int w = 0; w < 3; ++w) dst[w] = src[w];
-                    ptx::mbar_arrive(&item_full[i]);
-                }
+                publish_item(ki, item_ring, item_full, item_empty, published, dead);
             } while (ki.kind > 1);
             kj = 0;
         };
@@ -292,7 +252,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             int n[kMine] = {}, steps = 0;     // key tiles that the query tiles meet in the item whose scores come next, and those of the item
             auto next = [&]() {
                 Item x;
-                do x = next_item<false>(item_ring, item_full, item_empty, items, dead);
+                do x = next_item<false, Item>(item_ring, item_full, item_empty, items, dead);
                 while (x.kind > 1);
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) n[i] = x.kind == 1 ? x.n(s0 + i) : 0;
@@ -484,7 +444,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             const uint64_t all = f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3]));
             l += f2_lo(all) + f2_hi(all);
         };
-        Item it = next_item<true>(item_ring, item_full, item_empty, items, dead);
+        Item it = next_item<true, Item>(item_ring, item_full, item_empty, items, dead);
         for (; it.kind != 0;) {
             const int head = it.h(s), n = it.n(s), t = it.t(s);
             if (it.kind > 1) {                           // rows of no sequence; once a head
@@ -494,7 +454,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                             make_uint4(0u, 0u, 0u, 0u);
             }
             if (it.kind > 1 || n == 0) {
-                it = next_item<true>(item_ring, item_full, item_empty, items, dead);
+                it = next_item<true, Item>(item_ring, item_full, item_empty, items, dead);
                 continue;
             }
             m = -INFINITY, l = 0.f;
@@ -508,7 +468,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 tile_weights(j, seen, mine);
             }
             const Item done = it;                        // the next one is read while the last products run
-            it = next_item<true>(item_ring, item_full, item_empty, items, dead);
+            it = next_item<true, Item>(item_ring, item_full, item_empty, items, dead);
             // O / l, one row a thread, nothing behind the sequence's end.  A row without a finite score has no softmax.
             wait_for(&pv_done[s], (uint32_t)(tiles - 1) & 1u, dead);
             ptx::tcgen05_fence_after();
@@ -570,7 +530,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         int it = 0, items = 0;
         uint32_t phases = 0;
         for (;;) {
-            const Item x = next_item<true>(item_ring, item_full, item_empty, items, dead);
+            const Item x = next_item<true, Item>(item_ring, item_full, item_empty, items, dead);
             if (x.kind == 0) break;
             if (x.kind > 1) continue;
             const int n = max(x.n0, x.n1), left = x.len - (n - 1) * kBN;
@@ -591,11 +551,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     ptx::tcgen05_fence_before();
     __syncthreads();
-    if (dead_word) {          // copies may still be on their way into this CTA's memory
-        const long long start = clock64();
-        while (clock64() - start < kWaitClocks / 100) {
-        }
-    }
+    if (dead_word) let_copies_land();
     if (warp == 8) ptx::tmem_dealloc<1>(tmem, 512);
 }
 

@@ -137,7 +137,7 @@ def _backward(q, k, v, o, lse, do, dq, dk, dv, packed: PackedSequences, scale: f
     Hkv = k.shape[1]
     tiles, entries, columns = packed.plan(causal)
     delta = torch.empty_like(lse)
-    acc = torch.zeros((Hq, D, columns), dtype=torch.float32, device=q.device)
+    acc = torch.empty((Hq, D, columns), dtype=torch.float32, device=q.device)
     splits = _lib.lib().nxd_packed_attn_bwd_splits(_c.c_longlong(T), _c.c_int(packed.count), _c.c_int(Hq), _c.c_int(Hkv))
     kv_acc = torch.zeros((2, Hkv, T, D), dtype=torch.float32, device=q.device) if splits > 1 else None
     rc = _lib.lib().nxd_packed_attn_bwd(
