@@ -129,20 +129,6 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedTile* tiles, int i
     return PackedTile{v.x, v.y, v.z, v.w};
 }
 
-// `valid` rows of D bf16 from global memory, then zeros, as a [D / 64 groups][rows][64] image of 128-byte swizzled rows: what a
-// TMA load of a tile gives at the end of the tensor, for a tile that ends inside it.  All lanes of a warp take part; the caller
-// fences (fence.proxy.async) and signals.
-template <int D>
-__device__ __forceinline__ void warp_load_tile(uint8_t* dst, const bf16* src, long long row_stride, int rows, int valid, int lane) {
-    constexpr int CH = D / 8;
-#pragma unroll 8
-    for (int i = lane; i < rows * CH; i += 32) {
-        const int r = i / CH, ch = i % CH;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < valid) v = *reinterpret_cast<const uint4*>(src + r * row_stride + ch * 8);
-        st_shared_v4(dst + (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
-    }
-}
 // zeros into `rows` rows of D bf16; all `threads` threads of the block take part
 template <int D>
 __device__ __forceinline__ void block_zero_rows(bf16* dst, long long row_stride, int rows, int tid, int threads) {

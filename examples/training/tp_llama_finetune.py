@@ -129,7 +129,10 @@ def main():
     ap.add_argument("--lora_rank", type=int, default=16)
     ap.add_argument("--lora_alpha", type=int, default=32)
     ap.add_argument("--lora_dropout", type=float, default=0.05)
+    ap.add_argument("--counter_dropout", type=int, default=0, help="LoRA dropout that stores no mask")
     ap.add_argument("--lora_target_modules", default="qkv_proj,o_proj")
+    ap.add_argument("--pack", type=int, default=0,
+                    help="samples end to end in rows of batch_size * seq_len tokens, without padding")
     ap.add_argument("--do_eval", type=int, default=0)
     ap.add_argument("--eval_max_new_tokens", type=int, default=32)
     ap.add_argument("--golden_rouge_score_path", default=None)
@@ -138,7 +141,8 @@ def main():
     device = C.init_process_group()
     sp = bool(args.use_sequence_parallel) and args.tensor_parallel_size > 1
     lora = LoraConfig(enable_lora=True, lora_rank=args.lora_rank, lora_alpha=args.lora_alpha,
-                      lora_dropout=args.lora_dropout, target_modules=args.lora_target_modules.split(","),
+                      lora_dropout=args.lora_dropout, counter_dropout=bool(args.counter_dropout),
+                      target_modules=args.lora_target_modules.split(","),
                       lora_verbose=True, save_lora_base=False, merge_lora=False) if args.enable_lora else None
     nxd_config = nxd.neuronx_distributed_config(
         tensor_parallel_size=args.tensor_parallel_size, sequence_parallel=sp,
@@ -153,8 +157,9 @@ def main():
     model = nxd.initialize_parallel_model(nxd_config, lambda: LlamaForCausalLM(cfg, device=device), device=device)
     dp, dp_rank = C.dp_coords()
     train_dl, eval_dl = create_instruction_based_dataset(args.data_dir, args.batch_size, dp, dp_rank, args.seed,
-                                                         tokenizer=load_tokenizer(args.tokenizer), seq_len=args.seq_len)
-    batches = ({"input_ids": b["input_ids"], "labels": b["labels"]} for b in DevicePrefetcher(train_dl, device))
+                                                         tokenizer=load_tokenizer(args.tokenizer), seq_len=args.seq_len,
+                                                         pack=bool(args.pack))
+    batches = ({k: b[k] for k in ("input_ids", "labels", "cu_seqlens") if k in b} for b in DevicePrefetcher(train_dl, device))
     eval_batches = list(DevicePrefetcher(eval_dl, device, loop=False)) if (args.do_eval and eval_dl is not None) else None
 
     C.fit(args, nxd_config, model, batches, teardown=False)

@@ -157,7 +157,8 @@ int nxd_flash_attn_bwd_tc(const void* q, const void* k, const void* v, const voi
 /* ---- attention over packed sequences (rows cu[s] .. cu[s + 1] of a row of T tokens each attend to themselves) ------------
  * nxd_packed_plan makes the tile list from the boundaries on the device (int32, or int64 with `wide`): room for
  * nxd_packed_plan_entries tiles of 16 bytes, `seqs` 16 bytes per sequence; nxd_packed_plan_columns is the row length of
- * the per-row scratch.  Tiles have 128 rows, but 256 for the forward call where Hq / Hkv is odd.  strides = {head, row} in elements: {q, k, v, o} forward, {q, k, v, o, dout, dq, dk, dv} backward, multiples of 8.
+ * the per-row scratch.  Tiles have 128 rows, but 256 for the forward call where Hq / Hkv is odd.  strides = {head, row} in
+ * elements: {q, k, v, o} forward, {q, k, v, o, dout, dq, dk, dv} backward, multiples of 8.
  * lse [Hq, columns] (NULL: not wanted), delta the same; dq_accum [Hq, D, columns] of scratch; dkv_accum: NULL, or ZEROED
  * [2, Hkv, T, D] where nxd_packed_attn_bwd_splits is above 1.  Rows outside every sequence come out as zeros. */
 int nxd_packed_plan_entries(long long T, int N, int rows);
@@ -171,6 +172,24 @@ int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void*
                         float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
                         const long long* strides, const void* tiles, int entries, long long columns, long long T, int N,
                         int Hq, int Hkv, int D, float scale, int causal, void* stream);
+
+/* ---- dropout: y = keep(i) ? x / (1 - p) : 0, plus residual (NULL: none); 0 < p < 1 ---------------------------------------
+ * keep(i): word i % 4 of Philox4x32-7 at counter (i / 4, offset) under key seed >= p 2^32.  dtype 0 fp32, 1 bf16, 2 fp16.
+ * state: NULL, or state_len (1 or 2) int64 on the device that replace the seed and add to the offset; used: NULL, or where
+ * the two numbers that the call drew with go, for the backward call. */
+int nxd_dropout(const void* x, const void* residual, void* y, long long n, int dtype, double p, unsigned long long seed,
+                unsigned long long offset, const long long* state, int state_len, long long* used, void* stream);
+
+/* ---- load-balancing loss of several layers' router logits: E / k sum_e share_e mean_prob_e, and its gradient -------------
+ * x, ld, rows: HOST arrays of `layers` device pointers, row strides (elements, unit stride along the experts) and row counts;
+ * dtype 0 fp32, 1 bf16, 2 fp16; mask: NULL, or a byte per row that all layers share.  counts: E int64 choices; share: E floats
+ * for the backward call; scratch: nxd_balance_loss_num_blocks * E * 8 bytes; grad: 1 float; dx: the layers' rows end to end. */
+int nxd_balance_loss_num_blocks(long long most_rows, int layers, int E);
+int nxd_balance_loss_fwd(const void* const* x, const long long* ld, const long long* rows, int layers, int dtype,
+                         const void* mask, int E, int k, float* loss, long long* counts, float* share, void* scratch,
+                         void* stream);
+int nxd_balance_loss_bwd(const void* const* x, const long long* ld, const long long* rows, int layers, int dtype,
+                         const void* mask, int E, int k, const float* share, const float* grad, void* dx, void* stream);
 
 /* ---- symmetric (peer-mapped) memory over CUDA IPC + fused compute/collective kernels ---------------------------
  * No counterpart in the reference (its collectives are XLA ops).  One process per GPU: every rank allocates a

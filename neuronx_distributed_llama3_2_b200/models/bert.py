@@ -12,19 +12,21 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops import attention as attn_ops
+from ..ops.dropout import Dropout
+from ..ops.packed_attention import PackedSequences
 from ..parallel import mappings
 from ..parallel import parallel_state as ps
 from ..parallel.layer_norm import LayerNorm
 from ..parallel.layers import ColumnParallelLinear, ParallelEmbedding, RowParallelLinear
 from ..parallel.loss_functions import parallel_cross_entropy
-from .llama import _init_fn
+from .llama import _init_fn, packed_row
 
 
 @dataclass
@@ -38,6 +40,7 @@ class BertConfig:
     type_vocab_size: int = 2
     layer_norm_eps: float = 1e-12
     initializer_range: float = 0.02
+    hidden_dropout_prob: float = 0.0        # on both residual branches of a layer and on the embeddings
     sequence_parallel_enabled: bool = False
     activation_checkpointing: bool = False
     torch_dtype: torch.dtype = torch.bfloat16
@@ -63,6 +66,11 @@ def _tag_sp(module: nn.Module, enabled: bool) -> None:
         setattr(p, "sequence_parallel_enabled", enabled)
 
 
+def _hidden_dropout(config: BertConfig) -> Dropout:
+    """Dropout of hidden states, with the residual added in the same pass; sequence shards draw different masks."""
+    return Dropout(config.hidden_dropout_prob, offset=ps.get_tensor_model_parallel_rank() if config.sequence_parallel_enabled else 0)
+
+
 class BertEmbeddings(nn.Module):
     def __init__(self, config: BertConfig, device=None):
         super().__init__()
@@ -75,24 +83,29 @@ class BertEmbeddings(nn.Module):
         self.token_type_embeddings = nn.Embedding(config.type_vocab_size, config.hidden_size, dtype=dt, device=device)
         self.LayerNorm = LayerNorm(config.hidden_size, eps=config.layer_norm_eps, sequence_parallel_enabled=sp, dtype=dt,
                                    device=device)
+        self.dropout = _hidden_dropout(config)
         # no sequence-parallel tag on these two: the scatter below all-gathers their gradient in its backward, so every
         # rank already holds the complete gradient
         for emb in (self.position_embeddings, self.token_type_embeddings):
             nn.init.normal_(emb.weight, std=config.initializer_range)
 
-    def forward(self, input_ids: torch.Tensor, token_type_ids: Optional[torch.Tensor]) -> torch.Tensor:
+    def forward(self, input_ids: torch.Tensor, token_type_ids: Optional[torch.Tensor],
+                packed: Optional[PackedSequences] = None) -> torch.Tensor:
         B, S = input_ids.shape
         tp = ps.get_tensor_model_parallel_size()
         words = self.word_embeddings(input_ids)                              # [S/tp, B, H] (or [S, B, H] at tp = 1)
         if token_type_ids is None:
             token_type_ids = torch.zeros_like(input_ids)
-        pos = torch.arange(S, device=input_ids.device)
+        if packed is None:
+            pos = torch.arange(S, device=input_ids.device)
+        else:               # (a sequence is no longer than the table; the bound keeps a wrong one from reading behind it)
+            pos = packed.positions().clamp(max=self.position_embeddings.num_embeddings - 1)
         extra = self.position_embeddings(pos)[:, None, :] + self.token_type_embeddings(token_type_ids.t())   # [S, B, H]
         if tp > 1 and self.sp:
             extra = mappings.scatter_to_sequence_parallel_region(extra)
         elif tp > 1:
             words = mappings.gather_from_sequence_parallel_region(words, to_model_parallel=False)
-        return self.LayerNorm(words + extra)
+        return self.dropout(self.LayerNorm(words + extra))
 
 
 class BertSelfAttention(nn.Module):
@@ -110,10 +123,15 @@ class BertSelfAttention(nn.Module):
         self.dense = RowParallelLinear(config.hidden_size, config.hidden_size, bias=True, input_is_parallel=True,
                                        init_method=init, sequence_parallel_enabled=sp, dtype=dt, device=device)
 
-    def forward(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor]) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor],
+                packed: Optional[PackedSequences] = None) -> torch.Tensor:
         h, D = self.heads_local, self.config.head_dim
         qkv = self.query_key_value(x)
         S, B = qkv.shape[0], qkv.shape[1]
+        if packed is not None:              # one row of sentences end to end: each attends to all of itself
+            qkv = qkv.reshape(S, h, 3, D)
+            o = attn_ops.flash_attn_packed_func(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], packed, causal=False)
+            return self.dense(o.reshape(S, B, h * D))
         qkv = qkv.reshape(S, B, h, 3, D)
         q, k, v = (qkv[:, :, :, i].permute(1, 2, 0, 3) for i in range(3))   # [B, h, S, D] views
         if key_padding_mask is None:
@@ -139,16 +157,22 @@ class BertLayer(nn.Module):
                                         init_method=init, sequence_parallel_enabled=sp, dtype=dt, device=device)
         self.output_layernorm = LayerNorm(config.hidden_size, eps=config.layer_norm_eps, sequence_parallel_enabled=sp,
                                           dtype=dt, device=device)
+        self.dropout = _hidden_dropout(config)
 
-    def forward(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor]) -> torch.Tensor:
-        x = self.attention_layernorm(x + self.attention(x, key_padding_mask))
-        return self.output_layernorm(x + self.output(F.gelu(self.intermediate(x))))
+    def forward(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor],
+                packed: Optional[PackedSequences] = None) -> torch.Tensor:
+        x = self.attention_layernorm(self.dropout(self.attention(x, key_padding_mask, packed), x))
+        return self.output_layernorm(self.dropout(self.output(F.gelu(self.intermediate(x))), x))
 
 
 class BertForPreTraining(nn.Module):
     """``forward(input_ids [B, S], token_type_ids, attention_mask, labels [B, S] (-100 = not masked),
     next_sentence_label [B])`` -> ``mlm_loss + nsp_loss``; without labels ``(vocab-parallel logits [S, B, V/tp],
-    nsp logits [B, 2])``."""
+    nsp logits [B, 2])``.
+
+    ``cu_seqlens [N + 1]`` with ``input_ids [1, S]``: the row holds N sentences (pairs) end to end instead of padded ones; each
+    attends to itself, its positions start at 0, and its first token is its CLS (``next_sentence_label [N]``, ``nsp logits
+    [N, 2]``).  No sentence is empty or longer than ``max_position_embeddings``; columns outside of them carry label -100."""
 
     def __init__(self, config: BertConfig, device=None):
         super().__init__()
@@ -174,8 +198,13 @@ class BertForPreTraining(nn.Module):
             nn.init.zeros_(lin.bias)
         _tag_sp(self.transform, sp)
 
-    def _cls_token(self, hidden: torch.Tensor) -> torch.Tensor:
-        """Hidden state of position 0 on every rank (with sequence parallelism only TP rank 0 holds it)."""
+    def _cls_token(self, hidden: torch.Tensor, packed: Optional[PackedSequences] = None) -> torch.Tensor:
+        """Hidden state of position 0 on every rank (with sequence parallelism only TP rank 0 holds it); ``packed``: of every
+        sequence's first token."""
+        if packed is not None:
+            if self.config.sequence_parallel_enabled and ps.get_tensor_model_parallel_size() > 1:
+                hidden = mappings.gather_from_sequence_parallel_region(hidden, to_model_parallel=False)
+            return hidden[packed.first_tokens(), 0]
         if not (self.config.sequence_parallel_enabled and ps.get_tensor_model_parallel_size() > 1):
             return hidden[0]
         mine = hidden[0] if ps.get_tensor_model_parallel_rank() == 0 else torch.zeros_like(hidden[0])
@@ -183,22 +212,26 @@ class BertForPreTraining(nn.Module):
 
     def forward(self, input_ids: torch.Tensor, token_type_ids: Optional[torch.Tensor] = None,
                 attention_mask: Optional[torch.Tensor] = None, labels: Optional[torch.Tensor] = None,
-                next_sentence_label: Optional[torch.Tensor] = None):
+                next_sentence_label: Optional[torch.Tensor] = None,
+                cu_seqlens: Optional[Union[torch.Tensor, PackedSequences]] = None):
         from torch.utils.checkpoint import checkpoint
 
         cfg = self.config
+        extra = () if cu_seqlens is None else (packed_row(input_ids, cu_seqlens),)
+        if extra and attention_mask is not None:
+            raise ValueError("packed sentences have no padding mask")
         if (attention_mask is not None and not isinstance(attention_mask, torch.fx.Proxy)
                 and bool(attention_mask.all())):       # nothing is padded: take the flash-attention path
             attention_mask = None
-        hidden = self.embeddings(input_ids, token_type_ids)
+        hidden = self.embeddings(input_ids, token_type_ids, *extra)
         for layer in self.layers:
             if cfg.activation_checkpointing and self.training and torch.is_grad_enabled():
-                hidden = checkpoint(layer, hidden, attention_mask, use_reentrant=False)
+                hidden = checkpoint(layer, hidden, attention_mask, *extra, use_reentrant=False)
             else:
-                hidden = layer(hidden, attention_mask)
+                hidden = layer(hidden, attention_mask, *extra)
         mlm = self.transform_layernorm(F.gelu(self.transform(hidden)))
         logits = self.decoder(mlm) + self.decoder_bias                    # [S, B, V/tp]
-        nsp_logits = self.seq_relationship(torch.tanh(self.pooler(self._cls_token(hidden))))
+        nsp_logits = self.seq_relationship(torch.tanh(self.pooler(self._cls_token(hidden, *extra))))
         if labels is None:
             return logits, nsp_logits
         per_token = parallel_cross_entropy(logits, labels.t().contiguous())          # [S, B]

@@ -77,11 +77,11 @@ class DbrxDecoderLayer(MixtralDecoderLayer):
         if config.clip_qkv:
             self.self_attn.qkv_proj.register_forward_hook(_clip_hook(float(config.clip_qkv)))
 
-    def forward(self, hidden, residual, cos, sin):
+    def forward(self, hidden, residual, cos, sin, packed=None):
         if residual is not None:
             hidden = hidden + residual
         residual = hidden
-        a = self.self_attn(self.input_layernorm(hidden), cos, sin)
+        a = self.self_attn(self.input_layernorm(hidden), cos, sin, packed)
         residual = residual + a
         h = self.post_attention_layernorm(residual)
         if self.is_moe:

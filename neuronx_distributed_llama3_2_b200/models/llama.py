@@ -21,9 +21,10 @@ B200 design notes
 from __future__ import annotations
 
 from dataclasses import asdict, dataclass, field
-from typing import Any, Dict, Optional, Tuple
+from typing import Any, Dict, Optional, Tuple, Union
 
 import torch
+import torch.fx
 import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
@@ -32,6 +33,7 @@ from ..ops import activation as act_ops
 from ..ops import attention as attn_ops
 from ..ops import norm as norm_ops
 from ..ops import rope as rope_ops
+from ..ops.packed_attention import PackedSequences, as_packed
 from ..parallel import mappings
 from ..parallel import parallel_state as ps
 from ..parallel.layer_norm import RMSNorm
@@ -184,6 +186,15 @@ def config_from_hf_json(path_or_dict, **overrides) -> LlamaConfig:
     return config_from_json(LlamaConfig, path_or_dict, **overrides)
 
 
+def packed_row(input_ids: torch.Tensor, cu_seqlens: Union[torch.Tensor, PackedSequences]) -> PackedSequences:
+    """The samples of a step whose ``input_ids [1, S]`` hold them end to end: one object for all its layers."""
+    if isinstance(cu_seqlens, torch.fx.Proxy):
+        raise NotImplementedError("packed samples under pipeline tracing")
+    if input_ids.dim() != 2 or input_ids.shape[0] != 1:
+        raise ValueError(f"packed samples lie in one row [1, S], not {tuple(input_ids.shape)}")
+    return as_packed(cu_seqlens, input_ids.shape[1], input_ids.device)
+
+
 def _init_fn(std: float):
     def f(w):
         return nn.init.normal_(w, mean=0.0, std=std)
@@ -273,13 +284,17 @@ class LlamaAttention(nn.Module):
         if o is not None:
             model_state_dict[base + "o_proj.weight"] = o[:, rows.to(o.device)]
 
-    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                packed: Optional[PackedSequences] = None) -> torch.Tensor:
         nq, nkv, D = self.q_heads_local, self.kv_heads_local, self.head_dim
         if self.config.fuse_qkv:
             qkv = self.qkv_proj(x, return_fused=True)            # [S, B, (nq + 2 nkv) * D]
         else:
             qkv = torch.cat(self.qkv_proj(x), dim=-1)
         S, B = qkv.shape[0], qkv.shape[1]
+        if packed is not None:      # one row of samples end to end: positions start again and attention stays inside each
+            o = attn_ops.rope_flash_attn_packed_func(qkv.reshape(S, nq + 2 * nkv, D), cos, sin, nq, nkv, packed)
+            return self.o_proj(o.reshape(S, B, nq * D))
         # q and k heads are rotated in one pass (token s sits at position s); [B, nq, S, D] stored as [S, B, nq, D]
         o = attn_ops.rope_flash_attn_func(qkv.reshape(S, B, nq + 2 * nkv, D), cos, sin, nq, nkv)
         o = o.permute(2, 0, 1, 3).reshape(S, B, nq * D)
@@ -298,7 +313,7 @@ class LlamaDecoderLayer(nn.Module):
                                                 sequence_parallel_enabled=sp, dtype=dt, device=device)
 
     def forward(self, hidden: torch.Tensor, residual: Optional[torch.Tensor], cos: torch.Tensor,
-                sin: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+                sin: torch.Tensor, packed: Optional[PackedSequences] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """``hidden`` is the previous block's un-added output, ``residual`` the stream it must be added to."""
         eps = self.input_layernorm.variance_epsilon
         if residual is None:
@@ -306,7 +321,7 @@ class LlamaDecoderLayer(nn.Module):
             h = norm_ops.rms_norm(hidden, self.input_layernorm.weight, eps)
         else:
             h, residual = norm_ops.fused_add_rms_norm(hidden, residual, self.input_layernorm.weight, eps)
-        a = self.self_attn(h, cos, sin)
+        a = self.self_attn(h, cos, sin, packed)
         h, residual = norm_ops.fused_add_rms_norm(a, residual, self.post_attention_layernorm.weight, eps)
         return self.mlp(h), residual
 
@@ -336,10 +351,12 @@ class CausalLMLoss(nn.Module):
 
     _nxd_fx_leaf = True
 
-    def forward(self, logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+    def forward(self, logits: torch.Tensor, labels: torch.Tensor, packed: Optional[PackedSequences] = None) -> torch.Tensor:
         B, S = labels.shape
         shifted = torch.full((S, B), -100, dtype=torch.long, device=labels.device)
         shifted[:-1] = labels[:, 1:].t()
+        if packed is not None:                          # the next token of a sample's last one belongs to another sample
+            shifted.masked_fill_(packed.last_tokens().unsqueeze(1), -100)
         per_token = parallel_cross_entropy(logits, shifted)        # [S, B] fp32
         valid = shifted >= 0
         return (per_token * valid).sum() / valid.sum().clamp(min=1)
@@ -359,7 +376,7 @@ class LlamaModel(nn.Module):
                             sequence_parallel_enabled=config.sequence_parallel_enabled, dtype=dt, device=device)
         self.rotary = RotaryTables(config)
 
-    def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def forward(self, input_ids: torch.Tensor, packed: Optional[PackedSequences] = None) -> torch.Tensor:
         """``input_ids [B, S]`` -> final normed hidden states ``[S(/tp), B, H]``."""
         cfg = self.config
         hidden = self.embed_tokens(input_ids)  # [S/tp, B, H] (reduce-scatter) -- SP region entered here
@@ -367,18 +384,24 @@ class LlamaModel(nn.Module):
             hidden = mappings.gather_from_sequence_parallel_region(hidden, to_model_parallel=False)
         cos_sin = self.rotary(input_ids)
         cos, sin = cos_sin[0], cos_sin[1]
+        extra = () if packed is None else (packed,)
         residual = None
         for layer in self.layers:
             if cfg.activation_checkpointing and self.training and torch.is_grad_enabled():
-                hidden, residual = checkpoint(layer, hidden, residual, cos, sin, use_reentrant=False)
+                hidden, residual = checkpoint(layer, hidden, residual, cos, sin, *extra, use_reentrant=False)
             else:
-                hidden, residual = layer(hidden, residual, cos, sin)
+                hidden, residual = layer(hidden, residual, cos, sin, *extra)
         return self.norm(hidden, residual)   # fused (hidden + residual) -> RMSNorm
 
 
 class LlamaForCausalLM(nn.Module):
     """``forward(input_ids, labels)`` returns the mean next-token loss (labels are shifted inside,
-    reference ``modeling_llama_nxd.py:733-747``); without labels returns vocab-parallel logits."""
+    reference ``modeling_llama_nxd.py:733-747``); without labels returns vocab-parallel logits.
+
+    ``cu_seqlens [N + 1]`` (int32 or int64, or a ``PackedSequences``) with ``input_ids [1, S]``: the row holds samples end to
+    end, sample ``s`` in columns ``cu_seqlens[s] .. cu_seqlens[s + 1]``.  Each attends to itself alone, its positions start at 0,
+    and no sample's last token predicts the next sample's first; columns outside of them (padding) enter neither attention nor
+    the loss."""
 
     def __init__(self, config: LlamaConfig, device=None):
         super().__init__()
@@ -403,12 +426,14 @@ class LlamaForCausalLM(nn.Module):
         return self.lm_head
 
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
-                attention_mask: Optional[torch.Tensor] = None):
-        hidden = self.model(input_ids)                 # [S/tp, B, H]
+                attention_mask: Optional[torch.Tensor] = None,
+                cu_seqlens: Optional[Union[torch.Tensor, PackedSequences]] = None):
+        extra = () if cu_seqlens is None else (packed_row(input_ids, cu_seqlens),)
+        hidden = self.model(input_ids, *extra)         # [S/tp, B, H]
         logits = self.lm_head(hidden)                  # [S, B, V/tp]  (AG->GEMM under SP)
         if labels is None:
             return logits
-        return self.loss_fn(logits, labels)
+        return self.loss_fn(logits, labels, *extra)
 
 
 def flops_per_token(cfg: LlamaConfig, seq_len: int) -> float:

@@ -5,7 +5,7 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import torch
 import torch.nn as nn
@@ -13,9 +13,10 @@ from torch.utils.checkpoint import checkpoint
 
 from ..modules.moe import ExpertMLPs, MoE, RouterTopK, load_balancing_loss_func
 from ..ops import norm as norm_ops
+from ..ops.packed_attention import PackedSequences
 from ..parallel.layer_norm import RMSNorm
 from ..parallel.layers import ColumnParallelLinear, ParallelEmbedding
-from .llama import CausalLMLoss, LlamaAttention, LlamaConfig, LlamaMLP, RotaryTables, _init_fn
+from .llama import CausalLMLoss, LlamaAttention, LlamaConfig, LlamaMLP, RotaryTables, _init_fn, packed_row
 
 
 @dataclass
@@ -68,14 +69,14 @@ class MixtralDecoderLayer(nn.Module):
         self.post_attention_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, sequence_parallel_enabled=sp,
                                                 dtype=dt, device=device)
 
-    def forward(self, hidden, residual, cos, sin):
+    def forward(self, hidden, residual, cos, sin, packed=None):
         eps = self.input_layernorm.variance_epsilon
         if residual is None:
             residual = hidden
             h = norm_ops.rms_norm(hidden, self.input_layernorm.weight, eps)
         else:
             h, residual = norm_ops.fused_add_rms_norm(hidden, residual, self.input_layernorm.weight, eps)
-        a = self.self_attn(h, cos, sin)
+        a = self.self_attn(h, cos, sin, packed)
         h, residual = norm_ops.fused_add_rms_norm(a, residual, self.post_attention_layernorm.weight, eps)
         if self.is_moe:
             out, router_logits = self.mlp(h)
@@ -85,7 +86,8 @@ class MixtralDecoderLayer(nn.Module):
 
 
 class MixtralForCausalLM(nn.Module):
-    """``forward(input_ids, labels)`` -> ``lm_loss + router_aux_loss_coef * load_balancing_loss``."""
+    """``forward(input_ids, labels)`` -> ``lm_loss + router_aux_loss_coef * load_balancing_loss``.  ``cu_seqlens``: samples end to
+    end in one row, as in ``LlamaForCausalLM``; columns outside of them do not count in the balancing loss either."""
 
     _fx_wrap_functions = [load_balancing_loss_func]       # kept opaque by the pipeline tracer (pipeline/trace.py)
 
@@ -107,7 +109,8 @@ class MixtralForCausalLM(nn.Module):
                                             device=device)
         self.loss_fn = CausalLMLoss()
 
-    def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None):
+    def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
+                cu_seqlens: Optional[Union[torch.Tensor, PackedSequences]] = None):
         from ..parallel import mappings
         from ..parallel import parallel_state as ps
 
@@ -116,24 +119,26 @@ class MixtralForCausalLM(nn.Module):
         if not cfg.sequence_parallel_enabled and ps.get_tensor_model_parallel_size() > 1:
             hidden = mappings.gather_from_sequence_parallel_region(hidden, to_model_parallel=False)
         cos, sin = self.rotary(input_ids)
+        extra = () if cu_seqlens is None else (packed_row(input_ids, cu_seqlens),)
         residual = None
         all_router_logits: List[torch.Tensor] = []
         for layer in self.layers:
             if cfg.activation_checkpointing and self.training and torch.is_grad_enabled():
-                hidden, residual, rl = checkpoint(layer, hidden, residual, cos, sin, use_reentrant=False)
+                hidden, residual, rl = checkpoint(layer, hidden, residual, cos, sin, *extra, use_reentrant=False)
             else:
-                hidden, residual, rl = layer(hidden, residual, cos, sin)
+                hidden, residual, rl = layer(hidden, residual, cos, sin, *extra)
             if rl is not None:
                 all_router_logits.append(rl)
         hidden = self.norm(hidden, residual)
         logits = self.lm_head(hidden)
         if labels is None:
             return logits
-        loss = self.loss_fn(logits, labels)
+        loss = self.loss_fn(logits, labels, *extra)
         if cfg.output_router_logits and all_router_logits:
             # the list goes in as is: under pipeline tracing the call is one opaque node (``_fx_wrap_functions``) whose
             # inputs are the per-layer router logits carried from their stages to the last one
-            aux = load_balancing_loss_func(all_router_logits, cfg.num_local_experts, cfg.num_experts_per_tok)
+            aux = load_balancing_loss_func(all_router_logits, cfg.num_local_experts, cfg.num_experts_per_tok,
+                                           *(x.inside() for x in extra))
             loss = loss + cfg.router_aux_loss_coef * aux
         return loss
 

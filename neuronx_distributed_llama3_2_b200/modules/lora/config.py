@@ -12,6 +12,7 @@ class LoraConfig:
     target_modules: Optional[List[str]] = None          # module-name suffixes or a regex; None -> per-arch default
     lora_alpha: int = 8
     lora_dropout: float = 0.0
+    counter_dropout: bool = False                        # the mask from ``ops.dropout``'s counter-based generator, not stored
     bias: Literal["none", "all", "lora_only"] = "none"
     use_rslora: bool = False                             # scale = alpha / sqrt(r) instead of alpha / r
     init_lora_weights: Literal["default", "gaussian"] = "default"

@@ -12,20 +12,25 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ...ops.dropout import Dropout
+
 
 class LoraLayer:
     """Mixin with the adapter bookkeeping shared by every wrapped layer type."""
 
     adapter_layer_names = ("lora_A", "lora_B", "lora_embedding_A", "lora_embedding_B")
 
-    def init_lora(self, base_layer: nn.Module, lora_config) -> None:
+    def init_lora(self, base_layer: nn.Module, lora_config, dropout_offset: int = 0) -> None:
         self.base_layer = base_layer
         self.lora_config = lora_config
         self.lora_rank = lora_config.lora_rank
         self.lora_alpha = lora_config.lora_alpha
         self.scaling = (self.lora_alpha / math.sqrt(self.lora_rank)) if lora_config.use_rslora \
             else (self.lora_alpha / self.lora_rank)
-        self.lora_dropout = nn.Dropout(p=lora_config.lora_dropout) if lora_config.lora_dropout > 0.0 else nn.Identity()
+        if lora_config.lora_dropout > 0.0 and getattr(lora_config, "counter_dropout", False):
+            self.lora_dropout = Dropout(lora_config.lora_dropout, offset=dropout_offset)
+        else:
+            self.lora_dropout = nn.Dropout(p=lora_config.lora_dropout) if lora_config.lora_dropout > 0.0 else nn.Identity()
         self.merged = False
 
     def get_base_layer(self) -> nn.Module:

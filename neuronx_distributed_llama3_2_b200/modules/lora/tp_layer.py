@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from ...parallel import parallel_state as ps
 from ...parallel.layers import ColumnParallelLinear, RowParallelLinear
 from ..qkv_linear import GQAQKVColumnParallelLinear
 from .layer import LoraLayer
@@ -18,10 +19,12 @@ from .layer import LoraLayer
 class LoraParallelLinear(nn.Module, LoraLayer):
     def __init__(self, base_layer, lora_config):
         super().__init__()
-        self.init_lora(base_layer, lora_config)
+        self.is_row = isinstance(base_layer, RowParallelLinear)
+        split = base_layer.input_is_parallel if self.is_row else base_layer.sequence_parallel_enabled
+        # a rank that holds a part of the input draws another mask than its neighbours, one that holds all of it the same
+        self.init_lora(base_layer, lora_config, ps.get_tensor_model_parallel_rank() if split else 0)
         dt = base_layer.weight.dtype
         dev = base_layer.weight.device
-        self.is_row = isinstance(base_layer, RowParallelLinear)
         if self.is_row:
             self.lora_A = RowParallelLinear(base_layer.input_size, self.lora_rank, bias=False,
                                             input_is_parallel=base_layer.input_is_parallel,
@@ -68,7 +71,7 @@ class LoraParallelLinear(nn.Module, LoraLayer):
 class LoraGQAQKVParallelLinear(nn.Module, LoraLayer):
     def __init__(self, base_layer: GQAQKVColumnParallelLinear, lora_config):
         super().__init__()
-        self.init_lora(base_layer, lora_config)
+        self.init_lora(base_layer, lora_config, ps.get_tensor_model_parallel_rank() if base_layer.sequence_parallel_enabled else 0)
         w = base_layer.weight_qkv if base_layer.fuse_qkv else base_layer.weight_q
         dt, dev = w.dtype, w.device
         q_out, kv_out = base_layer.output_sizes

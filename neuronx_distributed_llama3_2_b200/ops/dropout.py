@@ -117,6 +117,8 @@ class Dropout(torch.nn.Module):
     """``torch.nn.Dropout`` on this generator: every training call draws its seed from torch's CPU generator; ``offset`` tells
     apart what ranks with one generator state hold (the tensor-parallel rank where activations are sharded)."""
 
+    _nxd_fx_leaf = True             # one node of a pipeline's graph
+
     def __init__(self, p: float = 0.5, offset: int = 0):
         super().__init__()
         if not 0.0 <= p <= 1.0:

@@ -69,6 +69,10 @@ class PackedSequences:
             self._positions = pos.to(torch.int32)
         return self._positions
 
+    def first_tokens(self) -> torch.Tensor:
+        """int64 ``[N]``: the row of every sequence's first token."""
+        return self.cu_seqlens[:-1].long().clamp(0, self.total - 1).cummax(0).values
+
     def last_tokens(self) -> torch.Tensor:
         """bool ``[total]``: the last token of a sequence (it has no next token to predict), and every row outside of them."""
         cu = self.cu_seqlens.long().clamp(0, self.total).cummax(0).values

@@ -97,9 +97,10 @@ def open_token_dataset(data_dir: str, seq_len: Optional[int] = None) -> Dataset:
     return TokenFileDataset(data_dir, seq_len)
 
 
-def _loader(ds: Dataset, mini_batch_size: int, dp_size: int, dp_rank: int, seed: int, shuffle: bool) -> DataLoader:
+def _loader(ds: Dataset, mini_batch_size: int, dp_size: int, dp_rank: int, seed: int, shuffle: bool,
+            collate: Callable = _collate) -> DataLoader:
     sampler = DistributedSampler(ds, num_replicas=dp_size, rank=dp_rank, shuffle=shuffle, seed=seed, drop_last=True)
-    return DataLoader(ds, batch_size=mini_batch_size, sampler=sampler, collate_fn=_collate, num_workers=0, drop_last=True,
+    return DataLoader(ds, batch_size=mini_batch_size, sampler=sampler, collate_fn=collate, num_workers=0, drop_last=True,
                       pin_memory=torch.cuda.is_available())
 
 
@@ -143,11 +144,52 @@ class InstructionDataset(Dataset):
         return self.rows[i]
 
 
+class PackedSamples(Dataset):
+    """The samples of a dataset without their padding, laid end to end in rows of ``row_len`` tokens: each row takes the next
+    samples that still fit, and ``cu_seqlens`` (int32) says where they begin.  What is left of a row is padding outside of
+    every sequence.  With ``shuffle`` the samples are first permuted by ``seed``, the same way on every rank."""
+
+    def __init__(self, samples: Dataset, row_len: int, pad_token_id: int = 0, shuffle: bool = False, seed: int = 0):
+        order = torch.randperm(len(samples), generator=torch.Generator().manual_seed(seed)).tolist() if shuffle else range(len(samples))
+        self.samples, self.row_len, self.pad_token_id = samples, row_len, pad_token_id
+        self.rows: List[List[int]] = []
+        room = 0
+        for i in order:
+            n = int(samples[i]["attention_mask"].sum())
+            if n > row_len:
+                raise ValueError(f"sample {i} has {n} tokens, a row {row_len}")
+            if not self.rows or n > room:
+                self.rows.append([])
+                room = row_len
+            self.rows[-1].append(i)
+            room -= n
+
+    def __len__(self) -> int:
+        return len(self.rows)
+
+    def __getitem__(self, i: int) -> Dict[str, torch.Tensor]:
+        ids = torch.full((self.row_len,), self.pad_token_id, dtype=torch.long)
+        labels = torch.full((self.row_len,), IGNORE_INDEX, dtype=torch.long)
+        ends = [0]
+        for j in self.rows[i]:
+            s = self.samples[j]
+            n = int(s["attention_mask"].sum())
+            ids[ends[-1]:ends[-1] + n], labels[ends[-1]:ends[-1] + n] = s["input_ids"][:n], s["labels"][:n]
+            ends.append(ends[-1] + n)
+        return {"input_ids": ids, "labels": labels, "cu_seqlens": torch.tensor(ends, dtype=torch.int32)}
+
+
+def _collate_packed(rows: List[Dict[str, torch.Tensor]]) -> Dict[str, torch.Tensor]:
+    (row,) = rows
+    return {k: v if k == "cu_seqlens" else v.unsqueeze(0) for k, v in row.items()}
+
+
 def create_instruction_based_dataset(data_dir: str, mini_batch_size: int, dp_size: int, dp_rank: int, seed: int,
-                                     tokenizer=None, task=None, seq_len: int = 2048):
+                                     tokenizer=None, task=None, seq_len: int = 2048, pack: bool = False):
     """``(train_dataloader, eval_dataloader)`` from ``train.jsonl`` / ``eval.jsonl`` (or one ``*.jsonl``/``*.json``,
     split 95/5) with ``instruction`` / ``input`` / ``output`` fields.  ``tokenizer`` is an HF tokenizer or any callable
-    ``str -> list[int]``."""
+    ``str -> list[int]``.  ``pack``: a training batch is one row ``[1, mini_batch_size * seq_len]`` of samples end to end with
+    their ``cu_seqlens`` instead of ``mini_batch_size`` padded rows."""
     def read(path):
         with open(path) as f:
             txt = f.read().strip()
@@ -168,7 +210,11 @@ def create_instruction_based_dataset(data_dir: str, mini_batch_size: int, dp_siz
     else:
         tok, pad, eos = tokenizer, 0, None
     make = lambda rows: InstructionDataset(rows, tok, seq_len, pad, eos)  # noqa: E731
-    train_dl = _loader(make(train), mini_batch_size, dp_size, dp_rank, seed, shuffle=True)
+    if pack:
+        rows = PackedSamples(make(train), mini_batch_size * seq_len, pad, shuffle=True, seed=seed)
+        train_dl = _loader(rows, 1, dp_size, dp_rank, seed, shuffle=True, collate=_collate_packed)
+    else:
+        train_dl = _loader(make(train), mini_batch_size, dp_size, dp_rank, seed, shuffle=True)
     eval_dl = _loader(make(ev), mini_batch_size, dp_size, dp_rank, seed, shuffle=False) if len(ev) >= mini_batch_size * dp_size else None
     return train_dl, eval_dl
 
