@@ -37,6 +37,7 @@ constexpr int kStages = 3;            // of Q_i, dO_i, L_i, Delta_i: a tile is a
 struct BwdParams {
     const PackedTile* tiles;
     const float *lse, *delta;
+    int* claimed;                // items that were given out behind everybody's first
     bf16 *dk, *dv;
     long long lse_row, dk_head, dk_row, dv_head, dv_row;
     int entries, Hkv, group, nsplit;          // nsplit: items that share a key block; each walks its part of the (head, query tile) list
@@ -71,8 +72,8 @@ struct alignas(16) Item {
 };
 
 template <bool CAUSAL>
-__device__ __forceinline__ Item fetch_item(const BwdParams& p, int round) {
-    const unsigned at = item_of_round(round), per = (unsigned)(p.Hkv * p.nsplit);
+__device__ __forceinline__ Item fetch_item(const BwdParams& p, unsigned at) {
+    const unsigned per = (unsigned)(p.Hkv * p.nsplit);
     Item it{};
     if (at >= (unsigned)p.entries * per) return it;
     const unsigned e = at / per, r = at - e * per;
@@ -192,10 +193,12 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar);
         };
-        Item ahead = fetch_item<CAUSAL>(p, 0);
-        for (int round = 1;; ++round) {
-            const Item x = ahead;
-            if (x.kind) ahead = fetch_item<CAUSAL>(p, round);          // read while this one is worked on
+        auto claim = [&]() {
+            unsigned at = 0;
+            if (lane == 0) at = (unsigned)atomicAdd(p.claimed, 1);
+            return fetch_item<CAUSAL>(p, gridDim.x + __shfl_sync(0xffffffffu, at, 0));
+        };
+        for (Item x = fetch_item<CAUSAL>(p, blockIdx.x);; x = claim()) {          // the last tiles are still worked on when the next item is asked for
             publish_item(x, item_ring, item_full, item_empty, published, dead);
             if (x.kind == 0) break;
             if (x.kind > 1) continue;
@@ -560,7 +563,7 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 // (nobody reads the padding).  kD / 8 lanes own a row.
 template <int kD>
 __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ dout, const PackedTile* tiles,
-                                                           float* __restrict__ delta, float* __restrict__ acc, long long o_head, long long o_row,
+                                                           float* __restrict__ delta, float* __restrict__ acc, int* claimed, long long o_head, long long o_row,
                                                            long long do_head, long long do_row, long long lse_row, int Hq) {
     pdl_trigger();
     pdl_wait();
@@ -568,6 +571,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
     const PackedTile pt = packed_tile(tiles, blockIdx.x / Hq);
     const int h = blockIdx.x % Hq, l = threadIdx.x % L;
     const int first = pt.t * kBN, rows = min(pt.len - first, kBN);        // negative where the entry is no tile
+    if (blockIdx.x == 0 && threadIdx.x == 0) *claimed = 0;
     if (pt.len == 0) return;
     {
         const int quads = (rows + 3) >> 2;
@@ -690,7 +694,7 @@ NXD_API int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv) {
 }
 
 // Backward of nxd_packed_attn_fwd.  strides: {head, row} in elements of q, k, v, o, dout, dq, dk, dv (16 values, multiples of 8);
-// lse: what the forward pass wrote; delta: Hq * lse_row floats of scratch; dq_accum: [Hq, D, lse_row] floats of scratch;
+// lse: what the forward pass wrote; delta: Hq * lse_row + 4 floats of scratch; dq_accum: [Hq, D, lse_row] floats of scratch;
 // dkv_accum: NULL, or ZEROED [2, Hkv, T, D] floats where nxd_packed_attn_bwd_splits says more than one.
 // dQ (with splits dK and dV too) is summed in fp32 in an order that is not fixed.
 NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
@@ -712,15 +716,16 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
     p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
     p.nsplit = dkv_accum ? nxd_packed_attn_bwd_splits(T, N, Hq, Hkv) : 1;
     p.tiles = pt;
+    p.claimed = (int*)(delta + (long long)Hq * lse_row);
     p.dk = (bf16*)dk; p.dk_head = strides[12]; p.dk_row = strides[13];
     p.dv = (bf16*)dv; p.dv_head = strides[14]; p.dv_row = strides[15];
     const unsigned per_head = (unsigned)entries * Hq;
     if (D == 128)
         NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<128>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const bf16*)dout, pt,
-            delta, dq_accum, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
+            delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
     else
         NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<64>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const bf16*)dout, pt,
-            delta, dq_accum, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
+            delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
     NXD_LAUNCH_CHECK();
     CUtensorMap tq, tdo, tk, tv, tdq, tdka, tdva;
     int rc;

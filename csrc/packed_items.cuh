@@ -8,15 +8,30 @@ namespace nxd_packed {
 // A try of a wait lasts 3900 clocks, so a wait ends after two seconds; the results of a CTA that gave up are NaN.
 constexpr int kTries = 1 << 20;
 
-// A wait with an end: after kTries the CTA is marked, and no wait of its lasts any more.  The end costs the threads that wait 3 to 6 % of the
-// backward pass (D = 128, 16384 tokens: 2980 us against 2800 without it; 3100 with two predicated tries ahead of the loop, 3290 with
-// the counting in one condition with the try).
+// A wait with an end: after kTries the CTA is marked, and no wait of its lasts any more (the mark leaves one try).  In one piece, because
+// the loop's shape counts: of the backward pass of 4 documents in 16384 tokens, 32 heads of 128 over 8, it takes 2050 us (one of 16384
+// tokens, 16 heads of 64 over 4: 1967) as here, 2090 (2057) as a loop in C++, 2106 (2166) as a call behind the first try, 2124 (2156)
+// with the first try counted too.
 __device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    if (ptx::mbar_try_wait(bar, parity)) return;
-    for (int i = 0; !ptx::mbar_try_wait(bar, parity); ++i) {
-        if (i == kTries) *dead = 1;
-        if (*dead) break;
-    }
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P, Q;\n\t"
+        ".reg .s32 left;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1;\n\t"
+        "@P bra DONE;\n\t"
+        "ld.volatile.shared.s32 left, [%2];\n\t"          // 0, or -kTries
+        "add.s32 left, left, %3;\n"
+        "TRY:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1;\n\t"
+        "@P bra DONE;\n\t"
+        "sub.s32 left, left, 1;\n\t"
+        "setp.gt.s32 Q, left, 0;\n\t"
+        "@Q bra TRY;\n\t"
+        "st.volatile.shared.s32 [%2], %4;\n"
+        "DONE:\n\t"
+        "}"
+        ::"r"(ptx::smem_u32(bar)), "r"(parity), "r"(ptx::smem_u32(const_cast<const int*>(dead))), "n"(kTries), "n"(-kTries)
+        : "memory");
 }
 
 // copies that were started may still be on their way into the memory of a CTA that gave up
@@ -26,8 +41,12 @@ __device__ __forceinline__ void let_copies_land() {
     }
 }
 
-// The items of a CTA: every gridDim.x-th of the list, which is sorted by weight, forwards and backwards in turn so that nobody gets the
-// longest of every round.  The TMA warp, which is ahead of the others, reads them and hands them on through a ring in shared memory.
+// The items of a CTA.  The list is sorted by weight, and the first item of a CTA is the one of its number.  Backward, whoever is done
+// claims the next from a counter; forward, every gridDim.x-th is its own, forwards and backwards in turn so that nobody gets the longest
+// of every round.  The counter needs a launch that clears it, which the backward pass has, and its items differ more (a key block's
+// walk covers all heads of the group: 24 samples in 8192 tokens, 32 heads of 64 over 8, worst CTA 26 % above the mean in turn, 5 % by
+// claims; 204 us and 181).  Forward the worst is 9 % above (claims: 3 %).  The TMA warp, which is ahead of the others, gets the
+// items and hands them on through a ring in shared memory.
 constexpr int kItems = 4;
 constexpr int kRowsOfNone = 1;           // added to the rows of an entry of no sequence, to tell its kind from an item's
 __device__ __forceinline__ unsigned item_of_round(int round) {          // below 2^31 + gridDim.x

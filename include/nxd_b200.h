@@ -159,7 +159,7 @@ int nxd_flash_attn_bwd_tc(const void* q, const void* k, const void* v, const voi
  * nxd_packed_plan_entries tiles of 16 bytes, `seqs` 16 bytes per sequence; nxd_packed_plan_columns is the row length of
  * the per-row scratch.  Tiles have 128 rows, but 256 for the forward call where Hq / Hkv is odd.  strides = {head, row} in
  * elements: {q, k, v, o} forward, {q, k, v, o, dout, dq, dk, dv} backward, multiples of 8.
- * lse [Hq, columns] (NULL: not wanted), delta the same; dq_accum [Hq, D, columns] of scratch; dkv_accum: NULL, or ZEROED
+ * lse [Hq, columns] (NULL: not wanted), delta the same and 4 floats more; dq_accum [Hq, D, columns] of scratch; dkv_accum: NULL, or ZEROED
  * [2, Hkv, T, D] where nxd_packed_attn_bwd_splits is above 1.  Rows outside every sequence come out as zeros. */
 int nxd_packed_plan_entries(long long T, int N, int rows);
 long long nxd_packed_plan_columns(long long T, int N);

@@ -2,7 +2,8 @@
 
 ``PackedSequences`` holds where the sequences of a step begin and the tile list that the kernels walk (``csrc/packed_plan.cu``);
 it is made on the device from ``cu_seqlens`` without a copy to the host and serves every layer of the step, forward and
-backward.  The kernels are ``csrc/packed_attention.cu`` and the packed instantiation of ``csrc/flash_attn_bwd_tc.cu``.  ``ops.attention`` has the public functions."""
+backward.  The kernels are ``csrc/packed_attention.cu`` and ``csrc/packed_attention_bwd.cu``.  ``ops.attention`` has the public
+functions."""
 from __future__ import annotations
 
 import ctypes as _c
@@ -140,7 +141,7 @@ def _backward(q, k, v, o, lse, do, dq, dk, dv, packed: PackedSequences, scale: f
     T, Hq, D = q.shape
     Hkv = k.shape[1]
     tiles, entries, columns = packed.plan(causal)
-    delta = torch.empty_like(lse)
+    delta = torch.empty(lse.numel() + 4, dtype=torch.float32, device=q.device)
     acc = torch.empty((Hq, D, columns), dtype=torch.float32, device=q.device)
     splits = _lib.lib().nxd_packed_attn_bwd_splits(_c.c_longlong(T), _c.c_int(packed.count), _c.c_int(Hq), _c.c_int(Hkv))
     kv_acc = torch.zeros((2, Hkv, T, D), dtype=torch.float32, device=q.device) if splits > 1 else None
