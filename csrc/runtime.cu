@@ -30,6 +30,16 @@ int nxd_pdl_enabled() {
 void nxd_count_launches(int n) { __atomic_fetch_add(&g_launches, (unsigned long long)n, __ATOMIC_RELAXED); }
 NXD_API unsigned long long nxd_kernel_launches() { return __atomic_load_n(&g_launches, __ATOMIC_RELAXED); }
 
+NXD_API unsigned long long nxd_capture_id(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
+        cudaGetLastError();          // the legacy stream while another one is captured
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 NXD_API int nxd_version() { return 100; }
 
 NXD_API int nxd_device_sm_count() { return nxd_num_sms(); }

@@ -23,6 +23,8 @@ int nxd_version(void);
 int nxd_device_sm_count(void);
 /* Kernel launches made by this library in the calling process so far (bench.py's "gpu_launches"). */
 unsigned long long nxd_kernel_launches(void);
+/* which capture goes on on the stream, 0: none */
+unsigned long long nxd_capture_id(void* stream);
 /* Overwrite `bytes` of `buf` (> L2 size) so the next timed iteration starts with a cold L2. */
 int nxd_l2_flush(void* buf, size_t bytes, void* stream);
 

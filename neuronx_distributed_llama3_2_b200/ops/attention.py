@@ -138,16 +138,27 @@ def flash_attn_packed_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 def rope_flash_attn_packed_func(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_q: int, n_kv: int,
                                 cu_seqlens: Union[torch.Tensor, "PackedSequences"]) -> torch.Tensor:
     """Causal attention inside the sequences of a packed projection ``qkv [T, n_q + 2 n_kv, D]`` (q | k | v heads) whose queries and
-    keys are first rotated at their position in their own sequence -> ``[T, n_q, D]``.  The tables need as many rows as the
-    longest sequence has tokens."""
+    keys are first rotated at their position in their own sequence -> ``[T, n_q, D]``.  The tables
+    (fp32, ``[rows, D / 2]``) need as many rows as the longest sequence has tokens; on the GPU, where a check would wait for the
+    device, the tokens behind turn by the last row."""
     if qkv.dim() != 3 or qkv.shape[1] != n_q + 2 * n_kv:
         raise ValueError(f"a projection of {n_q} + 2 x {n_kv} heads, not {tuple(qkv.shape)}")
     packed = as_packed(cu_seqlens, qkv.shape[0], qkv.device)
+    if cos.dim() != 2 or cos.shape[1] * 2 != qkv.shape[2] or cos.shape != sin.shape or not cos.shape[0]:
+        raise ValueError(f"tables {tuple(cos.shape)} and {tuple(sin.shape)} for heads of {qkv.shape[2]}")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != qkv.device or sin.device != qkv.device:
+        raise ValueError(f"tables in fp32 on {qkv.device}, not {cos.dtype} on {cos.device}")
+    cos, sin = cos.contiguous(), sin.contiguous()
     if qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.shape[-1] in (64, 128) and _backend(qkv) == "nxd":
         return rope_packed_attn(qkv, cos, sin, n_q, n_kv, packed)
     from .rope import apply_rope
 
-    x = apply_rope(qkv, cos, sin, n_q + n_kv, positions=packed.positions())
+    positions = packed.positions()
+    if cos.shape[0] < packed.total:
+        if not qkv.is_cuda and int(positions.max()) >= cos.shape[0]:
+            raise ValueError(f"a sequence of {int(positions.max()) + 1} tokens, tables of {cos.shape[0]} rows")
+        positions = positions.clamp(max=cos.shape[0] - 1)
+    x = apply_rope(qkv, cos, sin, n_q + n_kv, positions=positions)
     return flash_attn_packed_func(x[:, :n_q], x[:, n_q:n_q + n_kv], x[:, n_q + n_kv:], packed)
 
 

@@ -23,9 +23,8 @@ class PackedSequences:
     ``cu_seqlens [N + 1]``: int32 or int64, rising (equal neighbours are an empty sequence), inside ``[0, total]``; rows ahead of the
     first boundary or behind the last belong to no sequence, attend to nothing and give zeros.  On the CPU this is checked; on
     the GPU, where a check would wait for the device, a boundary that falls or leaves the row is taken as the nearest one
-    that does not.  What is made of the boundaries (tile lists, positions) is made once, on the stream of the first call that needs it:
-    lengths that change want a new object.  One that is made while a CUDA graph is captured reads ``cu_seqlens`` again in
-    every replay, and is of use inside that graph only."""
+    that does not.  What is made of the boundaries (tile lists, positions) is made once for every stream, and once inside every
+    captured graph, which reads ``cu_seqlens`` again in each replay; elsewhere lengths that change want a new object."""
 
     def __init__(self, cu_seqlens: torch.Tensor, total: int):
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
@@ -34,7 +33,7 @@ class PackedSequences:
             raise ValueError(f"a packed row of {total} tokens")
         self.cu_seqlens, self.total, self.count = cu_seqlens.contiguous(), int(total), cu_seqlens.numel() - 1
         self._plans: dict = {}
-        self._positions: Optional[torch.Tensor] = None
+        self._positions: dict = {}
         if not cu_seqlens.is_cuda:
             ends = cu_seqlens.tolist()
             if any(b < a for a, b in zip(ends, ends[1:])) or ends[0] < 0 or ends[-1] > total:
@@ -44,9 +43,16 @@ class PackedSequences:
     def device(self) -> torch.device:
         return self.cu_seqlens.device
 
+    def _here(self) -> Tuple[int, int]:
+        """The current stream, and which capture goes on there: another one's lists may be unwritten still, or gone with its graph."""
+        if not self.cu_seqlens.is_cuda:
+            return 0, 0
+        stream = torch._C._cuda_getCurrentRawStream(self.cu_seqlens.get_device())
+        return stream, _lib.lib().nxd_capture_id(_c.c_void_p(stream)) if _lib.available() else 0
+
     def plan(self, causal: bool, rows: int = 128) -> Tuple[torch.Tensor, int, int]:
         """``(list of tiles of that many rows, its entries, columns of the per-row scratch)`` for the kernels, made on first use."""
-        key = (causal, rows)
+        key = (causal, rows, self._here())
         if key not in self._plans:
             most = min(self.count, self.total)
             entries = self.total // rows + most + 2                         # nxd_packed_plan_entries
@@ -61,14 +67,15 @@ class PackedSequences:
 
     def positions(self) -> torch.Tensor:
         """int32 ``[total]``: every token's position in its own sequence (0 outside of them), for the rotation."""
-        if self._positions is None:
+        here = self._here()
+        if here not in self._positions:
             cu = self.cu_seqlens.long().clamp(0, self.total).cummax(0).values
             rows = torch.arange(self.total, device=self.device)
             s = torch.searchsorted(cu, rows, right=True) - 1
             inside = (s >= 0) & (s < self.count)
             pos = torch.where(inside, rows - cu[s.clamp(0, self.count)], 0)
-            self._positions = pos.to(torch.int32)
-        return self._positions
+            self._positions[here] = pos.to(torch.int32)
+        return self._positions[here]
 
     def first_tokens(self) -> torch.Tensor:
         """int64 ``[N]``: the row of every sequence's first token."""
@@ -135,20 +142,20 @@ def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, want_
     return o, lse
 
 
-def _backward(q, k, v, o, lse, do, dq, dk, dv, packed: PackedSequences, scale: float, causal: bool) -> None:
-    """Every element of ``dq / dk / dv`` is written."""
+def _backward(q, k, v, o, lse, do, dq, dk, dv, plan, count: int, scale: float, causal: bool) -> None:
+    """Every element of ``dq / dk / dv`` is written.  ``plan``: the list that the forward pass had, or one made with it."""
     do = _fix(do)
     T, Hq, D = q.shape
     Hkv = k.shape[1]
-    tiles, entries, columns = packed.plan(causal)
+    tiles, entries, columns = plan
     delta = torch.empty(lse.numel() + 4, dtype=torch.float32, device=q.device)
     acc = torch.empty((Hq, D, columns), dtype=torch.float32, device=q.device)
-    splits = _lib.lib().nxd_packed_attn_bwd_splits(_c.c_longlong(T), _c.c_int(packed.count), _c.c_int(Hq), _c.c_int(Hkv))
+    splits = _lib.lib().nxd_packed_attn_bwd_splits(_c.c_longlong(T), _c.c_int(count), _c.c_int(Hq), _c.c_int(Hkv))
     kv_acc = torch.zeros((2, Hkv, T, D), dtype=torch.float32, device=q.device) if splits > 1 else None
     rc = _lib.lib().nxd_packed_attn_bwd(
         _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(do), _lib.ptr(lse), _lib.ptr(delta), _lib.ptr(acc), _lib.ptr(kv_acc),
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _strides(q, k, v, o, do, dq, dk, dv), _lib.ptr(tiles), _c.c_int(entries),
-        _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(packed.count), _c.c_int(Hq), _c.c_int(Hkv), _c.c_int(D), _c.c_float(scale),
+        _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(count), _c.c_int(Hq), _c.c_int(Hkv), _c.c_int(D), _c.c_float(scale),
         _c.c_int(causal), _lib.stream_ptr())
     _lib.check(rc, "nxd_packed_attn_bwd")
 
@@ -160,9 +167,9 @@ class _PackedAttnFn(torch.autograd.Function):
         grad = any(ctx.needs_input_grad[:3])
         with _lib.on_device_of(q):
             o, lse = _forward(q, k, v, packed, scale, causal, grad)
-        if grad:
-            ctx.save_for_backward(q, k, v, o, lse)
-            ctx.args = (packed, scale, causal)
+            if grad:
+                ctx.save_for_backward(q, k, v, o, lse)
+                ctx.args = (packed.plan(causal), packed.count, scale, causal)
         return o
 
     @staticmethod
@@ -186,22 +193,24 @@ class _RopePackedAttnFn(torch.autograd.Function):
             qkv = _rope_aligned(qkv)
             rot = torch.empty_like(qkv)
             positions = packed.positions()
+            if cos.shape[0] < packed.total:          # the bound keeps a sequence that is too long for the tables from reading behind them
+                positions = positions.clamp(max=cos.shape[0] - 1)
             _rope_launch(qkv, cos, sin, n_q + n_kv, 1, 1 << 30, positions, False, rot)
             o, lse = _forward(rot[:, :n_q], rot[:, n_q:n_q + n_kv], rot[:, n_q + n_kv:], packed, scale, True, ctx.needs_input_grad[0])
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(rot, o, lse, cos, sin, positions)
-            ctx.args = (n_q, n_kv, packed, scale)
+            if ctx.needs_input_grad[0]:
+                ctx.save_for_backward(rot, o, lse, cos, sin, positions)
+                ctx.args = (n_q, n_kv, packed.plan(True), packed.count, scale)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
         rot, o, lse, cos, sin, positions = ctx.saved_tensors
-        n_q, n_kv, packed, scale = ctx.args
+        n_q, n_kv, plan, count, scale = ctx.args
         parts = lambda x: (x[:, :n_q], x[:, n_q:n_q + n_kv], x[:, n_q + n_kv:])     # noqa: E731
         with _lib.on_device_of(rot):
             d = torch.empty_like(rot)
-            _backward(*parts(rot), o, lse, do, *parts(d), packed, scale, True)
+            _backward(*parts(rot), o, lse, do, *parts(d), plan, count, scale, True)
             _rope_launch(d, cos, sin, n_q + n_kv, 1, 1 << 30, positions, True)
         return d, None, None, None, None, None, None
 

@@ -76,3 +76,19 @@ def test_bad_tensors_are_refused():
         attention.flash_attn_packed_func(q, k, v, PackedSequences(torch.tensor([0, 4]), 8))
     with pytest.raises(ValueError):
         attention.rope_flash_attn_packed_func(q, None, None, 2, 2, cu)
+
+
+def test_bad_tables_are_refused():
+    qkv, cu = torch.randn(9, 8, 16), torch.tensor([0, 4, 9])
+    table = torch.ones(9, 8)
+    short, half, odd = torch.ones(4, 8), table.half(), torch.ones(9, 4)
+    for cos, sin in ((odd, odd), (table, short), (half, half), (short, short), (table[:0], table[:0])):
+        with pytest.raises(ValueError):
+            attention.rope_flash_attn_packed_func(qkv, cos, sin, 4, 2, cu)
+    attention.rope_flash_attn_packed_func(qkv, table[:5], table[:5], 4, 2, cu)
+
+
+def test_first_tokens():
+    assert PackedSequences(torch.tensor([1, 4, 4, 6]), 8).first_tokens().tolist() == [1, 4, 4]
+    assert PackedSequences(torch.tensor([0, 8, 8]), 8).first_tokens().tolist() == [0, 7]
+    assert PackedSequences(torch.tensor([3]), 8).first_tokens().tolist() == []

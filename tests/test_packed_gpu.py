@@ -197,6 +197,81 @@ def test_captured_step_follows_new_lengths():
             check(x, want, name)
 
 
+@pytest.mark.parametrize("G", [2, 4])
+def test_two_graphs_and_two_streams_of_one_object(G):
+    """Each capture and each stream makes its own lists: those of a graph that is gone are nobody else's."""
+    from neuronx_distributed_llama3_2_b200.ops import attention, rope
+    from neuronx_distributed_llama3_2_b200.ops.packed_attention import PackedSequences
+
+    T, ends = 700, [0, 300, 301, 690]
+    q, k, v, do = (x.contiguous() for x in _inputs(T, 4, G, 64))
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    qkv = torch.cat([q, k, v], 1)
+    cos, sin = rope.build_rope_cache(T, 64, 10000.0, None, device="cuda")
+    p = PackedSequences(torch.tensor(ends, device="cuda"), T)
+    want = packed(q, k, v, ends, True, do)
+
+    def step():
+        o = attention.flash_attn_packed_func(*leaves, p)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do), attention.rope_flash_attn_packed_func(qkv, cos, sin, 4, G, p))
+
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    graph, out = graphs.pop(1)
+    graphs.clear()                                              # the first one's memory goes back
+    torch.cuda.empty_cache()
+    trash = [torch.full((1 << 20,), 0x7f, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    graph.replay()
+    turned = step()[-1]                                         # eager, behind the captures
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    late = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for s in streams:                                           # at the same time
+        with torch.cuda.stream(s):
+            late.append(step())
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for results in (out, *late):
+        for name, x in zip(("o", "dq", "dk", "dv"), results):
+            check(x, want, name)
+        assert torch.equal(results[-1], turned)
+    del trash
+
+
+def test_backward_has_the_lists_of_its_forward():
+    """Boundaries that are overwritten before the backward pass, with heads that take other lists there."""
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+
+    T, ends = 640, [0, 100, 640]
+    q, k, v, do = (x.contiguous() for x in _inputs(T, 4, 4, 64))
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    cu = torch.tensor(ends, device="cuda")
+    o = flash_attn_packed_func(*leaves, cu)
+    cu.fill_(640)
+    want = packed(q, k, v, ends, True, do)
+    for name, x in zip(("o", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, leaves, do))):
+        check(x, want, name)
+
+
+def test_tables_shorter_than_the_row():
+    """Rotation tables as long as the longest sequence are enough, and a sequence that is longer reads no further."""
+    from neuronx_distributed_llama3_2_b200.ops import attention, rope
+
+    T, D = 400, 64
+    qkv = torch.randn(T, 8, D, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").bfloat16()
+    cos, sin = rope.build_rope_cache(T, D, 10000.0, None, device="cuda")
+    cu = torch.tensor([0, 200, 400], device="cuda")
+    whole = attention.rope_flash_attn_packed_func(qkv, cos, sin, 4, 2, cu)
+    assert torch.equal(whole, attention.rope_flash_attn_packed_func(qkv, cos[:200], sin[:200], 4, 2, cu))
+    short = attention.rope_flash_attn_packed_func(qkv, cos[:150], sin[:150], 4, 2, cu)
+    assert short.isfinite().all() and torch.equal(short[:150], whole[:150])
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_rotation_and_attention(D):
     from neuronx_distributed_llama3_2_b200.ops import attention, rope
