@@ -7,11 +7,17 @@
 // added tile by tile to a d-major fp32 accumulator by TMA, in an order that is not fixed.
 //
 // Here one CTA per SM stays for the whole call (items: packed_items.cuh; the list is sorted by the key tiles that a query tile meets, and
-// mirrored for key blocks: the block as far from the end meets as many query rows).  A block of a fine-tuning sequence meets a few
+// mirrored for key blocks: the block as far from the end meets as many query rows).  A block of a short sequence meets a few
 // query tiles, and with a CTA per block its start, its end and the copies of tiles that cross the sequence's end by a warp were
-// two thirds of the time (24 samples in 8192 tokens, 32 heads of 64 over 8: 178 us).  Tiles that cross the end are loaded whole and
-// cleared behind it once they are there: 0 * NaN is NaN, and behind the end is the next sequence.
-//   warp 0      TMA: K, V of an item, then Q_i, dO_i, L_i, Delta_i through a ring of three; zeros behind the end of a sequence
+// more than half of the time (120 sentences in 24576 tokens, 16 heads of 64, no mask: 410 us against 210).  Tiles that cross the end
+// are loaded whole and cleared behind it once they are there: 0 * NaN is NaN, and behind the end is the next sequence.
+//
+// Measured (the whole pass: Delta, this kernel, dQ): 4 documents in 16384 tokens, 32 heads of 128 over 8: 2.0 ms, 727 TFLOP/s, bound by
+// the products' dependences on P^T and dS^T of the same tile (tensor memory holds one of each) and by the power limit; 24 samples in 8192
+// tokens, heads of 64: 178 us, 325; the sentences above: 294 us, 262, where a block's end (dK, dV out of tensor memory, while
+// nothing else may use it) and 78 us of passes over the fp32 accumulator weigh most.  Two pairs of accumulators for heads of 64, so that
+// the warps of dQ write the results under the next block: 309 us, since those warps then hold up dQ.
+//   warp 0      claims items; TMA: K, V of an item, then Q_i, dO_i, L_i, Delta_i through a ring of three; zeros behind the end of a sequence
 //   warp 1      MMA: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q, dQ^T = K^T dS^T
 //   warps 2-9   P^T and dS^T, two warps to a lane quadrant with 32 of the 64 queries each; then dV (one half) and dK (the other)
 //   warps 10-13 dQ^T -> fp32 accumulator
@@ -560,7 +566,8 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 }
 
 // Delta of one entry (up to 128 rows) of one head, at the plan's padded columns, and zeros into the dQ accumulator's columns of those rows
-// (nobody reads the padding).  kD / 8 lanes own a row.
+// (nobody reads the padding) and the counter of claims.  kD / 8 lanes own a row.  Bound by memory: 24576 rows of 16 heads of 64,
+// 201 MB, 35 us.
 template <int kD>
 __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ dout, const PackedTile* tiles,
                                                            float* __restrict__ delta, float* __restrict__ acc, int* claimed, long long o_head, long long o_row,
@@ -607,7 +614,8 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
     }
 }
 
-// d-major fp32 accumulator [Hq, D, lse_row] -> dq, half an entry (64 rows) of one head per block; rows of no sequence get zeros.
+// d-major fp32 accumulator [Hq, D, lse_row] -> dq, half an entry (64 rows) of one head per block; rows of no sequence get zeros.  Bound by
+// memory (24576 rows of 16 heads of 64: 43 us; whole entries: the same).
 template <int kD>
 __global__ void __launch_bounds__(256) packed_dq_kernel(const float* __restrict__ acc, bf16* __restrict__ dq, const PackedTile* tiles,
                                                         long long head, long long row, long long lse_row, int Hq) {

@@ -1,5 +1,5 @@
 // The tile list of a packed batch: sequences of different lengths laid end to end in `T` rows, bounded by cu[0 .. N], for the
-// attention kernels, which work by tiles of 128 (flash_attn_bwd_tc.cu, packed_attention.cu) or 256 rows (the latter) of one sequence.
+// attention kernels, which work by tiles of 128 (packed_attention.cu, packed_attention_bwd.cu) or 256 rows (the former) of one sequence.
 //
 // The lengths stay on the device, so that a step needs no copy to the host and can be captured: the list has room for
 // T / 128 + N + 2 tiles whatever the lengths are, and entries without a tile cost nothing.  Boundaries that fall or leave [0, T] are

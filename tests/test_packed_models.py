@@ -189,6 +189,47 @@ def test_finetune_example_runs_on_packed_rows(tmp_path):
     assert out.returncode == 0, out.stdout[-2000:] + out.stderr[-2000:]
 
 
+def _two_ranks(rank, world, sp):
+    from test_llama_tp_cpu import _shard_from_full, _solo
+
+    cu = torch.tensor([0, 7, 8, 8, 30])
+    ids = torch.randint(0, 512, (1, 32), generator=torch.Generator().manual_seed(1))
+    torch.manual_seed(3)
+    with _solo():
+        full = M.LlamaForCausalLM(M.tiny_llama(sequence_parallel_enabled=False))
+        want = full(ids, ids, cu_seqlens=cu)
+    model = M.LlamaForCausalLM(M.tiny_llama(sequence_parallel_enabled=sp))
+    _shard_from_full(full, model, world, rank)
+    got = model(ids, ids, cu_seqlens=cu)
+    got.backward()
+    assert abs(got - want) <= FP32 * want, (got, want)
+    # a rank with a part of the input draws a mask of its own
+    lora = _lora(model)
+    offsets = {n.split(".")[-2]: m.offset for n, m in lora.named_modules() if isinstance(m, dropout.Dropout)}
+    assert offsets == {"qkv_proj": rank if sp else 0, "o_proj": rank}, offsets
+    # the first token of every sentence, wherever its row lives
+    bert = BertForPreTraining(tiny_bert(sequence_parallel_enabled=sp))
+    hidden = torch.arange(32.0).view(32, 1, 1).expand(32, 1, 128)
+    mine = hidden.chunk(world)[rank] if sp else hidden
+    packed = PackedSequences(torch.tensor([0, 7, 20, 32]), 32)
+    assert bert._cls_token(mine.contiguous(), packed)[:, 0].tolist() == [0.0, 7.0, 20.0]
+
+
+@pytest.mark.parametrize("sp", [False, True])
+def test_two_ranks(sp):
+    from conftest import run_distributed
+
+    run_distributed(_two_ranks_entry, 2, sp)
+
+
+def _two_ranks_entry(rank, world, sp):
+    from neuronx_distributed_llama3_2_b200.parallel import parallel_state as ps
+
+    if not ps.model_parallel_is_initialized():
+        ps.initialize_model_parallel(tensor_model_parallel_size=world)
+    _two_ranks(rank, world, sp)
+
+
 # -- on the GPU --------------------------------------------------------------------------------------------------------------
 GPU_ENDS, GPU_ROW = [0, 130, 131, 131, 448, 700], 768
 
