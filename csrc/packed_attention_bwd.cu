@@ -614,45 +614,41 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
     }
 }
 
-// d-major fp32 accumulator [Hq, D, lse_row] -> dq, half an entry (64 rows) of one head per block; rows of no sequence get zeros.  Bound by
-// memory (24576 rows of 16 heads of 64: 43 us; whole entries: the same).
+// d-major fp32 accumulator [Hq, D, lse_row] -> dq, 64 of the D of an entry (128 rows) of one head per block; rows of no sequence get
+// zeros.
 template <int kD>
 __global__ void __launch_bounds__(256) packed_dq_kernel(const float* __restrict__ acc, bf16* __restrict__ dq, const PackedTile* tiles,
                                                         long long head, long long row, long long lse_row, int Hq) {
     pdl_trigger();
     pdl_wait();
-    __shared__ float tile[kD][65];
-    const PackedTile pt = packed_tile(tiles, blockIdx.x / Hq);
-    const int h = blockIdx.x % Hq;
-    const int half = blockIdx.y;
+    __shared__ float4 tile[64][32];          // four columns of row d at place (columns / 4) ^ (d / 8 % 8): no bank twice, either way
+    constexpr int kParts = kD / 64;
+    const unsigned at = blockIdx.x / kParts;
+    const PackedTile pt = packed_tile(tiles, at / Hq);
+    const int h = at % Hq, d0 = blockIdx.x % kParts * 64;
     if (pt.len == 0) {
-        if (half == 0) block_zero_rows<kD>(dq + (long long)pt.start * row + h * head, row, pt.t, threadIdx.x, 256);
+        if (d0 == 0) block_zero_rows<kD>(dq + (long long)pt.start * row + h * head, row, pt.t, threadIdx.x, 256);
         return;
     }
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int col = (threadIdx.x & 15) * 4, d0 = threadIdx.x >> 4;
-    const int q0 = pt.t * kBN + half * 64;
-    if (q0 >= pt.len) return;
-    const float* src = acc + (long long)h * kD * lse_row + pt.pad + q0;
-    float4 v[kD / 16];
+    const int q0 = pt.t * kBN, left = pt.len - q0;
+    const float* src = acc + ((long long)h * kD + d0) * lse_row + pt.pad + q0;
+    float4 v[8];
 #pragma unroll
-    for (int j = 0; j < kD / 16; ++j)        // columns in fours: those of a sequence are padded to a multiple of four
-        v[j] = q0 + col < pt.len ? *reinterpret_cast<const float4*>(src + (d0 + 16 * j) * lse_row + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < 8; ++j)              // columns in fours: those of a sequence are padded to a multiple of four
+        v[j] = 4 * lane < left ? *reinterpret_cast<const float4*>(src + (w + 8 * j) * lse_row + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < kD / 16; ++j) {
-        float* t = &tile[d0 + 16 * j][col];
-        t[0] = v[j].x, t[1] = v[j].y, t[2] = v[j].z, t[3] = v[j].w;
-    }
+    for (int j = 0; j < 8; ++j) tile[w + 8 * j][lane ^ j] = v[j];
     __syncthreads();
-    const int r = w * 8 + (lane >> 2);
-    if (q0 + r >= pt.len) return;
-    bf16* dst = dq + h * head + (long long)(pt.start + q0 + r) * row;
 #pragma unroll
-    for (int c = lane & 3; c < kD / 8; c += 4) {
-        float f[8];
+    for (int i = 0; i < 4; ++i) {            // eight lanes write 128 bytes of a row
+        const int r = w * 16 + i * 4 + (lane >> 3), c = lane & 7;
+        if (r < left) {
+            float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = tile[c * 8 + e][r];
-        reinterpret_cast<bf16x8*>(dst)[c] = pack8(f);
+            for (int e = 0; e < 8; ++e) f[e] = reinterpret_cast<const float*>(&tile[c * 8 + e][(r >> 2) ^ c])[r & 3];
+            reinterpret_cast<bf16x8*>(dq + h * head + (long long)(pt.start + q0 + r) * row + d0)[c] = pack8(f);
+        }
     }
 }
 
@@ -764,10 +760,10 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
         NXD_LAUNCH_CHECK_N(2);
     }
     if (D == 128)
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<128>, dim3(per_head, 2), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<128>, dim3(per_head * 2), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
             strides[10], strides[11], lse_row, Hq)));
     else
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<64>, dim3(per_head, 2), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<64>, dim3(per_head), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
             strides[10], strides[11], lse_row, Hq)));
     NXD_LAUNCH_CHECK();
     return 0;
