@@ -38,6 +38,7 @@ constexpr float kRescale = 8.0f;                  // log2 units
 struct FwdParams {
     const PackedTile* tiles;
     float* lse;
+    uint8_t* rest;                                // what rounding to bf16 took from o (attn_tc_common.cuh), NULL: not wanted
     bf16* o;
     const bf16* v;
     long long lse_row, o_head, o_row, v_head, v_row;
@@ -502,6 +503,27 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                         w[i] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * i]) * inv, __uint_as_float(o[8 * c + 2 * i + 1]) * inv);
                     st_shared_v4(stage + lane * 128 + ((c ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
                 }
+                if (p.rest != nullptr && n == 1) {           // eight bits of what the rounding took, for Delta of the backward pass
+                    uint32_t most = 0u;
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) {
+                        o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+                        o[e + 1] = __float_as_uint(__uint_as_float(o[e + 1]) * inv);
+                        most = __vmaxu2(most, pack_bf16x2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])) & 0x7fff7fffu);
+                    }
+                    const float up = rest_up(most);
+                    uint8_t* to = p.rest + rest_offset<D>(head * p.lse_row + done.pad + at, g * 4);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t* x = o + 16 * c + 4 * i;
+                            w[i] = rest_pack(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3]), up);
+                        }
+                        if (real) *reinterpret_cast<uint4*>(to + c * 64) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
                 if (first + 32 <= done.len) {
                     ptx::fence_proxy_async();
                     __syncwarp();
@@ -582,9 +604,9 @@ int launch_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& t
 
 // Attention inside each sequence of a packed batch: q [T, Hq, D], k and v [T, Hkv, D], o [T, Hq, D], strides {q_h, q_row, k_h,
 // k_row, v_h, v_row, o_h, o_row} in elements (multiples of 8), 16-byte aligned bases; tiles: the `entries` tiles that
-// nxd_packed_plan has made; lse NULL or [Hq, lse_row] floats, log2 units, written at the plan's padded columns.  Rows
-// outside every sequence get zeros.
-NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const long long* strides,
+// nxd_packed_plan has made; lse NULL or [Hq, lse_row] floats, log2 units, written at the plan's padded columns; rest NULL or [Hq, lse_row,
+// D] bytes, for the backward pass.  Rows outside every sequence get zeros.
+NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const long long* strides,
                                 const void* tiles, int entries, long long lse_row, long long T, int Hq, int Hkv, int D, float scale,
                                 int causal, void* stream) {
     NXD_REQUIRE(D == 64 || D == 128, "packed_attn: head dim %d not supported (64 or 128)", D);
@@ -592,12 +614,13 @@ NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, voi
                 "packed_attn: bad problem");
     for (int i = 0; i < 8; ++i)
         NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
-    NXD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)tiles) & 15) == 0,
-                "packed_attn: tensors must be 16-byte aligned");
+    NXD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)tiles) & 15) == 0 && lse_row % 4 == 0,
+                "packed_attn: tensors must be 16-byte aligned, rows of the scratch multiples of four");
     FwdParams p{};
     p.tiles = (const PackedTile*)tiles;
     p.entries = entries;
     p.lse = lse; p.lse_row = lse_row;
+    p.rest = (uint8_t*)rest;
     p.Hq = Hq; p.group = Hq / Hkv;
     p.pairs = p.group % 2 == 0 ? Hq / 2 : Hq;
     p.scale_log2 = scale * 1.4426950408889634f;

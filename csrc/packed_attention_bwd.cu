@@ -569,9 +569,9 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 // (nobody reads the padding) and the counter of claims.  kD / 8 lanes own a row.  Bound by memory: 24576 rows of 16 heads of 64,
 // 201 MB, 35 us.
 template <int kD>
-__global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ dout, const PackedTile* tiles,
+__global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __restrict__ o, const uint8_t* __restrict__ rest, const bf16* __restrict__ dout, const PackedTile* tiles,
                                                            float* __restrict__ delta, float* __restrict__ acc, int* claimed, long long o_head, long long o_row,
-                                                           long long do_head, long long do_row, long long lse_row, int Hq) {
+                                                           long long do_head, long long do_row, long long lse_row, int Hq, int causal) {
     pdl_wait();         // and no trigger: CTAs of the next kernel that come while the SMs are full of this one's blocks stay slower for good
                         // (4 documents in 16384 tokens, 32 heads of 128 over 8: 2060 us for the pass instead of 1750)
     constexpr int L = kD / 8, R = 256 / L;
@@ -587,30 +587,52 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
         for (int i = threadIdx.x; i < kD * 32; i += 256)
             if ((i & 31) < quads) *reinterpret_cast<float4*>(to + (i >> 5) * lse_row + (i & 31) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    bf16x8 a[kBN / R], g[kBN / R];
+    const long long col = h * lse_row + pt.pad + first;
+    const bool one_tile = causal ? pt.t == 0 : pt.len <= kBN;          // of keys: these rows have what the rounding took
+    constexpr int U = 4;                     // rows of a lane on their way
+#pragma unroll 1
+    for (int r0 = threadIdx.x / L; r0 < kBN; r0 += U * R) {
+        bf16x8 a[U], g[U];
+        uint2 less[U];
 #pragma unroll
-    for (int u = 0; u < kBN / R; ++u) {
-        const int r = u * R + threadIdx.x / L;
-        const long long row = pt.start + first + r;
-        if (r < rows) {
-            a[u] = reinterpret_cast<const bf16x8*>(o + h * o_head + row * o_row)[l];
-            g[u] = reinterpret_cast<const bf16x8*>(dout + h * do_head + row * do_row)[l];
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < kBN / R; ++u) {
-        const int r = u * R + threadIdx.x / L;
-        float acc = 0.f;
-        if (r < rows) {
-            float fa[8], fg[8];
-            unpack8(a[u], fa);
-            unpack8(g[u], fg);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fg[e], acc);
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * R;
+            const long long row = pt.start + first + r;
+            if (r < rows) {
+                a[u] = reinterpret_cast<const bf16x8*>(o + h * o_head + row * o_row)[l];
+                g[u] = reinterpret_cast<const bf16x8*>(dout + h * do_head + row * do_row)[l];
+                if (one_tile) less[u] = *reinterpret_cast<const uint2*>(rest + rest_offset<kD>(col + r, l >> 1) + (l & 1) * 8);
+            }
         }
 #pragma unroll
-        for (int off = L / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-        if (l == 0 && r < rows) delta[h * lse_row + pt.pad + first + r] = acc;
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * R;
+            float acc = 0.f;
+            uint32_t most = 0u;              // of the row's 64 neighbours
+            if (one_tile && r < rows) {
+                const uint4 w = *reinterpret_cast<const uint4*>(&a[u]);
+                most = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+            }
+            if (one_tile) {
+#pragma unroll
+                for (int off = 4; off > 0; off >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, off));
+            }
+            if (r < rows) {
+                float fa[8], fg[8];
+                unpack8(a[u], fa);
+                unpack8(g[u], fg);
+                if (one_tile) {
+                    const float down = rest_down(most);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) fa[e] = fmaf(rest_of(e < 4 ? less[u].x : less[u].y, e & 3), down, fa[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fg[e], acc);
+            }
+#pragma unroll
+            for (int off = L / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+            if (l == 0 && r < rows) delta[col + r] = acc;
+        }
     }
 }
 
@@ -699,10 +721,10 @@ NXD_API int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv) {
 }
 
 // Backward of nxd_packed_attn_fwd.  strides: {head, row} in elements of q, k, v, o, dout, dq, dk, dv (16 values, multiples of 8);
-// lse: what the forward pass wrote; delta: Hq * lse_row + 4 floats of scratch; dq_accum: [Hq, D, lse_row] floats of scratch;
+// lse, rest: what the forward pass wrote; delta: Hq * lse_row + 4 floats of scratch; dq_accum: [Hq, D, lse_row] floats of scratch;
 // dkv_accum: NULL, or ZEROED [2, Hkv, T, D] floats where nxd_packed_attn_bwd_splits says more than one.
 // dQ (with splits dK and dV too) is summed in fp32 in an order that is not fixed.
-NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse,
                                 float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
                                 const long long* strides, const void* tiles, int entries, long long lse_row, long long T, int N, int Hq,
                                 int Hkv, int D, float scale, int causal, void* stream) {
@@ -711,7 +733,7 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
                 (long long)entries * Hq * 16 < (1ll << 31), "packed_attn_bwd: bad problem");
     for (int i = 0; i < 16; ++i)
         NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn_bwd: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
-    const void* bases[] = {q, k, v, o, dout, lse, delta, dq_accum, dkv_accum, dq, dk, dv, tiles};
+    const void* bases[] = {q, k, v, o, rest, dout, lse, delta, dq_accum, dkv_accum, dq, dk, dv, tiles};
     for (const void* x : bases) NXD_REQUIRE(((uintptr_t)x & 15) == 0, "packed_attn_bwd: tensors must be %s", "16-byte aligned");
     cudaStream_t st = (cudaStream_t)stream;
     const PackedTile* pt = (const PackedTile*)tiles;
@@ -726,11 +748,11 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
     p.dv = (bf16*)dv; p.dv_head = strides[14]; p.dv_row = strides[15];
     const unsigned per_head = (unsigned)entries * Hq;
     if (D == 128)
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<128>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const bf16*)dout, pt,
-            delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<128>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const uint8_t*)rest, (const bf16*)dout, pt,
+            delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq, causal)));
     else
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<64>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const bf16*)dout, pt,
-            delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq)));
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<64>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const uint8_t*)rest, (const bf16*)dout, pt,
+            delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq, causal)));
     NXD_LAUNCH_CHECK();
     CUtensorMap tq, tdo, tk, tv, tdq, tdka, tdva;
     int rc;

@@ -128,21 +128,23 @@ def _strides(*ts: torch.Tensor):
     return (_c.c_longlong * len(vals))(*vals)
 
 
-def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, want_lse: bool):
+def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad: bool):
+    """``(o, lse, rest)``; the two that the backward pass takes are ``None`` without it."""
     T, Hq, D = q.shape
     # an odd number of heads to a key head: two neighbouring tiles of one head are worked on together (csrc/packed_attention.cu)
     tiles, entries, columns = packed.plan(causal, 128 if Hq // k.shape[1] % 2 == 0 else 256)
     o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((Hq, columns), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((Hq, columns), dtype=torch.float32, device=q.device) if grad else None
+    rest = torch.empty((Hq, columns, D), dtype=torch.uint8, device=q.device) if grad else None
     rc = _lib.lib().nxd_packed_attn_fwd(
-        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(lse), _strides(q, k, v, o), _lib.ptr(tiles), _c.c_int(entries),
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(lse), _lib.ptr(rest), _strides(q, k, v, o), _lib.ptr(tiles), _c.c_int(entries),
         _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(Hq), _c.c_int(k.shape[1]), _c.c_int(D), _c.c_float(scale), _c.c_int(causal),
         _lib.stream_ptr())
     _lib.check(rc, "nxd_packed_attn_fwd")
-    return o, lse
+    return o, lse, rest
 
 
-def _backward(q, k, v, o, lse, do, dq, dk, dv, plan, count: int, scale: float, causal: bool) -> None:
+def _backward(q, k, v, o, lse, rest, do, dq, dk, dv, plan, count: int, scale: float, causal: bool) -> None:
     """Every element of ``dq / dk / dv`` is written.  ``plan``: the list that the forward pass had, or one made with it."""
     do = _fix(do)
     T, Hq, D = q.shape
@@ -153,7 +155,7 @@ def _backward(q, k, v, o, lse, do, dq, dk, dv, plan, count: int, scale: float, c
     splits = _lib.lib().nxd_packed_attn_bwd_splits(_c.c_longlong(T), _c.c_int(count), _c.c_int(Hq), _c.c_int(Hkv))
     kv_acc = torch.zeros((2, Hkv, T, D), dtype=torch.float32, device=q.device) if splits > 1 else None
     rc = _lib.lib().nxd_packed_attn_bwd(
-        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(do), _lib.ptr(lse), _lib.ptr(delta), _lib.ptr(acc), _lib.ptr(kv_acc),
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(rest), _lib.ptr(do), _lib.ptr(lse), _lib.ptr(delta), _lib.ptr(acc), _lib.ptr(kv_acc),
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _strides(q, k, v, o, do, dq, dk, dv), _lib.ptr(tiles), _c.c_int(entries),
         _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(count), _c.c_int(Hq), _c.c_int(Hkv), _c.c_int(D), _c.c_float(scale),
         _c.c_int(causal), _lib.stream_ptr())
@@ -166,19 +168,19 @@ class _PackedAttnFn(torch.autograd.Function):
         q, k, v = _fix(q), _fix(k), _fix(v)
         grad = any(ctx.needs_input_grad[:3])
         with _lib.on_device_of(q):
-            o, lse = _forward(q, k, v, packed, scale, causal, grad)
+            o, lse, rest = _forward(q, k, v, packed, scale, causal, grad)
             if grad:
-                ctx.save_for_backward(q, k, v, o, lse)
+                ctx.save_for_backward(q, k, v, o, lse, rest)
                 ctx.args = (packed.plan(causal), packed.count, scale, causal)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, o, lse, rest = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         with _lib.on_device_of(q):
-            _backward(q, k, v, o, lse, do, dq, dk, dv, *ctx.args)
+            _backward(q, k, v, o, lse, rest, do, dq, dk, dv, *ctx.args)
         return dq, dk, dv, None, None, None
 
 
@@ -196,21 +198,21 @@ class _RopePackedAttnFn(torch.autograd.Function):
             if cos.shape[0] < packed.total:          # the bound keeps a sequence that is too long for the tables from reading behind them
                 positions = positions.clamp(max=cos.shape[0] - 1)
             _rope_launch(qkv, cos, sin, n_q + n_kv, 1, 1 << 30, positions, False, rot)
-            o, lse = _forward(rot[:, :n_q], rot[:, n_q:n_q + n_kv], rot[:, n_q + n_kv:], packed, scale, True, ctx.needs_input_grad[0])
+            o, lse, rest = _forward(rot[:, :n_q], rot[:, n_q:n_q + n_kv], rot[:, n_q + n_kv:], packed, scale, True, ctx.needs_input_grad[0])
             if ctx.needs_input_grad[0]:
-                ctx.save_for_backward(rot, o, lse, cos, sin, positions)
+                ctx.save_for_backward(rot, o, lse, rest, cos, sin, positions)
                 ctx.args = (n_q, n_kv, packed.plan(True), packed.count, scale)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        rot, o, lse, cos, sin, positions = ctx.saved_tensors
+        rot, o, lse, rest, cos, sin, positions = ctx.saved_tensors
         n_q, n_kv, plan, count, scale = ctx.args
         parts = lambda x: (x[:, :n_q], x[:, n_q:n_q + n_kv], x[:, n_q + n_kv:])     # noqa: E731
         with _lib.on_device_of(rot):
             d = torch.empty_like(rot)
-            _backward(*parts(rot), o, lse, do, *parts(d), plan, count, scale, True)
+            _backward(*parts(rot), o, lse, rest, do, *parts(d), plan, count, scale, True)
             _rope_launch(d, cos, sin, n_q + n_kv, 1, 1 << 30, positions, True)
         return d, None, None, None, None, None, None
 

@@ -258,6 +258,19 @@ def test_backward_has_the_lists_of_its_forward():
         check(x, want, name)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_delta_is_not_of_the_rounded_result(D):
+    """Two tokens that see one another, queries of zero: weights of one half, score gradients of d and -d.  With keys of ones dQ is the sum
+    of the two, each rounded, so it is zero unless Delta's error e moves them apart: that takes a border between two numbers of bf16,
+    2^-8 |d| apart, inside 2 e.  With Delta of the rounded result e is some 2^-9 |o| |dO| and most elements are not zero; with what the
+    rounding took (to 2^-8 of it) and fp32 sums less than one in fifty moves."""
+    T, H = 512, 4
+    _, _, v, do = _inputs(T, H, H, D)
+    q, k = torch.zeros_like(v), torch.ones_like(v)
+    got = _run(q, k, v, do, list(range(0, T + 1, 2)), False)
+    assert (got["dq"] != 0).any(-1).float().mean() <= 0.1
+
+
 def test_tables_shorter_than_the_row():
     """Rotation tables as long as the longest sequence are enough, and a sequence that is longer reads no further."""
     from neuronx_distributed_llama3_2_b200.ops import attention, rope
