@@ -20,8 +20,8 @@
 // thread of each query tile, so the softmax warps, which bound this size (128 exponentials a row for half the products), never wait.
 //
 // Measured, 32 heads over 8: 7 prompts in 32768 tokens, heads of 128: bound by the tensor core at the power limit, 3.0 ms, 1190 TFLOP/s;
-// 4 documents in 16384 tokens: 551 us, 1059; 24 samples in 8192 tokens, heads of 64: 62 us, 376, as tiles of 128 x 128 are a half full
-// and an item is a few tiles.  120 sentences in 24576 tokens, 16 heads of 64, no mask: 99 us, 309 (by the length of an item too).
+// 4 documents in 16384 tokens: 0.50 ms, 1160; 24 samples in 8192 tokens, heads of 64: 67 us, 346, as tiles of 128 x 128 are a half full
+// and an item is a few tiles.  120 sentences in 24576 tokens, 16 heads of 64, no mask: 102 us, 301 (by the length of an item too).
 #include "attn_tc_common.cuh"
 #include "gemm_tcgen05.cuh"
 #include "packed_items.cuh"
@@ -614,7 +614,7 @@ NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, voi
                 "packed_attn: bad problem");
     for (int i = 0; i < 8; ++i)
         NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
-    NXD_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)tiles) & 15) == 0 && lse_row % 4 == 0,
+    NXD_REQUIRE(q && k && v && o && tiles && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)tiles) & 15) == 0 && lse_row % 4 == 0,
                 "packed_attn: tensors must be 16-byte aligned, rows of the scratch multiples of four");
     FwdParams p{};
     p.tiles = (const PackedTile*)tiles;

@@ -12,11 +12,11 @@
 // more than half of the time (120 sentences in 24576 tokens, 16 heads of 64, no mask: 410 us against 210).  Tiles that cross the end
 // are loaded whole and cleared behind it once they are there: 0 * NaN is NaN, and behind the end is the next sequence.
 //
-// Measured (the whole pass: Delta, this kernel, dQ): 4 documents in 16384 tokens, 32 heads of 128 over 8: 2.0 ms, 727 TFLOP/s, bound by
+// Measured (the whole pass: Delta, this kernel, dQ): 4 documents in 16384 tokens, 32 heads of 128 over 8: 1.8 ms, 810 TFLOP/s, bound by
 // the products' dependences on P^T and dS^T of the same tile (tensor memory holds one of each) and by the power limit; 24 samples in 8192
-// tokens, heads of 64: 178 us, 325; the sentences above: 294 us, 262, where a block's end (dK, dV out of tensor memory, while
-// nothing else may use it) and 78 us of passes over the fp32 accumulator weigh most.  Two pairs of accumulators for heads of 64, so that
-// the warps of dQ write the results under the next block: 309 us, since those warps then hold up dQ.
+// tokens, heads of 64: 171 us, 338; the sentences above: 290 us, 265, where a block's end (dK, dV out of tensor memory, while
+// nothing else may use it) and 69 us of passes over the fp32 accumulator weigh most.  Two pairs of accumulators for heads of 64, so that
+// the warps of dQ write the results under the next block: 309 us instead of 297, since those warps then hold up dQ.
 //   warp 0      claims items; TMA: K, V of an item, then Q_i, dO_i, L_i, Delta_i through a ring of three; zeros behind the end of a sequence
 //   warp 1      MMA: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q, dQ^T = K^T dS^T
 //   warps 2-9   P^T and dS^T, two warps to a lane quadrant with 32 of the 64 queries each; then dV (one half) and dK (the other)
@@ -567,7 +567,7 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 
 // Delta of one entry (up to 128 rows) of one head, at the plan's padded columns, and zeros into the dQ accumulator's columns of those rows
 // (nobody reads the padding) and the counter of claims.  kD / 8 lanes own a row.  Bound by memory: 24576 rows of 16 heads of 64,
-// 201 MB, 35 us.
+// 201 MB, 38 us.
 template <int kD>
 __global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __restrict__ o, const uint8_t* __restrict__ rest, const bf16* __restrict__ dout, const PackedTile* tiles,
                                                            float* __restrict__ delta, float* __restrict__ acc, int* claimed, long long o_head, long long o_row,
@@ -637,7 +637,8 @@ __global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __rest
 }
 
 // d-major fp32 accumulator [Hq, D, lse_row] -> dq, 64 of the D of an entry (128 rows) of one head per block; rows of no sequence get
-// zeros.
+// zeros.  Bound by memory: 24576 rows of 16 heads of 64, 151 MB, 31 us; 16384 rows of 32 heads of 128, 403 MB, 79 us (142 as half
+// entries through padded rows of shared memory, which two to four lanes met at one bank).
 template <int kD>
 __global__ void __launch_bounds__(256) packed_dq_kernel(const float* __restrict__ acc, bf16* __restrict__ dq, const PackedTile* tiles,
                                                         long long head, long long row, long long lse_row, int Hq) {
@@ -734,7 +735,8 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
     for (int i = 0; i < 16; ++i)
         NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn_bwd: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
     const void* bases[] = {q, k, v, o, rest, dout, lse, delta, dq_accum, dkv_accum, dq, dk, dv, tiles};
-    for (const void* x : bases) NXD_REQUIRE(((uintptr_t)x & 15) == 0, "packed_attn_bwd: tensors must be %s", "16-byte aligned");
+    for (const void* x : bases)
+        NXD_REQUIRE(((uintptr_t)x & 15) == 0 && (x != nullptr || x == dkv_accum), "packed_attn_bwd: tensors must be %s", "there and 16-byte aligned");
     cudaStream_t st = (cudaStream_t)stream;
     const PackedTile* pt = (const PackedTile*)tiles;
     BwdParams p{};
