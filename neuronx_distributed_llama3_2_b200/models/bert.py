@@ -174,6 +174,8 @@ class BertForPreTraining(nn.Module):
     attends to itself, its positions start at 0, and its first token is its CLS (``next_sentence_label [N]``, ``nsp logits
     [N, 2]``).  No sentence is empty or longer than ``max_position_embeddings``; columns outside of them carry label -100."""
 
+    _fx_default_inputs = ("cu_seqlens",)                  # not an input of a pipeline's graph unless it is named
+
     def __init__(self, config: BertConfig, device=None):
         super().__init__()
         self.config = config

@@ -403,6 +403,8 @@ class LlamaForCausalLM(nn.Module):
     and no sample's last token predicts the next sample's first; columns outside of them (padding) enter neither attention nor
     the loss."""
 
+    _fx_default_inputs = ("cu_seqlens",)                  # not an input of a pipeline's graph unless it is named
+
     def __init__(self, config: LlamaConfig, device=None):
         super().__init__()
         self.config = config

@@ -89,6 +89,8 @@ class MixtralForCausalLM(nn.Module):
     """``forward(input_ids, labels)`` -> ``lm_loss + router_aux_loss_coef * load_balancing_loss``.  ``cu_seqlens``: samples end to
     end in one row, as in ``LlamaForCausalLM``; columns outside of them do not count in the balancing loss either."""
 
+    _fx_default_inputs = ("cu_seqlens",)                  # not an input of a pipeline's graph unless it is named
+
     _fx_wrap_functions = [load_balancing_loss_func]       # kept opaque by the pipeline tracer (pipeline/trace.py)
 
     def __init__(self, config: MixtralConfig, device=None):

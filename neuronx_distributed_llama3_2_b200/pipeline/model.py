@@ -290,6 +290,9 @@ class NxDPPModel(nn.Module):
     def _split_microbatches(self, kwargs: Dict[str, Any]) -> List[Dict[str, Any]]:
         n = self.num_microbatches
         out = [dict() for _ in range(n)]
+        for name in getattr(self.original_torch_module, "_fx_default_inputs", ()):
+            if kwargs.get(name) is not None and name not in (self.input_names or ()):
+                raise ValueError(f"`{name}` is fixed to its default in a pipeline")
         for name, val in kwargs.items():
             if isinstance(val, torch.Tensor) and val.dim() > 0:
                 if val.shape[0] % n != 0:

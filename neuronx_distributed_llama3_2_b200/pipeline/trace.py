@@ -48,10 +48,11 @@ class NxDTracer(fx.Tracer):
 
 
 def get_concrete_args(model: torch.nn.Module, input_names: Optional[List[str]]) -> Dict[str, Any]:
-    """Every ``forward`` parameter that is not a traced input is fixed to its default (reference ``:77-104``)."""
+    """Every ``forward`` parameter that is not a traced input is fixed to its default (reference ``:77-104``).  Without
+    ``input_names`` all are inputs but those that the model lists in ``_fx_default_inputs``."""
     sig = inspect.signature(model.forward)
     if input_names is None:
-        return {}
+        return {name: sig.parameters[name].default for name in getattr(model, "_fx_default_inputs", ()) if name in sig.parameters}
     concrete = {}
     for name, prm in sig.parameters.items():
         if name in input_names or prm.kind in (prm.VAR_POSITIONAL, prm.VAR_KEYWORD):

@@ -137,6 +137,35 @@ def test_bert_hidden_dropout():
         assert torch.equal(got[n], want[n]), n
 
 
+@pytest.mark.parametrize("family", ["llama", "mixtral", "bert"])
+def test_pipelines_trace_models_without_packed_rows(family):
+    from neuronx_distributed_llama3_2_b200.models.bert import BertLayer
+    from neuronx_distributed_llama3_2_b200.models.llama import LlamaDecoderLayer
+    from neuronx_distributed_llama3_2_b200.models.mixtral import MixtralDecoderLayer
+    from neuronx_distributed_llama3_2_b200.pipeline.model import NxDPPModel
+    from neuronx_distributed_llama3_2_b200.pipeline.trace import trace_model
+
+    make, config, layer = {"llama": (M.LlamaForCausalLM, M.tiny_llama, LlamaDecoderLayer), "bert": (BertForPreTraining, tiny_bert, BertLayer),
+                           "mixtral": (M.MixtralForCausalLM, M.tiny_mixtral, MixtralDecoderLayer)}[family]
+    torch.manual_seed(1)
+    model = make(config())
+    ids = torch.randint(0, 512, (1, 8))
+    want = model(ids, labels=ids)
+    everything = trace_model(model, leaf_modules=[layer])                  # as inputs, but those that have to be named
+    if family != "bert":                                                    # whose graph then takes a mask and token types
+        assert torch.equal(everything(ids, labels=ids), want)
+    traced = trace_model(model, input_names=["input_ids", "labels"], leaf_modules=[layer])
+    assert torch.equal(traced(input_ids=ids, labels=ids), want)
+    with pytest.raises(NotImplementedError):
+        trace_model(model, input_names=["input_ids", "labels", "cu_seqlens"], leaf_modules=[layer])
+    pipe = NxDPPModel.__new__(NxDPPModel)
+    torch.nn.Module.__init__(pipe)
+    pipe.original_torch_module, pipe.input_names, pipe.num_microbatches = model, None, 1
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        pipe._split_microbatches({"input_ids": ids, "cu_seqlens": torch.tensor([0, 8])})
+    assert pipe._split_microbatches({"input_ids": ids, "cu_seqlens": None})[0]["input_ids"] is not None
+
+
 def test_models_refuse():
     llama, bert = M.LlamaForCausalLM(M.tiny_llama()), BertForPreTraining(tiny_bert())
     cu, two, one = torch.tensor([0, 8]), torch.zeros(2, 8, dtype=torch.long), torch.zeros(1, 8, dtype=torch.long)
