@@ -105,7 +105,8 @@ class BertEmbeddings(nn.Module):
             extra = mappings.scatter_to_sequence_parallel_region(extra)
         elif tp > 1:
             words = mappings.gather_from_sequence_parallel_region(words, to_model_parallel=False)
-        return self.dropout(self.LayerNorm(words + extra))
+        hidden = self.LayerNorm(words + extra)
+        return self.dropout(hidden) if self.dropout.p else hidden
 
 
 class BertSelfAttention(nn.Module):
@@ -161,8 +162,11 @@ class BertLayer(nn.Module):
 
     def forward(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor],
                 packed: Optional[PackedSequences] = None) -> torch.Tensor:
-        x = self.attention_layernorm(self.dropout(self.attention(x, key_padding_mask, packed), x))
-        return self.output_layernorm(self.dropout(self.output(F.gelu(self.intermediate(x))), x))
+        x = self.attention_layernorm(self._add(x, self.attention(x, key_padding_mask, *(() if packed is None else (packed,)))))
+        return self.output_layernorm(self._add(x, self.output(F.gelu(self.intermediate(x)))))
+
+    def _add(self, x: torch.Tensor, branch: torch.Tensor) -> torch.Tensor:
+        return self.dropout(branch, x) if self.dropout.p else x + branch
 
 
 class BertForPreTraining(nn.Module):

@@ -81,7 +81,7 @@ class DbrxDecoderLayer(MixtralDecoderLayer):
         if residual is not None:
             hidden = hidden + residual
         residual = hidden
-        a = self.self_attn(self.input_layernorm(hidden), cos, sin, packed)
+        a = self.self_attn(self.input_layernorm(hidden), cos, sin, *(() if packed is None else (packed,)))
         residual = residual + a
         h = self.post_attention_layernorm(residual)
         if self.is_moe:

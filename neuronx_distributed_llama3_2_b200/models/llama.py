@@ -321,7 +321,7 @@ class LlamaDecoderLayer(nn.Module):
             h = norm_ops.rms_norm(hidden, self.input_layernorm.weight, eps)
         else:
             h, residual = norm_ops.fused_add_rms_norm(hidden, residual, self.input_layernorm.weight, eps)
-        a = self.self_attn(h, cos, sin, packed)
+        a = self.self_attn(h, cos, sin, *(() if packed is None else (packed,)))
         h, residual = norm_ops.fused_add_rms_norm(a, residual, self.post_attention_layernorm.weight, eps)
         return self.mlp(h), residual
 
