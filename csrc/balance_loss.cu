@@ -9,6 +9,9 @@
 // each, so a row is read in 16-byte pieces and the softmax is L-lane shuffles; a thread keeps its experts' sums and counts in
 // registers over all its rows.  Sums of a block go to global memory in a fixed order and a second kernel adds the blocks' in
 // double precision: no atomics, the loss does not depend on the schedule.
+//
+// Forward is bound by issue (half of the instructions are comparisons and selections, two clocks each): 240042 rows of 128 experts in
+// fp32, 8 of each, 73 us (memory alone: 19), 524288 rows of 64 66 us; backward by memory: 43 us (38).
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -190,13 +193,19 @@ __global__ void __launch_bounds__(kThreads) balance_fwd_kernel(const __grid_cons
         const long long r = r0 + threadIdx.x / L;
         const bool valid = r < rows && (a.mask == nullptr || a.mask[r] != 0);
         float x[V];
-        load_row<T, V>(x0 + min(r, rows - 1) * ld, e0, a.E, a.vec, x);
+        if (valid) {
+            load_row<T, V>(x0 + r * ld, e0, a.E, a.vec, x);
+        } else {                             // a row like any other, which counts nothing
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = 0.f;
+        }
         uint32_t key[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) key[i] = e0 + i < a.E ? order_key<T>(x[i], e0 + i) : 0u;
         softmax_row<L, V>(x);
+        const float one = valid ? 1.f : 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += valid ? x[i] : 0.f;
+        for (int i = 0; i < V; ++i) sum[i] = fmaf(x[i], one, sum[i]);
         // The k-th largest key: every lane's largest ones in order, and k times the largest first one of the row's lanes leaves its list.
         // Equal keys (fp32 only) would leave together: then more than k keys are as large as the last one, and the row's warp takes them
         // one by one, the lowest expert first.
@@ -204,12 +213,13 @@ __global__ void __launch_bounds__(kThreads) balance_fwd_kernel(const __grid_cons
         if (exact) {
             uint32_t h[8], last = 0u;
             top8<V>(key, h);
-            for (int j = 0; j < a.k; ++j) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j == a.k) break;
                 last = row_max<L>(h[0]);
                 const bool pop = h[0] == last;
 #pragma unroll
-                for (int i = 0; i < 7; ++i) h[i] = pop ? h[i + 1] : h[i];
-                h[7] = pop ? 0u : h[7];
+                for (int i = 0; i < 7 - j; ++i) h[i] = pop ? h[i + 1] : h[i];          // no more are asked for
             }
             int chosen = 0;
 #pragma unroll
@@ -218,11 +228,12 @@ __global__ void __launch_bounds__(kThreads) balance_fwd_kernel(const __grid_cons
                 int all = chosen;
 #pragma unroll
                 for (int o = 1; o < L; o <<= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-                exact = __all_sync(0xffffffffu, all == a.k);
+                exact = __all_sync(0xffffffffu, !valid || all == a.k);
             }
             if (exact) {
+                if (!valid) last = 0xffffffffu;          // above a zero's key
 #pragma unroll
-                for (int i = 0; i < V; ++i) count[i] += valid && key[i] >= last;
+                for (int i = 0; i < V; ++i) count[i] += key[i] >= last;
             }
         }
         if (!exact) {
@@ -372,14 +383,16 @@ __global__ void __launch_bounds__(kBwdThreads) balance_bwd_kernel(const __grid_c
 struct Plan {
     Layers layers;
     RouterArgs args;
+    long long most;                      // rows of the largest layer
     int blocks_x, n;
 };
 
-// blocks of a layer: enough of all layers together to fill the chip, no more than there are rows for
-int blocks_of(long long most_rows, int layers, int lanes, bool backward) {
-    const int threads = backward ? kBwdThreads : kThreads;
+// Blocks of a layer: all layers' together are on the chip at once and no more than that (half of a second round costs as much as a
+// whole one; with three blocks for each SM, whatever fits, 524288 rows of 64 experts took 88 us instead of 72, 160000 of 512 209
+// instead of 170, 240042 of 128 86 instead of 82), and no more than there are rows for.
+int blocks_of(long long most_rows, int layers, int lanes, int threads, int per_sm) {
     const long long want = (most_rows + threads / lanes - 1) / (threads / lanes);
-    const long long fill = ((backward ? 8ll : 3ll) * 148 + layers - 1) / layers, n = want < fill ? want : fill;
+    const long long fill = (long long)per_sm * nxd_num_sms() / layers, n = want < fill ? want : fill;
     return n < 1 ? 1 : (int)n;
 }
 int lanes_of(int E) {
@@ -406,45 +419,59 @@ int make_plan(Plan* p, const void* const* x, const long long* ld, const long lon
     NXD_REQUIRE(total < (1ll << 31) && total * k < (1ll << 40), "balance_loss: %lld rows", total);
     p->args = RouterArgs{(const unsigned char*)mask, E, k, vec};
     p->n = n;
-    p->blocks_x = blocks_of(most, n, lanes_of(E), dx != nullptr);
+    p->most = most;
     return 0;
 }
 
+template <auto Kernel>
+int blocks_per_sm(int threads) {
+    static const int n = [threads] {
+        int m = 0;
+        return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&m, Kernel, threads, 0) == cudaSuccess && m > 0 ? m : 1;
+    }();
+    return n;
+}
+
 template <typename T, int L, int V>
-int run(const Plan& p, float* part_p, int* part_c, const float* share, const float* grad, void* dx, cudaStream_t st) {
-    const dim3 grid(p.blocks_x, p.n);
-    if (dx == nullptr)
-        NXD_CHECK_CUDA((nxd_launch_pdl(balance_fwd_kernel<T, L, V>, grid, dim3(kThreads), 0, st, p.layers, p.args, part_p, part_c)));
-    else
-        NXD_CHECK_CUDA((nxd_launch_pdl(balance_bwd_kernel<T, L, V>, grid, dim3(kBwdThreads), 0, st, p.layers, p.args, share, grad, (T*)dx)));
+int run(Plan& p, float* scratch, const float* share, const float* grad, void* dx, cudaStream_t st) {
+    if (dx == nullptr) {
+        constexpr auto kern = balance_fwd_kernel<T, L, V>;
+        p.blocks_x = blocks_of(p.most, p.n, L, kThreads, blocks_per_sm<kern>(kThreads));
+        int* part_c = (int*)(scratch + (long long)p.blocks_x * p.n * p.args.E);
+        NXD_CHECK_CUDA((nxd_launch_pdl(kern, dim3(p.blocks_x, p.n), dim3(kThreads), 0, st, p.layers, p.args, scratch, part_c)));
+    } else {
+        constexpr auto kern = balance_bwd_kernel<T, L, V>;
+        p.blocks_x = blocks_of(p.most, p.n, L, kBwdThreads, blocks_per_sm<kern>(kBwdThreads));
+        NXD_CHECK_CUDA((nxd_launch_pdl(kern, dim3(p.blocks_x, p.n), dim3(kBwdThreads), 0, st, p.layers, p.args, share, grad, (T*)dx)));
+    }
     NXD_LAUNCH_CHECK();
     return 0;
 }
 
 template <typename T>
-int run_sized(const Plan& p, float* part_p, int* part_c, const float* share, const float* grad, void* dx, cudaStream_t st) {
+int run_sized(Plan& p, float* scratch, const float* share, const float* grad, void* dx, cudaStream_t st) {
     const int E = p.args.E;
-    if (E <= 8) return run<T, 1, 8>(p, part_p, part_c, share, grad, dx, st);
-    if (E <= 16) return run<T, 2, 8>(p, part_p, part_c, share, grad, dx, st);
-    if (E <= 32) return run<T, 4, 8>(p, part_p, part_c, share, grad, dx, st);
-    if (E <= 64) return run<T, 8, 8>(p, part_p, part_c, share, grad, dx, st);
-    if (E <= 128) return run<T, 16, 8>(p, part_p, part_c, share, grad, dx, st);
-    if (E <= 256) return run<T, 32, 8>(p, part_p, part_c, share, grad, dx, st);
-    if (E <= 512) return run<T, 32, 16>(p, part_p, part_c, share, grad, dx, st);
-    return run<T, 32, 32>(p, part_p, part_c, share, grad, dx, st);
+    if (E <= 8) return run<T, 1, 8>(p, scratch, share, grad, dx, st);
+    if (E <= 16) return run<T, 2, 8>(p, scratch, share, grad, dx, st);
+    if (E <= 32) return run<T, 4, 8>(p, scratch, share, grad, dx, st);
+    if (E <= 64) return run<T, 8, 8>(p, scratch, share, grad, dx, st);
+    if (E <= 128) return run<T, 16, 8>(p, scratch, share, grad, dx, st);
+    if (E <= 256) return run<T, 32, 8>(p, scratch, share, grad, dx, st);
+    if (E <= 512) return run<T, 32, 16>(p, scratch, share, grad, dx, st);
+    return run<T, 32, 32>(p, scratch, share, grad, dx, st);
 }
 
-int run_typed(const Plan& p, int dtype, float* part_p, int* part_c, const float* share, const float* grad, void* dx, cudaStream_t st) {
-    if (dtype == 0) return run_sized<float>(p, part_p, part_c, share, grad, dx, st);
-    if (dtype == 1) return run_sized<bf16>(p, part_p, part_c, share, grad, dx, st);
-    return run_sized<__half>(p, part_p, part_c, share, grad, dx, st);
+int run_typed(Plan& p, int dtype, float* scratch, const float* share, const float* grad, void* dx, cudaStream_t st) {
+    if (dtype == 0) return run_sized<float>(p, scratch, share, grad, dx, st);
+    if (dtype == 1) return run_sized<bf16>(p, scratch, share, grad, dx, st);
+    return run_sized<__half>(p, scratch, share, grad, dx, st);
 }
 
 }  // namespace
 
-// Blocks of the first kernel: its scratch is that many times E floats and as many ints.
+// Blocks of the first kernel at most: its scratch is that many times E floats and as many ints.
 NXD_API int nxd_balance_loss_num_blocks(long long most_rows, int layers, int E) {
-    return blocks_of(most_rows, layers, lanes_of(E), false) * layers;
+    return blocks_of(most_rows, layers, lanes_of(E), kThreads, 2048 / kThreads) * layers;
 }
 
 // x, ld, rows: HOST arrays of `layers` device pointers, row strides (elements; unit stride along the experts) and row counts;
@@ -457,13 +484,12 @@ NXD_API int nxd_balance_loss_fwd(const void* const* x, const long long* ld, cons
     Plan p;
     int rc = make_plan(&p, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, nullptr);
     if (rc) return rc;
-    const int blocks = p.blocks_x * layers;
-    float* part_p = (float*)scratch;
-    int* part_c = (int*)(part_p + (long long)blocks * E);
     cudaStream_t st = (cudaStream_t)stream;
-    if ((rc = run_typed(p, dtype, part_p, part_c, nullptr, nullptr, nullptr, st))) return rc;
-    NXD_CHECK_CUDA(nxd_launch_pdl(balance_final_kernel, dim3(1), dim3(kFinalThreads), 0, st, (const float*)part_p, (const int*)part_c, blocks,
-                                  E, k, loss, counts, share));
+    if ((rc = run_typed(p, dtype, (float*)scratch, nullptr, nullptr, nullptr, st))) return rc;
+    const int blocks = p.blocks_x * layers;
+    const float* part_p = (const float*)scratch;
+    const int* part_c = (const int*)(part_p + (long long)blocks * E);
+    NXD_CHECK_CUDA(nxd_launch_pdl(balance_final_kernel, dim3(1), dim3(kFinalThreads), 0, st, part_p, part_c, blocks, E, k, loss, counts, share));
     NXD_LAUNCH_CHECK();
     return 0;
 }
@@ -475,5 +501,5 @@ NXD_API int nxd_balance_loss_bwd(const void* const* x, const long long* ld, cons
     Plan p;
     int rc = make_plan(&p, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, dx);
     if (rc) return rc;
-    return run_typed(p, dtype, nullptr, nullptr, share, grad, dx, (cudaStream_t)stream);
+    return run_typed(p, dtype, nullptr, share, grad, dx, (cudaStream_t)stream);
 }
