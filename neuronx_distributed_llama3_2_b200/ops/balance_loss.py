@@ -47,6 +47,7 @@ class _BalanceLossFn(torch.autograd.Function):
                                           _c.c_void_p(share.data_ptr() + 4 * E), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_fwd")
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)         # no zeros for the counts' gradient
         ctx.save_for_backward(share, mask, *rows)
         ctx.args = (table, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
         return loss, counts
@@ -54,6 +55,8 @@ class _BalanceLossFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _):
+        if grad is None:
+            return (None,) * len(ctx.needs_input_grad)
         saved = ctx.saved_tensors          # all of them: none may have been written since
         share, x = saved[0], saved[2]
         table, sizes, shapes = ctx.args
