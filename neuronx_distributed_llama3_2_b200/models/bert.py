@@ -40,7 +40,9 @@ class BertConfig:
     type_vocab_size: int = 2
     layer_norm_eps: float = 1e-12
     initializer_range: float = 0.02
-    hidden_dropout_prob: float = 0.0        # on both residual branches of a layer and on the embeddings
+    # on both residual branches of a layer and on the embeddings; a name of its own: the dropout entries of a checkpoint's
+    # ``config.json`` stay unread
+    residual_dropout: float = 0.0
     sequence_parallel_enabled: bool = False
     activation_checkpointing: bool = False
     torch_dtype: torch.dtype = torch.bfloat16
@@ -68,7 +70,7 @@ def _tag_sp(module: nn.Module, enabled: bool) -> None:
 
 def _hidden_dropout(config: BertConfig) -> Dropout:
     """Dropout of hidden states, with the residual added in the same pass; sequence shards draw different masks."""
-    return Dropout(config.hidden_dropout_prob, offset=ps.get_tensor_model_parallel_rank() if config.sequence_parallel_enabled else 0)
+    return Dropout(config.residual_dropout, offset=ps.get_tensor_model_parallel_rank() if config.sequence_parallel_enabled else 0)
 
 
 class BertEmbeddings(nn.Module):

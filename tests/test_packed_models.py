@@ -113,8 +113,15 @@ def test_bert_row_of_sentences():
     _compare(got, _grads(model))
 
 
+def test_dropout_of_a_checkpoint_file_stays_unread():
+    from neuronx_distributed_llama3_2_b200.models.llama import config_from_json
+
+    cfg = config_from_json(type(tiny_bert()), {"hidden_size": 128, "hidden_dropout_prob": 0.1, "attention_probs_dropout_prob": 0.1})
+    assert cfg.residual_dropout == 0.0 and cfg.hidden_size == 128
+
+
 def test_bert_hidden_dropout():
-    cfg = tiny_bert(hidden_dropout_prob=0.3)
+    cfg = tiny_bert(residual_dropout=0.3)
     torch.manual_seed(6)
     model = BertForPreTraining(cfg)
     torch.manual_seed(6)
