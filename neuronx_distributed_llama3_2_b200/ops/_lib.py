@@ -210,7 +210,6 @@ def lib(group: Optional[str] = None) -> ctypes.CDLL:
                 try:
                     cdll = ctypes.CDLL(build(group=group))
                     cdll.nxd_last_error.restype = ctypes.c_char_p
-                    cdll.nxd_capture_id.restype = ctypes.c_ulonglong
                     handle = _GroupLibrary(cdll)
                 except OSError:          # a source of the group needs a symbol from outside it: use the full library
                     handle = None
@@ -231,7 +230,6 @@ def _full_lib() -> ctypes.CDLL:
                 build()
             handle = ctypes.CDLL(LIB_PATH)
             handle.nxd_last_error.restype = ctypes.c_char_p
-            handle.nxd_capture_id.restype = ctypes.c_ulonglong
             _lib = handle
     return _lib
 

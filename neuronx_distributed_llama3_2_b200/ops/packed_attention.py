@@ -48,7 +48,11 @@ class PackedSequences:
         if not self.cu_seqlens.is_cuda:
             return 0, 0
         stream = torch._C._cuda_getCurrentRawStream(self.cu_seqlens.get_device())
-        return stream, _lib.lib().nxd_capture_id(_c.c_void_p(stream)) if _lib.available() else 0
+        if not _lib.available():
+            return stream, 0
+        capture_id = _lib.lib().nxd_capture_id
+        capture_id.restype = _c.c_ulonglong
+        return stream, capture_id(_c.c_void_p(stream))
 
     def plan(self, causal: bool, rows: int = 128) -> Tuple[torch.Tensor, int, int]:
         """``(list of tiles of that many rows, its entries, columns of the per-row scratch)`` for the kernels, made on first use."""
