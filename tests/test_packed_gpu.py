@@ -154,6 +154,21 @@ def test_strides_and_a_second_stream():
         check(got[name], want, name)
 
 
+def test_rows_further_apart_than_32_bits():
+    """Queries and the results' gradients as views of a row store of 2.4e9 elements."""
+    T, H, G, D = 300, 4, 2, 64
+    q, k, v, do = _inputs(T, H, G, D)
+    store = torch.empty((T, 8 << 20), dtype=torch.bfloat16, device="cuda")
+    views = [store[:, at:at + H * D].view(T, H, D) for at in (0, 1 << 22)]
+    for view, x in zip(views, (q, do)):
+        view.copy_(x)
+    ends = [0, 130, 290]
+    want = packed(q, k, v, ends, True, do)
+    got = _run(views[0], k, v, views[1], ends, True)
+    for name in got:
+        check(got[name], want, name)
+
+
 def test_one_list_for_several_calls_and_no_gradients():
     from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
     from neuronx_distributed_llama3_2_b200.ops.packed_attention import PackedSequences
