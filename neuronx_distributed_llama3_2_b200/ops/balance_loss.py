@@ -38,11 +38,11 @@ class _BalanceLossFn(torch.autograd.Function):
         table = ((_c.c_void_p * n)(*[t.data_ptr() for t in rows]), (_c.c_longlong * n)(*[t.stride(0) for t in rows]),
                  (_c.c_longlong * n)(*sizes), _c.c_int(n), _c.c_int(_DTYPES[x.dtype]), _lib.ptr(mask), _c.c_int(E), _c.c_int(top_k))
         lib = _lib.lib()
-        blocks = lib.nxd_balance_loss_num_blocks(_c.c_longlong(max(sizes)), _c.c_int(n), _c.c_int(E))
         loss = torch.empty((), dtype=torch.float32, device=x.device)
         counts = torch.empty(E, dtype=torch.int64, device=x.device)
-        share = torch.empty(E + 2 * blocks * E, dtype=torch.float32, device=x.device)     # the shares, then the call's scratch
         with _lib.on_device_of(x):
+            blocks = lib.nxd_balance_loss_num_blocks(_c.c_longlong(max(sizes)), _c.c_int(n), _c.c_int(E))
+            share = torch.empty(E + 2 * blocks * E, dtype=torch.float32, device=x.device)     # the shares, then the call's scratch
             rc = lib.nxd_balance_loss_fwd(*table, _lib.ptr(loss), _lib.ptr(counts), _lib.ptr(share),
                                           _c.c_void_p(share.data_ptr() + 4 * E), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_fwd")
