@@ -3,7 +3,7 @@ forward (and a small one that adds up), one backward.  ``modules.moe.load_balanc
 from __future__ import annotations
 
 import ctypes as _c
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -28,28 +28,32 @@ def qualifies(logits: List[torch.Tensor], E: int) -> bool:
             and all(t.dtype is dtype and t.get_device() == device for t in logits) and _lib.available())
 
 
+def _table(rows: Sequence[torch.Tensor], mask: Optional[torch.Tensor], E: int, top_k: int) -> tuple:
+    """The entry points' first arguments: pointers, row strides and rows of the layers, and what they share."""
+    n = len(rows)
+    return ((_c.c_void_p * n)(*[t.data_ptr() for t in rows]), (_c.c_longlong * n)(*[t.stride(0) for t in rows]),
+            (_c.c_longlong * n)(*[t.shape[0] for t in rows]), _c.c_int(n), _c.c_int(_DTYPES[rows[0].dtype]), _lib.ptr(mask), _c.c_int(E),
+            _c.c_int(top_k))
+
+
 class _BalanceLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, E, top_k, mask, *logits):
         rows = [_rows(t, E) for t in logits]
         sizes = [t.shape[0] for t in rows]
-        n, x = len(rows), rows[0]
-        # pointers, row strides, rows: built once, the backward call reads the same tensors
-        table = ((_c.c_void_p * n)(*[t.data_ptr() for t in rows]), (_c.c_longlong * n)(*[t.stride(0) for t in rows]),
-                 (_c.c_longlong * n)(*sizes), _c.c_int(n), _c.c_int(_DTYPES[x.dtype]), _lib.ptr(mask), _c.c_int(E), _c.c_int(top_k))
-        lib = _lib.lib()
+        n, x, lib = len(rows), rows[0], _lib.lib()
         loss = torch.empty((), dtype=torch.float32, device=x.device)
         counts = torch.empty(E, dtype=torch.int64, device=x.device)
         with _lib.on_device_of(x):
             blocks = lib.nxd_balance_loss_num_blocks(_c.c_longlong(max(sizes)), _c.c_int(n), _c.c_int(E))
             share = torch.empty(E + 2 * blocks * E, dtype=torch.float32, device=x.device)     # the shares, then the call's scratch
-            rc = lib.nxd_balance_loss_fwd(*table, _lib.ptr(loss), _lib.ptr(counts), _lib.ptr(share),
+            rc = lib.nxd_balance_loss_fwd(*_table(rows, mask, E, top_k), _lib.ptr(loss), _lib.ptr(counts), _lib.ptr(share),
                                           _c.c_void_p(share.data_ptr() + 4 * E), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_fwd")
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)         # no zeros for the counts' gradient
         ctx.save_for_backward(share, mask, *rows)
-        ctx.args = (table, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
+        ctx.args = (E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
         return loss, counts
 
     @staticmethod
@@ -57,13 +61,14 @@ class _BalanceLossFn(torch.autograd.Function):
     def backward(ctx, grad, _):
         if grad is None:
             return (None,) * len(ctx.needs_input_grad)
-        saved = ctx.saved_tensors          # all of them: none may have been written since
-        share, x = saved[0], saved[2]
-        table, sizes, shapes = ctx.args
+        share, mask, *rows = ctx.saved_tensors          # which may lie elsewhere now (checkpointing, offloading)
+        E, top_k, sizes, shapes = ctx.args
+        rows = [_rows(t, E) for t in rows]
+        x = rows[0]
         dx = torch.empty((sum(sizes), x.shape[1]), dtype=x.dtype, device=x.device)
         grad = grad.float()
         with _lib.on_device_of(x):
-            rc = _lib.lib().nxd_balance_loss_bwd(*table, _lib.ptr(share), _lib.ptr(grad), _lib.ptr(dx), _lib.stream_ptr())
+            rc = _lib.lib().nxd_balance_loss_bwd(*_table(rows, mask, E, top_k), _lib.ptr(share), _lib.ptr(grad), _lib.ptr(dx), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_bwd")
         grads = dx.split(sizes)
         if any(s is not None for s in shapes):

@@ -150,7 +150,7 @@ def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad:
 
 def _backward(q, k, v, o, lse, rest, do, dq, dk, dv, plan, count: int, scale: float, causal: bool) -> None:
     """Every element of ``dq / dk / dv`` is written.  ``plan``: the list that the forward pass had, or one made with it."""
-    do = _fix(do)
+    q, k, v, o, do = (_fix(t) for t in (q, k, v, o, do))          # what was saved may have been moved
     T, Hq, D = q.shape
     Hkv = k.shape[1]
     tiles, entries, columns = plan

@@ -164,6 +164,32 @@ def test_same_bits_twice_captured_and_on_another_stream():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how", ["checkpoint", "on the host"])
+def test_saved_logits_that_move(how):
+    """What the backward pass reads is computed again, or copied back, and lies elsewhere than in the forward pass."""
+    from torch.utils.checkpoint import checkpoint
+
+    weight = torch.randn(16, 8, generator=torch.Generator().manual_seed(2)).cuda().requires_grad_()
+    hidden = [torch.randn(200, 16, generator=torch.Generator().manual_seed(i)).cuda() for i in range(3)]
+
+    def loss():
+        return load_balancing_loss_func([h @ weight for h in hidden], 8, 2)
+
+    def again():
+        if how == "checkpoint":
+            return checkpoint(loss, use_reentrant=False)
+        with torch.autograd.graph.save_on_cpu():
+            return loss()
+
+    (want,) = torch.autograd.grad(loss(), weight)
+    out = again()
+    trash = [torch.full((200, 8), math.nan, device="cuda") for _ in range(64)]          # where the logits were
+    (got,) = torch.autograd.grad(out, weight)
+    assert torch.equal(got, want)
+    del trash
+
+
+@pytest.mark.gpu
 def test_part_of_the_layers_needs_gradients():
     a, b = _logits(2, 40, 8, torch.float32, "cuda")
     a.requires_grad_()

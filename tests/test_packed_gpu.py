@@ -286,6 +286,31 @@ def test_delta_is_not_of_the_rounded_result(D):
     assert (got["dq"] != 0).any(-1).float().mean() <= 0.1
 
 
+@pytest.mark.parametrize("how", ["checkpoint", "on the host"])
+def test_saved_tensors_that_move(how):
+    from torch.utils.checkpoint import checkpoint
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+
+    T, ends = 300, [0, 120, 290]
+    q, k, v, do = _inputs(T, 4, 2, 64)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    cu = torch.tensor(ends, device="cuda")
+
+    def attend():
+        return flash_attn_packed_func(*(x * 1.0 for x in leaves), cu)
+
+    if how == "checkpoint":
+        o = checkpoint(attend, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            o = attend()
+    trash = [torch.full((T, 4, 64), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(32)]
+    want = packed(q, k, v, ends, True, do)
+    for name, x in zip(("o", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, leaves, do))):
+        check(x, want, name)
+    del trash
+
+
 def test_tables_shorter_than_the_row():
     """Rotation tables as long as the longest sequence are enough, and a sequence that is longer reads no further."""
     from neuronx_distributed_llama3_2_b200.ops import attention, rope
