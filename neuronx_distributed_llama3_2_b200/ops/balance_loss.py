@@ -36,6 +36,10 @@ def _table(rows: Sequence[torch.Tensor], mask: Optional[torch.Tensor], E: int, t
             _c.c_int(top_k))
 
 
+# what moves saved tensors: the innermost pair of hooks, None without one
+_saved_hooks = getattr(torch._C._autograd, "_top_saved_tensors_default_hooks", lambda _: "unknown")
+
+
 class _BalanceLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, E, top_k, mask, *logits):
@@ -44,16 +48,18 @@ class _BalanceLossFn(torch.autograd.Function):
         n, x, lib = len(rows), rows[0], _lib.lib()
         loss = torch.empty((), dtype=torch.float32, device=x.device)
         counts = torch.empty(E, dtype=torch.int64, device=x.device)
+        table = _table(rows, mask, E, top_k)
         with _lib.on_device_of(x):
             blocks = lib.nxd_balance_loss_num_blocks(_c.c_longlong(max(sizes)), _c.c_int(n), _c.c_int(E))
             share = torch.empty(E + 2 * blocks * E, dtype=torch.float32, device=x.device)     # the shares, then the call's scratch
-            rc = lib.nxd_balance_loss_fwd(*_table(rows, mask, E, top_k), _lib.ptr(loss), _lib.ptr(counts), _lib.ptr(share),
+            rc = lib.nxd_balance_loss_fwd(*table, _lib.ptr(loss), _lib.ptr(counts), _lib.ptr(share),
                                           _c.c_void_p(share.data_ptr() + 4 * E), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_fwd")
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)         # no zeros for the counts' gradient
         ctx.save_for_backward(share, mask, *rows)
-        ctx.args = (E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
+        # 32 layers' table costs a tenth of the call: the backward pass makes it again only where what was saved may have moved
+        ctx.args = (table if _saved_hooks(True) is None else None, E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
         return loss, counts
 
     @staticmethod
@@ -61,14 +67,16 @@ class _BalanceLossFn(torch.autograd.Function):
     def backward(ctx, grad, _):
         if grad is None:
             return (None,) * len(ctx.needs_input_grad)
-        share, mask, *rows = ctx.saved_tensors          # which may lie elsewhere now (checkpointing, offloading)
-        E, top_k, sizes, shapes = ctx.args
-        rows = [_rows(t, E) for t in rows]
-        x = rows[0]
+        saved = ctx.saved_tensors          # all of them: none may have been written since
+        table, E, top_k, sizes, shapes = ctx.args
+        share, x = saved[0], saved[2]
+        if table is None:                  # checkpointing, offloading
+            rows = [_rows(t, E) for t in saved[2:]]
+            table = _table(rows, saved[1], E, top_k)
         dx = torch.empty((sum(sizes), x.shape[1]), dtype=x.dtype, device=x.device)
         grad = grad.float()
         with _lib.on_device_of(x):
-            rc = _lib.lib().nxd_balance_loss_bwd(*_table(rows, mask, E, top_k), _lib.ptr(share), _lib.ptr(grad), _lib.ptr(dx), _lib.stream_ptr())
+            rc = _lib.lib().nxd_balance_loss_bwd(*table, _lib.ptr(share), _lib.ptr(grad), _lib.ptr(dx), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_bwd")
         grads = dx.split(sizes)
         if any(s is not None for s in shapes):
