@@ -65,7 +65,8 @@ struct FwdSmem {
 static_assert(FwdSmem<128>::kBytes <= 232448 && FwdSmem<64>::kBytes > 116 * 1024, "one CTA per SM");
 
 struct alignas(16) Item {
-    int kind, start, len, pad;           // kind: 0 end of the list, 1 an item, above: that many (less kRowsOfNone) rows from `start` are of no sequence
+    int kind, start, len, pad;           // kind: 0 end of the items (`start`: the CTA's round that comes next), 1 an item, above: that many (less
+                                         // kRowsOfNone) rows from `start` are of no sequence
     int t0, t1, n0, n1;                  // query tiles and the key tiles that they meet (0: there is no second one)
     int h0, h1, hkv, unused;
     __device__ __forceinline__ int t(int s) const { return s ? t1 : t0; }
@@ -84,7 +85,7 @@ __device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
     it.start = pt.start, it.len = pt.len, it.pad = pt.pad;
     it.h0 = HEADS ? 2 * pr : pr;
     it.h1 = HEADS ? it.h0 + 1 : it.h0;
-    if (pt.len == 0) {                   // an entry without anything: all that follow are like it
+    if (pt.len == 0) {                   // behind all items; an entry without anything: all that follow are like it
         it.kind = pt.t > 0 ? pt.t + kRowsOfNone : 0;
         return it;
     }
@@ -187,12 +188,17 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         // the item whose keys come next and its next key tile; the same of the values, which are one tile behind at most
         Item ki{}, vi{}, ahead = fetch_item<CAUSAL, HEADS>(p, round++);
         int kj = 0, vj = 0;
-        auto publish = [&]() {               // goes on to the next item with scores; the one behind it is read meanwhile
-            do {
-                ki = ahead;
-                if (ki.kind) ahead = fetch_item<CAUSAL, HEADS>(p, round++);
-                publish_item(ki, item_ring, item_full, item_empty, published, dead);
-            } while (ki.kind > 1);
+        // Goes on to the next item, of which the last value tile of this one must not wait for more than one: the readers take one more
+        // before they end this one.  Rows of no sequence are behind all items and do not go through the ring.
+        auto publish = [&]() {
+            ki = ahead;
+            if (ki.kind == 1) {              // the one behind it is read meanwhile
+                ahead = fetch_item<CAUSAL, HEADS>(p, round++);
+            } else {
+                ki = Item{};
+                ki.start = round - 1;
+            }
+            publish_item(ki, item_ring, item_full, item_empty, published, dead);
             kj = 0;
         };
         auto load = [&](const CUtensorMap* map, const int* pos, uint64_t* bar, uint8_t* dst, int row, int h) {
@@ -257,12 +263,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             int it = 0, items = 0, loads[kMine] = {}, tiles[kMine] = {}, done[kMine] = {};
             int n[kMine] = {}, steps = 0;     // key tiles that the query tiles meet in the item whose scores come next, and those of the item
             auto next = [&]() {
-                Item x;
-                do x = next_item<false, Item>(item_ring, item_full, item_empty, items, dead);
-                while (x.kind > 1);
+                const Item x = next_item<false, Item>(item_ring, item_full, item_empty, items, dead);
 #pragma unroll
-                for (int i = 0; i < kMine; ++i) n[i] = x.kind == 1 ? x.n(s0 + i) : 0;
-                steps = x.kind == 1 ? max(x.n0, x.n1) : 0;
+                for (int i = 0; i < kMine; ++i) n[i] = x.n(s0 + i);
+                steps = max(x.n0, x.n1);
             };
             auto slot = [&]() {
                 const int at = it % L::kSlots;
@@ -453,13 +457,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         Item it = next_item<true, Item>(item_ring, item_full, item_empty, items, dead);
         for (; it.kind != 0;) {
             const int head = it.h(s), n = it.n(s), t = it.t(s);
-            if (it.kind > 1) {                           // rows of no sequence; once a head
-                if (HEADS || s == 0)
-                    for (int i = threadIdx.x & 127; i < (it.kind - kRowsOfNone) * (D / 8); i += 128)
-                        *reinterpret_cast<uint4*>(p.o + head * p.o_head + (long long)(it.start + i / (D / 8)) * p.o_row + (i % (D / 8)) * 8) =
-                            make_uint4(0u, 0u, 0u, 0u);
-            }
-            if (it.kind > 1 || n == 0) {
+            if (n == 0) {
                 it = next_item<true, Item>(item_ring, item_full, item_empty, items, dead);
                 continue;
             }
@@ -548,6 +546,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             }
             ptx::tcgen05_fence_before();
         }
+        // zeros for rows of no sequence, once a head
+        for (int round = it.start;; ++round) {
+            it = fetch_item<CAUSAL, HEADS>(p, round);
+            if (it.kind <= 1) break;
+            if (HEADS || s == 0)
+                for (int i = threadIdx.x & 127; i < (it.kind - kRowsOfNone) * (D / 8); i += 128)
+                    *reinterpret_cast<uint4*>(p.o + it.h(s) * p.o_head + (long long)(it.start + i / (D / 8)) * p.o_row + (i % (D / 8)) * 8) =
+                        make_uint4(0u, 0u, 0u, 0u);
+        }
         if (lane == 0) ptx::bulk_wait<0>();
     } else if (warp == 10) {
         // ============================ ends of sequences ============================
@@ -559,7 +566,6 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         for (;;) {
             const Item x = next_item<true, Item>(item_ring, item_full, item_empty, items, dead);
             if (x.kind == 0) break;
-            if (x.kind > 1) continue;
             const int n = max(x.n0, x.n1), left = x.len - (n - 1) * kBN;
             it += 2 * n;                       // keys and values of the item; its last values are the last of them
             if (left >= kBN) continue;

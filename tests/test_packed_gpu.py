@@ -94,6 +94,24 @@ def test_long_and_many(lens, H, G, D, causal):
         check(got[name], want, name)
 
 
+# long stretches of no sequence: so many entries that every CTA has several of them in a row behind its items, whose last value tiles are
+# whole or cut
+@pytest.mark.parametrize("lens,first,T", [([3400], 0, 8192), ([100], 0, 8192), ([8000], 0, 16384), ([3192], 5000, 8192), ([300, 1664], 3000, 9000),
+                                          ([2000, 128], 4000, 12000)])
+@pytest.mark.parametrize("H,G,D,causal", [(32, 8, 64, True), (32, 8, 128, False), (12, 12, 64, False), (9, 3, 128, True)])
+def test_long_gaps(lens, first, T, H, G, D, causal):
+    q, k, v, do = _inputs(T, H, G, D)
+    ends = _ends(lens, first)
+    inside = slice(first, ends[-1])
+    for x in (q, k, v, do):                          # what lies between is nobody's
+        x[:first], x[ends[-1]:] = float("nan"), float("nan")
+    got = _run(q, k, v, do, ends, causal)
+    want = packed(*(x[inside] for x in (q, k, v)), [e - first for e in ends], causal, do[inside])
+    for name in got:
+        check(got[name][inside], want, name)
+        assert not got[name][:first].any() and not got[name][ends[-1]:].any()
+
+
 # scores that rise along the keys (the running maximum moves in every tile) and scores that leave one weight
 @pytest.mark.parametrize("scale", [0.01, 1.0, None])
 def test_scales(scale):
