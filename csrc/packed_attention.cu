@@ -40,9 +40,10 @@ struct FwdParams {
     float* lse;
     uint8_t* rest;                                // what rounding to bf16 took from o (attn_tc_common.cuh), NULL: not wanted
     bf16* o;
-    const bf16* v;
-    long long lse_row, o_head, o_row, v_head, v_row;
-    int entries, Hq, group, pairs;                // pairs: items of one tile-list entry
+    int* gave_up;                                 // host memory (packed_items.cuh)
+    long long lse_row, o_head, o_row;
+    int entries, group, pairs;                    // pairs: items of one tile-list entry
+    int tries;                                    // of a wait
     int pos_q[3], pos_k[3], pos_v[3], pos_o[3];
     float scale_log2;
 };
@@ -116,6 +117,26 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// What a CTA that gave up a wait leaves: NaN for all its items, those among them that were ready, and zeros for rows of no sequence.
+template <int D, bool CAUSAL, bool HEADS>
+__device__ __forceinline__ void leave_nan(const FwdParams& p) {
+    for (int round = 0;; ++round) {
+        const Item x = fetch_item<CAUSAL, HEADS>(p, round);
+        if (x.kind == 0) break;
+        for (int s = 0; s < 2; ++s) {
+            if (x.kind > 1 ? s == 1 && !HEADS : x.n(s) == 0) continue;
+            const int first = x.kind > 1 ? 0 : x.t(s) * kBM, rows = x.kind > 1 ? x.kind - kRowsOfNone : min(x.len - first, kBM);
+            const uint32_t fill = x.kind > 1 ? 0u : 0x7fff7fffu;
+            for (int i = threadIdx.x; i < rows * (D / 8); i += kThreads)
+                *reinterpret_cast<uint4*>(p.o + x.h(s) * p.o_head + (long long)(x.start + first + i / (D / 8)) * p.o_row + (i % (D / 8)) * 8) =
+                    make_uint4(fill, fill, fill, fill);
+            if (x.kind == 1 && p.lse != nullptr)
+                for (int i = threadIdx.x; i < rows; i += kThreads) p.lse[x.h(s) * p.lse_row + x.pad + first + i] = NAN;
+        }
+    }
+    if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(p.gave_up) = 1;
+}
+
 template <int D, bool CAUSAL, bool HEADS>
 __global__ void __launch_bounds__(kThreads, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -145,7 +166,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        dead_word = 0;
+        dead_word = p.tries - kTries;
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(&q_full[s], 1);
             ptx::mbar_init(&q_empty[s], 1);
@@ -192,6 +213,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         // before they end this one.  Rows of no sequence are behind all items and do not go through the ring.
         auto publish = [&]() {
             ki = ahead;
+            if (__shfl_sync(0xffffffffu, gave_up(dead), 0)) ki.kind = 0;
             if (ki.kind == 1) {              // the one behind it is read meanwhile
                 ahead = fetch_item<CAUSAL, HEADS>(p, round++);
             } else {
@@ -202,6 +224,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             kj = 0;
         };
         auto load = [&](const CUtensorMap* map, const int* pos, uint64_t* bar, uint8_t* dst, int row, int h) {
+            if (gave_up(dead)) return;           // what was loaded there before may be on its way still
             ptx::mbar_arrive_expect_tx(bar, L::kTileBytes);
             int c[4];
 #pragma unroll
@@ -478,7 +501,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             ptx::tcgen05_fence_after();
             const int at = t * kBM + row;
             const bool real = at < done.len;
-            if (m == -INFINITY || *dead) l = NAN;
+            if (m == -INFINITY) l = NAN;
             const float inv = 1.f / l;
             if (p.lse != nullptr && real) p.lse[head * p.lse_row + done.pad + at] = m * sc + log2f(l);
             // through shared memory, 32 rows x 64 columns at a time: stored by rows from the registers, a warp's 16-byte pieces fall into
@@ -584,7 +607,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     ptx::tcgen05_fence_before();
     __syncthreads();
-    if (dead_word) let_copies_land();
+    if (gave_up(dead)) {
+        let_copies_land();
+        leave_nan<D, CAUSAL, HEADS>(p);
+    }
     if (warp == 8) ptx::tmem_dealloc<1>(tmem, 512);
 }
 
@@ -608,13 +634,38 @@ int launch_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& t
 
 }  // namespace
 
+// The word is there as long as the process, for graphs that are replayed.
+int nxd_packed::begin_call(int** word) {
+    static int* const shared = [] {
+        int* w = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;          // the first call may be a captured one
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (cudaHostAlloc((void**)&w, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) w = nullptr;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (w != nullptr) *w = 0;
+        return w;
+    }();
+    NXD_REQUIRE(shared != nullptr, "packed_attn: no host memory for %s", "the status word");
+    *word = shared;
+    NXD_REQUIRE(__atomic_exchange_n(shared, 0, __ATOMIC_RELAXED) == 0, "packed_attn: a call before this one gave up a wait; %s", "its results are NaN");
+    return 0;
+}
+
+// *gave_up <- whether a call gave up a wait since the last one that failed or asked for it.  Waits for the stream.
+NXD_API int nxd_packed_attn_status(int* gave_up, void* stream) {
+    int* word;
+    NXD_CHECK_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+    *gave_up = nxd_packed::begin_call(&word) != 0;
+    return 0;
+}
+
 // Attention inside each sequence of a packed batch: q [T, Hq, D], k and v [T, Hkv, D], o [T, Hq, D], strides {q_h, q_row, k_h,
 // k_row, v_h, v_row, o_h, o_row} in elements (multiples of 8), 16-byte aligned bases; tiles: the `entries` tiles that
 // nxd_packed_plan has made; lse NULL or [Hq, lse_row] floats, log2 units, written at the plan's padded columns; rest NULL or [Hq, lse_row,
-// D] bytes, for the backward pass.  Rows outside every sequence get zeros.
+// D] bytes, for the backward pass.  Rows outside every sequence get zeros.  wait_tries: after which a wait gives up, -1: two seconds.
 NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const long long* strides,
                                 const void* tiles, int entries, long long lse_row, long long T, int Hq, int Hkv, int D, float scale,
-                                int causal, void* stream) {
+                                int causal, int wait_tries, void* stream) {
     NXD_REQUIRE(D == 64 || D == 128, "packed_attn: head dim %d not supported (64 or 128)", D);
     NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && (long long)entries * Hq < (1ll << 31),
                 "packed_attn: bad problem");
@@ -623,17 +674,18 @@ NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, voi
     NXD_REQUIRE(q && k && v && o && tiles && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)tiles) & 15) == 0 && lse_row % 4 == 0,
                 "packed_attn: tensors must be 16-byte aligned, rows of the scratch multiples of four");
     FwdParams p{};
+    int rc;
+    if ((rc = begin_call(&p.gave_up))) return rc;
+    p.tries = wait_tries < 0 || wait_tries > kTries ? kTries : wait_tries;
     p.tiles = (const PackedTile*)tiles;
     p.entries = entries;
     p.lse = lse; p.lse_row = lse_row;
     p.rest = (uint8_t*)rest;
-    p.Hq = Hq; p.group = Hq / Hkv;
+    p.group = Hq / Hkv;
     p.pairs = p.group % 2 == 0 ? Hq / 2 : Hq;
     p.scale_log2 = scale * 1.4426950408889634f;
-    p.v = (const bf16*)v; p.v_head = strides[4]; p.v_row = strides[5];
     p.o = (bf16*)o; p.o_head = strides[6]; p.o_row = strides[7];
     CUtensorMap tq, tk, tv, to;
-    int rc;
     if ((rc = make_tmap_bhsd(&tq, q, D, T, Hq, 1, strides[1], strides[0], 0, kBM, p.pos_q))) return rc;
     if ((rc = make_tmap_bhsd(&tk, k, D, T, Hkv, 1, strides[3], strides[2], 0, kBN, p.pos_k))) return rc;
     if ((rc = make_tmap_bhsd(&tv, v, D, T, Hkv, 1, strides[5], strides[4], 0, kBN, p.pos_v))) return rc;

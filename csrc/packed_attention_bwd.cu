@@ -43,7 +43,9 @@ constexpr int kStages = 3;            // of Q_i, dO_i, L_i, Delta_i: a tile is a
 struct BwdParams {
     const PackedTile* tiles;
     const float *lse, *delta;
-    int* claimed;                // items that were given out behind everybody's first
+    int* claimed;                // items that were given out behind everybody's first; then whether a CTA gave up a wait
+    int* gave_up;                // host memory (packed_items.cuh)
+    int tries;                   // of a wait
     bf16 *dk, *dv;
     long long lse_row, dk_head, dk_row, dv_head, dv_row;
     int entries, Hkv, group, nsplit;          // nsplit: items that share a key block; each walks its part of the (head, query tile) list
@@ -145,7 +147,7 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        dead_word = 0;
+        dead_word = p.tries - kTries;
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&k_full[i], 1);
             ptx::mbar_init(&k_cut[i], 1);
@@ -206,14 +208,14 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         };
         for (Item x = fetch_item<CAUSAL>(p, blockIdx.x);; x = claim()) {          // the last tiles are still worked on when the next item is asked for
             publish_item(x, item_ring, item_full, item_empty, published, dead);
-            if (x.kind == 0) break;
+            if (x.kind == 0 || __shfl_sync(0xffffffffu, gave_up(dead), 0)) break;
             if (x.kind > 1) continue;
             const int buf = blocks % L::kBufs;
             const uint32_t ph = ((uint32_t)(blocks / L::kBufs) & 1u) ^ 1u;
             ++blocks;
             int c[4];
             wait_for(&v_empty[buf], ph, dead);
-            if (lane == 0) {
+            if (lane == 0 && !gave_up(dead)) {
                 ptx::mbar_arrive_expect_tx(&v_full[buf], L::kKvBytes);
 #pragma unroll
                 for (int g = 0; g < D / 64; ++g) {
@@ -223,7 +225,7 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 }
             }
             wait_for(&k_empty[buf], ph, dead);
-            if (lane == 0) {
+            if (lane == 0 && !gave_up(dead)) {
                 uint64_t* bar = x.keys_cut() ? &k_cut[buf] : &k_full[buf];
                 ptx::mbar_arrive_expect_tx(bar, L::kKvBytes);
 #pragma unroll
@@ -237,7 +239,7 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             for (int it = 0; it < x.total; ++it, ++gi) {
                 const int st = gi % kStages, m0 = (x.first + th) * kBM;
                 wait_for(&qdo_empty[st], ((uint32_t)(gi / kStages) & 1u) ^ 1u, dead);
-                if (lane == 0) {
+                if (lane == 0 && !gave_up(dead)) {
                     uint64_t* bar = m0 + kBM > x.len ? &qdo_cut[st] : &qdo_full[st];
                     ptx::mbar_arrive_expect_tx(bar, L::kTxPerStage);
 #pragma unroll
@@ -490,7 +492,7 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             wait_for(pds_empty, ((uint32_t)(gi - 1)) & 1u, dead);          // the commit behind the last product: dK and dV are final
             ptx::tcgen05_fence_after();
             const uint32_t col = half == 0 ? kColDV : kColDK;
-            const float mul = *dead ? NAN : half == 0 ? 1.f : p.scale;
+            const float mul = half == 0 ? 1.f : p.scale;
             if (p.nsplit > 1) {
                 // partial dV / dK -> fp32 -> TMA reduce-add into the accumulators, 8 rows x 32 columns at a time
 #pragma unroll 1
@@ -561,12 +563,18 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     ptx::tcgen05_fence_before();
     __syncthreads();
-    if (dead_word) let_copies_land();
+    if (gave_up(dead)) {
+        let_copies_land();
+        if (threadIdx.x == 0) {
+            p.claimed[1] = 1;            // the last kernel of the call then writes NaN
+            *reinterpret_cast<volatile int*>(p.gave_up) = 1;
+        }
+    }
     if (warp == 1) ptx::tmem_dealloc<1>(tmem, 512);
 }
 
 // Delta of one entry (up to 128 rows) of one head, at the plan's padded columns, and zeros into the dQ accumulator's columns of those rows
-// (nobody reads the padding) and the counter of claims.  kD / 8 lanes own a row.  Bound by memory: 24576 rows of 16 heads of 64,
+// (nobody reads the padding), the counter of claims and the mark behind it.  kD / 8 lanes own a row.  Bound by memory: 24576 rows of 16 heads of 64,
 // 201 MB, 38 us.
 template <int kD>
 __global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __restrict__ o, const uint8_t* __restrict__ rest, const bf16* __restrict__ dout, const PackedTile* tiles,
@@ -578,7 +586,7 @@ __global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __rest
     const PackedTile pt = packed_tile(tiles, blockIdx.x / Hq);
     const int h = blockIdx.x % Hq, l = threadIdx.x % L;
     const int first = pt.t * kBN, rows = min(pt.len - first, kBN);        // negative where the entry is no tile
-    if (blockIdx.x == 0 && threadIdx.x == 0) *claimed = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) claimed[0] = claimed[1] = 0;
     if (pt.len == 0) return;
     {
         const int quads = (rows + 3) >> 2;
@@ -637,20 +645,26 @@ __global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __rest
 }
 
 // d-major fp32 accumulator [Hq, D, lse_row] -> dq, 64 of the D of an entry (128 rows) of one head per block; rows of no sequence get
-// zeros.  Bound by memory: 24576 rows of 16 heads of 64, 151 MB, 31 us; 16384 rows of 32 heads of 128, 403 MB, 79 us (142 as half
+// zeros.  Where a CTA of the kernel before gave up a wait, dQ, dK and dV become NaN: what it and others had added is a part.  Bound by memory: 24576 rows of 16 heads of 64, 151 MB, 31 us; 16384 rows of 32 heads of 128, 403 MB, 79 us (142 as half
 // entries through padded rows of shared memory, which two to four lanes met at one bank).
 template <int kD>
-__global__ void __launch_bounds__(256) packed_dq_kernel(const float* __restrict__ acc, bf16* __restrict__ dq, const PackedTile* tiles,
-                                                        long long head, long long row, long long lse_row, int Hq) {
+__global__ void __launch_bounds__(256) packed_dq_kernel(const float* __restrict__ acc, bf16* __restrict__ dq, const BwdParams p, long long head,
+                                                        long long row, int Hq) {
+    const long long lse_row = p.lse_row;
     pdl_trigger();
     pdl_wait();
     __shared__ float4 tile[64][32];          // four columns of row d at place (columns / 4) ^ (d / 8 % 8): no bank twice, either way
     constexpr int kParts = kD / 64;
     const unsigned at = blockIdx.x / kParts;
-    const PackedTile pt = packed_tile(tiles, at / Hq);
+    const PackedTile pt = packed_tile(p.tiles, at / Hq);
     const int h = at % Hq, d0 = blockIdx.x % kParts * 64;
     if (pt.len == 0) {
-        if (d0 == 0) block_zero_rows<kD>(dq + (long long)pt.start * row + h * head, row, pt.t, threadIdx.x, 256);
+        if (d0 != 0) return;
+        block_zero_rows<kD>(dq + (long long)pt.start * row + h * head, row, pt.t, threadIdx.x, 256);
+        if (p.claimed[1] && h % p.group == 0) {
+            block_zero_rows<kD>(p.dk + (long long)pt.start * p.dk_row + h / p.group * p.dk_head, p.dk_row, pt.t, threadIdx.x, 256);
+            block_zero_rows<kD>(p.dv + (long long)pt.start * p.dv_row + h / p.group * p.dv_head, p.dv_row, pt.t, threadIdx.x, 256);
+        }
         return;
     }
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -660,6 +674,19 @@ __global__ void __launch_bounds__(256) packed_dq_kernel(const float* __restrict_
 #pragma unroll
     for (int j = 0; j < 8; ++j)              // columns in fours: those of a sequence are padded to a multiple of four
         v[j] = 4 * lane < left ? *reinterpret_cast<const float4*>(src + (w + 8 * j) * lse_row + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.claimed[1]) {                      // asked for behind the loads
+        const int key_head = h / p.group;
+        for (int i = threadIdx.x; i < min(left, kBN) * 8; i += 256) {
+            const long long r = pt.start + q0 + (i >> 3);
+            const int c = d0 + (i & 7) * 8;
+            const uint4 nan = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            *reinterpret_cast<uint4*>(dq + h * head + r * row + c) = nan;
+            if (h % p.group) continue;
+            *reinterpret_cast<uint4*>(p.dk + key_head * p.dk_head + r * p.dk_row + c) = nan;
+            *reinterpret_cast<uint4*>(p.dv + key_head * p.dv_head + r * p.dv_row + c) = nan;
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) tile[w + 8 * j][lane ^ j] = v[j];
     __syncthreads();
@@ -724,11 +751,11 @@ NXD_API int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv) {
 // Backward of nxd_packed_attn_fwd.  strides: {head, row} in elements of q, k, v, o, dout, dq, dk, dv (16 values, multiples of 8);
 // lse, rest: what the forward pass wrote; delta: Hq * lse_row + 4 floats of scratch; dq_accum: [Hq, D, lse_row] floats of scratch;
 // dkv_accum: NULL, or ZEROED [2, Hkv, T, D] floats where nxd_packed_attn_bwd_splits says more than one.
-// dQ (with splits dK and dV too) is summed in fp32 in an order that is not fixed.
+// dQ (with splits dK and dV too) is summed in fp32 in an order that is not fixed.  wait_tries: as forward.
 NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse,
                                 float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
                                 const long long* strides, const void* tiles, int entries, long long lse_row, long long T, int N, int Hq,
-                                int Hkv, int D, float scale, int causal, void* stream) {
+                                int Hkv, int D, float scale, int causal, int wait_tries, void* stream) {
     NXD_REQUIRE(D == 64 || D == 128, "packed_attn_bwd: head dim %d not supported (64 or 128)", D);
     NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && lse_row % 4 == 0 &&
                 (long long)entries * Hq * 16 < (1ll << 31), "packed_attn_bwd: bad problem");
@@ -740,6 +767,9 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
     cudaStream_t st = (cudaStream_t)stream;
     const PackedTile* pt = (const PackedTile*)tiles;
     BwdParams p{};
+    int rc;
+    if ((rc = begin_call(&p.gave_up))) return rc;
+    p.tries = wait_tries < 0 || wait_tries > kTries ? kTries : wait_tries;
     p.entries = entries; p.Hkv = Hkv; p.group = Hq / Hkv;
     p.lse = lse; p.delta = delta; p.lse_row = lse_row;
     p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
@@ -757,7 +787,6 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
             delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq, causal)));
     NXD_LAUNCH_CHECK();
     CUtensorMap tq, tdo, tk, tv, tdq, tdka, tdva;
-    int rc;
     if ((rc = make_tmap_bhsd(&tq, q, D, T, Hq, 1, strides[1], strides[0], 0, kBM, p.pos_q))) return rc;
     if ((rc = make_tmap_bhsd(&tk, k, D, T, Hkv, 1, strides[3], strides[2], 0, kBN, p.pos_k))) return rc;
     if ((rc = make_tmap_bhsd(&tv, v, D, T, Hkv, 1, strides[5], strides[4], 0, kBN, p.pos_v))) return rc;
@@ -785,11 +814,11 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
         NXD_LAUNCH_CHECK_N(2);
     }
     if (D == 128)
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<128>, dim3(per_head * 2), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
-            strides[10], strides[11], lse_row, Hq)));
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<128>, dim3(per_head * 2), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, p,
+            strides[10], strides[11], Hq)));
     else
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<64>, dim3(per_head), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, pt,
-            strides[10], strides[11], lse_row, Hq)));
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_dq_kernel<64>, dim3(per_head), dim3(256), 0, st, (const float*)dq_accum, (bf16*)dq, p,
+            strides[10], strides[11], Hq)));
     NXD_LAUNCH_CHECK();
     return 0;
 }

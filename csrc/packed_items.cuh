@@ -5,8 +5,14 @@
 
 namespace nxd_packed {
 
-// A try of a wait lasts 3900 clocks, so a wait ends after two seconds; the results of a CTA that gave up are NaN.
+// A try of a wait lasts 3900 clocks, so a wait ends after two seconds.  A CTA that gave one up loads no more and leaves NaN: forward in the
+// results of all its items, backward in all gradients of the call.  It sets a word of pinned host memory, and the next call fails.
 constexpr int kTries = 1 << 20;
+constexpr int kGaveUp = -kTries;         // the CTA's mark; below that many tries a wait starts with their number less kTries
+__device__ __forceinline__ bool gave_up(const volatile int* dead) { return *dead == kGaveUp; }
+
+// Sets *word to the word above; fails where a call before this one has set it, and clears it.
+int begin_call(int** word);
 
 // A wait with an end: after kTries the CTA is marked, and no wait of its lasts any more (the mark leaves one try).  In one piece, because
 // the loop's shape counts: of the backward pass of 4 documents in 16384 tokens, 32 heads of 128 over 8, it takes 2050 us (one of 16384
@@ -19,7 +25,7 @@ __device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, volatil
         ".reg .s32 left;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1;\n\t"
         "@P bra DONE;\n\t"
-        "ld.volatile.shared.s32 left, [%2];\n\t"          // 0, or -kTries
+        "ld.volatile.shared.s32 left, [%2];\n\t"          // 0, or kGaveUp, or (a smaller limit) between the two
         "add.s32 left, left, %3;\n"
         "TRY:\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1;\n\t"
@@ -30,7 +36,7 @@ __device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, volatil
         "st.volatile.shared.s32 [%2], %4;\n"
         "DONE:\n\t"
         "}"
-        ::"r"(ptx::smem_u32(bar)), "r"(parity), "r"(ptx::smem_u32(const_cast<const int*>(dead))), "n"(kTries), "n"(-kTries)
+        ::"r"(ptx::smem_u32(bar)), "r"(parity), "r"(ptx::smem_u32(const_cast<const int*>(dead))), "n"(kTries), "n"(kGaveUp)
         : "memory");
 }
 
@@ -75,7 +81,7 @@ __device__ __forceinline__ Item next_item(const Item* ring, uint64_t* full, uint
     wait_for(&full[i], (uint32_t)(count / kItems) & 1u, dead);
     ++count;
     Item it{};
-    if (!*dead) {
+    if (!gave_up(dead)) {
         const int4* src = reinterpret_cast<const int4*>(&ring[i]);
         int4* dst = reinterpret_cast<int4*>(&it);
 #pragma unroll

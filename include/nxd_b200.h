@@ -162,18 +162,21 @@ int nxd_flash_attn_bwd_tc(const void* q, const void* k, const void* v, const voi
  * the per-row scratch.  Tiles have 128 rows, but 256 for the forward call where Hq / Hkv is odd.  strides = {head, row} in
  * elements: {q, k, v, o} forward, {q, k, v, o, dout, dq, dk, dv} backward, multiples of 8.
  * lse [Hq, columns] and rest [Hq, columns, D] bytes (NULL: not wanted; the backward call needs both), delta the same and 4 floats more; dq_accum [Hq, D, columns] of scratch; dkv_accum: NULL, or ZEROED
- * [2, Hkv, T, D] where nxd_packed_attn_bwd_splits is above 1.  Rows outside every sequence come out as zeros. */
+ * [2, Hkv, T, D] where nxd_packed_attn_bwd_splits is above 1.  Rows outside every sequence come out as zeros.
+ * wait_tries: tries of 3900 clocks after which a wait inside a kernel gives up, -1: two seconds.  The results are NaN then (forward those
+ * that the giving block owed, backward all), and the next call fails, or nxd_packed_attn_status (waits for the stream) says so. */
 int nxd_packed_plan_entries(long long T, int N, int rows);
 long long nxd_packed_plan_columns(long long T, int N);
 int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, int rows, void* tiles, void* seqs, void* stream);
 int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const long long* strides,
                         const void* tiles, int entries, long long columns, long long T, int Hq, int Hkv, int D, float scale,
-                        int causal, void* stream);
+                        int causal, int wait_tries, void* stream);
+int nxd_packed_attn_status(int* gave_up, void* stream);
 int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv);
 int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse,
                         float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
                         const long long* strides, const void* tiles, int entries, long long columns, long long T, int N,
-                        int Hq, int Hkv, int D, float scale, int causal, void* stream);
+                        int Hq, int Hkv, int D, float scale, int causal, int wait_tries, void* stream);
 
 /* ---- dropout: y = keep(i) ? x / (1 - p) : 0, plus residual (NULL: none); 0 < p < 1 ---------------------------------------
  * keep(i): word i % 4 of Philox4x32-7 at counter (i / 4, offset) under key seed >= p 2^32.  dtype 0 fp32, 1 bf16, 2 fp16.

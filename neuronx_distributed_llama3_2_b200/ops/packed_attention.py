@@ -132,8 +132,17 @@ def _strides(*ts: torch.Tensor):
     return (_c.c_longlong * len(vals))(*vals)
 
 
-def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad: bool):
-    """``(o, lse, rest)``; the two that the backward pass takes are ``None`` without it."""
+def gave_up() -> bool:
+    """Whether a call of packed attention gave up waiting inside its kernel since the last one that failed for it or was asked: its results
+    are NaN.  Waits for the current stream."""
+    flag = _c.c_int(0)
+    _lib.check(_lib.lib().nxd_packed_attn_status(_c.byref(flag), _lib.stream_ptr()), "nxd_packed_attn_status")
+    return bool(flag.value)
+
+
+def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad: bool, wait_tries: int = -1):
+    """``(o, lse, rest)``; the two that the backward pass takes are ``None`` without it.  ``wait_tries``: of a wait inside the kernel, -1: two
+    seconds (``gave_up``; the next call raises)."""
     T, Hq, D = q.shape
     # an odd number of heads to a key head: two neighbouring tiles of one head are worked on together (csrc/packed_attention.cu)
     tiles, entries, columns = packed.plan(causal, 128 if Hq // k.shape[1] % 2 == 0 else 256)
@@ -143,12 +152,12 @@ def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad:
     rc = _lib.lib().nxd_packed_attn_fwd(
         _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(lse), _lib.ptr(rest), _strides(q, k, v, o), _lib.ptr(tiles), _c.c_int(entries),
         _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(Hq), _c.c_int(k.shape[1]), _c.c_int(D), _c.c_float(scale), _c.c_int(causal),
-        _lib.stream_ptr())
+        _c.c_int(wait_tries), _lib.stream_ptr())
     _lib.check(rc, "nxd_packed_attn_fwd")
     return o, lse, rest
 
 
-def _backward(q, k, v, o, lse, rest, do, dq, dk, dv, plan, count: int, scale: float, causal: bool) -> None:
+def _backward(q, k, v, o, lse, rest, do, dq, dk, dv, plan, count: int, scale: float, causal: bool, wait_tries: int = -1) -> None:
     """Every element of ``dq / dk / dv`` is written.  ``plan``: the list that the forward pass had, or one made with it."""
     q, k, v, o, do = (_fix(t) for t in (q, k, v, o, do))          # what was saved may have been moved
     T, Hq, D = q.shape
@@ -162,7 +171,7 @@ def _backward(q, k, v, o, lse, rest, do, dq, dk, dv, plan, count: int, scale: fl
         _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(rest), _lib.ptr(do), _lib.ptr(lse), _lib.ptr(delta), _lib.ptr(acc), _lib.ptr(kv_acc),
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _strides(q, k, v, o, do, dq, dk, dv), _lib.ptr(tiles), _c.c_int(entries),
         _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(count), _c.c_int(Hq), _c.c_int(Hkv), _c.c_int(D), _c.c_float(scale),
-        _c.c_int(causal), _lib.stream_ptr())
+        _c.c_int(causal), _c.c_int(wait_tries), _lib.stream_ptr())
     _lib.check(rc, "nxd_packed_attn_bwd")
 
 

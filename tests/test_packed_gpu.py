@@ -112,6 +112,44 @@ def test_long_gaps(lens, first, T, H, G, D, causal):
         assert not got[name][:first].any() and not got[name][ends[-1]:].any()
 
 
+@pytest.mark.parametrize("lens,first,T,H,G,D,causal", [([300, 130], 7, 600, 4, 2, 64, True), ([2500], 100, 2700, 4, 1, 128, True),
+                                                       ([60] * 80, 0, 5000, 3, 1, 64, False), ([700] * 20, 500, 16000, 8, 4, 128, False)])
+def test_waits_that_run_out(lens, first, T, H, G, D, causal):
+    """A call whose waits give up at once leaves NaN in every sequence and zeros outside, the next call fails, and those behind it are sound."""
+    from neuronx_distributed_llama3_2_b200.ops import packed_attention as pa
+
+    q, k, v, do = _inputs(T, H, G, D)
+    ends = _ends(lens, first)
+    p = pa.PackedSequences(torch.tensor(ends, device="cuda"), T)
+    scale = D ** -0.5
+    inside = slice(first, ends[-1])
+    grads = [torch.full(x.shape, 7.0, dtype=x.dtype, device="cuda") for x in (q, k, v)]
+
+    def all_nan(*xs):
+        return all(x[inside].isnan().all() and not x[:first].any() and not x[ends[-1]:].any() for x in xs)
+
+    assert not pa.gave_up()
+    o, lse, rest = pa._forward(q, k, v, p, scale, causal, True)
+    assert not pa.gave_up() and o.isfinite().all()
+    lost, lost_lse, lost_rest = pa._forward(q, k, v, p, scale, causal, True, wait_tries=0)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="gave up"):
+        pa._forward(q, k, v, p, scale, causal, True)
+    assert all_nan(lost)
+    pa._backward(q, k, v, lost, lost_lse, lost_rest, do, *grads, p.plan(causal), p.count, scale, causal)
+    assert all_nan(*grads) and not pa.gave_up()
+    pa._backward(q, k, v, o, lse, rest, do, *grads, p.plan(causal), p.count, scale, causal, wait_tries=0)
+    torch.cuda.synchronize()
+    assert all_nan(*grads)
+    with pytest.raises(RuntimeError, match="gave up"):
+        pa._backward(q, k, v, o, lse, rest, do, *grads, p.plan(causal), p.count, scale, causal)
+    pa._forward(q, k, v, p, scale, causal, True, wait_tries=0)
+    assert pa.gave_up() and not pa.gave_up()
+    got, want = _run(q, k, v, do, ends, causal), packed(q, k, v, ends, causal, do)
+    for name in got:
+        check(got[name], want, name)
+
+
 # scores that rise along the keys (the running maximum moves in every tile) and scores that leave one weight
 @pytest.mark.parametrize("scale", [0.01, 1.0, None])
 def test_scales(scale):
