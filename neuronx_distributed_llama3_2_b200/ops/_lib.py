@@ -22,6 +22,7 @@ from concurrent.futures import ThreadPoolExecutor
 from typing import List, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _REPO = os.path.dirname(os.path.dirname(_HERE))
@@ -290,6 +291,14 @@ def on_device_of(t: torch.Tensor):
     """Context in which ``t``'s device is the current one (launches go to its current stream); free of charge where it is already."""
     index = t.get_device()
     return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def transformed(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a tensor carries a forward-mode tangent, or a ``torch.func`` transform goes on: a kernel that writes through addresses takes
+    such a tensor's values and loses the rest, while ``requires_grad`` is False."""
+    if torch._C._are_functorch_transforms_active():
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def check(code: int, what: str, handle: Optional[ctypes.CDLL] = None) -> None:

@@ -100,7 +100,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: Seed = None, offset: int = 0,
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a captured dropout would drop the same elements in every replay: pass its seed as a tensor")
         seed = int(torch.randint(0, 2 ** 62, (1,)).item())
-    if x.is_cuda and x.dtype in _DTYPES and _lib.available():
+    if x.is_cuda and x.dtype in _DTYPES and _lib.available() and not _lib.transformed(x, residual):
         if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
             return _DropoutFn.apply(x, residual, p, seed & _M64, offset & _M64, state)
         return _launch(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed & _M64, offset & _M64, state, None)

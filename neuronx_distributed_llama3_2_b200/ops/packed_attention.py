@@ -232,7 +232,8 @@ class _RopePackedAttnFn(torch.autograd.Function):
 
 def packed_attn_nxd(q, k, v, packed: PackedSequences, softmax_scale: Optional[float], causal: bool) -> torch.Tensor:
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or v.requires_grad):
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    if not grad and not _lib.transformed(q, k, v):          # forward-mode derivatives and ``torch.func`` are refused by the node
         with _lib.on_device_of(q):
             return _forward(_fix(q), _fix(k), _fix(v), packed, float(scale), bool(causal), False)[0]
     return _PackedAttnFn.apply(q, k, v, packed, float(scale), bool(causal))

@@ -183,6 +183,35 @@ def test_captured_with_a_state_on_the_device():
             dropout(x, 0.5)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_forward_mode_and_func(device):
+    """A tangent is dropped where its element is, and torch.func's transforms see what autograd does."""
+    import torch.autograd.forward_ad as fw
+
+    g = torch.Generator().manual_seed(0)
+    x, t, r, rt = (torch.randn(300, generator=g).to(device) for _ in range(4))
+    keep = dropout_keep((300,), 0.25, 9, 2, device)
+    slope = torch.where(keep, 1.0 / 0.75, 0.0)
+    state = torch.tensor([9, 2], device=device)
+    for kw in (dict(seed=9, offset=2), dict(seed=state)):
+        for residual, rest in ((None, None), (r, None), (r, rt)):
+            with fw.dual_level(), torch.no_grad():
+                dual = fw.make_dual(x, t)
+                add = residual if rest is None else fw.make_dual(residual, rest)
+                y, tangent = fw.unpack_dual(dropout(dual, 0.25, residual=add, **kw))
+            # the kernel rounds a product and its sum with the residual once, torch each: the product's half step, and one of either sum
+            want = dropout(x, 0.25, residual=residual, **kw)
+            assert ((y - want).abs() <= 2.0 ** -24 * (1.0001 * x.abs() / 0.75 + y.abs() + want.abs())).all()
+            # a product of fp32 and a sum
+            assert (tangent - (slope * t + (0.0 if rest is None else rest))).abs().max() <= 2.0 ** -22 * 8
+    with fw.dual_level():
+        assert fw.unpack_dual(dropout(x, 0.25, 9, 2, residual=fw.make_dual(r, rt))).tangent.equal(rt)
+        assert fw.unpack_dual(dropout(x, 0.25, 9, 2)).tangent is None
+    grad = torch.func.grad(lambda z: (dropout(z, 0.25, 9, 2) * t).sum())(x)
+    assert (grad - slope * t).abs().max() <= 2.0 ** -22 * 8
+    assert torch.equal(torch.func.jvp(lambda z: dropout(z, 0.25, 9, 2), (x,), (torch.ones_like(x),))[1] != 0, keep)
+
+
 @pytest.mark.gpu
 def test_float64_on_the_gpu():
     x = torch.randn(100, device="cuda", dtype=torch.float64)

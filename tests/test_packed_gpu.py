@@ -404,6 +404,24 @@ def test_rotation_and_attention(D):
     assert not o[470:].any() and not grad[470:].any()
 
 
+def test_forward_mode_is_refused():
+    """Not taken as a call without derivatives, with autograd on and off."""
+    import torch.autograd.forward_ad as fw
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+
+    q, k, v, _ = _inputs(100, 4, 2, 64)
+    cu = torch.tensor([0, 60, 100], device="cuda")
+    with fw.dual_level():
+        for on in (True, False):
+            for at in range(3):
+                args = [fw.make_dual(x, torch.ones_like(x)) if i == at else x for i, x in enumerate((q, k, v))]
+                with torch.set_grad_enabled(on), pytest.raises((NotImplementedError, RuntimeError), match="jvp"):
+                    flash_attn_packed_func(*args, cu)
+        assert flash_attn_packed_func(q, k, v, cu).isfinite().all()
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: flash_attn_packed_func(x, k, v, cu), (q,), (q,))
+
+
 def test_other_types_take_one_sequence_after_the_other():
     q, k, v, do = (x.float() for x in _inputs(130, 4, 2, 64))
     ends = [0, 60, 120]
