@@ -36,6 +36,11 @@ def _table(rows: Sequence[torch.Tensor], mask: Optional[torch.Tensor], E: int, t
             _c.c_int(top_k))
 
 
+def _where(mask: Optional[torch.Tensor], rows: Sequence[torch.Tensor]) -> list:
+    """What the table says of its tensors but their sizes."""
+    return [mask is not None and mask.data_ptr(), *[t.data_ptr() for t in rows], *[t.stride(0) for t in rows]]
+
+
 # what moves saved tensors: the innermost pair of hooks, None without one
 _saved_hooks = getattr(torch._C._autograd, "_top_saved_tensors_default_hooks", lambda _: "unknown")
 
@@ -57,9 +62,11 @@ class _BalanceLossFn(torch.autograd.Function):
         _lib.check(rc, "nxd_balance_loss_fwd")
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)         # no zeros for the counts' gradient
-        ctx.save_for_backward(share, mask, *rows)
-        # 32 layers' table costs a tenth of the call: the backward pass makes it again only where what was saved may have moved
-        ctx.args = (table if _saved_hooks(True) is None else None, E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
+        # Without hooks the program's own tensors are saved as they are, so that ``logits.data = ...`` gives them other storage: what is
+        # saved is another tensor on the storage of this call (the gradient wants its values), and its writes are counted with theirs.
+        hooks = _saved_hooks(True) is not None
+        ctx.save_for_backward(share, mask, *(rows if hooks else [r.detach() if r is t else r for r, t in zip(rows, logits)]))
+        ctx.args = (table, _where(mask, rows), E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
         return loss, counts
 
     @staticmethod
@@ -68,11 +75,14 @@ class _BalanceLossFn(torch.autograd.Function):
         if grad is None:
             return (None,) * len(ctx.needs_input_grad)
         saved = ctx.saved_tensors          # all of them: none may have been written since
-        table, E, top_k, sizes, shapes = ctx.args
-        share, x = saved[0], saved[2]
-        if table is None:                  # checkpointing, offloading
-            rows = [_rows(t, E) for t in saved[2:]]
-            table = _table(rows, saved[1], E, top_k)
+        table, where, E, top_k, sizes, shapes = ctx.args
+        share, mask, rows = saved[0], saved[1], saved[2:]
+        if _where(mask, rows) != where:    # checkpointing, offloading; the table of 32 layers costs a tenth of the call
+            rows = [_rows(t, E) for t in rows]
+            if [tuple(t.shape) for t in rows] != [(n, E) for n in sizes]:
+                raise RuntimeError(f"router logits saved for the balance loss have become {[tuple(t.shape) for t in rows]}")
+            table = _table(rows, mask, E, top_k)
+        x = rows[0]
         dx = torch.empty((sum(sizes), x.shape[1]), dtype=x.dtype, device=x.device)
         grad = grad.float()
         with _lib.on_device_of(x):

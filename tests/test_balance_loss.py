@@ -190,6 +190,33 @@ def test_saved_logits_that_move(how):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how", ["other data", "smaller data", "hooks of the node", "a view moved"])
+def test_saved_logits_that_get_other_storage(how):
+    """The gradient is that of the logits as the loss saw them, wherever they lie by then."""
+    for leaf in (True, False):
+        logits = [t.requires_grad_() for t in _logits(3, 200, 8, torch.float32, "cuda", seed=5)]
+        seen = logits if leaf else [t * 1.0 for t in logits]
+        (want,) = torch.autograd.grad(load_balancing_loss_func(seen, 8, 2), logits[1], retain_graph=True)
+        mask = torch.arange(200, device="cuda") % 7 > 0
+        (want_masked,) = torch.autograd.grad(load_balancing_loss_func(seen, 8, 2, mask=mask), logits[1], retain_graph=True)
+        loss, masked = load_balancing_loss_func(seen, 8, 2), load_balancing_loss_func(seen, 8, 2, mask=mask)
+        if how == "hooks of the node":
+            kept = []
+            for out in (loss, masked):
+                for saved in out.grad_fn._raw_saved_tensors[2:]:
+                    saved.register_hooks(lambda t: kept.append(t.cpu()) or len(kept) - 1, lambda i: kept[i].cuda())
+        else:
+            for t in seen:
+                t.data = {"other data": lambda: torch.full_like(t, math.nan), "smaller data": lambda: t.data[:1, :1].clone(),
+                          "a view moved": lambda: torch.full((200, 16), math.nan, device="cuda")[:, ::2]}[how]()
+        trash = [torch.full((200, 8), math.nan, device="cuda") for _ in range(64)]          # where the logits were
+        for out, same in ((loss, want), (masked, want_masked)):
+            (got,) = torch.autograd.grad(out, logits[1], retain_graph=True)
+            assert torch.equal(got, same)
+        del trash
+
+
+@pytest.mark.gpu
 def test_part_of_the_layers_needs_gradients():
     a, b = _logits(2, 40, 8, torch.float32, "cuda")
     a.requires_grad_()
