@@ -385,6 +385,7 @@ struct Plan {
     RouterArgs args;
     long long most;                      // rows of the largest layer
     int blocks_x, n;
+    bool backward;
 };
 
 // Blocks of a layer: all layers' together are on the chip at once and no more than that (half of a second round costs as much as a
@@ -401,8 +402,8 @@ int lanes_of(int E) {
     return l;
 }
 
-int make_plan(Plan* p, const void* const* x, const long long* ld, const long long* rows, int n, int elem, const void* mask, int E, int k,
-              const void* dx) {
+int make_plan(Plan* p, bool backward, const void* const* x, const long long* ld, const long long* rows, int n, int elem, const void* mask,
+              int E, int k, const void* dx) {
     NXD_REQUIRE(n > 0 && n <= kMaxLayers && E > 0 && E <= 1024 && k > 0 && k <= E, "balance_loss: %d tensors, %d of %d experts", n, k, E);
     long long most = 0, total = 0;
     bool vec = (long long)E * elem % 16 == 0 && ((uintptr_t)dx & 15) == 0;
@@ -418,8 +419,10 @@ int make_plan(Plan* p, const void* const* x, const long long* ld, const long lon
     p->layers.first[n] = total;
     NXD_REQUIRE(total < (1ll << 31) && total * k < (1ll << 40), "balance_loss: %lld rows", total);
     p->args = RouterArgs{(const unsigned char*)mask, E, k, vec};
+    NXD_REQUIRE(!backward || dx != nullptr || total == 0, "balance_loss: no gradients' memory for %lld rows", total);
     p->n = n;
     p->most = most;
+    p->backward = backward;
     return 0;
 }
 
@@ -434,7 +437,7 @@ int blocks_per_sm(int threads) {
 
 template <typename T, int L, int V>
 int run(Plan& p, float* scratch, const float* share, const float* grad, void* dx, cudaStream_t st) {
-    if (dx == nullptr) {
+    if (!p.backward) {
         constexpr auto kern = balance_fwd_kernel<T, L, V>;
         p.blocks_x = blocks_of(p.most, p.n, L, kThreads, blocks_per_sm<kern>(kThreads));
         int* part_c = (int*)(scratch + (long long)p.blocks_x * p.n * p.args.E);
@@ -482,7 +485,7 @@ NXD_API int nxd_balance_loss_fwd(const void* const* x, const long long* ld, cons
                                  void* stream) {
     NXD_REQUIRE(dtype >= 0 && dtype <= 2, "balance_loss: dtype %d", dtype);
     Plan p;
-    int rc = make_plan(&p, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, nullptr);
+    int rc = make_plan(&p, false, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, nullptr);
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     if ((rc = run_typed(p, dtype, (float*)scratch, nullptr, nullptr, nullptr, st))) return rc;
@@ -494,12 +497,12 @@ NXD_API int nxd_balance_loss_fwd(const void* const* x, const long long* ld, cons
     return 0;
 }
 
-// dx: [all rows, E] in x's type, the layers one after the other; grad: the loss's gradient, 1 float on the device.
+// dx: [all rows, E] in x's type, the layers one after the other (NULL where there are no rows); grad: the loss's gradient, 1 float on the device.
 NXD_API int nxd_balance_loss_bwd(const void* const* x, const long long* ld, const long long* rows, int layers, int dtype,
                                  const void* mask, int E, int k, const float* share, const float* grad, void* dx, void* stream) {
-    NXD_REQUIRE(dtype >= 0 && dtype <= 2 && dx != nullptr, "balance_loss: dtype %d", dtype);
+    NXD_REQUIRE(dtype >= 0 && dtype <= 2, "balance_loss: dtype %d", dtype);
     Plan p;
-    int rc = make_plan(&p, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, dx);
-    if (rc) return rc;
+    int rc = make_plan(&p, true, x, ld, rows, layers, dtype == 0 ? 4 : 2, mask, E, k, dx);
+    if (rc || p.most == 0) return rc;          // no rows, no gradients
     return run_typed(p, dtype, nullptr, share, grad, dx, (cudaStream_t)stream);
 }

@@ -104,6 +104,16 @@ def test_kernel_of_many_layers_and_rows():
     _check(uneven, 8, 2, None)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("layers", [1, 3])
+def test_no_rows_at_all(layers, device):
+    logits = [torch.zeros(0, 8, device=device, requires_grad=True) for _ in range(layers)]
+    for mask in (None, torch.zeros(0, dtype=torch.bool, device=device)):
+        loss, counts = load_balancing_loss_func(logits, 8, 2, mask=mask, return_counts=True)
+        grads = torch.autograd.grad(loss, logits)
+        assert loss.item() == 0.0 and not counts.any() and all(g.shape == (0, 8) for g in grads)
+
+
 @pytest.mark.gpu
 def test_kernel_reads_views():
     g = torch.Generator(device="cuda").manual_seed(0)
