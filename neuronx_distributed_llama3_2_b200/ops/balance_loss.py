@@ -6,7 +6,6 @@ import ctypes as _c
 from typing import List, Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -25,7 +24,8 @@ def qualifies(logits: List[torch.Tensor], E: int) -> bool:
     x = logits[0]
     dtype, device = x.dtype, x.get_device()
     return (x.is_cuda and dtype in _DTYPES and len(logits) <= MAX_LAYERS and E <= MAX_EXPERTS
-            and all(t.dtype is dtype and t.get_device() == device for t in logits) and _lib.available())
+            and all(t.dtype is dtype and t.get_device() == device for t in logits) and _lib.available()
+            and not _lib.transformed(*logits))          # forward-mode derivatives and ``torch.func`` take the torch form
 
 
 def _table(rows: Sequence[torch.Tensor], mask: Optional[torch.Tensor], E: int, top_k: int) -> tuple:
@@ -63,21 +63,31 @@ class _BalanceLossFn(torch.autograd.Function):
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)         # no zeros for the counts' gradient
         # Without hooks the program's own tensors are saved as they are, so that ``logits.data = ...`` gives them other storage: what is
-        # saved is another tensor on the storage of this call (the gradient wants its values), and its writes are counted with theirs.
-        hooks = _saved_hooks(True) is not None
-        ctx.save_for_backward(share, mask, *(rows if hooks else [r.detach() if r is t else r for r, t in zip(rows, logits)]))
-        ctx.args = (table, _where(mask, rows), E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
+        # saved is another tensor on the storage of this call (the gradient wants its values), and its writes are counted with theirs.  The
+        # tensors themselves are for a gradient that is differentiated.
+        where = None
+        if _saved_hooks(True) is None:
+            where = _where(mask, rows)
+            ctx.save_for_backward(share, mask, *[r.detach() if r is t else r for r, t in zip(rows, logits)], *logits)
+        else:
+            ctx.save_for_backward(share, mask, *logits)
+        ctx.args = (table, where, E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
             return (None,) * len(ctx.needs_input_grad)
         saved = ctx.saved_tensors          # all of them: none may have been written since
         table, where, E, top_k, sizes, shapes = ctx.args
-        share, mask, rows = saved[0], saved[1], saved[2:]
-        if _where(mask, rows) != where:    # checkpointing, offloading; the table of 32 layers costs a tenth of the call
+        n = len(sizes)
+        share, mask, rows = saved[0], saved[1], saved[2:2 + n]
+        if torch.is_grad_enabled():        # this gradient is differentiated itself: in torch operations, on the program's own tensors
+            logits, need = saved[-n:], ctx.needs_input_grad[3:]
+            loss, _ = balance_loss_ref(list(logits), E, top_k, mask)
+            grads = iter(torch.autograd.grad(loss, [t for t, x in zip(logits, need) if x], grad.to(loss.dtype), create_graph=True))
+            return (None, None, None, *[next(grads) if x else None for x in need])
+        if where is None or _where(mask, rows) != where:    # checkpointing, offloading; the table of 32 layers costs a tenth of the call
             rows = [_rows(t, E) for t in rows]
             if [tuple(t.shape) for t in rows] != [(n, E) for n in sizes]:
                 raise RuntimeError(f"router logits saved for the balance loss have become {[tuple(t.shape) for t in rows]}")

@@ -226,6 +226,46 @@ def test_saved_logits_that_get_other_storage(how):
         del trash
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_other_derivatives(masked, device):
+    """Second derivatives, forward mode and torch.func, against the formulas in float64."""
+    import torch.autograd.forward_ad as fw
+
+    E, k, layers, rows = 8, 2, 3, 50
+    logits = [t.to(device) for t in _logits(layers, rows, E, torch.float32, "cpu")]
+    v = [t.to(device) for t in _logits(layers, rows, E, torch.float32, "cpu", seed=7)]
+    mask = (torch.arange(rows, device=device) % 3 > 0) if masked else None
+
+    def loss_of(*x):
+        return load_balancing_loss_func(list(x), E, k, mask=mask)
+
+    _, counts, dx = oracle(logits, E, k, mask)
+    n = int(counts.sum()) // k
+    p = torch.softmax(torch.cat(logits).double(), -1) * (1.0 if mask is None else mask.repeat(layers)[:, None])
+    f, t = counts.double() / n, torch.cat(v).double()
+    dp = p * (t - (p * t).sum(-1, keepdim=True))
+    second = E / (k * n) * (dp * (f - (p * f).sum(-1, keepdim=True)) - p * (dp * f).sum(-1, keepdim=True))
+    # a softmax and three more products and sums over E, 2^-24 each, of terms that are no larger than these
+    size = E / (k * n) * (p * (t.abs() + (p * t.abs()).sum(-1, keepdim=True))) * f.max() * 4
+    leaves = [x.clone().requires_grad_() for x in logits]
+    first = torch.autograd.grad(loss_of(*leaves), leaves, create_graph=True)
+    again = torch.autograd.grad(sum((a * b).sum() for a, b in zip(first, v)), leaves)
+    assert ((torch.cat(again).double() - second).abs() <= 2.0 ** -24 * (24 + 3 * E) * (size + size.mean(-1, keepdim=True))).all()
+    slope = (dx * t).sum()
+    # rows of E products, then some hundred sums
+    near = 2.0 ** -24 * (24 + 4 * E) * (E / (k * n) * (p * t.abs()).sum() * f.max() * 4)
+    with fw.dual_level():
+        _, tangent = fw.unpack_dual(loss_of(*[fw.make_dual(x, y) for x, y in zip(logits, v)]))
+    assert abs(tangent.double() - slope) <= near
+    assert abs(torch.func.jvp(loss_of, tuple(logits), tuple(v))[1].double() - slope) <= near
+    grads = torch.func.grad(loss_of, argnums=tuple(range(layers)))(*logits)
+    for a, b, c in zip(grads, first, torch.autograd.grad(loss_of(*leaves), leaves)):
+        assert (a - b).abs().max() <= 2.0 ** -24 * (24 + E) * 4 * a.abs().max() and (b - c).abs().max() <= 2.0 ** -24 * (24 + E) * 4 * c.abs().max()
+    only = torch.autograd.grad(loss_of(logits[0], leaves[1], logits[2]), leaves[1], create_graph=True)[0]
+    assert only.requires_grad and torch.equal(only, first[1])
+
+
 @pytest.mark.gpu
 def test_part_of_the_layers_needs_gradients():
     a, b = _logits(2, 40, 8, torch.float32, "cuda")
