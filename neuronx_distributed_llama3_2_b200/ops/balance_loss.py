@@ -114,14 +114,16 @@ def balance_loss(logits: List[torch.Tensor], E: int, top_k: int, mask: Optional[
 def balance_loss_ref(logits: List[torch.Tensor], E: int, top_k: int, mask: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
     """The same in torch operations."""
     x = torch.cat([t.reshape(-1, E) for t in logits]).float() if len(logits) > 1 else logits[0].reshape(-1, E).float()
+    rows = mask.repeat(len(logits)) if mask is not None else None
+    if rows is not None:          # ahead of the softmax, whose gradient turns a zero into NaN where the row holds one
+        x = torch.where(rows[:, None], x, 0.0)
     probs = torch.softmax(x, dim=-1)
     # the largest logits, ties to the lowest expert (a top-k leaves open which of two equal ones it takes)
     selected = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :top_k]
-    if mask is None:
+    if rows is None:
         n = torch.full((), float(x.shape[0]), device=x.device)
         ones = torch.ones(selected.shape, dtype=torch.int64, device=x.device)
     else:
-        rows = mask.repeat(len(logits))
         n = rows.sum().float()
         ones = rows[:, None].expand_as(selected).long()
         probs = torch.where(rows[:, None], probs, 0.0)

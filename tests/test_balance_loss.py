@@ -114,6 +114,22 @@ def test_no_rows_at_all(layers, device):
         assert loss.item() == 0.0 and not counts.any() and all(g.shape == (0, 8) for g in grads)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("fill", [math.nan, math.inf, -math.inf])
+def test_rows_left_out_hold_anything(fill, device):
+    logits = [t.to(device) for t in _logits(2, 30, 8, torch.float32, "cpu")]
+    mask = torch.arange(30, device=device) % 4 > 0
+    leaves = [[x.clone().requires_grad_() for x in logits] for _ in range(2)]
+    with torch.no_grad():
+        for x in leaves[1]:
+            x[~mask] = fill
+    clean, dirty = (load_balancing_loss_func(x, 8, 2, mask=mask, return_counts=True) for x in leaves)
+    assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+    for create in (False, True):
+        for a, b in zip(*(torch.autograd.grad(out[0], x, create_graph=create, retain_graph=True) for out, x in zip((clean, dirty), leaves))):
+            assert torch.equal(a, b) and not b[~mask].any()
+
+
 @pytest.mark.gpu
 def test_kernel_reads_views():
     g = torch.Generator(device="cuda").manual_seed(0)
