@@ -11,7 +11,9 @@
 // double precision: no atomics, the loss does not depend on the schedule.
 //
 // Forward is bound by issue (half of the instructions are comparisons and selections, two clocks each): 240042 rows of 128 experts in
-// fp32, 8 of each, 73 us (memory alone: 19), 524288 rows of 64 66 us; backward by memory: 43 us (38).
+// fp32, 8 of each, 77 us (memory alone: 19), 524288 rows of 64 69 us; backward by memory: 43 us (38).  Exponentials and the division are
+// the library's exact ones (5 % forward; backward in fp32 nothing), and a row's sums are trees: the fp32 gradients of 16 experts are off by
+// 2.65e-7 by norm, torch's by 2.7e-7 (sums one after the other: 3.2e-7).
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -90,27 +92,36 @@ __device__ __forceinline__ float group_max(float v) {
     return v;
 }
 
-// 2^x by the hardware instruction: within 2 units in the last place, and the rounding of its argument (x - max) log2 e adds 2^-24 of
-// that argument, so a probability of 2^-10 is off by 6e-7 of itself at most.
-__device__ __forceinline__ float exp_of(float x) {
+// 2^x by the hardware instruction, within 2 units in the last place; the rounding of its argument (x - max) log2 e adds 2^-24 of that
+// argument.  For gradients that are rounded to 16 bits, 2^-11 of them at best: a probability as small as 2^-126 is off by 2^-17
+// of itself, of which a rounding in some hundred of fp16 takes notice.  expf costs 5 us more for 240042 rows of 128 experts in bf16 (33).
+__device__ __forceinline__ float exp_near(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
     return y;
 }
 
-// x <- softmax of the row.  A NaN, or a maximum that is infinite, makes the whole row NaN, as exp(x - max) / sum does.
-template <int L, int V>
-__device__ __forceinline__ void softmax_row(float (&x)[V]) {
+// pairs, pairs of pairs and so on: the rounding of a sum grows with the logarithm of V
+template <int N>
+__device__ __forceinline__ float tree_sum(float (&v)[N]) {
+#pragma unroll
+    for (int d = 1; d < N; d <<= 1)
+#pragma unroll
+        for (int i = 0; i + d < N; i += 2 * d) v[i] += v[i + d];
+    return v[0];
+}
+
+// x <- exp(x - max) of the row; their sum.  A NaN, or a maximum that is infinite, makes all of it NaN.
+template <int L, bool NEAR, int V>
+__device__ __forceinline__ float exp_row(float (&x)[V]) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
     m = group_max<L>(m);
-    float s = 0.f;
+    float s[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s += x[i] = exp_of(x[i] - m);
-    const float inv = __fdividef(1.f, group_sum<L>(s));          // 1 <= sum <= E: the approximate reciprocal is off by 2^-23
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] *= inv;
+    for (int i = 0; i < V; ++i) s[i] = x[i] = NEAR ? exp_near(x[i] - m) : expf(x[i] - m);
+    return group_sum<L>(tree_sum(s));
 }
 
 // Larger numbers have larger keys, +0 and -0 the same one, NaN the largest; 0 is below every number's.  Numbers of 16 bits leave room
@@ -202,10 +213,9 @@ __global__ void __launch_bounds__(kThreads) balance_fwd_kernel(const __grid_cons
         uint32_t key[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) key[i] = e0 + i < a.E ? order_key<T>(x[i], e0 + i) : 0u;
-        softmax_row<L, V>(x);
-        const float one = valid ? 1.f : 0.f;
+        const float total = exp_row<L, false>(x), inv = valid ? 1.f / total : 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] = fmaf(x[i], one, sum[i]);
+        for (int i = 0; i < V; ++i) sum[i] = fmaf(x[i], inv, sum[i]);
         // The k-th largest key: every lane's largest ones in order, and k times the largest first one of the row's lanes leaves its list.
         // Equal keys (fp32 only) would leave together: then more than k keys are as large as the last one, and the row's warp takes them
         // one by one, the lowest expert first.
@@ -369,13 +379,14 @@ __global__ void __launch_bounds__(kBwdThreads) balance_bwd_kernel(const __grid_c
         const bool valid = r < rows && (a.mask == nullptr || a.mask[r] != 0);
         float x[V];
         load_row<T, V>(x0 + min(r, rows - 1) * ld, e0, a.E, a.vec, x);
-        softmax_row<L, V>(x);
-        float s = 0.f;
+        // p (f - sum p f) with p = x / total: the reciprocal's rounding, which all p share, stays out of the difference
+        const float total = exp_row<L, sizeof(T) == 2>(x), inv = 1.f / total;
+        float pairs[V / 2];
 #pragma unroll
-        for (int i = 0; i < V; ++i) s = fmaf(x[i], e0 + i < a.E ? f[i] : 0.f, s);
-        s = group_sum<L>(s);
+        for (int i = 0; i < V; i += 2) pairs[i / 2] = fmaf(x[i], f[i], x[i + 1] * f[i + 1]);
+        const float s = group_sum<L>(tree_sum(pairs));
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = valid ? x[i] * (f[i] - s) * g : 0.f;
+        for (int i = 0; i < V; ++i) x[i] = valid ? x[i] * inv * (fmaf(f[i], total, -s) * (inv * g)) : 0.f;
         if (r < rows) store_row<T, V>(dx + (first + r) * a.E, e0, a.E, a.vec, x);
     }
 }

@@ -84,8 +84,8 @@ GROUPS["state_space_serving"] = ["window_attention.cu", "state_space.cu", "strea
                                  "runtime.cu", "gemm_tcgen05.cu", "gemm_smallm.cu", "fused_gemm_ar.cu", "tma_host.cu",
                                  "flash_attn_tc.cu", "attn_tc_host.cu"]
 
-# sources whose fp32 state is carried over thousands of steps, or whose fp32 results are exact to a rounding: no approximate exp /
-# tanh / division, no flushed subnormals
+# sources whose fp32 state is carried over thousands of steps, or whose fp32 results are exact to a few roundings: compiled without
+# approximate exp / tanh / division and without flushed subnormals
 PRECISE_SOURCES = {"mlstm.cu", "delta_rule.cu", "delta_chunks.cu", "retention.cu", "retention_tc.cu", "hyper_connection.cu", "stream_norm.cu",
                    "state_space.cu", "balance_loss.cu", "dropout.cu"}
 

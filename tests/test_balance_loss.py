@@ -130,6 +130,21 @@ def test_rows_left_out_hold_anything(fill, device):
             assert torch.equal(a, b) and not b[~mask].any()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("E", [8, 200])
+def test_small_probabilities(E, device):
+    """Gradients of experts far below the largest logit, whose differences from it are exact in fp32."""
+    x = torch.full((5, E), -50.0)
+    x[:, 0] = 0.0
+    x[:, 1:5] = torch.tensor([-11.3125, -29.59375, -58.71875, -83.03125])
+    leaf = x.to(device).requires_grad_()
+    (grad,) = torch.autograd.grad(load_balancing_loss_func(leaf, E, 1), leaf)
+    want = oracle([x], E, 1)[2]
+    # the exponential, 2 units in the last place (4 half steps), its sum, the division, two products, the share and the rows' sum
+    # p f, whose one large term is 1: less than 16 half steps
+    assert ((grad.double().cpu() - want).abs() <= 16 * FP32 * want.abs())[:, 1:].all()
+
+
 @pytest.mark.gpu
 def test_kernel_reads_views():
     g = torch.Generator(device="cuda").manual_seed(0)
