@@ -2,7 +2,7 @@
 
 Element ``i`` of the row-major tensor is kept when word ``i % 4`` of Philox4x32-7 (Salmon et al., SC 2011) at counter ``(i // 4,
 offset)`` under the key ``seed`` is at least ``p 2^32``, so the mask is the same on every device, in every layout and type, and for
-a call that activation checkpointing repeats."""
+a call that activation checkpointing repeats (one whose seed is a tensor: as long as that holds what it held, see ``dropout``)."""
 from __future__ import annotations
 
 import ctypes as _c
@@ -79,7 +79,11 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: Seed = None, offset: int = 0,
     ``seed``: a number (64 bits); or an int64 tensor of one or two on ``x``'s device, the seed and a number that is added to
     ``offset``, read when the kernel runs, so that a captured step which counts it on draws another mask in every replay; or
     ``None``: drawn from torch's CPU generator, which activation checkpointing winds back.  Two calls with the same seed and
-    offset drop the same elements: calls of one step take different offsets or seeds."""
+    offset drop the same elements: calls of one step take different offsets or seeds.
+
+    The backward pass of a call takes the numbers that the call read, whatever a seed tensor holds by then.  Activation checkpointing
+    calls again and reads again, and winds back torch's generators but no tensor of the program: under it a seed tensor is counted on
+    behind the backward pass, or the call gets a copy that stays (``state.clone()``, made outside the repeated part)."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability {p} not in [0, 1]")
     if not x.is_floating_point():

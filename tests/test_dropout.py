@@ -104,6 +104,27 @@ def test_module_draws_from_the_cpu_generator_and_checkpoints():
     assert m.eval()(x) is x
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_checkpointed_with_a_seed_tensor(device):
+    """Counted on behind the backward pass, or a copy that stays: both are the numbers that the first call read."""
+    from torch.utils.checkpoint import checkpoint
+
+    x = torch.ones(4096, device=device, requires_grad=True)
+    state = torch.tensor([5, 0], device=device)
+    for step in range(3):
+        y = checkpoint(lambda t: dropout(t, 0.5, state, 7) * t, x, use_reentrant=False)
+        (grad,) = torch.autograd.grad(y.sum(), x)
+        keep = dropout_keep((4096,), 0.5, 5, 7 + step, device)
+        assert torch.equal(y != 0, keep) and torch.equal(grad, 2 * y)
+        state[1] += 1
+    for step in range(3, 6):
+        now = state.clone()
+        y = checkpoint(lambda t: dropout(t, 0.5, now, 7) * t, x, use_reentrant=False)
+        state[1] += 1
+        (grad,) = torch.autograd.grad(y.sum(), x)
+        assert torch.equal(y != 0, dropout_keep((4096,), 0.5, 5, 7 + step, device)) and torch.equal(grad, 2 * y)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 7, 8, 9, 4095, 4096, 4097, 8192 * 3 + 1, 1 << 20])
