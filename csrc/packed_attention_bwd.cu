@@ -759,6 +759,7 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
     NXD_REQUIRE(D == 64 || D == 128, "packed_attn_bwd: head dim %d not supported (64 or 128)", D);
     NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && lse_row % 4 == 0 &&
                 (long long)entries * Hq * 16 < (1ll << 31), "packed_attn_bwd: bad problem");
+    NXD_REQUIRE(scale >= 1.17549435e-38f && scale <= 1.7014118e38f, "packed_attn_bwd: a scale of %g", scale);
     for (int i = 0; i < 16; ++i)
         NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn_bwd: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
     const void* bases[] = {q, k, v, o, rest, dout, lse, delta, dq_accum, dkv_accum, dq, dk, dv, tiles};

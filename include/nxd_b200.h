@@ -163,7 +163,7 @@ int nxd_flash_attn_bwd_tc(const void* q, const void* k, const void* v, const voi
  * elements: {q, k, v, o} forward, {q, k, v, o, dout, dq, dk, dv} backward, multiples of 8.
  * lse [Hq, columns] and rest [Hq, columns, D] bytes (NULL: not wanted; the backward call needs both), delta the same and 4 floats more; dq_accum [Hq, D, columns] of scratch; dkv_accum: NULL, or ZEROED
  * [2, Hkv, T, D] where nxd_packed_attn_bwd_splits is above 1.  Rows outside every sequence come out as zeros.
- * wait_tries: tries of 3900 clocks after which a wait inside a kernel gives up, -1: two seconds.  The results are NaN then (forward those
+ * scale: positive.  wait_tries: tries of 3900 clocks after which a wait inside a kernel gives up, -1: two seconds.  The results are NaN then (forward those
  * that the giving block owed, backward all), and the next call fails, or nxd_packed_attn_status (waits for the stream) says so. */
 int nxd_packed_plan_entries(long long T, int N, int rows);
 long long nxd_packed_plan_columns(long long T, int N);

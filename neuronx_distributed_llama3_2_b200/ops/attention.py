@@ -109,7 +109,8 @@ def flash_attn_packed_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """Attention of every sequence of a packed row to itself: q ``[T, Hq, D]``, k / v ``[T, Hkv, D]`` (``Hq`` a multiple of ``Hkv``)
     -> ``[T, Hq, D]``.  ``cu_seqlens [N + 1]`` (int32 or int64, on the tensors' device): sequence ``s`` is rows ``cu_seqlens[s] ..
     cu_seqlens[s + 1]``, or a ``PackedSequences`` that several calls share.  ``causal``: a token sees its sequence up to itself,
-    else all of it.  Rows outside every sequence give zeros and get zero gradients.
+    else all of it.  Rows outside every sequence give zeros and get zero gradients.  ``softmax_scale``: any number that fp32 holds as a
+    normal one, 0 (equal weights) and negative ones among them.
 
     Backends as ``flash_attn_func``; other types and head sizes than the kernel's run that function on one sequence after the
     other (the lengths are read on the host then)."""
@@ -119,6 +120,8 @@ def flash_attn_packed_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError(f"{q.shape[1]} query heads over {k.shape[1]} key heads")
     if q.dtype != k.dtype or q.dtype != v.dtype or q.device != k.device or q.device != v.device:
         raise ValueError("packed attention needs q, k and v of one type on one device")
+    if softmax_scale is not None and softmax_scale != 0 and not 2.0 ** -126 <= abs(softmax_scale) <= 2.0 ** 127:
+        raise ValueError(f"a softmax scale of {softmax_scale}")
     packed = as_packed(cu_seqlens, q.shape[0], q.device)
     if _backend(q) == "nxd":
         return packed_attn_nxd(q, k, v, packed, softmax_scale, causal)

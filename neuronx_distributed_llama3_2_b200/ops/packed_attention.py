@@ -231,12 +231,14 @@ class _RopePackedAttnFn(torch.autograd.Function):
 
 
 def packed_attn_nxd(q, k, v, packed: PackedSequences, softmax_scale: Optional[float], causal: bool) -> torch.Tensor:
-    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if scale <= 0.0:                # the kernels keep the maximum of the raw scores, which wants a positive scale
+        q, scale = (-q, -scale) if scale < 0.0 else (q * 0.0, 1.0)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if not grad and not _lib.transformed(q, k, v):          # forward-mode derivatives and ``torch.func`` are refused by the node
         with _lib.on_device_of(q):
-            return _forward(_fix(q), _fix(k), _fix(v), packed, float(scale), bool(causal), False)[0]
-    return _PackedAttnFn.apply(q, k, v, packed, float(scale), bool(causal))
+            return _forward(_fix(q), _fix(k), _fix(v), packed, scale, bool(causal), False)[0]
+    return _PackedAttnFn.apply(q, k, v, packed, scale, bool(causal))
 
 
 def rope_packed_attn(qkv, cos, sin, n_q: int, n_kv: int, packed: PackedSequences) -> torch.Tensor:

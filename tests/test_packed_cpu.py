@@ -78,6 +78,23 @@ def test_bad_tensors_are_refused():
         attention.rope_flash_attn_packed_func(q, None, None, 2, 2, cu)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.5, -2.0])
+def test_scales_that_are_not_positive(scale):
+    q, k, v, do = (x.requires_grad_() for x in _inputs(9, 4, 2, 8, torch.float32))
+    o = attention.flash_attn_packed_func(q, k, v, torch.tensor([0, 4, 9]), softmax_scale=scale)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, (q, k, v), do)), o=o)
+    want = packed(q, k, v, [0, 4, 9], True, do.detach(), scale)
+    for name, x in got.items():          # as in the test of the fp32 path, with scores up to six times as large
+        assert (x.double() - want[name][0]).abs().max() <= 2.0 ** -24 * 9 * 64 * 6
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e-39, 3e38, 1e300])
+def test_bad_scales_are_refused(scale):
+    q, k, v, _ = _inputs(9, 4, 2, 8, torch.float32)
+    with pytest.raises(ValueError):
+        attention.flash_attn_packed_func(q, k, v, torch.tensor([0, 9]), softmax_scale=scale)
+
+
 def test_bad_tables_are_refused():
     qkv, cu = torch.randn(9, 8, 16), torch.tensor([0, 4, 9])
     table = torch.ones(9, 8)

@@ -163,6 +163,23 @@ def test_scales(scale):
         assert (got[n].double() - want[n][0]).norm() <= 4 * 2.0 ** -8 * want[n][0].norm()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.125, -1.0, 2.0 ** -126])
+@pytest.mark.parametrize("causal,D", [(True, 64), (False, 128)])
+def test_scales_that_are_not_positive(scale, causal, D):
+    q, k, v, do = _inputs(400, 4, 2, D)
+    ends = [0, 150, 390]
+    got, want = _run(q, k, v, do, ends, causal, scale=scale), packed(q, k, v, ends, causal, do, scale)
+    bounds = packed(-q, k, v, ends, causal, do, -scale) if scale < 0.0 else want          # bounds of the same sums, with the scale's size
+    for name in got:
+        check(got[name], {name: (want[name][0], bounds[name][1])}, name)
+    from neuronx_distributed_llama3_2_b200.ops import packed_attention as pa
+
+    p = pa.PackedSequences(torch.tensor(ends, device="cuda"), 400)
+    for bad in (0.0, -1.0, float("nan"), float("inf"), 2.0 ** -130):
+        with pytest.raises(RuntimeError, match="scale"):
+            pa._forward(q, k, v, p, bad, causal, False)
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("D", [64, 128])
 def test_sequences_do_not_touch(causal, D):
