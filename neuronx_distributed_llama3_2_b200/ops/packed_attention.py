@@ -24,7 +24,8 @@ class PackedSequences:
     first boundary or behind the last belong to no sequence, attend to nothing and give zeros.  On the CPU this is checked; on
     the GPU, where a check would wait for the device, a boundary that falls or leaves the row is taken as the nearest one
     that does not.  What is made of the boundaries (tile lists, positions) is made once for every stream, and once inside every
-    captured graph, which reads ``cu_seqlens`` again in each replay; elsewhere lengths that change want a new object."""
+    captured graph, which reads ``cu_seqlens`` again in each replay; elsewhere lengths that change want a new object.  The object
+    holds what it made for each stream and for the last capture there: what earlier captures made is their graphs' alone."""
 
     def __init__(self, cu_seqlens: torch.Tensor, total: int):
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
@@ -56,8 +57,9 @@ class PackedSequences:
 
     def plan(self, causal: bool, rows: int = 128) -> Tuple[torch.Tensor, int, int]:
         """``(list of tiles of that many rows, its entries, columns of the per-row scratch)`` for the kernels, made on first use."""
-        key = (causal, rows, self._here())
-        if key not in self._plans:
+        stream, capture = self._here()
+        key = (causal, rows, stream, capture != 0)
+        if key not in self._plans or self._plans[key][0] != capture:
             most = min(self.count, self.total)
             entries = self.total // rows + most + 2                         # nxd_packed_plan_entries
             columns = (self.total + 3 * most + 3 & ~3) + 64                 # nxd_packed_plan_columns
@@ -66,20 +68,21 @@ class PackedSequences:
                                             _c.c_longlong(self.total), _c.c_int(causal), _c.c_int(rows), _lib.ptr(lists),
                                             _c.c_void_p(lists.data_ptr() + 16 * entries), _lib.stream_ptr())
             _lib.check(rc, "nxd_packed_plan")
-            self._plans[key] = (lists, entries, columns)
-        return self._plans[key]
+            self._plans[key] = (capture, (lists, entries, columns))
+        return self._plans[key][1]
 
     def positions(self) -> torch.Tensor:
         """int32 ``[total]``: every token's position in its own sequence (0 outside of them), for the rotation."""
-        here = self._here()
-        if here not in self._positions:
+        stream, capture = self._here()
+        key = (stream, capture != 0)
+        if key not in self._positions or self._positions[key][0] != capture:
             cu = self.cu_seqlens.long().clamp(0, self.total).cummax(0).values
             rows = torch.arange(self.total, device=self.device)
             s = torch.searchsorted(cu, rows, right=True) - 1
             inside = (s >= 0) & (s < self.count)
             pos = torch.where(inside, rows - cu[s.clamp(0, self.count)], 0)
-            self._positions[here] = pos.to(torch.int32)
-        return self._positions[here]
+            self._positions[key] = (capture, pos.to(torch.int32))
+        return self._positions[key][1]
 
     def first_tokens(self) -> torch.Tensor:
         """int64 ``[N]``: the row of every sequence's first token."""

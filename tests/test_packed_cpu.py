@@ -95,6 +95,27 @@ def test_bad_scales_are_refused(scale):
         attention.flash_attn_packed_func(q, k, v, torch.tensor([0, 9]), softmax_scale=scale)
 
 
+def test_captures_that_are_over_are_let_go(monkeypatch):
+    """A long-lived object keeps what the last capture of each stream made, and what the streams share without one."""
+    import weakref
+
+    p = PackedSequences(torch.tensor([0, 4, 9]), 9)
+    here = {"at": (1, 0)}
+    monkeypatch.setattr(p, "_here", lambda: here["at"])
+    eager = p.positions()
+    made = []
+    for capture in range(1, 20):
+        for stream in (1, 2):
+            here["at"] = (stream, capture)
+            x = p.positions()
+            assert x is p.positions() and x.tolist() == eager.tolist() and x is not eager
+            made.append(weakref.ref(x))
+            del x
+    assert sum(r() is not None for r in made) == 2 and all(r() is not None for r in made[-2:])
+    here["at"] = (1, 0)
+    assert p.positions() is eager
+
+
 def test_bad_tables_are_refused():
     qkv, cu = torch.randn(9, 8, 16), torch.tensor([0, 4, 9])
     table = torch.ones(9, 8)

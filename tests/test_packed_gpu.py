@@ -331,6 +331,34 @@ def test_two_graphs_and_two_streams_of_one_object(G):
     del trash
 
 
+def test_graphs_whose_lists_the_object_let_go():
+    """Earlier graphs of one object are replayed behind later captures, follow new lengths, and their memory goes back with them."""
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+    from neuronx_distributed_llama3_2_b200.ops.packed_attention import PackedSequences
+
+    T = 500
+    q, k, v, _ = (x.contiguous() for x in _inputs(T, 4, 2, 64))
+    cu = torch.tensor([0, 100, 500], dtype=torch.int32, device="cuda")
+    p = PackedSequences(cu, T)
+    flash_attn_packed_func(q, k, v, p)
+    graphs = []
+    for _ in range(4):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = flash_attn_packed_func(q, k, v, p)
+        graphs.append((graph, out))
+    assert len(p._plans) <= 2          # one list without a capture, one of the last
+    trash = [torch.full((T, 4), 1 << 20, dtype=torch.int32, device="cuda") for _ in range(64)]
+    for ends in ([0, 100, 500], [0, 333, 334], [7, 7, 480]):
+        cu.copy_(torch.tensor(ends))
+        want = packed(q, k, v, ends, True)
+        for graph, out in graphs[::-1]:
+            out.fill_(float("nan"))
+            graph.replay()
+            check(out, want, "o")
+    del trash
+
+
 def test_backward_has_the_lists_of_its_forward():
     """Boundaries that are overwritten before the backward pass, with heads that take other lists there."""
     from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
