@@ -135,7 +135,8 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedTile* tiles, int i
 // 0.0041, 16 tokens 0.0023 and 0.0028).  It falls with the root of the keys that a row averages over, so only query tiles that
 // meet one key tile have it (150 tokens: 0.0024 and 0.0026, 340: both 0.0024); for all tiles, 24 samples in 8192 tokens took 239 us
 // forward and backward instead of 228.
-// Four rows of the padded scratch at a time: [row / 4][D / 16][row % 4][16 bytes].
+// At most the first 128 rows of a sequence, so a head has 128 rows for each sequence, or, where that is less, the padded columns of the
+// per-row scratch.  Four rows at a time: [row / 4][D / 16][row % 4][16 bytes].
 template <int D>
 __device__ __forceinline__ long long rest_offset(long long row, int sixteenth) {
     return (row >> 2) * (4 * D) + sixteenth * 64 + (row & 3) * 16;

@@ -39,6 +39,8 @@ struct FwdParams {
     const PackedTile* tiles;
     float* lse;
     uint8_t* rest;                                // what rounding to bf16 took from o (attn_tc_common.cuh), NULL: not wanted
+    const int* which;                             // sequence of an entry; NULL: the rows of `rest` are the padded columns
+    long long rest_row;
     bf16* o;
     int* gave_up;                                 // host memory (packed_items.cuh)
     long long lse_row, o_head, o_row;
@@ -69,7 +71,7 @@ struct alignas(16) Item {
     int kind, start, len, pad;           // kind: 0 end of the items (`start`: the CTA's round that comes next), 1 an item, above: that many (less
                                          // kRowsOfNone) rows from `start` are of no sequence
     int t0, t1, n0, n1;                  // query tiles and the key tiles that they meet (0: there is no second one)
-    int h0, h1, hkv, unused;
+    int h0, h1, hkv, rest;               // rest: row of `rest` of the sequence's first
     __device__ __forceinline__ int t(int s) const { return s ? t1 : t0; }
     __device__ __forceinline__ int n(int s) const { return s ? n1 : n0; }
     __device__ __forceinline__ int h(int s) const { return s ? h1 : h0; }
@@ -83,7 +85,8 @@ __device__ __forceinline__ Item fetch_item(const FwdParams& p, int round) {
     const unsigned e = at / (unsigned)p.pairs;
     const int pr = (int)(at - e * p.pairs);
     const PackedTile pt = packed_tile(p.tiles, (int)e);
-    it.start = pt.start, it.len = pt.len, it.pad = pt.pad;
+    it.start = pt.start, it.len = pt.len, it.pad = it.rest = pt.pad;
+    if (p.which != nullptr) it.rest = (int)((unsigned)p.which[e] * kBN);          // (of no use where the entry is no item)
     it.h0 = HEADS ? 2 * pr : pr;
     it.h1 = HEADS ? it.h0 + 1 : it.h0;
     if (pt.len == 0) {                   // behind all items; an entry without anything: all that follow are like it
@@ -533,7 +536,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                         most = __vmaxu2(most, pack_bf16x2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])) & 0x7fff7fffu);
                     }
                     const float up = rest_up(most);
-                    uint8_t* to = p.rest + rest_offset<D>(head * p.lse_row + done.pad + at, g * 4);
+                    uint8_t* to = p.rest + rest_offset<D>(head * p.rest_row + done.rest + at, g * 4);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t w[4];
@@ -661,10 +664,10 @@ NXD_API int nxd_packed_attn_status(int* gave_up, void* stream) {
 
 // Attention inside each sequence of a packed batch: q [T, Hq, D], k and v [T, Hkv, D], o [T, Hq, D], strides {q_h, q_row, k_h,
 // k_row, v_h, v_row, o_h, o_row} in elements (multiples of 8), 16-byte aligned bases; tiles: the `entries` tiles that
-// nxd_packed_plan has made; lse NULL or [Hq, lse_row] floats, log2 units, written at the plan's padded columns; rest NULL or [Hq, lse_row,
-// D] bytes, for the backward pass.  Rows outside every sequence get zeros.  wait_tries: after which a wait gives up, -1: two seconds.
+// nxd_packed_plan has made; lse NULL or [Hq, lse_row] floats, log2 units, written at the plan's padded columns; rest NULL or [Hq, rest_row,
+// D] bytes, for the backward pass, where rest_row is 128 for each sequence and `which` the plan's, or NULL and rest_row is lse_row.  Rows outside every sequence get zeros.  wait_tries: after which a wait gives up, -1: two seconds.
 NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const long long* strides,
-                                const void* tiles, int entries, long long lse_row, long long T, int Hq, int Hkv, int D, float scale,
+                                const void* tiles, const int* which, long long rest_row, int entries, long long lse_row, long long T, int Hq, int Hkv, int D, float scale,
                                 int causal, int wait_tries, void* stream) {
     NXD_REQUIRE(D == 64 || D == 128, "packed_attn: head dim %d not supported (64 or 128)", D);
     NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && (long long)entries * Hq < (1ll << 31),
@@ -672,7 +675,7 @@ NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, voi
     NXD_REQUIRE(scale >= 1.17549435e-38f && scale <= 1.7014118e38f, "packed_attn: a scale of %g", scale);
     for (int i = 0; i < 8; ++i)
         NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
-    NXD_REQUIRE(q && k && v && o && tiles && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)tiles) & 15) == 0 && lse_row % 4 == 0,
+    NXD_REQUIRE(q && k && v && o && tiles && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)tiles) & 15) == 0 && lse_row % 4 == 0 && rest_row % 4 == 0,
                 "packed_attn: tensors must be 16-byte aligned, rows of the scratch multiples of four");
     FwdParams p{};
     int rc;
@@ -681,7 +684,7 @@ NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, voi
     p.tiles = (const PackedTile*)tiles;
     p.entries = entries;
     p.lse = lse; p.lse_row = lse_row;
-    p.rest = (uint8_t*)rest;
+    p.rest = (uint8_t*)rest; p.which = rest ? which : nullptr; p.rest_row = rest_row;
     p.group = Hq / Hkv;
     p.pairs = p.group % 2 == 0 ? Hq / 2 : Hq;
     p.scale_log2 = scale * 1.4426950408889634f;

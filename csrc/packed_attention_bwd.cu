@@ -577,8 +577,9 @@ packed_bwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 // (nobody reads the padding), the counter of claims and the mark behind it.  kD / 8 lanes own a row.  Bound by memory: 24576 rows of 16 heads of 64,
 // 201 MB, 38 us.
 template <int kD>
-__global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __restrict__ o, const uint8_t* __restrict__ rest, const bf16* __restrict__ dout, const PackedTile* tiles,
-                                                           float* __restrict__ delta, float* __restrict__ acc, int* claimed, long long o_head, long long o_row,
+__global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __restrict__ o, const uint8_t* __restrict__ rest, const bf16* __restrict__ dout,
+                                                           const PackedTile* tiles, const int* which, long long rest_row, float* __restrict__ delta,
+                                                           float* __restrict__ acc, int* claimed, long long o_head, long long o_row,
                                                            long long do_head, long long do_row, long long lse_row, int Hq, int causal) {
     pdl_wait();         // and no trigger: CTAs of the next kernel that come while the SMs are full of this one's blocks stay slower for good
                         // (4 documents in 16384 tokens, 32 heads of 128 over 8: 2060 us for the pass instead of 1750)
@@ -597,6 +598,7 @@ __global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __rest
     }
     const long long col = h * lse_row + pt.pad + first;
     const bool one_tile = causal ? pt.t == 0 : pt.len <= kBN;          // of keys: these rows have what the rounding took
+    const long long rest_at = h * rest_row + (which == nullptr ? pt.pad : (int)((unsigned)which[blockIdx.x / Hq] * kBN));
     constexpr int U = 4;                     // rows of a lane on their way
 #pragma unroll 1
     for (int r0 = threadIdx.x / L; r0 < kBN; r0 += U * R) {
@@ -609,7 +611,7 @@ __global__ void __launch_bounds__(256, 4) packed_delta_kernel(const bf16* __rest
             if (r < rows) {
                 a[u] = reinterpret_cast<const bf16x8*>(o + h * o_head + row * o_row)[l];
                 g[u] = reinterpret_cast<const bf16x8*>(dout + h * do_head + row * do_row)[l];
-                if (one_tile) less[u] = *reinterpret_cast<const uint2*>(rest + rest_offset<kD>(col + r, l >> 1) + (l & 1) * 8);
+                if (one_tile) less[u] = *reinterpret_cast<const uint2*>(rest + rest_offset<kD>(rest_at + r, l >> 1) + (l & 1) * 8);
             }
         }
 #pragma unroll
@@ -749,15 +751,15 @@ NXD_API int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv) {
 }
 
 // Backward of nxd_packed_attn_fwd.  strides: {head, row} in elements of q, k, v, o, dout, dq, dk, dv (16 values, multiples of 8);
-// lse, rest: what the forward pass wrote; delta: Hq * lse_row + 4 floats of scratch; dq_accum: [Hq, D, lse_row] floats of scratch;
+// lse, rest: what the forward pass wrote (which, rest_row: as there); delta: Hq * lse_row + 4 floats of scratch; dq_accum: [Hq, D, lse_row] floats of scratch;
 // dkv_accum: NULL, or ZEROED [2, Hkv, T, D] floats where nxd_packed_attn_bwd_splits says more than one.
 // dQ (with splits dK and dV too) is summed in fp32 in an order that is not fixed.  wait_tries: as forward.
 NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse,
                                 float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
-                                const long long* strides, const void* tiles, int entries, long long lse_row, long long T, int N, int Hq,
+                                const long long* strides, const void* tiles, const int* which, long long rest_row, int entries, long long lse_row, long long T, int N, int Hq,
                                 int Hkv, int D, float scale, int causal, int wait_tries, void* stream) {
     NXD_REQUIRE(D == 64 || D == 128, "packed_attn_bwd: head dim %d not supported (64 or 128)", D);
-    NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && lse_row % 4 == 0 &&
+    NXD_REQUIRE(T > 0 && T < (1ll << 31) - 256 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && entries > 0 && lse_row % 4 == 0 && rest_row % 4 == 0 &&
                 (long long)entries * Hq * 16 < (1ll << 31), "packed_attn_bwd: bad problem");
     NXD_REQUIRE(scale >= 1.17549435e-38f && scale <= 1.7014118e38f, "packed_attn_bwd: a scale of %g", scale);
     for (int i = 0; i < 16; ++i)
@@ -781,10 +783,10 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
     p.dv = (bf16*)dv; p.dv_head = strides[14]; p.dv_row = strides[15];
     const unsigned per_head = (unsigned)entries * Hq;
     if (D == 128)
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<128>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const uint8_t*)rest, (const bf16*)dout, pt,
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<128>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const uint8_t*)rest, (const bf16*)dout, pt, which, rest_row,
             delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq, causal)));
     else
-        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<64>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const uint8_t*)rest, (const bf16*)dout, pt,
+        NXD_CHECK_CUDA((nxd_launch_pdl(packed_delta_kernel<64>, dim3(per_head), dim3(256), 0, st, (const bf16*)o, (const uint8_t*)rest, (const bf16*)dout, pt, which, rest_row,
             delta, dq_accum, p.claimed, strides[6], strides[7], strides[8], strides[9], lse_row, Hq, causal)));
     NXD_LAUNCH_CHECK();
     CUtensorMap tq, tdo, tk, tv, tdq, tdka, tdva;

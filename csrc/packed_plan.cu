@@ -56,7 +56,7 @@ __device__ int block_scan(int v, int* warps, int& total) {
 
 template <typename Index>
 __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const Index* __restrict__ cu, int N, int T, int causal, int rows, PackedTile* tiles,
-                                                              int entries, int4* seqs) {
+                                                              int entries, int4* seqs, int* which) {
     __shared__ int bins[kBins + 2], warps[32];
     const int tid = threadIdx.x, lane = tid & 31;
     pdl_trigger();
@@ -124,19 +124,21 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const Index* __re
         }
     }
     __syncthreads();
-    const auto place = [&](const int4& s, int t) {
+    const auto place = [&](const int4& s, int t, int sequence) {
         const int at = atomicAdd(&bins[min(causal ? t + 1 : s.w, kBins)], 1);
-        if (at < entries) reinterpret_cast<int4*>(tiles)[at] = make_int4(s.x, s.y, t, s.z);
+        if (at >= entries) return;
+        reinterpret_cast<int4*>(tiles)[at] = make_int4(s.x, s.y, t, s.z);
+        which[at] = sequence;
     };
     for (int base = 0; base < N; base += kThreads) {
         const int i = base + tid;
         const int4 s = i < N ? seqs[i] : make_int4(0, 0, 0, 0);
-        for (int t = 0; t < min(s.w, kOwn); ++t) place(s, t);
+        for (int t = 0; t < min(s.w, kOwn); ++t) place(s, t, i);
         for (unsigned more = __ballot_sync(0xffffffffu, s.w > kOwn); more; more &= more - 1) {
             const int from = __ffs(more) - 1;
             const int4 q = make_int4(__shfl_sync(0xffffffffu, s.x, from), __shfl_sync(0xffffffffu, s.y, from),
                                      __shfl_sync(0xffffffffu, s.z, from), __shfl_sync(0xffffffffu, s.w, from));
-            for (int t = kOwn + lane; t < q.w; t += 32) place(q, t);
+            for (int t = kOwn + lane; t < q.w; t += 32) place(q, t, base + (tid & ~31) + from);
         }
     }
     // rows before the first and behind the last sequence, then entries without work
@@ -165,8 +167,8 @@ NXD_API long long nxd_packed_plan_columns(long long T, int N) {
 }
 
 // cu: N + 1 boundaries, int32 or (wide) int64; rows of a tile: 128 or 256; tiles: nxd_packed_plan_entries entries of 16 bytes; seqs: 16 bytes of scratch
-// per sequence, afterwards {first row, rows, first padded column, tiles} of each.
-NXD_API int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, int rows, void* tiles, void* seqs, void* stream) {
+// per sequence, afterwards {first row, rows, first padded column, tiles} of each; which: an int per entry, the number of the tile's sequence.
+NXD_API int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, int rows, void* tiles, void* seqs, int* which, void* stream) {
     NXD_REQUIRE(rows == 128 || rows == 256, "packed_plan: tiles of %d rows", rows);
     const int entries = nxd_packed_plan_entries(T, N, rows);
     NXD_REQUIRE(N >= 0 && T > 0 && T < (1ll << 31) - 256 && entries > 0, "packed_plan: %d sequences in %lld rows", N, T);
@@ -174,10 +176,10 @@ NXD_API int nxd_packed_plan(const void* cu, int wide, int N, long long T, int ca
     cudaStream_t st = (cudaStream_t)stream;
     if (wide)
         NXD_CHECK_CUDA((nxd_launch_pdl(packed_plan_kernel<long long>, dim3(1), dim3(kThreads), 0, st, (const long long*)cu, N, (int)T, causal, rows,
-            (PackedTile*)tiles, entries, (int4*)seqs)));
+            (PackedTile*)tiles, entries, (int4*)seqs, which)));
     else
         NXD_CHECK_CUDA((nxd_launch_pdl(packed_plan_kernel<int>, dim3(1), dim3(kThreads), 0, st, (const int*)cu, N, (int)T, causal, rows,
-            (PackedTile*)tiles, entries, (int4*)seqs)));
+            (PackedTile*)tiles, entries, (int4*)seqs, which)));
     NXD_LAUNCH_CHECK();
     return 0;
 }

@@ -158,24 +158,27 @@ int nxd_flash_attn_bwd_tc(const void* q, const void* k, const void* v, const voi
 
 /* ---- attention over packed sequences (rows cu[s] .. cu[s + 1] of a row of T tokens each attend to themselves) ------------
  * nxd_packed_plan makes the tile list from the boundaries on the device (int32, or int64 with `wide`): room for
- * nxd_packed_plan_entries tiles of 16 bytes, `seqs` 16 bytes per sequence; nxd_packed_plan_columns is the row length of
+ * nxd_packed_plan_entries tiles of 16 bytes and as many ints (`which`), `seqs` 16 bytes per sequence; nxd_packed_plan_columns is the row length of
  * the per-row scratch.  Tiles have 128 rows, but 256 for the forward call where Hq / Hkv is odd.  strides = {head, row} in
  * elements: {q, k, v, o} forward, {q, k, v, o, dout, dq, dk, dv} backward, multiples of 8.
- * lse [Hq, columns] and rest [Hq, columns, D] bytes (NULL: not wanted; the backward call needs both), delta the same and 4 floats more; dq_accum [Hq, D, columns] of scratch; dkv_accum: NULL, or ZEROED
+ * lse [Hq, columns] and rest [Hq, rest_row, D] bytes (NULL: not wanted; the backward call needs both; rest_row: 128 N, or columns with
+ * `which` NULL), delta the same and 4 floats more; dq_accum [Hq, D, columns] of scratch; dkv_accum: NULL, or ZEROED
  * [2, Hkv, T, D] where nxd_packed_attn_bwd_splits is above 1.  Rows outside every sequence come out as zeros.
  * scale: positive.  wait_tries: tries of 3900 clocks after which a wait inside a kernel gives up, -1: two seconds.  The results are NaN then (forward those
  * that the giving block owed, backward all), and the next call fails, or nxd_packed_attn_status (waits for the stream) says so. */
 int nxd_packed_plan_entries(long long T, int N, int rows);
 long long nxd_packed_plan_columns(long long T, int N);
-int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, int rows, void* tiles, void* seqs, void* stream);
+int nxd_packed_plan(const void* cu, int wide, int N, long long T, int causal, int rows, void* tiles, void* seqs, int* which, void* stream);
 int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const long long* strides,
-                        const void* tiles, int entries, long long columns, long long T, int Hq, int Hkv, int D, float scale,
+                        const void* tiles, const int* which, long long rest_row, int entries, long long columns, long long T, int Hq, int Hkv,
+                        int D, float scale,
                         int causal, int wait_tries, void* stream);
 int nxd_packed_attn_status(int* gave_up, void* stream);
 int nxd_packed_attn_bwd_splits(long long T, int N, int Hq, int Hkv);
 int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse,
                         float* delta, float* dq_accum, float* dkv_accum, void* dq, void* dk, void* dv,
-                        const long long* strides, const void* tiles, int entries, long long columns, long long T, int N,
+                        const long long* strides, const void* tiles, const int* which, long long rest_row, int entries, long long columns,
+                        long long T, int N,
                         int Hq, int Hkv, int D, float scale, int causal, int wait_tries, void* stream);
 
 /* ---- dropout: y = keep(i) ? x / (1 - p) : 0, plus residual (NULL: none); 0 < p < 1 ---------------------------------------

@@ -63,10 +63,10 @@ class PackedSequences:
             most = min(self.count, self.total)
             entries = self.total // rows + most + 2                         # nxd_packed_plan_entries
             columns = (self.total + 3 * most + 3 & ~3) + 64                 # nxd_packed_plan_columns
-            lists = torch.empty((entries + self.count, 4), dtype=torch.int32, device=self.device)
+            lists = torch.empty((entries + self.count + (entries + 3) // 4, 4), dtype=torch.int32, device=self.device)
             rc = _lib.lib().nxd_packed_plan(_lib.ptr(self.cu_seqlens), _c.c_int(self.cu_seqlens.dtype == torch.int64), _c.c_int(self.count),
                                             _c.c_longlong(self.total), _c.c_int(causal), _c.c_int(rows), _lib.ptr(lists),
-                                            _c.c_void_p(lists.data_ptr() + 16 * entries), _lib.stream_ptr())
+                                            _c.c_void_p(lists.data_ptr() + 16 * entries), _which(lists, entries, self.count), _lib.stream_ptr())
             _lib.check(rc, "nxd_packed_plan")
             self._plans[key] = (capture, (lists, entries, columns))
         return self._plans[key][1]
@@ -143,6 +143,18 @@ def gave_up() -> bool:
     return bool(flag.value)
 
 
+def _which(lists: torch.Tensor, entries: int, count: int) -> _c.c_void_p:
+    """Where a plan's list has the sequences' numbers of its tiles: behind the tiles and the sequences."""
+    return _c.c_void_p(lists.data_ptr() + 16 * (entries + count))
+
+
+def _rest_of(rest: Optional[torch.Tensor], lists: torch.Tensor, entries: int, columns: int, count: int) -> tuple:
+    """Of what the rounding took from the result: the sequences' numbers if it has 128 rows for each (``None``: one row a column), rows."""
+    if rest is None or rest.shape[1] == columns:
+        return None, _c.c_longlong(columns)
+    return _which(lists, entries, count), _c.c_longlong(rest.shape[1])
+
+
 def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad: bool, wait_tries: int = -1):
     """``(o, lse, rest)``; the two that the backward pass takes are ``None`` without it.  ``wait_tries``: of a wait inside the kernel, -1: two
     seconds (``gave_up``; the next call raises)."""
@@ -151,9 +163,10 @@ def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad:
     tiles, entries, columns = packed.plan(causal, 128 if Hq // k.shape[1] % 2 == 0 else 256)
     o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((Hq, columns), dtype=torch.float32, device=q.device) if grad else None
-    rest = torch.empty((Hq, columns, D), dtype=torch.uint8, device=q.device) if grad else None
+    rest = torch.empty((Hq, min(columns, 128 * max(1, packed.count)), D), dtype=torch.uint8, device=q.device) if grad else None
     rc = _lib.lib().nxd_packed_attn_fwd(
-        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(lse), _lib.ptr(rest), _strides(q, k, v, o), _lib.ptr(tiles), _c.c_int(entries),
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(lse), _lib.ptr(rest), _strides(q, k, v, o), _lib.ptr(tiles),
+        *_rest_of(rest, tiles, entries, columns, packed.count), _c.c_int(entries),
         _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(Hq), _c.c_int(k.shape[1]), _c.c_int(D), _c.c_float(scale), _c.c_int(causal),
         _c.c_int(wait_tries), _lib.stream_ptr())
     _lib.check(rc, "nxd_packed_attn_fwd")
@@ -172,7 +185,8 @@ def _backward(q, k, v, o, lse, rest, do, dq, dk, dv, plan, count: int, scale: fl
     kv_acc = torch.zeros((2, Hkv, T, D), dtype=torch.float32, device=q.device) if splits > 1 else None
     rc = _lib.lib().nxd_packed_attn_bwd(
         _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(o), _lib.ptr(rest), _lib.ptr(do), _lib.ptr(lse), _lib.ptr(delta), _lib.ptr(acc), _lib.ptr(kv_acc),
-        _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _strides(q, k, v, o, do, dq, dk, dv), _lib.ptr(tiles), _c.c_int(entries),
+        _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _strides(q, k, v, o, do, dq, dk, dv), _lib.ptr(tiles),
+        *_rest_of(rest, tiles, entries, columns, count), _c.c_int(entries),
         _c.c_longlong(columns), _c.c_longlong(T), _c.c_int(count), _c.c_int(Hq), _c.c_int(Hkv), _c.c_int(D), _c.c_float(scale),
         _c.c_int(causal), _c.c_int(wait_tries), _lib.stream_ptr())
     _lib.check(rc, "nxd_packed_attn_bwd")

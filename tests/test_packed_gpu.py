@@ -387,6 +387,26 @@ def test_delta_is_not_of_the_rounded_result(D):
     assert (got["dq"] != 0).any(-1).float().mean() <= 0.1
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_what_rounding_took_is_kept_by_sequence(D, causal):
+    """As above in a long row with few sequences, some of them long or empty; what is kept for it grows with the sequences, not the row."""
+    from neuronx_distributed_llama3_2_b200.ops import packed_attention as pa
+
+    lens, H = [2] * 40 + [0, 5000, 0, 300] + [2] * 40 + [0], 4
+    T = sum(lens) + 9000
+    ends = _ends(lens, 200)
+    _, _, v, do = _inputs(T, H, H, D)
+    q, k = torch.zeros_like(v), torch.ones_like(v)
+    p = pa.PackedSequences(torch.tensor(ends, device="cuda"), T)
+    _, _, rest = pa._forward(q, k, v, p, D ** -0.5, causal, True)
+    assert rest.numel() == H * 128 * len(lens) * D < H * T * D
+    dq = _run(q, k, v, do, torch.tensor(ends, device="cuda"), causal)["dq"]
+    # causal: the first token sees itself alone, and its score gradient is fp32's rounding; the second has the two of one half
+    pairs = [a + i for a, n in zip(ends, lens) if n == 2 for i in range(causal, 2)]
+    assert (dq[pairs] != 0).any(-1).float().mean() <= 0.1
+
+
 @pytest.mark.parametrize("how", ["checkpoint", "on the host"])
 def test_saved_tensors_that_move(how):
     from torch.utils.checkpoint import checkpoint
