@@ -36,13 +36,21 @@ def _table(rows: Sequence[torch.Tensor], mask: Optional[torch.Tensor], E: int, t
             _c.c_int(top_k))
 
 
-def _where(mask: Optional[torch.Tensor], rows: Sequence[torch.Tensor]) -> list:
-    """What the table says of its tensors but their sizes."""
-    return [mask is not None and mask.data_ptr(), *[t.data_ptr() for t in rows], *[t.stride(0) for t in rows]]
-
-
-# what moves saved tensors: the innermost pair of hooks, None without one
+# what moves saved tensors: the innermost pair of hooks, None without one; whether the backward pass that goes on leaves the graph for another
 _saved_hooks = getattr(torch._C._autograd, "_top_saved_tensors_default_hooks", lambda _: "unknown")
+_keeps_graph = getattr(torch._C._autograd, "_get_current_graph_task_keep_graph", lambda: True)
+
+
+class _Kept:
+    """A call's table of addresses with the storages that it points into: ``logits.data = ...`` behind the loss, or hooks on what the node
+    saved, give the saved tensors other storage, while the gradient wants the values that the loss saw."""
+
+    def __init__(self, table: tuple, tensors: Sequence[torch.Tensor]):
+        self.table, self.storages = table, [t.untyped_storage() for t in tensors]
+        self.at = [s.data_ptr() for s in self.storages]
+
+    def valid(self) -> bool:          # a storage can be resized
+        return [s.data_ptr() for s in self.storages] == self.at
 
 
 class _BalanceLossFn(torch.autograd.Function):
@@ -62,16 +70,10 @@ class _BalanceLossFn(torch.autograd.Function):
         _lib.check(rc, "nxd_balance_loss_fwd")
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)         # no zeros for the counts' gradient
-        # Without hooks the program's own tensors are saved as they are, so that ``logits.data = ...`` gives them other storage: what is
-        # saved is another tensor on the storage of this call (the gradient wants its values), and its writes are counted with theirs.  The
-        # tensors themselves are for a gradient that is differentiated.
-        where = None
-        if _saved_hooks(True) is None:
-            where = _where(mask, rows)
-            ctx.save_for_backward(share, mask, *[r.detach() if r is t else r for r, t in zip(rows, logits)], *logits)
-        else:
-            ctx.save_for_backward(share, mask, *logits)
-        ctx.args = (table, where, E, top_k, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
+        ctx.save_for_backward(share, mask, *logits)
+        # hooks (checkpointing, offloading) are there to let the memory go; what they give back is read where it lies
+        ctx.kept = None if _saved_hooks(True) is not None else _Kept(table, rows if mask is None else [*rows, mask])
+        ctx.args = (E, top_k, x.dtype, sizes, [None if r is t else t.shape for r, t in zip(rows, logits)])
         return loss, counts
 
     @staticmethod
@@ -79,30 +81,32 @@ class _BalanceLossFn(torch.autograd.Function):
         if grad is None:
             return (None,) * len(ctx.needs_input_grad)
         saved = ctx.saved_tensors          # all of them: none may have been written since
-        table, where, E, top_k, sizes, shapes = ctx.args
-        n = len(sizes)
-        share, mask, rows = saved[0], saved[1], saved[2:2 + n]
+        E, top_k, dtype, sizes, shapes = ctx.args
+        share, mask, logits = saved[0], saved[1], saved[2:]
+        kept, need = ctx.kept, ctx.needs_input_grad[3:]
+        if not _keeps_graph():             # like what is saved, these go with the last pass
+            ctx.kept = None
         if torch.is_grad_enabled():        # this gradient is differentiated itself: in torch operations, on the program's own tensors
-            logits, need = saved[-n:], ctx.needs_input_grad[3:]
             loss, _ = balance_loss_ref(list(logits), E, top_k, mask)
             grads = iter(torch.autograd.grad(loss, [t for t, x in zip(logits, need) if x], grad.to(loss.dtype), create_graph=True))
             return (None, None, None, *[next(grads) if x else None for x in need])
-        if where is None or _where(mask, rows) != where:    # checkpointing, offloading; the table of 32 layers costs a tenth of the call
-            rows = [_rows(t, E) for t in rows]
-            if [tuple(t.shape) for t in rows] != [(n, E) for n in sizes]:
-                raise RuntimeError(f"router logits saved for the balance loss have become {[tuple(t.shape) for t in rows]}")
+        if kept is not None and kept.valid():          # the table of 32 layers costs a tenth of the call
+            table = kept.table
+        else:
+            rows = [_rows(t, E) for t in logits]
+            if [(*t.shape, t.dtype, t.device) for t in rows] != [(n, E, dtype, share.device) for n in sizes]:
+                raise RuntimeError(f"router logits saved for the balance loss have become {[(*t.shape, t.dtype, t.device) for t in rows]}")
             table = _table(rows, mask, E, top_k)
-        x = rows[0]
-        dx = torch.empty((sum(sizes), x.shape[1]), dtype=x.dtype, device=x.device)
+        dx = torch.empty((sum(sizes), E), dtype=dtype, device=share.device)
         grad = grad.float()
-        with _lib.on_device_of(x):
+        with _lib.on_device_of(share):
             rc = _lib.lib().nxd_balance_loss_bwd(*table, _lib.ptr(share), _lib.ptr(grad), _lib.ptr(dx), _lib.stream_ptr())
         _lib.check(rc, "nxd_balance_loss_bwd")
         grads = dx.split(sizes)
         if any(s is not None for s in shapes):
             grads = [g if s is None else g.view(s) for g, s in zip(grads, shapes)]
-        if not all(ctx.needs_input_grad[3:]):
-            grads = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[3:])]
+        if not all(need):
+            grads = [g if x else None for g, x in zip(grads, need)]
         return (None, None, None, *grads)
 
 

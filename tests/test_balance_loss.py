@@ -231,10 +231,36 @@ def test_saved_logits_that_move(how):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("how", ["other data", "smaller data", "hooks of the node", "a view moved"])
+def test_logits_written_behind_the_loss():
+    leaf = _logits(1, 200, 8, torch.float32, "cuda")[0].requires_grad_()
+    for x in (leaf, leaf * 1.0):
+        loss = load_balancing_loss_func(x, 8, 2)
+        with torch.no_grad():
+            x.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, leaf)
+
+
+@pytest.mark.gpu
+def test_memory_goes_with_the_last_pass():
+    """A loss that the program keeps does not hold the logits beyond the passes through its graph."""
+    for again in (False, True):
+        leaf = torch.randn(8, 8, device="cuda", requires_grad=True)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = load_balancing_loss_func(torch.ones(1 << 20, 8, device="cuda") @ leaf, 8, 2)
+        if again:
+            torch.autograd.grad(loss, leaf, retain_graph=True)
+            assert torch.cuda.memory_allocated() - before >= 32 << 20
+        torch.autograd.grad(loss, leaf)
+        assert torch.cuda.memory_allocated() - before < 1 << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["other data", "smaller data", "data on the host", "hooks of the node", "a view moved"])
 def test_saved_logits_that_get_other_storage(how):
     """The gradient is that of the logits as the loss saw them, wherever they lie by then."""
-    for leaf in (True, False):
+    for leaf in (False,) if how == "data on the host" else (True, False):          # torch refuses a leaf that went to another device
         logits = [t.requires_grad_() for t in _logits(3, 200, 8, torch.float32, "cuda", seed=5)]
         seen = logits if leaf else [t * 1.0 for t in logits]
         (want,) = torch.autograd.grad(load_balancing_loss_func(seen, 8, 2), logits[1], retain_graph=True)
@@ -248,12 +274,13 @@ def test_saved_logits_that_get_other_storage(how):
                     saved.register_hooks(lambda t: kept.append(t.cpu()) or len(kept) - 1, lambda i: kept[i].cuda())
         else:
             for t in seen:
-                t.data = {"other data": lambda: torch.full_like(t, math.nan), "smaller data": lambda: t.data[:1, :1].clone(),
+                t.data = {"other data": lambda: torch.full_like(t, math.nan), "smaller data": lambda: t.data[:1, :1].clone(), "data on the host": lambda: t.data.cpu(),
                           "a view moved": lambda: torch.full((200, 16), math.nan, device="cuda")[:, ::2]}[how]()
         trash = [torch.full((200, 8), math.nan, device="cuda") for _ in range(64)]          # where the logits were
-        for out, same in ((loss, want), (masked, want_masked)):
-            (got,) = torch.autograd.grad(out, logits[1], retain_graph=True)
-            assert torch.equal(got, same)
+        for _ in range(2):          # the graph is kept
+            for out, same in ((loss, want), (masked, want_masked)):
+                (got,) = torch.autograd.grad(out, logits[1], retain_graph=True)
+                assert torch.equal(got, same)
         del trash
 
 
