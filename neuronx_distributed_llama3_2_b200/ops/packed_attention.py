@@ -176,9 +176,13 @@ def _forward(q, k, v, packed: PackedSequences, scale: float, causal: bool, grad:
 def _backward(q, k, v, o, lse, rest, do, dq, dk, dv, plan, count: int, scale: float, causal: bool, wait_tries: int = -1) -> None:
     """Every element of ``dq / dk / dv`` is written.  ``plan``: the list that the forward pass had, or one made with it."""
     q, k, v, o, do = (_fix(t) for t in (q, k, v, o, do))          # what was saved may have been moved
-    T, Hq, D = q.shape
+    T, Hq, D = o.shape
     Hkv = k.shape[1]
     tiles, entries, columns = plan
+    if (q.shape != o.shape or do.shape != o.shape or k.shape != (T, Hkv, D) or v.shape != k.shape or not Hkv or Hq % Hkv
+            or any(x.dtype != o.dtype or x.device != o.device for x in (q, k, v, do))):          # ``q.data = ...`` since
+        raise RuntimeError(f"packed attention saved q, k and v for a result {tuple(o.shape)} {o.dtype} on {o.device}; they have become "
+                           + ", ".join(f"{tuple(x.shape)} {x.dtype} on {x.device}" for x in (q, k, v)))
     delta = torch.empty(lse.numel() + 4, dtype=torch.float32, device=q.device)
     acc = torch.empty((Hq, D, columns), dtype=torch.float32, device=q.device)
     splits = _lib.lib().nxd_packed_attn_bwd_splits(_c.c_longlong(T), _c.c_int(count), _c.c_int(Hq), _c.c_int(Hkv))

@@ -432,6 +432,23 @@ def test_saved_tensors_that_move(how):
     del trash
 
 
+def test_saved_tensors_that_do_not_fit_are_refused():
+    """Tensors that got other data behind the forward pass: no kernel reads beyond what they have now."""
+    from neuronx_distributed_llama3_2_b200.ops.attention import flash_attn_packed_func
+
+    T, ends = 300, [0, 120, 290]
+    q, k, v, do = (x.contiguous() for x in _inputs(T, 4, 2, 64))
+    cu = torch.tensor(ends, device="cuda")
+    for at in range(3):
+        for other in (lambda x: x[:7].clone(), lambda x: x[:, :1].clone(), lambda x: x[..., :32].clone(), lambda x: x.float(), lambda x: x.cpu()):
+            leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+            args = [x * 1.0 for x in leaves]
+            o = flash_attn_packed_func(*args, cu)
+            args[at].data = other(args[at].data)
+            with pytest.raises(RuntimeError, match="have become"):
+                torch.autograd.grad(o, leaves, do)
+
+
 def test_tables_shorter_than_the_row():
     """Rotation tables as long as the longest sequence are enough, and a sequence that is longer reads no further."""
     from neuronx_distributed_llama3_2_b200.ops import attention, rope
