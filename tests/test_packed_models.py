@@ -266,6 +266,54 @@ def _two_ranks_entry(rank, world, sp):
     _two_ranks(rank, world, sp)
 
 
+
+def _two_ranks_gradients(rank, world, family, sp):
+    from test_llama_tp_cpu import _shard_from_full, _solo
+    from neuronx_distributed_llama3_2_b200.parallel import parallel_state as ps
+    from neuronx_distributed_llama3_2_b200.parallel.grads import allreduce_sequence_parallel_gradients
+
+    if not ps.model_parallel_is_initialized():
+        ps.initialize_model_parallel(tensor_model_parallel_size=world)
+    # every rank of a tensor-parallel group adds the balance loss's gradient to the routers' sum, with and without packed rows: left out
+    make, config, kw = {"llama": (M.LlamaForCausalLM, M.tiny_llama, {}), "bert": (BertForPreTraining, tiny_bert, {}),
+                        "mixtral": (M.MixtralForCausalLM, M.tiny_mixtral, {"capacity_factor": None, "router_aux_loss_coef": 0.0})}[family]
+    g = torch.Generator().manual_seed(1)
+    ends, row = [0, 7, 8, 20, 30], 32
+    ids = torch.randint(0, 512, (1, row), generator=g)
+    batch = {"input_ids": ids, "labels": ids, "cu_seqlens": torch.tensor(ends)}
+    if family == "bert":
+        labels = torch.where(torch.rand(1, row, generator=g) < 0.5, ids, -100)
+        labels[:, ends[-1]:] = -100
+        batch.update(labels=labels, token_type_ids=torch.randint(0, 2, (1, row), generator=g), next_sentence_label=torch.tensor([1, 0, 1, 1]))
+    torch.manual_seed(3)
+    with _solo():
+        full = make(config(sequence_parallel_enabled=False, **kw)).train()
+        want = full(**batch)
+        want.backward()
+    model = make(config(sequence_parallel_enabled=sp, **kw)).train()
+    _shard_from_full(full, model, world, rank)
+    got = model(**batch)
+    got.backward()
+    if sp:
+        allreduce_sequence_parallel_gradients(list(model.parameters()))
+    assert abs(got - want) <= FP32 * abs(want), (got, want)
+    grads = {n: p.grad for n, p in model.named_parameters()}
+    with torch.no_grad():          # the whole model's gradients, cut as its weights are
+        for p in full.parameters():
+            p.copy_(p.grad)
+    _shard_from_full(full, model, world, rank)
+    for n, p in model.named_parameters():
+        _near(grads[n], p.detach(), n)
+
+
+@pytest.mark.parametrize("family", ["llama", "mixtral", "bert"])
+@pytest.mark.parametrize("sp", [False, True])
+def test_two_ranks_gradients(family, sp):
+    from conftest import run_distributed
+
+    run_distributed(_two_ranks_gradients, 2, family, sp)
+
+
 # -- on the GPU --------------------------------------------------------------------------------------------------------------
 GPU_ENDS, GPU_ROW = [0, 130, 131, 131, 448, 700], 768
 
@@ -316,6 +364,33 @@ def test_llama_lora_step_follows_fp32(head_dim, kv):
     assert abs(runs[0][0] - runs[1][0]) <= bound * runs[0][0]
     for n, want in runs[0][1].items():
         assert (runs[1][1][n] - want).norm() <= bound * want.norm(), (n, ((runs[1][1][n] - want).norm() / want.norm()).item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [4, 2])
+def test_bert_step_follows_fp32(heads):
+    """A pre-training step on a row of sentences in bf16 on the kernels against fp32 without them, with the same dropout masks."""
+    ends, g = [0, 130, 131, 448, 700], torch.Generator().manual_seed(1)
+    ids, types = torch.randint(0, 512, (1, GPU_ROW), generator=g), torch.randint(0, 2, (1, GPU_ROW), generator=g)
+    labels = torch.where(torch.rand(1, GPU_ROW, generator=g) < 0.3, ids, -100)
+    labels[:, ends[-1]:] = -100
+    runs = []
+    for dev, dt in (("cpu", torch.float32), ("cuda", torch.bfloat16)):
+        torch.manual_seed(8)
+        cfg = tiny_bert(hidden_size=256, num_attention_heads=heads, max_position_embeddings=512, residual_dropout=0.1)
+        model = BertForPreTraining(cfg).bfloat16().to(dev, dt).train()
+        torch.manual_seed(11)
+        loss = model(ids.to(dev), types.to(dev), labels=labels.to(dev), next_sentence_label=torch.tensor([1, 0, 1, 1], device=dev),
+                     cu_seqlens=torch.tensor(ends, device=dev))
+        loss.backward()
+        runs.append((loss.detach().double().cpu(), {n: g.double().cpu() for n, g in _grads(model).items()}))
+    # about 10 rounded tensors a layer each way, 40 roundings of half a step of bf16 between the ids and a gradient
+    bound = 40 * 2.0 ** -8
+    assert abs(runs[0][0] - runs[1][0]) <= bound * runs[0][0]
+    for n, want in runs[0][1].items():
+        # a bias behind which nothing changes with it (of keys: the softmax does not see it) has a gradient of roundings alone
+        if not n.endswith("query_key_value.bias"):
+            assert (runs[1][1][n] - want).norm() <= bound * want.norm(), (n, ((runs[1][1][n] - want).norm() / want.norm()).item())
 
 
 @pytest.mark.gpu
