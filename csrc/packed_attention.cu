@@ -19,8 +19,8 @@
 // each).  D = 64: P_s has columns of its own, and S_s of the next tile is computed as soon as the scores are in registers, by a
 // thread of each query tile, so the softmax warps, which bound this size (128 exponentials a row for half the products), never wait.
 //
-// Measured, 32 heads over 8: 7 prompts in 32768 tokens, heads of 128: bound by the tensor core at the power limit, 3.0 ms, 1190 TFLOP/s;
-// 4 documents in 16384 tokens: 0.50 ms, 1160; 24 samples in 8192 tokens, heads of 64: 67 us, 346, as tiles of 128 x 128 are a half full
+// Measured, 32 heads over 8: 7 prompts in 32768 tokens, heads of 128: bound by the tensor core at the power limit, 3.1 ms, 1140 TFLOP/s;
+// 4 documents in 16384 tokens: 0.50 ms, 1160 (tensor cores busy 66 % of the cycles, exponentials 65 %); 24 samples in 8192 tokens, heads of 64: 67 us, 346, as tiles of 128 x 128 are a half full
 // and an item is a few tiles.  120 sentences in 24576 tokens, 16 heads of 64, no mask: 102 us, 301 (by the length of an item too).
 #include "attn_tc_common.cuh"
 #include "gemm_tcgen05.cuh"

@@ -12,9 +12,9 @@
 // more than half of the time (120 sentences in 24576 tokens, 16 heads of 64, no mask: 410 us against 210).  Tiles that cross the end
 // are loaded whole and cleared behind it once they are there: 0 * NaN is NaN, and behind the end is the next sequence.
 //
-// Measured (the whole pass: Delta, this kernel, dQ): 4 documents in 16384 tokens, 32 heads of 128 over 8: 1.8 ms, 810 TFLOP/s, bound by
-// the products' dependences on P^T and dS^T of the same tile (tensor memory holds one of each) and by the power limit; 24 samples in 8192
-// tokens, heads of 64: 171 us, 338; the sentences above: 290 us, 265, where a block's end (dK, dV out of tensor memory, while
+// Measured (the whole pass: Delta, this kernel, dQ): 4 documents in 16384 tokens, 32 heads of 128 over 8: 1.8 ms, 810 TFLOP/s, shared memory
+// busy 82 % of the cycles, the tensor cores 60 %, under the power limit; one sequence of 16384 tokens, 16 heads of 128 over 4: 990 TFLOP/s,
+// the dense kernel in turn 1011; 24 samples in 8192 tokens, heads of 64: 171 us, 338; the sentences above: 290 us, 265, where a block's end (dK, dV out of tensor memory, while
 // nothing else may use it) and 69 us of passes over the fp32 accumulator weigh most.  Two pairs of accumulators for heads of 64, so that
 // the warps of dQ write the results under the next block: 309 us instead of 297, since those warps then hold up dQ.
 //   warp 0      claims items; TMA: K, V of an item, then Q_i, dO_i, L_i, Delta_i through a ring of three; zeros behind the end of a sequence
