@@ -677,6 +677,7 @@ NXD_API int nxd_packed_attn_fwd(const void* q, const void* k, const void* v, voi
         NXD_REQUIRE(strides[i] % 8 == 0, "packed_attn: stride %d (=%lld) must be a multiple of 8 elements", i, strides[i]);
     NXD_REQUIRE(q && k && v && o && tiles && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)tiles) & 15) == 0 && lse_row % 4 == 0 && rest_row % 4 == 0,
                 "packed_attn: tensors must be 16-byte aligned, rows of the scratch multiples of four");
+    NXD_REQUIRE(rest == nullptr || rest_row >= (which ? kBN : lse_row), "packed_attn: %lld rows of what the rounding took", rest_row);
     FwdParams p{};
     int rc;
     if ((rc = begin_call(&p.gave_up))) return rc;

@@ -767,6 +767,7 @@ NXD_API int nxd_packed_attn_bwd(const void* q, const void* k, const void* v, con
     const void* bases[] = {q, k, v, o, rest, dout, lse, delta, dq_accum, dkv_accum, dq, dk, dv, tiles};
     for (const void* x : bases)
         NXD_REQUIRE(((uintptr_t)x & 15) == 0 && (x != nullptr || x == dkv_accum), "packed_attn_bwd: tensors must be %s", "there and 16-byte aligned");
+    NXD_REQUIRE(rest_row >= (which ? kBN : lse_row), "packed_attn_bwd: %lld rows of what the rounding took", rest_row);
     cudaStream_t st = (cudaStream_t)stream;
     const PackedTile* pt = (const PackedTile*)tiles;
     BwdParams p{};

@@ -172,6 +172,7 @@ NXD_API int nxd_packed_plan(const void* cu, int wide, int N, long long T, int ca
     NXD_REQUIRE(rows == 128 || rows == 256, "packed_plan: tiles of %d rows", rows);
     const int entries = nxd_packed_plan_entries(T, N, rows);
     NXD_REQUIRE(N >= 0 && T > 0 && T < (1ll << 31) - 256 && entries > 0, "packed_plan: %d sequences in %lld rows", N, T);
+    NXD_REQUIRE(cu && tiles && which && (seqs || N == 0), "packed_plan: %s", "a list is missing");
     NXD_REQUIRE((((uintptr_t)tiles | (uintptr_t)seqs) & 15) == 0, "packed_plan: the lists must be %s", "16-byte aligned");
     cudaStream_t st = (cudaStream_t)stream;
     if (wide)

@@ -449,6 +449,28 @@ def test_saved_tensors_that_do_not_fit_are_refused():
                 torch.autograd.grad(o, leaves, do)
 
 
+def test_entry_points_refuse_what_is_missing():
+    import ctypes as c
+
+    from neuronx_distributed_llama3_2_b200.ops import _lib
+
+    x = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda" if torch.cuda.is_available() else "cpu")
+    lib, at = _lib.lib(), c.c_void_p(x.data_ptr() + (-x.data_ptr() & 15))
+    nothing, n = c.c_void_p(None), c.c_longlong
+    plan = [at, c.c_int(0), c.c_int(1), n(100), c.c_int(1), c.c_int(128), at, at, at, nothing]
+    for i in (0, 6, 7, 8):
+        assert lib.nxd_packed_plan(*[nothing if j == i else a for j, a in enumerate(plan)]) == -1 and b"missing" in lib.nxd_last_error()
+    strides = (n * 16)(*([64] * 16))
+    sizes = lambda rows, columns: (n(rows), c.c_int(2), n(columns), n(100))                 # noqa: E731
+    tail = (c.c_int(1), c.c_int(1), c.c_int(64), c.c_float(1.0), c.c_int(1), c.c_int(-1), nothing)
+    for which, rows in ((nothing, 128), (at, 64)):
+        assert lib.nxd_packed_attn_fwd(at, at, at, at, at, at, strides, at, which, *sizes(rows, 192), *tail) == -1
+        assert b"rows of what" in lib.nxd_last_error()
+        assert lib.nxd_packed_attn_bwd(at, at, at, at, at, at, at, at, at, nothing, at, at, at, strides, at, which, *sizes(rows, 192), c.c_int(1),
+                                       *tail) == -1
+        assert b"rows of what" in lib.nxd_last_error()
+
+
 def test_tables_shorter_than_the_row():
     """Rotation tables as long as the longest sequence are enough, and a sequence that is longer reads no further."""
     from neuronx_distributed_llama3_2_b200.ops import attention, rope
