@@ -188,6 +188,15 @@ def _books(case, rng, groups, W, step):
     return scores, lengths, slots, done
 
 
+def _laid_out(cache, states=()):
+    """A program's cache is laid out for the kernels once."""
+    if not own:
+        return None
+    from neuronx_distributed_llama3_2_b200.ops.kv_lines import CacheTensors
+
+    return CacheTensors(cache, states)
+
+
 def prepare(case, seed):
     dev = _device()
     g = torch.Generator(device=dev).manual_seed(seed)
@@ -231,11 +240,11 @@ def prepare(case, seed):
         cache = [normal(lines, case["heads"], case["rows"], case["dim"]) for _ in range(2 * case["layers"])]
         states = [normal(lines, case["state"], dtype=torch.float32) for _ in range(case["states"])]
         lo, hi = zip(*ranges_of(case))
-        return {"case": case, "cache": cache, "states": states, "lo": lo, "hi": hi,
+        return {"case": case, "cache": cache, "states": states, "laid_out": _laid_out(cache, states), "lo": lo, "hi": hi,
                 "parents": torch.tensor(parents_of(case), device=dev), "start": torch.tensor(lo, device=dev), "end": torch.tensor(hi, device=dev)}
     cache = [normal(case["pages"], case["heads"], case["page"], case["dim"]) for _ in range(2 * case["layers"])]
     src, dst, rows = (torch.tensor(a, device=dev) for a in moves_of(case))
-    return {"case": case, "cache": cache, "src": src, "dst": dst, "rows": rows if case["partial"] else None, "counts": moves_of(case)[2]}
+    return {"case": case, "cache": cache, "laid_out": _laid_out(cache), "src": src, "dst": dst, "rows": rows if case["partial"] else None, "counts": moves_of(case)[2]}
 
 
 # ---- the plain forms --------------------------------------------------------------------------------------------------
@@ -376,14 +385,14 @@ def _own_finish(s):
 def _own_reorder(s):
     from neuronx_distributed_llama3_2_b200.ops.kv_lines import reorder_lines_
 
-    reorder_lines_(s["cache"], s["parents"], s["start"], s["end"], states=s["states"])
+    reorder_lines_(s["laid_out"] or _laid_out(s["cache"], s["states"]), s["parents"], s["start"], s["end"])
     return {"cache": s["cache"], "states": s["states"]}
 
 
 def _own_pages(s):
     from neuronx_distributed_llama3_2_b200.ops.kv_lines import copy_pages_
 
-    copy_pages_(s["cache"], s["src"], s["dst"], rows=s["rows"])
+    copy_pages_(s["laid_out"] or _laid_out(s["cache"]), s["src"], s["dst"], rows=s["rows"])
     return {"cache": s["cache"]}
 
 
