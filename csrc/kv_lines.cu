@@ -1,0 +1,233 @@
+// Whole lines and pages of a key/value cache, in every layer at once: lines that continue other lines (beam search), and pages that are copied
+// (a line forks, a shared page is about to be written, a pool is compacted).
+//
+// Both only move bytes, so HBM bounds them: 699 MB (16 layers, 32 lines of up to 900 rows, recurrent states) are 107 us at 6555 GB/s.  All
+// tensors of one shape share a launch; their addresses travel as kernel parameters.
+#include "common.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTensors = 256;          // of a launch: 2 KB of parameters
+constexpr int kMaxBeams = 32;
+
+struct Tensors {
+    char* base[kMaxTensors];
+    int n;
+};
+
+// What all tensors of a launch have in common, in units of U bytes (per_row) and in bytes (strides).
+struct Shape {
+    int heads, rows, per_row;
+    long long line_stride, head_stride;
+};
+
+// The order in which a group's lines can be written in place: no line is written before those that continue it have read it.  Where
+// lines continue each other in a circle, one of them is set aside first.  Entries (to, from); from = kAside: what was set aside, to = kAside: it.
+constexpr int kAside = -1, kMaxMoves = kMaxBeams + kMaxBeams / 2;
+struct Moves {
+    signed char to[kMaxMoves], from[kMaxMoves];
+    int n;
+};
+
+// By one warp, lane w for line w; from[w] = w: it stays.
+__device__ __forceinline__ void order_moves(int from, int lane, Moves& m) {
+    unsigned left = __ballot_sync(0xffffffffu, from != lane);          // lines to be written
+    int n = 0;
+    while (left != 0) {
+        // lines that a line still to be written reads
+        const unsigned read = __reduce_or_sync(0xffffffffu, left >> lane & 1 ? 1u << from : 0u);
+        const unsigned ready = left & ~read;
+        if (ready != 0) {
+            if (ready >> lane & 1) {
+                const int at = n + __popc(ready & ((1u << lane) - 1u));
+                m.to[at] = (signed char)lane;
+                m.from[at] = (signed char)from;
+            }
+            n += __popc(ready);
+            left &= ~ready;
+        } else {          // circles only: the first one, around
+            const int first = __ffs(left) - 1;
+            if (lane == 0) m.to[n] = kAside, m.from[n] = (signed char)first;
+            ++n;
+            int at = first;
+            do {
+                const int next = __shfl_sync(0xffffffffu, from, at);
+                if (lane == 0) m.to[n] = (signed char)at, m.from[n] = next == first ? (signed char)kAside : (signed char)next;
+                ++n;
+                left &= ~(1u << at);
+                at = next;
+            } while (at != first);
+        }
+    }
+    if (lane == 0) m.n = n;
+}
+
+// Lines g * W + w of a group continue its lines g * W + parent[w], rows [start, end) of every head.  A thread takes one unit of all the
+// group's lines in an order that works in place, so there is no scratch and each line that is wanted is read once from memory however
+// many continue it.  Four reads are under way before the first of them is written.
+template <typename U>
+__global__ void __launch_bounds__(kThreads) reorder_lines_kernel(const __grid_constant__ Tensors t, Shape s, int W, const long long* __restrict__ parents,
+                                                                 const long long* __restrict__ start, const long long* __restrict__ end,
+                                                                 const int* __restrict__ table, int page_size, int max_pages, int num_pages) {
+    __shared__ Moves moves;
+    const int g = blockIdx.y;
+    const long long line0 = (long long)g * W;
+    if (threadIdx.x < 32) {
+        const int w = threadIdx.x;
+        long long p = w < W ? parents[line0 + w] : w;
+        if (p < 0 || p >= W) p = w;          // a line whose parent is none of the group's stays as it is
+        order_moves((int)p, w, moves);
+    }
+    __syncthreads();
+    const int n = moves.n;
+    const long long lo = start != nullptr ? max(start[g], 0LL) : 0, hi = end != nullptr ? min(end[g], (long long)s.rows) : s.rows;
+    if (n == 0 || hi <= lo) return;
+    const unsigned per_head = (unsigned)(hi - lo) * (unsigned)s.per_row, per_tensor = per_head * (unsigned)s.heads;
+    const unsigned total = per_tensor * (unsigned)t.n;          // the host keeps it below 2^31
+    for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
+        const unsigned tensor = i / per_tensor, in_tensor = i - tensor * per_tensor;
+        const unsigned head = in_tensor / per_head, unit = in_tensor - head * per_head;
+        char* base = t.base[tensor] + (long long)head * s.head_stride;
+        int page = 0;
+        if (table == nullptr) {
+            base += line0 * s.line_stride + (lo * s.per_row + unit) * (long long)sizeof(U);
+        } else {
+            const unsigned r = unit / (unsigned)s.per_row, row = (unsigned)lo + r;
+            page = (int)(row / (unsigned)page_size);
+            base += ((long long)(row - (unsigned)page * (unsigned)page_size) * s.per_row + (unit - r * (unsigned)s.per_row)) * (long long)sizeof(U);
+        }
+        auto place = [&](int w) -> U* {
+            if (table == nullptr) return reinterpret_cast<U*>(base + w * s.line_stride);
+            const int p = table[(line0 + w) * max_pages + page];
+            return p < 0 || p >= num_pages ? nullptr : reinterpret_cast<U*>(base + p * s.line_stride);
+        };
+        U aside{};
+        bool has_aside = false;
+        for (int k0 = 0; k0 < n; k0 += 4) {
+            U v[4];
+            U* to[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                to[k] = nullptr;
+                if (k0 + k >= n) continue;
+                const int d = moves.to[k0 + k], f = moves.from[k0 + k];
+                const U* src = f == kAside ? nullptr : place(f);
+                if (d == kAside) {
+                    has_aside = src != nullptr;
+                    if (has_aside) aside = *src;
+                } else {
+                    if (src != nullptr) v[k] = *src;
+                    else if (f == kAside) v[k] = aside;
+                    if (f == kAside ? has_aside : src != nullptr) to[k] = place(d);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (to[k] != nullptr) *to[k] = v[k];
+        }
+    }
+}
+
+// Page dst[i] becomes page src[i], its first rows[i] rows of every head.  No page that is read is written by the same call.
+template <typename U>
+__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ Tensors t, Shape s, int pages, int pairs, const long long* __restrict__ src,
+                                                              const long long* __restrict__ dst, const long long* __restrict__ rows) {
+    for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
+        const long long from = src[pair], to = dst[pair];
+        if (from < 0 || to < 0 || from >= pages || to >= pages || from == to) continue;
+        const int n = rows != nullptr ? (int)min(max(rows[pair], 0LL), (long long)s.rows) : s.rows;
+        const unsigned per_head = (unsigned)n * (unsigned)s.per_row, per_tensor = per_head * (unsigned)s.heads;
+        const unsigned total = per_tensor * (unsigned)t.n;
+        constexpr int kDeep = 4;
+        for (unsigned i0 = blockIdx.x * (kThreads * kDeep) + threadIdx.x; i0 < total; i0 += gridDim.x * (kThreads * kDeep)) {
+            U v[kDeep];
+            U* at[kDeep];
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const unsigned i = i0 + k * kThreads;
+                at[k] = nullptr;
+                if (i < total) {
+                    const unsigned tensor = i / per_tensor, in_tensor = i - tensor * per_tensor;
+                    const unsigned head = in_tensor / per_head, unit = in_tensor - head * per_head;
+                    char* base = t.base[tensor] + head * s.head_stride + (long long)unit * (long long)sizeof(U);
+                    v[k] = *reinterpret_cast<const U*>(base + from * s.line_stride);
+                    at[k] = reinterpret_cast<U*>(base + to * s.line_stride);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k)
+                if (at[k] != nullptr) *at[k] = v[k];
+        }
+    }
+}
+
+// The widest unit that rows, strides and addresses allow.
+int unit_of(void* const* base, int n, long long row_bytes, long long line_stride, long long head_stride) {
+    unsigned long long all = (unsigned long long)row_bytes | (unsigned long long)line_stride | (unsigned long long)head_stride;
+    for (int i = 0; i < n; ++i) all |= (unsigned long long)(uintptr_t)base[i];
+    return (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : (all & 1) == 0 ? 2 : 1;
+}
+
+// Blocks beside each other for one group or pair: what its units can use, and no more than fill the GPU.
+unsigned blocks_for(long long units, long long per_block, long long beside) {
+    const long long want = (units + per_block - 1) / per_block, room = (8LL * nxd_num_sms() + beside - 1) / beside;
+    const long long least = nxd_num_sms();
+    return (unsigned)(want < room ? want : room < least ? (want < least ? want : least) : room);
+}
+
+constexpr long long kMaxUnits = (1LL << 31) - (1LL << 22);          // of a group or pair in a launch: the strides of the loops stay below 2^32
+
+}  // namespace
+
+// n tensors of one shape at `base` (host array of device addresses): [lines, heads, rows, row_bytes] or, with a block table
+// [lines, max_pages], pages [num_pages, heads, page_size, row_bytes]; strides in bytes, rows side by side.
+NXD_API int nxd_reorder_lines(void* const* base, int n, int heads, long long rows, long long row_bytes, long long line_stride, long long head_stride,
+                              int groups, int W, const long long* parents, const long long* start, const long long* end, const int* table,
+                              int page_size, int max_pages, int num_pages, void* stream) {
+    NXD_REQUIRE(W >= 1 && W <= kMaxBeams, "reorder_lines: %d lines of a group are not between 1 and %d", W, kMaxBeams);
+    NXD_REQUIRE(groups >= 0 && groups <= 65535, "reorder_lines: %d groups are more than 65535", groups);
+    if (n == 0 || groups == 0 || rows == 0 || row_bytes == 0 || heads == 0) return 0;
+    const int unit = unit_of(base, n, row_bytes, line_stride, head_stride);
+    const long long per_row = row_bytes / unit, per_tensor = rows * per_row * heads;
+    NXD_REQUIRE(per_tensor <= kMaxUnits, "reorder_lines: a line of %lld rows of %lld bytes in %d heads is too long", rows, row_bytes, heads);
+    const int most = (int)(kMaxUnits / per_tensor < kMaxTensors ? kMaxUnits / per_tensor : kMaxTensors);
+    for (int at = 0; at < n; at += most) {
+        Tensors t;
+        t.n = n - at < most ? n - at : most;
+        for (int i = 0; i < kMaxTensors; ++i) t.base[i] = i < t.n ? (char*)base[at + i] : nullptr;
+        const Shape s = {heads, (int)rows, (int)per_row, line_stride, head_stride};
+        const dim3 grid(blocks_for(per_tensor * t.n, kThreads, groups), groups);
+        cudaStream_t st = (cudaStream_t)stream;
+        if (unit == 16) reorder_lines_kernel<uint4><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        else if (unit == 4) reorder_lines_kernel<uint32_t><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        else if (unit == 2) reorder_lines_kernel<uint16_t><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        else reorder_lines_kernel<uint8_t><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        NXD_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+// n tensors of one shape [pages, heads, rows, row_bytes] at `base` (host array of device addresses).
+NXD_API int nxd_copy_pages(void* const* base, int n, int pages, int heads, long long rows, long long row_bytes, long long page_stride,
+                           long long head_stride, int pairs, const long long* src, const long long* dst, const long long* used, void* stream) {
+    if (n == 0 || pairs == 0 || rows == 0 || row_bytes == 0 || heads == 0) return 0;
+    const int unit = unit_of(base, n, row_bytes, page_stride, head_stride);
+    const long long per_row = row_bytes / unit, per_tensor = rows * per_row * heads;
+    NXD_REQUIRE(per_tensor <= kMaxUnits, "copy_pages: a page of %lld rows of %lld bytes in %d heads is too large", rows, row_bytes, heads);
+    const int most = (int)(kMaxUnits / per_tensor < kMaxTensors ? kMaxUnits / per_tensor : kMaxTensors);
+    for (int at = 0; at < n; at += most) {
+        Tensors t;
+        t.n = n - at < most ? n - at : most;
+        for (int i = 0; i < kMaxTensors; ++i) t.base[i] = i < t.n ? (char*)base[at + i] : nullptr;
+        const Shape s = {heads, (int)rows, (int)per_row, page_stride, head_stride};
+        const dim3 grid(blocks_for(per_tensor * t.n, kThreads * 4, pairs), pairs < 65535 ? pairs : 65535);
+        cudaStream_t st = (cudaStream_t)stream;
+        if (unit == 16) copy_pages_kernel<uint4><<<grid, kThreads, 0, st>>>(t, s, pages, pairs, src, dst, used);
+        else if (unit == 4) copy_pages_kernel<uint32_t><<<grid, kThreads, 0, st>>>(t, s, pages, pairs, src, dst, used);
+        else if (unit == 2) copy_pages_kernel<uint16_t><<<grid, kThreads, 0, st>>>(t, s, pages, pairs, src, dst, used);
+        else copy_pages_kernel<uint8_t><<<grid, kThreads, 0, st>>>(t, s, pages, pairs, src, dst, used);
+        NXD_LAUNCH_CHECK();
+    }
+    return 0;
+}

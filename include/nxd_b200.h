@@ -111,6 +111,35 @@ int nxd_kv_cache_update(const void* new_k, const void* new_v, void* cache_k, voi
                         const int* seq_ids, const int* block_table, long long stride_b, long long stride_h,
                         int page_size, int max_pages, int B, int n_kv, int T_new, int D, void* stream);
 
+/* ---- beam search (csrc/beam_search.cu) -----------------------------------------------------------
+ * select: logits [B * W, V] (dtype 0 fp32, 1 bf16, 2 fp16; rows `stride` elements apart), scores [B, W] -> the n best of
+ * scores[w] + log_softmax(logits[w])[v] of every group, best first, ties to the lowest w * V + v.  Scratch in floats, 0: outside what is
+ * compiled (W <= 32, n <= 64). */
+long long nxd_beam_select_scratch(int dtype, int B, int W, int V, int n);
+int nxd_beam_select(int dtype, const void* logits, long long stride, const float* scores, int B, int W, int V, int n, float* scratch,
+                    float* out_scores, long long* out_beams, long long* out_tokens, void* stream);
+/* one step of the books: candidates [B, N], running scores and the pool [B, W] -> the same behind the step, tokens and parents [B, W] by line, a row
+ * of the history [B, W].  norm = length ** penalty, length = tokens with this step's; eos -1: none. */
+int nxd_beam_advance(const float* cand_scores, const long long* cand_beams, const long long* cand_tokens, int B, int W, int N,
+                     const float* running, const float* pool_scores, const int* pool_lengths, const int* pool_slots,
+                     const unsigned char* done, float norm, long long eos, long long pad, int early_stopping, int length,
+                     float* out_running, long long* out_tokens, long long* out_parents, float* out_pool_scores, int* out_pool_lengths,
+                     int* out_pool_slots, unsigned char* out_done, int* hist_tokens, int* hist_parents, void* stream);
+/* the best W hypotheses of every group: tokens [B, W, step], lengths and scores [B, W]; history [>= step, B, W] */
+int nxd_beam_finish(const float* running, const float* pool_scores, const int* pool_lengths, const int* pool_slots, const unsigned char* done,
+                    int B, int W, int step, float norm, long long eos, long long pad, const int* hist_tokens, const int* hist_parents,
+                    long long* tokens, long long* lengths, float* scores, void* stream);
+
+/* ---- cache lines and pages (csrc/kv_lines.cu) -------------------------------------------------------
+ * n tensors of one shape at `base` (a HOST array of device addresses), strides and rows in bytes.  reorder: line g * W + w becomes what line
+ * g * W + parents[g, w] was, rows [start[g], end[g]) (NULL: all), in place; with a block table [lines, max_pages] the tensors are pages.
+ * copy: page dst[i] becomes page src[i], its first used[i] rows of every head (NULL: all). */
+int nxd_reorder_lines(void* const* base, int n, int heads, long long rows, long long row_bytes, long long line_stride, long long head_stride,
+                      int groups, int W, const long long* parents, const long long* start, const long long* end, const int* table,
+                      int page_size, int max_pages, int num_pages, void* stream);
+int nxd_copy_pages(void* const* base, int n, int pages, int heads, long long rows, long long row_bytes, long long page_stride,
+                   long long head_stride, int pairs, const long long* src, const long long* dst, const long long* used, void* stream);
+
 /* all decoder layers of a token step of one sequence in one launch (csrc/token_stack.cu); bytes of scratch, 0: does not apply */
 int nxd_token_stack_runs_on(void* stream);        /* 0: the stream has not all SMs of the device, as the launch needs */
 long long nxd_token_stack_scratch(int layers, int B, int H, int I, int n_q, int n_kv, int D);

@@ -87,7 +87,7 @@ GROUPS["state_space_serving"] = ["window_attention.cu", "state_space.cu", "strea
 # sources whose fp32 state is carried over thousands of steps, or whose fp32 results are exact to a few roundings: compiled without
 # approximate exp / tanh / division and without flushed subnormals
 PRECISE_SOURCES = {"mlstm.cu", "delta_rule.cu", "delta_chunks.cu", "retention.cu", "retention_tc.cu", "hyper_connection.cu", "stream_norm.cu",
-                   "state_space.cu", "balance_loss.cu", "dropout.cu"}
+                   "state_space.cu", "balance_loss.cu", "dropout.cu", "beam_search.cu"}
 
 _lib: Optional[ctypes.CDLL] = None
 _group_libs = {}
