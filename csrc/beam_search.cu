@@ -10,15 +10,17 @@
 // Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace {
 
-constexpr int kRowThreads = 256;
 constexpr int kMaxN = 64;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 4096;          // chunks of a group
-constexpr int kCollect = kRowThreads;    // values that a chunk's short way ranks
+constexpr int kStages = 3;               // rounds under way
+constexpr int kCollect = 512;            // candidates that a CTA holds
 constexpr unsigned kFull = 0xffffffffu;
 
 // order-preserving keys; -0 and +0 are one value (the caller adds 0)
@@ -28,12 +30,17 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 constexpr uint32_t kLowestKey = 0x00800000u;          // of the lowest finite number
-// the upper half of the same for 64 bits: sign, exponent and 20 bits of the fraction
-__device__ __forceinline__ uint32_t order_key_hi(double d) {
-    const uint32_t u = (uint32_t)((unsigned long long)__double_as_longlong(d + 0.0) >> 32);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// a value with its index, greater for greater values and of equal ones for lower indices
+__device__ __forceinline__ unsigned long long entry_key(float f, int index) {
+    return (unsigned long long)order_key(f + 0.f) << 32 | (uint32_t)~index;
 }
-constexpr uint32_t kLowestKeyHi = 0x00100000u;
+// the same for 64 bits
+__device__ __forceinline__ unsigned long long order_key(double d) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(d + 0.0);
+    return (u >> 63) ? ~u : (u | 1ull << 63);
+}
+__device__ __forceinline__ double key_value(unsigned long long k) { return __longlong_as_double((long long)((k >> 63) ? (k & ~(1ull << 63)) : ~k)); }
+constexpr uint32_t kLowestKeyHi = 0x00100000u;          // the upper half of the lowest finite number's
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -58,28 +65,204 @@ __device__ __forceinline__ int block_count(int v, int* red) {
     return t;
 }
 
-// What a call leaves for the second kernel: per chunk its maximum, the sum of exponentials behind it, and n (value, index) in order.
+// What a call leaves for the second kernel: per chunk its maximum, the sum of exponentials behind it, and n entries in order, 0 behind the last.
 struct Lists {
-    float* top;       // [rows, splits]
-    float* sum;       // [rows, splits]
-    float* value;     // [rows, splits, n], -inf behind the last
-    int* index;       // [rows, splits, n]
+    unsigned long long* entry;       // [rows, splits, n]
+    float2* sum;                     // [rows, splits]: maximum, sum
 };
 
-__host__ __device__ inline Lists lists_of(float* scratch, long long lists, int n) {
-    return {scratch, scratch + lists, scratch + 2 * lists, reinterpret_cast<int*>(scratch + 2 * lists + lists * n)};
+__host__ __device__ inline Lists lists_of(void* scratch, long long lists, int n) {
+    unsigned long long* entry = reinterpret_cast<unsigned long long*>(scratch);
+    return {entry, reinterpret_cast<float2*>(entry + lists * n)};
 }
 
-template <typename T, int E>
-__global__ void __launch_bounds__(kRowThreads) beam_rows_kernel(const T* __restrict__ logits, int V, long long stride, int splits, int n, Lists out) {
-    constexpr int VE = 16 / sizeof(T), NV = E / VE;
-    __shared__ uint32_t keys[kRowThreads];
-    __shared__ float cand_v[kCollect];
-    __shared__ int cand_i[kCollect];
-    __shared__ uint32_t warp_key[kRowThreads / 32];
-    __shared__ float warp_part[kRowThreads / 32];
+// 16 bytes of logits
+template <typename T> struct Vec { static constexpr int n = 16 / sizeof(T); };
+
+template <typename T> __device__ __forceinline__ uint32_t bits_of(T x);
+template <> __device__ __forceinline__ uint32_t bits_of<float>(float x) { return __float_as_uint(x); }
+template <> __device__ __forceinline__ uint32_t bits_of<bf16>(bf16 x) { return __bfloat16_as_ushort(x); }
+template <> __device__ __forceinline__ uint32_t bits_of<__half>(__half x) { return __half_as_ushort(x); }
+
+template <typename T>
+__device__ __forceinline__ uint4 load_vec(const T* row, int at, int V) {
+    if (at >= 0 && at + Vec<T>::n <= V) return __ldg(reinterpret_cast<const uint4*>(row + at));
+    // over an end of the row: its elements one by one, -inf outside
+    constexpr uint32_t kOut = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, bf16> ? 0xff80u : 0xfc00u;
+    constexpr int kBits = 8 * sizeof(T);
+    unsigned long long lo = 0, hi = 0;
+#pragma unroll 1
+    for (int j = Vec<T>::n - 1; j >= 0; --j) {
+        const int k = at + j;
+        hi = hi << kBits | lo >> (64 - kBits);
+        lo = lo << kBits | (k >= 0 && k < V ? bits_of<T>(row[k]) : kOut);
+    }
+    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+
+__device__ __forceinline__ void fetch_vec(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
+// A thread's vectors of a round on their way into shared memory (one group of copies; the ends of a row are stored at once).  Whether a round
+// lies inside the row the block decides at once.
+template <typename T, int NT, int NV>
+__device__ __forceinline__ void fetch_round(uint4* stage, const T* row, int first, int V) {
+    constexpr int VE = Vec<T>::n;
+    const int begin = first - (int)threadIdx.x * VE;
+    if (begin >= 0 && begin + NT * NV * VE <= V) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) fetch_vec(stage + i * NT + threadIdx.x, row + first + i * NT * VE);
+        return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < NV; ++i) {
+        const int at = first + i * NT * VE;
+        if (at >= 0 && at + VE <= V) fetch_vec(stage + i * NT + threadIdx.x, row + at);
+        else stage[i * NT + threadIdx.x] = load_vec<T>(row, at, V);
+    }
+}
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A 32-bit word's one or two values.
+template <typename T>
+__device__ __forceinline__ void unpack_word(uint32_t w, float* f) {
+    if constexpr (sizeof(T) == 4) {
+        f[0] = __uint_as_float(w);
+    } else if constexpr (std::is_same_v<T, bf16>) {
+        f[0] = __uint_as_float(w << 16);
+        f[1] = __uint_as_float(w & 0xffff0000u);
+    } else {
+        f[0] = __half2float(__ushort_as_half((unsigned short)(w & 0xffffu)));
+        f[1] = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_vec(const uint4& raw, float* f) {
+    constexpr int per = Vec<T>::n / 4;
+    unpack_word<T>(raw.x, f);
+    unpack_word<T>(raw.y, f + per);
+    unpack_word<T>(raw.z, f + 2 * per);
+    unpack_word<T>(raw.w, f + 3 * per);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (sizeof(T) == 4) r = __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    else if constexpr (std::is_same_v<T, bf16>) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// The largest of a thread's values, of NaN and a number the number.
+template <typename T, int NV>
+__device__ __forceinline__ float max_of(const uint4 (&raw)[NV]) {
+    uint32_t m = max_word<T>(max_word<T>(raw[0].x, raw[0].y), max_word<T>(raw[0].z, raw[0].w));
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = max_word<T>(m, max_word<T>(max_word<T>(raw[i].x, raw[i].y), max_word<T>(raw[i].z, raw[i].w)));
+    float f[2] = {-INFINITY, -INFINITY};
+    unpack_word<T>(m, f);
+    return fmaxf(fmaxf(f[0], f[1]), -INFINITY);
+}
+
+// The k-th largest key of a warp (0 where fewer threads have one).
+__device__ __forceinline__ uint32_t kth_of_warp(uint32_t key, int k, int lane) {
+    uint32_t v = 0;
+    for (int i = 0; i < k; ++i) {
+        v = __reduce_max_sync(kFull, key);
+        if (lane == __ffs(__ballot_sync(kFull, key == v)) - 1) key = 0;
+    }
+    return v;
+}
+
+// Many values, equal ones as a rule: the n-th key of a round bit by bit, then what is above it, then its ties in the order of their indices, behind
+// the `have` candidates that there are.  Reads the round's values once more, so that they hold no registers meanwhile.
+template <typename T, int NT, int NV>
+__device__ __noinline__ int collect_exactly(const T* row, int first, int V, int n, int have, unsigned long long* cand, int* s_count, int* red) {
+    constexpr int VE = Vec<T>::n, kWarps = NT / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint4 raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = load_vec<T>(row, first + i * NT * VE, V);
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | (1u << bit);
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float f[VE];
+            unpack_vec<T>(raw[i], f);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) mine += f[j] == f[j] && order_key(f[j] + 0.f) >= c;
+        }
+        if (block_count(mine, red) >= n) t = c;
+    }
+    const float tie = key_value(max(t, kLowestKey));          // fewer than n finite ones: all of them
+    if (tid == 0) *s_count = have;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[VE];
+        unpack_vec<T>(raw[i], f);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if (f[j] > tie) {                // fewer than n
+                cand[atomicAdd(s_count, 1)] = entry_key(f[j], first + i * NT * VE + j);
+            }
+        }
+    }
+    __syncthreads();
+    int filled = *s_count;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[VE];
+        unpack_vec<T>(raw[i], f);
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) mine += f[j] == tie;
+        int before = mine;               // of this thread and the ones before it
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(kFull, before, o);
+            if (lane >= o) before += x;
+        }
+        __syncthreads();
+        if (lane == 31) red[warp] = before;
+        __syncthreads();
+        int at = filled + before - mine;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) at += red[w];
+            filled += red[w];
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if (f[j] == tie) {
+                if (at < have + n) cand[at] = entry_key(tie, first + i * NT * VE + j);
+                ++at;
+            }
+        }
+    }
+    __syncthreads();
+    return min(filled, have + n);
+}
+
+// A CTA takes `rounds` rounds of 256 threads x NV vectors of one row.  Between rounds it keeps candidates, at least the n best so far; only values above
+// the n-th of those are looked at further.
+template <typename T, int NT, int NV>
+__global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __restrict__ logits, int V, long long stride, int splits, int rounds, int n,
+                                                                   Lists out) {
+    constexpr int VE = Vec<T>::n, E = NV * VE, kWarps = NT / 32;
+    __shared__ unsigned long long cand[kCollect];
+    extern __shared__ uint4 ring[];            // [kStages][NV][NT]
+    __shared__ unsigned char looker[kWarps][32];
+    __shared__ uint32_t warp_top[kWarps], warp_kth[kWarps];
+    __shared__ float warp_sum_of[kWarps];
     __shared__ int red[32];
-    __shared__ uint32_t s_floor;
+    __shared__ unsigned long long best[kMaxN];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long list = blockIdx.x;
@@ -87,282 +270,269 @@ __global__ void __launch_bounds__(kRowThreads) beam_rows_kernel(const T* __restr
     const T* row = logits + (list / splits) * stride;
     // vectors start on 16 bytes: the row's first element is element `mis` of the first one
     const int mis = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % VE);
-    const int first = split * (kRowThreads * E) + tid * VE - mis;          // index of this thread's first element
+    int first = split * rounds * (NT * E) + tid * VE - mis;          // index of this thread's first element of the round
 
-    float f[E];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = first + i * kRowThreads * VE;
-        if (at >= 0 && at + VE <= V) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + at));
-            const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) f[i * VE + j] = to_float<T>(e[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VE; ++j) f[i * VE + j] = (at + j >= 0 && at + j < V) ? to_float<T>(row[at + j]) : -INFINITY;
-        }
-    }
-    float m = f[0];
-#pragma unroll
-    for (int j = 1; j < E; ++j) m = fmaxf(m, f[j]);          // passes NaN by
-    m = m == m ? m + 0.f : -INFINITY;
-    // the differences first: a product of the maximum would lose their last bits.  A NaN, or an infinity, makes the sum NaN and takes the row out
-    const float base = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < E; ++j) sum += exp2_approx((f[j] - base) * kLog2e);
-    const uint32_t key = order_key(m);
-    keys[tid] = key;
-    const uint32_t wk = __reduce_max_sync(kFull, key);
-    if (lane == 0) warp_key[warp] = wk;
     if (tid == 0) s_count = 0;
-    __syncthreads();
-    uint32_t block_key = 0;
 #pragma unroll
-    for (int i = 0; i < kRowThreads / 32; ++i) block_key = max(block_key, warp_key[i]);
-    const float top = key_value(block_key);
-    sum *= m == -INFINITY ? (sum == sum ? 0.f : 1.f) : exp2_approx((m - top) * kLog2e);
-    sum = warp_sum(sum);
-    if (lane == 0) warp_part[warp] = sum;
-    if (warp == 0) {
-        // the n-th largest of the threads' maxima, its upper 16 bits (all that bf16 has): 8 keys a lane
-        uint32_t k[kRowThreads / 32];
-#pragma unroll
-        for (int i = 0; i < kRowThreads / 32; ++i) k[i] = keys[i * 32 + lane];
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t c = t | (1u << bit);
-            int mine = 0;
-#pragma unroll
-            for (int i = 0; i < kRowThreads / 32; ++i) mine += k[i] >= c;
-            if (__reduce_add_sync(kFull, mine) >= n) t = c;
-        }
-        if (lane == 0) s_floor = max(t, kLowestKey);
+    for (int q = 0; q < kStages; ++q) {
+        if (q < rounds) fetch_round<T, NT, NV>(ring + q * (NV * NT), row, first + q * (NT * E), V);
+        fetch_commit();
     }
+    float top = -INFINITY, sum = 0.f;          // this thread's
+    float floor = -INFINITY;                   // only what is above it counts
+    int until = 1;                             // the next round that puts the candidates in order
+    bool crowded = false;
+    // the n best candidates in order; eight lanes compare one with all
+    auto keep_best = [&](int count) {
+        for (int i0 = 0; i0 < count; i0 += NT / 8) {
+            const int i = i0 + tid / 8;
+            const unsigned long long own = i < count ? cand[i] : ~0ull;
+            int before = 0;
+#pragma unroll 4
+            for (int j = tid % 8; j < count; j += 8) before += cand[j] > own;
+            before += __shfl_xor_sync(kFull, before, 1);
+            before += __shfl_xor_sync(kFull, before, 2);
+            before += __shfl_xor_sync(kFull, before, 4);
+            if (i < count && before < n && tid % 8 == 0) best[before] = own;
+        }
+        count = min(count, n);
+        __syncthreads();
+        if (tid < count) cand[tid] = best[tid];
+        if (tid == 0) s_count = count;
+        __syncthreads();
+        floor = count == n ? key_value((uint32_t)(best[n - 1] >> 32)) : -INFINITY;
+    };
+    for (int r = 0; r < rounds; ++r) {
+        uint4* stage = ring + r % kStages * (NV * NT);
+        fetch_wait<kStages - 1>();
+        uint4 raw[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = stage[i * NT + tid];
+        float m = max_of<T, NV>(raw) + 0.f;          // no -0; passes NaN by
+        {
+            // the differences first: a product of the maximum would lose their last bits.  A NaN, or an infinity, makes the sum NaN
+            const float big = fmaxf(top, m), base = big == -INFINITY ? 0.f : big;
+            if (top != -INFINITY) sum *= exp2_approx((top - base) * kLog2e);
+            top = big;
+            const uint64_t away = f2_pack(-base, -base), one = f2_pack(1.f, 1.f), log2e = f2_pack(kLog2e, kLog2e);
+            uint64_t part[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float f[VE];
+                unpack_vec<T>(raw[i], f);
+#pragma unroll
+                for (int j = 0; j < VE; j += 2) {
+                    const uint64_t d = f2_mul(f2_fma(f2_pack(f[j], f[j + 1]), one, away), log2e);
+                    part[j / 2 % 2] = f2_fma(f2_pack(exp2_approx(f2_lo(d)), exp2_approx(f2_hi(d))), one, part[j / 2 % 2]);
+                }
+            }
+            sum += (f2_lo(part[0]) + f2_hi(part[0])) + (f2_lo(part[1]) + f2_hi(part[1]));
+        }
+        if (r == 0) {
+            // a k-th largest maximum of each warp that has values, warps * k >= n: the least of them has n values that are not below it
+            const int vecs = (V + mis - split * rounds * (NT * E) + VE - 1) / VE, filled = min(max((vecs + 31) / 32, 1), kWarps);
+            const uint32_t key = order_key(m), kth = kth_of_warp(key, (n + filled - 1) / filled, lane);
+            if (lane == 0) warp_kth[warp] = kth;
+            __syncthreads();
+            uint32_t least = warp_kth[0];
+#pragma unroll
+            for (int i = 1; i < kWarps; ++i) least = i < filled ? min(least, warp_kth[i]) : least;
+            // the number below that bound (below zero one that is not equal to it), so that what is above it is looked at in every round
+            least = max(least, kLowestKey) - 1;
+            floor = key_value(least == 0x7fffffffu ? least - 1 : least);
+        }
+        // the values of the threads that have some are looked at by their warp
+        const bool look = m > floor;
+        const unsigned lookers = __ballot_sync(kFull, look);
+        if (lookers != 0) {
+            if (look) looker[warp][__popc(lookers & ((1u << lane) - 1u))] = (unsigned char)lane;
+            __syncwarp();
+            for (int e = lane; e < __popc(lookers) * E; e += 32) {
+                const int who = looker[warp][e / E], i = e % E / VE, j = e % VE;
+                const float f = to_float<T>(reinterpret_cast<const T*>(stage + i * NT + warp * 32 + who)[j]);
+                if (f > floor) {
+                    const int to = atomicAdd(&s_count, 1);
+                    if (to < kCollect) cand[to] = entry_key(f, first + (who - lane) * VE + i * NT * VE + j);
+                }
+            }
+            __syncwarp();
+        }
+        if (r + kStages < rounds) fetch_round<T, NT, NV>(stage, row, first + kStages * (NT * E), V);          // the warp is done with its part
+        fetch_commit();
+        if (r == until || r + 1 == rounds) {
+            __syncthreads();
+            const int count = s_count;
+            if (count > kCollect) {
+                crowded = true;                  // more than there is room for: the rest only adds up
+                floor = INFINITY;
+                until = rounds;
+            } else if (!crowded) {
+                keep_best(count);
+                until = 4 * r + 2;          // 1, 6, 26: few pass the bound between these
+            }
+        }
+        first += NT * E;
+    }
+    pdl_trigger();
+    if (crowded) {
+        int count = 0;
+        for (int q = 0; q < rounds; ++q) {
+            __syncthreads();
+            count = collect_exactly<T, NT, NV>(row, split * rounds * (NT * E) + q * (NT * E) + tid * VE - mis, V, n, count, cand, &s_count, red);
+            keep_best(count);
+            count = min(count, n);
+        }
+    }
+    const uint32_t block_key = __reduce_max_sync(kFull, order_key(top));
+    if (lane == 0) warp_top[warp] = block_key;
+    __syncthreads();
+    uint32_t most = warp_top[0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) most = max(most, warp_top[i]);
+    const float all = key_value(most);
+    if (top != -INFINITY) sum *= exp2_approx((top - all) * kLog2e);
+    sum = warp_sum(sum);
+    if (lane == 0) warp_sum_of[warp] = sum;
     __syncthreads();
     if (tid == 0) {
         float total = 0.f;
 #pragma unroll
-        for (int i = 0; i < kRowThreads / 32; ++i) total += warp_part[i];
-        out.top[list] = top;
-        out.sum[list] = total;
+        for (int i = 0; i < kWarps; ++i) total += warp_sum_of[i];
+        out.sum[list] = make_float2(all, total);
     }
-    if (key >= s_floor) {
-        const float floor = key_value(s_floor);
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-            if (f[j] >= floor) {
-                const int at = atomicAdd(&s_count, 1);
-                if (at < kCollect) {
-                    cand_v[at] = f[j];
-                    cand_i[at] = first + (j / VE) * kRowThreads * VE + j % VE;
-                }
-            }
-        }
-    }
-    __syncthreads();
-    int count = s_count;
-    if (count > kCollect) {
-        // many equal values: the n-th key bit by bit, then what is above it, then its ties in the order of their indices
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t c = t | (1u << bit);
-            int mine = 0;
-#pragma unroll
-            for (int j = 0; j < E; ++j) mine += f[j] == f[j] && order_key(f[j] + 0.f) >= c;
-            if (block_count(mine, red) >= n) t = c;
-        }
-        const float tie = key_value(t);
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-            if (f[j] > tie) {                // fewer than n
-                const int at = atomicAdd(&s_count, 1);
-                cand_v[at] = f[j];
-                cand_i[at] = first + (j / VE) * kRowThreads * VE + j % VE;
-            }
-        }
-        __syncthreads();
-        int have = s_count;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            int mine = 0;
-#pragma unroll
-            for (int j = 0; j < VE; ++j) mine += f[i * VE + j] == tie;
-            int before = mine;               // of this thread and the ones before it
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(kFull, before, o);
-                if (lane >= o) before += x;
-            }
-            __syncthreads();
-            if (lane == 31) red[warp] = before;
-            __syncthreads();
-            int at = have + before - mine;
-            for (int w = 0; w < kRowThreads / 32; ++w) {
-                if (w < warp) at += red[w];
-                have += red[w];
-            }
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                if (f[i * VE + j] == tie) {
-                    if (at < n) {
-                        cand_v[at] = tie;
-                        cand_i[at] = first + i * kRowThreads * VE + j;
-                    }
-                    ++at;
-                }
-            }
-        }
-        __syncthreads();
-        count = min(have, n);
-    }
-    if (tid < count) {
-        const float v = cand_v[tid];
-        const int idx = cand_i[tid];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += cand_v[j] > v || (cand_v[j] == v && cand_i[j] < idx);
-        if (rank < n) {
-            out.value[list * n + rank] = v;
-            out.index[list * n + rank] = idx;
-        }
-    }
-    if (tid >= count && tid < n) out.value[list * n + tid] = -INFINITY;
+    if (tid < n) out.entry[list * n + tid] = tid < s_count ? cand[tid] : 0;
 }
 
-// The rank of (score, order) among `count` of them: greater scores first, of equal ones the lower order.
-__device__ __forceinline__ int rank_of(const double* score, const int* order, int count, int i) {
-    const double s = score[i];
-    const int o = order[i];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += score[j] > s || (score[j] == s && order[j] < o);
-    return rank;
+// The rank of an entry among `count` of them, by the eight lanes around it: greater scores (as keys) first, of equal ones the lower order.
+__device__ __forceinline__ int rank_by_eight(const unsigned long long* score, const int* order, int count, unsigned long long s, int o) {
+    int before = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x % 8; j < count; j += 8) before += (int)(score[j] > s) | ((int)(score[j] == s) & (int)(order[j] < o));
+    before += __shfl_xor_sync(kFull, before, 1);
+    before += __shfl_xor_sync(kFull, before, 2);
+    before += __shfl_xor_sync(kFull, before, 4);
+    return before;
 }
 
 // One CTA joins the lists of one group's rows.  Every list is in order, so its head is its best: the n lists with the best heads hold
 // the n best values, and none of those is below the n-th head.
-__global__ void __launch_bounds__(1024) beam_join_kernel(const float* __restrict__ scores, int W, int V, int splits, int n, Lists in, float* __restrict__ out_scores,
-                                 long long* __restrict__ out_beams, long long* __restrict__ out_tokens) {
-    extern __shared__ double smem[];
+__global__ void __launch_bounds__(1024, 1) beam_join_kernel(const float* __restrict__ scores, int W, int V, int splits, int n, int room, Lists in,
+                                                            float* __restrict__ out_scores, long long* __restrict__ out_beams,
+                                                            long long* __restrict__ out_tokens) {
+    extern __shared__ unsigned long long smem[];
     __shared__ double so_far[kMaxBeams], lse[kMaxBeams];
+    __shared__ uint32_t kth_of[2][32];
     __shared__ int sel[kMaxN];
-    __shared__ int red[32];
-    __shared__ uint32_t s_floor;
-    __shared__ int s_count;
+    __shared__ int s_count, s_heads;
     __shared__ unsigned char used[2 * kMaxN];
-    const int lists = W * splits, room = max(lists, n * min(n, lists));
-    double* head = smem;                                     // [lists]
-    double* cand = head + lists;                             // [room]
-    int* cand_i = reinterpret_cast<int*>(cand + room);       // [room]
+    const int lists = W * splits;
+    unsigned long long* cand = smem;                         // [room], keys of scores
+    unsigned long long* head = cand + room;                  // [lists]
+    int* cand_i = reinterpret_cast<int*>(head + lists);      // [room]
+    int* list_of = cand_i + room;                            // [lists]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nth = blockDim.x, warps = nth >> 5;
     const long long g = blockIdx.x, l0 = g * lists;
+    if (tid == 0) s_count = s_heads = 0;
+    if (tid < 2 * kMaxN) used[tid] = 0;
     pdl_wait();
+    const unsigned long long first = lane * warps + warp < lists ? in.entry[(l0 + lane * warps + warp) * n] : 0;          // of this thread's first list
     for (int w = warp; w < W; w += warps) {
-        const long long at = l0 + (long long)w * splits;
-        float top = -INFINITY;
-        for (int i = lane; i < splits; i += 32) top = fmaxf(top, in.top[at + i]);
-        top = warp_max(top);
-        double sum = 0.0;
-        for (int i = lane; i < splits; i += 32) {
-            const float t = in.top[at + i];
-            sum += (double)in.sum[at + i] * (t == -INFINITY ? 1.0 : exp((double)t - (double)top));
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+        const float2* part = in.sum + l0 + (long long)w * splits;
         const float own = scores[g * W + w];
+        const float2 mine = lane < splits ? part[lane] : make_float2(-INFINITY, 0.f);
+        float top = mine.x;
+        for (int i = lane + 32; i < splits; i += 32) top = fmaxf(top, part[i].x);
+        top = warp_max(top);
+        double sum = mine.x == -INFINITY ? (double)mine.y : (double)mine.y * exp((double)mine.x - (double)top);
+        for (int i = lane + 32; i < splits; i += 32) {
+            const float2 p = part[i];
+            sum += p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)top);
+        }
+        for (int o = splits > 16 ? 16 : splits > 1 ? 8 : 0; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
         // a row with NaN, with +inf or without a finite logit has no candidates
         if (lane == 0) {
             so_far[w] = sum > 0.0 && own > -INFINITY ? (double)own : -INFINITY;
             lse[w] = sum > 0.0 ? (double)top + log(sum) : 0.0;
         }
     }
-    if (tid == 0) s_count = 0;
-    if (tid < 2 * kMaxN) used[tid] = 0;
     __syncthreads();
-    for (int l = tid; l < lists; l += nth) {
-        const float v = in.value[(l0 + l) * n];
-        const int w = l / splits;
-        head[l] = v > -INFINITY && so_far[w] > -INFINITY ? so_far[w] + ((double)v - lse[w]) : -INFINITY;
+    auto score_of = [&](unsigned long long entry, int w) -> unsigned long long {          // as a key, that of -inf where there is none
+        return order_key(entry != 0 && so_far[w] > -INFINITY ? so_far[w] + ((double)key_value((uint32_t)(entry >> 32)) - lse[w]) : -INFINITY);
+    };
+    // lists go around the warps; of the best heads of its threads each warp has a k-th largest, warps * k >= n
+    const int k = (n + warps - 1) / warps;
+    uint32_t own = 0;
+    for (int l = lane * warps + warp; l < lists; l += nth) {
+        const unsigned long long h = score_of(l < nth ? first : in.entry[(l0 + l) * n], l / splits);
+        head[l] = h;
+        own = max(own, (uint32_t)(h >> 32));
     }
+    uint32_t kth = kth_of_warp(own, k, lane);
+    if (lane == 0) kth_of[0][warp] = kth;
     __syncthreads();
-    if (warp == 0) {
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t c = t | (1u << bit);
-            int mine = 0;
-            for (int l = lane; l < lists; l += 32) mine += order_key_hi(head[l]) >= c;
-            if (__reduce_add_sync(kFull, mine) >= n) t = c;
-        }
-        if (lane == 0) s_floor = max(t, kLowestKeyHi);
+    uint32_t floor = __reduce_min_sync(kFull, lane < warps ? kth_of[0][lane] : kFull);
+    floor = max(floor, kLowestKeyHi);
+    for (int l = tid; l < lists; l += nth)
+        if ((uint32_t)(head[l] >> 32) >= floor) list_of[atomicAdd(&s_heads, 1)] = l;
+    __syncthreads();
+    const int heads = s_heads;
+    // what these lists hold bounds the n-th score once more
+    own = 0;
+    for (int e = tid; e < heads * n; e += nth) {
+        const int l = list_of[e / n];
+        own = max(own, (uint32_t)(score_of(in.entry[(l0 + l) * n + e % n], l / splits) >> 32));
     }
+    kth = kth_of_warp(own, k, lane);
+    if (lane == 0) kth_of[1][warp] = kth;
     __syncthreads();
-    for (int l = tid; l < lists; l += nth) {
-        if (order_key_hi(head[l]) >= s_floor) {
+    floor = max(floor, __reduce_min_sync(kFull, lane < warps ? kth_of[1][lane] : kFull));
+    auto take = [&](int l, int e, unsigned long long least) {
+        const unsigned long long entry = in.entry[(l0 + l) * n + e], s = score_of(entry, l / splits);
+        if (s >= least) {
             const int at = atomicAdd(&s_count, 1);
-            cand[at] = head[l];
-            cand_i[at] = l;          // heads of a row are in the order of their lists
+            if (at < room) {
+                cand[at] = s;
+                cand_i[at] = l / splits * V + (int)~(uint32_t)entry;
+            }
         }
-    }
-    __syncthreads();
-    const int heads = s_count;
-    for (int i = tid; i < heads; i += nth) {
-        const int r = rank_of(cand, cand_i, heads, i);
-        if (r < n) sel[r] = cand_i[i];
-    }
-    __syncthreads();
-    const int picked = min(heads, n);
-    const double least = heads >= n ? head[sel[n - 1]] : -INFINITY;
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-    for (int e = tid; e < picked * n; e += nth) {
-        const int l = sel[e / n], w = l / splits;
-        const float v = in.value[(l0 + l) * n + e % n];
-        const double s = so_far[w] + ((double)v - lse[w]);
-        if (v > -INFINITY && so_far[w] > -INFINITY && s >= least) {
-            const int at = atomicAdd(&s_count, 1);
-            cand[at] = s;
-            cand_i[at] = w * V + in.index[(l0 + l) * n + e % n];
-        }
-    }
+    };
+    for (int e = tid; e < heads * n; e += nth) take(list_of[e / n], e % n, (unsigned long long)floor << 32);
     __syncthreads();
     int count = s_count;
-    if (count > 4 * n && count > 128) {
-        // few lists hold much that is not below the least head: the n-th score's upper half bit by bit, and what is not below that
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t c = t | (1u << bit);
-            int mine = 0;
-            for (int i = tid; i < count; i += nth) mine += order_key_hi(cand[i]) >= c;
-            if (block_count(mine, red) >= n) t = c;
+    if (count > room) {
+        // equal scores in numbers: of the lists only the n with the best heads (those of a row are in the order of the lists), and nothing below
+        // the n-th head
+        for (int i0 = 0; i0 < heads; i0 += nth) {
+            if (i0 + tid < heads) cand[i0 + tid] = head[list_of[i0 + tid]];
         }
-        // moved to the front in rounds, each read before any of it is written
+        __syncthreads();
+        for (int i0 = 0; i0 < heads; i0 += nth / 8) {
+            const int i = i0 + tid / 8;
+            const int r = rank_by_eight(cand, list_of, heads, i < heads ? cand[i] : 0, i < heads ? list_of[i] : 0);
+            if (i < heads && r < n && tid % 8 == 0) sel[r] = list_of[i];
+        }
         if (tid == 0) s_count = 0;
         __syncthreads();
-        for (int at = 0; at < count; at += nth) {
-            const int i = at + tid;
-            const double s = i < count ? cand[i] : 0.0;
-            const int o = i < count ? cand_i[i] : 0;
-            const bool keep = i < count && order_key_hi(s) >= t;
-            __syncthreads();
-            if (keep) {
-                const int to = atomicAdd(&s_count, 1);
-                cand[to] = s;
-                cand_i[to] = o;
-            }
-            __syncthreads();
-        }
+        const int picked = min(heads, n);
+        const unsigned long long least = max(heads >= n ? head[sel[n - 1]] : 0ull, (unsigned long long)kLowestKeyHi << 32);
+        for (int e = tid; e < picked * n; e += nth) take(sel[e / n], e % n, least);
+        __syncthreads();
         count = s_count;
     }
-    for (int i = tid; i < count; i += nth) {
-        const int r = rank_of(cand, cand_i, count, i), o = cand_i[i];
-        if (r < n) {
-            out_scores[g * n + r] = (float)cand[i];
-            out_beams[g * n + r] = o / V;
-            out_tokens[g * n + r] = o % V;
+    for (int i0 = 0; i0 < count; i0 += nth / 8) {
+        const int i = i0 + tid / 8;
+        const unsigned long long s = i < count ? cand[i] : 0;
+        const int o = i < count ? cand_i[i] : 0;
+        const int r = rank_by_eight(cand, cand_i, count, s, o);
+        if (i < count && tid % 8 == 0) {
+            if (r < n) {
+                const int w = o / V;
+                out_scores[g * n + r] = (float)key_value(s);
+                out_beams[g * n + r] = w;
+                out_tokens[g * n + r] = o - w * V;
+            }
+            if (count < n && o < 2 * kMaxN) used[o] = 1;
         }
-        if (count < n && o < 2 * kMaxN) used[o] = 1;
     }
     __syncthreads();
     if (tid == 0 && count < n) {             // the rest are -inf, from the lowest index on
@@ -581,50 +751,70 @@ __global__ void __launch_bounds__(1024) beam_finish_kernel(Books in, int W, int 
     if (warp == 0 && lane < W) lengths[b * W + lane] = n;
 }
 
-// Values a thread of the first kernel takes: 32, or 8 where the rows are so few that longer chunks leave SMs idle.
-int values_per_thread(long long rows, int W, int V) {
-    const bool few = rows * ((V + 8191) / 8192) < 2LL * nxd_num_sms();
-    return few && (long long)W * ((V + 7 + 2047) / 2048) <= kMaxLists ? 8 : 32;
+// How rows are split: threads and vectors a thread of a round, rounds of a CTA, CTAs of a row.
+struct Split {
+    int threads, vecs, rounds, splits;
+};
+
+// Rounds of 512 threads x 4 vectors where that leaves no SM without a CTA, as many of them per CTA as leave one wave (two CTAs an SM); rounds of 256 x 2
+// where rows are few.
+Split split_of(long long rows, int W, int V, int elem) {
+    const int per_vec = 16 / elem;
+    const long long sms = nxd_num_sms(), span = V + per_vec - 1, large = 512LL * 4 * per_vec;
+    Split s;
+    const bool few = rows * ((span + large - 1) / large) < sms;
+    s.threads = few ? 256 : 512;
+    s.vecs = few ? 2 : 4;
+    const long long round = (long long)s.threads * s.vecs * per_vec, chunks = (span + round - 1) / round;
+    long long beside = (few ? 4 : 2) * sms / rows;
+    if (beside < 1) beside = 1;
+    if (beside > kMaxLists / W) beside = kMaxLists / W;
+    s.rounds = (int)((chunks + beside - 1) / beside);
+    s.splits = (int)((chunks + s.rounds - 1) / s.rounds);
+    return s;
 }
 
-int splits_of(int V, int elem, int E) { return (V + 16 / elem - 1 + kRowThreads * E - 1) / (kRowThreads * E); }
-
 template <typename T>
-void launch_rows(int E, long long ctas, cudaStream_t s, const void* logits, int V, long long stride, int splits, int n, Lists out) {
-    if (E == 8) beam_rows_kernel<T, 8><<<(unsigned)ctas, kRowThreads, 0, s>>>((const T*)logits, V, stride, splits, n, out);
-    else beam_rows_kernel<T, 32><<<(unsigned)ctas, kRowThreads, 0, s>>>((const T*)logits, V, stride, splits, n, out);
+cudaError_t launch_rows(const Split& p, long long ctas, cudaStream_t s, const void* logits, int V, long long stride, int n, Lists out) {
+    const int smem = (p.rounds < kStages ? p.rounds : kStages) * p.vecs * p.threads * 16;
+    if (p.threads == 256) {
+        beam_rows_kernel<T, 256, 2><<<(unsigned)ctas, 256, smem, s>>>((const T*)logits, V, stride, p.splits, p.rounds, n, out);
+    } else {
+        const cudaError_t e = nxd_allow_smem<beam_rows_kernel<T, 512, 4>>(kStages * 4 * 512 * 16);
+        if (e != cudaSuccess) return e;
+        beam_rows_kernel<T, 512, 4><<<(unsigned)ctas, 512, smem, s>>>((const T*)logits, V, stride, p.splits, p.rounds, n, out);
+    }
+    return cudaSuccess;
 }
 
 }  // namespace
 
-// Scratch of a call in floats, or 0 where the sizes are outside what is compiled.
+// Scratch of a call in bytes, or 0 where the sizes are outside what is compiled.
 NXD_API long long nxd_beam_select_scratch(int dtype, int B, int W, int V, int n) {
-    if (dtype < 0 || dtype > 2 || B < 1 || W < 1 || W > kMaxBeams || V < 1 || n < 1 || n > kMaxN || (long long)W * V >= (1LL << 31) - 16 || n > (long long)W * V)
+    if (dtype < 0 || dtype > 2 || B < 1 || W < 1 || W > kMaxBeams || V < 1 || V > 1 << 30 || n < 1 || n > kMaxN || (long long)W * V >= (1LL << 31) - 16 || n > (long long)W * V)
         return 0;
-    const long long rows = (long long)B * W;
-    const int splits = splits_of(V, dtype == 0 ? 4 : 2, values_per_thread(rows, W, V));
-    if ((long long)W * splits > kMaxLists || rows * splits >= (1LL << 31)) return 0;
-    return rows * splits * (2 + 2LL * n);
+    const long long rows = (long long)B * W, lists = rows * split_of(rows, W, V, dtype == 0 ? 4 : 2).splits;
+    return lists < (1LL << 31) ? lists * (8 + 8LL * n) : 0;
 }
 
 // logits [B * W, V] (0 fp32, 1 bf16, 2 fp16; rows `stride` elements apart), scores [B, W] -> the n best candidates of every group.
-NXD_API int nxd_beam_select(int dtype, const void* logits, long long stride, const float* scores, int B, int W, int V, int n, float* scratch,
+NXD_API int nxd_beam_select(int dtype, const void* logits, long long stride, const float* scores, int B, int W, int V, int n, void* scratch,
                             float* out_scores, long long* out_beams, long long* out_tokens, void* stream) {
     if (B == 0) return 0;
     NXD_REQUIRE(nxd_beam_select_scratch(dtype, B, W, V, n) > 0, "beam_select: %d beams of %d tokens, %d candidates are outside what is compiled", W, V, n);
     cudaStream_t s = (cudaStream_t)stream;
     const long long rows = (long long)B * W;
-    const int E = values_per_thread(rows, W, V), splits = splits_of(V, dtype == 0 ? 4 : 2, E), lists = W * splits;
+    const Split p = split_of(rows, W, V, dtype == 0 ? 4 : 2);
+    const int splits = p.splits, lists = W * splits;
     const Lists l = lists_of(scratch, rows * splits, n);
-    if (dtype == 0) launch_rows<float>(E, rows * splits, s, logits, V, stride, splits, n, l);
-    else if (dtype == 1) launch_rows<bf16>(E, rows * splits, s, logits, V, stride, splits, n, l);
-    else launch_rows<__half>(E, rows * splits, s, logits, V, stride, splits, n, l);
+    if (dtype == 0) NXD_CHECK_CUDA(launch_rows<float>(p, rows * splits, s, logits, V, stride, n, l));
+    else if (dtype == 1) NXD_CHECK_CUDA(launch_rows<bf16>(p, rows * splits, s, logits, V, stride, n, l));
+    else NXD_CHECK_CUDA(launch_rows<__half>(p, rows * splits, s, logits, V, stride, n, l));
     NXD_LAUNCH_CHECK();
     const int room = lists > n * (n < lists ? n : lists) ? lists : n * (n < lists ? n : lists);
-    const int smem = lists * 8 + room * 12;
-    NXD_CHECK_CUDA(nxd_allow_smem<beam_join_kernel>(kMaxLists * 20));
-    const int threads = lists > 256 || n > 16 ? 1024 : 256;
-    beam_join_kernel<<<B, threads, smem, s>>>(scores, W, V, splits, n, l, out_scores, out_beams, out_tokens);
+    const int smem = (lists + room) * 12, threads = lists > 256 || n > 16 ? 1024 : 256;
+    NXD_CHECK_CUDA(nxd_allow_smem<beam_join_kernel>(kMaxLists * 24));
+    NXD_CHECK_CUDA(nxd_launch_pdl(beam_join_kernel, dim3(B), dim3(threads), smem, s, scores, W, V, splits, n, room, l, out_scores, out_beams, out_tokens));
     NXD_LAUNCH_CHECK();
     return 0;
 }

@@ -113,10 +113,10 @@ int nxd_kv_cache_update(const void* new_k, const void* new_v, void* cache_k, voi
 
 /* ---- beam search (csrc/beam_search.cu) -----------------------------------------------------------
  * select: logits [B * W, V] (dtype 0 fp32, 1 bf16, 2 fp16; rows `stride` elements apart), scores [B, W] -> the n best of
- * scores[w] + log_softmax(logits[w])[v] of every group, best first, ties to the lowest w * V + v.  Scratch in floats, 0: outside what is
+ * scores[w] + log_softmax(logits[w])[v] of every group, best first, ties to the lowest w * V + v.  Scratch in bytes (16-byte aligned), 0: outside what is
  * compiled (W <= 32, n <= 64). */
 long long nxd_beam_select_scratch(int dtype, int B, int W, int V, int n);
-int nxd_beam_select(int dtype, const void* logits, long long stride, const float* scores, int B, int W, int V, int n, float* scratch,
+int nxd_beam_select(int dtype, const void* logits, long long stride, const float* scores, int B, int W, int V, int n, void* scratch,
                     float* out_scores, long long* out_beams, long long* out_tokens, void* stream);
 /* one step of the books: candidates [B, N], running scores and the pool [B, W] -> the same behind the step, tokens and parents [B, W] by line, a row
  * of the history [B, W].  norm = length ** penalty, length = tokens with this step's; eos -1: none. */

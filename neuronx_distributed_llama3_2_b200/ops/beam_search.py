@@ -6,6 +6,7 @@ move; at the end ``beam_finish``.  Nothing of it needs the host.  ``inference.be
 from __future__ import annotations
 
 import ctypes as _c
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -58,14 +59,9 @@ def _kernel(t: torch.Tensor) -> bool:
     return t.is_cuda and _lib.available()
 
 
-def _need(ok: bool, text: str) -> None:
-    if not ok:
-        raise ValueError(text)
-
-
-def _alike(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous {dtype} tensor {tuple(shape)} on {device} is expected, not {t.dtype} {tuple(t.shape)} on {t.device}"
+def _alike(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, like: torch.Tensor) -> None:
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != like.get_device() or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor {tuple(shape)} on {like.device} is expected, not {t.dtype} {tuple(t.shape)} on {t.device}"
                          + ("" if t.is_contiguous() else " with strides"))
 
 
@@ -79,37 +75,50 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
     ``-inf`` and beams with the score ``-inf`` are left out, and so is a beam whose logits hold NaN or ``+inf``, or nothing finite; where fewer
     than ``n`` candidates are left the rest have the score ``-inf``, from the lowest ``w * V + v`` on.  Scores are compared in 64 bits; tokens of one
     beam by their logits.  Returns ``(scores [B, n] fp32, beams [B, n] int64, tokens [B, n] int64)``; not differentiable."""
-    _need(scores.dim() == 2 and scores.dtype == torch.float32, f"scores: an fp32 tensor [B, W] is expected, not {scores.dtype} {tuple(scores.shape)}")
+    if scores.dim() != 2 or scores.dtype is not torch.float32:
+        raise ValueError(f"scores: an fp32 tensor [B, W] is expected, not {scores.dtype} {tuple(scores.shape)}")
     B, W = scores.shape
-    _need(logits.dim() in (2, 3) and tuple(logits.shape[:-1]) in ((B, W), (B * W,)),
-          f"logits {tuple(logits.shape)} do not go with scores of {B} x {W} beams")
-    _need(logits.is_floating_point(), f"logits of {logits.dtype} are no floating-point numbers")
-    _need(logits.device == scores.device, f"logits on {logits.device}, scores on {scores.device}")
+    if logits.dim() not in (2, 3) or logits.shape[:-1] != ((B, W) if logits.dim() == 3 else (B * W,)):
+        raise ValueError(f"logits {tuple(logits.shape)} do not go with scores of {B} x {W} beams")
+    if not logits.is_floating_point():
+        raise ValueError(f"logits of {logits.dtype} are no floating-point numbers")
+    if logits.get_device() != scores.get_device():
+        raise ValueError(f"logits on {logits.device}, scores on {scores.device}")
     V = logits.shape[-1]
     n = int(n)
-    _need(1 <= n <= MAX_CANDIDATES, f"between 1 and {MAX_CANDIDATES} candidates are taken, not {n}")
-    _need(1 <= W <= MAX_BEAMS, f"between 1 and {MAX_BEAMS} beams are taken, not {W}")
-    _need(n <= W * V, f"{n} candidates are more than {W} beams of {V} tokens have")
+    if not 1 <= n <= MAX_CANDIDATES:
+        raise ValueError(f"between 1 and {MAX_CANDIDATES} candidates are taken, not {n}")
+    if not 1 <= W <= MAX_BEAMS:
+        raise ValueError(f"between 1 and {MAX_BEAMS} beams are taken, not {W}")
+    if n > W * V:
+        raise ValueError(f"{n} candidates are more than {W} beams of {V} tokens have")
     if not _kernel(logits):
         return beam_select_ref(logits, scores, n)
-    _need(logits.dtype in _DTYPES, f"logits of {logits.dtype} are not taken on the GPU: fp32, bf16 or fp16")
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"logits of {logits.dtype} are not taken on the GPU: fp32, bf16 or fp16")
     if logits.dim() == 3 and not (W == 1 or B == 1 or logits.stride(0) == W * logits.stride(1)) or (logits.stride(-1) != 1 and V != 1):
         logits = logits.contiguous()
     stride = (logits.stride(1) if W > 1 else logits.stride(0)) if logits.dim() == 3 else logits.stride(0)
     scores = scores.contiguous()
-    code = _DTYPES[logits.dtype]
-    out = torch.empty((2, B, n), dtype=torch.int64, device=logits.device)
-    best = torch.empty((B, n), dtype=torch.float32, device=logits.device)
+    code, device = _DTYPES[logits.dtype], logits.device
+    out = torch.empty((2, B, n), dtype=torch.int64, device=device)
+    best = torch.empty((B, n), dtype=torch.float32, device=device)
     if B:
         with _lib.on_device_of(logits):
-            size = _entry("nxd_beam_select_scratch")(code, B, W, V, n)
-            _need(size > 0, f"{W} beams of {V} tokens are more than one call takes")
-            scratch = torch.empty(size, dtype=torch.float32, device=logits.device)          # the call's own
+            size = _scratch_bytes(code, B, W, V, n)
+            if size <= 0:
+                raise ValueError(f"{W} beams of {V} tokens are more than one call takes")
+            scratch = torch.empty(size, dtype=torch.uint8, device=device)          # the call's own
             at = out.data_ptr()
             rc = _entry("nxd_beam_select")(code, logits.data_ptr(), stride, scores.data_ptr(), B, W, V, n, scratch.data_ptr(), best.data_ptr(), at,
                                            at + 8 * B * n, _lib.stream_ptr())
         _lib.check(rc, "nxd_beam_select")
-    return best, out[0], out[1]
+    return (best, *out.unbind(0))
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(code: int, B: int, W: int, V: int, n: int) -> int:
+    return _entry("nxd_beam_select_scratch")(code, B, W, V, n)
 
 
 def beam_select_ref(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -139,16 +148,19 @@ def beam_advance(candidates: Tuple[torch.Tensor, torch.Tensor, torch.Tensor], sc
     ``candidates``: scores, beams, tokens ``[B, N]``, the best first; ``scores``: the running ``[B, W]`` (of a request that is over they are handed
     on).  Writes row ``step`` of the history.  Returns ``(scores [B, W], tokens [B, W], parents [B, W], pool)``, by line."""
     cand_scores, cand_beams, cand_tokens = candidates
-    _need(scores.dim() == 2, f"scores: [B, W] is expected, not {tuple(scores.shape)}")
+    if scores.dim() != 2:
+        raise ValueError(f"scores: [B, W] is expected, not {tuple(scores.shape)}")
     (B, W), N, dev = scores.shape, cand_scores.shape[-1], scores.device
-    _need(1 <= W <= MAX_BEAMS and 1 <= N <= MAX_CANDIDATES, f"{W} beams and {N} candidates: up to {MAX_BEAMS} and {MAX_CANDIDATES} are taken")
+    if not (1 <= W <= MAX_BEAMS and 1 <= N <= MAX_CANDIDATES):
+        raise ValueError(f"{W} beams and {N} candidates: up to {MAX_BEAMS} and {MAX_CANDIDATES} are taken")
     step = int(step)
-    _need(history.tokens.dim() == 3 and 0 <= step < history.tokens.shape[0], f"step {step} is outside a history of {tuple(history.tokens.shape)}")
-    _alike("scores", scores, (B, W), torch.float32, dev)
-    _check_books(pool, history, B, W, dev)
+    if not (history.tokens.dim() == 3 and 0 <= step < history.tokens.shape[0]):
+        raise ValueError(f"step {step} is outside a history of {tuple(history.tokens.shape)}")
+    _alike("scores", scores, (B, W), torch.float32, scores)
+    _check_books(pool, history, B, W, scores)
     for name, t, dtype in (("candidates' scores", cand_scores, torch.float32), ("candidates' beams", cand_beams, torch.int64),
                            ("candidates' tokens", cand_tokens, torch.int64)):
-        _alike(name, t, (B, N), dtype, dev)
+        _alike(name, t, (B, N), dtype, scores)
     eos, pad = _ids(eos_token_id, pad_token_id)
     norm = _norm(step + 1, length_penalty)
     if not _kernel(scores):
@@ -173,8 +185,10 @@ def beam_advance(candidates: Tuple[torch.Tensor, torch.Tensor, torch.Tensor], sc
 
 def _ids(eos_token_id: Optional[int], pad_token_id: int) -> Tuple[int, int]:
     eos, pad = -1 if eos_token_id is None else int(eos_token_id), int(pad_token_id)
-    _need(eos_token_id is None or 0 <= eos < 2 ** 31, f"eos_token_id {eos_token_id} is no token")
-    _need(-2 ** 31 <= pad < 2 ** 31, f"pad_token_id {pad_token_id} does not fit 32 bits")
+    if eos_token_id is not None and not 0 <= eos < 2 ** 31:
+        raise ValueError(f"eos_token_id {eos_token_id} is no token")
+    if not -2 ** 31 <= pad < 2 ** 31:
+        raise ValueError(f"pad_token_id {pad_token_id} does not fit 32 bits")
     return eos, pad
 
 
@@ -183,18 +197,19 @@ def _norm(length: int, penalty: float) -> float:
         norm = float(length) ** float(penalty)
     except OverflowError:
         norm = float("inf")
-    _need(1e-37 < norm < 3e38, f"a length of {length} to the power of {penalty} is no fp32 number")
+    if not 1e-37 < norm < 3e38:
+        raise ValueError(f"a length of {length} to the power of {penalty} is no fp32 number")
     return norm
 
 
-def _check_books(pool: BeamPool, history: BeamHistory, B: int, W: int, dev: torch.device) -> None:
-    _alike("pool.scores", pool.scores, (B, W), torch.float32, dev)
-    _alike("pool.lengths", pool.lengths, (B, W), torch.int32, dev)
-    _alike("pool.slots", pool.slots, (B, W), torch.int32, dev)
-    _alike("pool.done", pool.done, (B,), torch.bool, dev)
+def _check_books(pool: BeamPool, history: BeamHistory, B: int, W: int, scores: torch.Tensor) -> None:
+    _alike("pool.scores", pool.scores, (B, W), torch.float32, scores)
+    _alike("pool.lengths", pool.lengths, (B, W), torch.int32, scores)
+    _alike("pool.slots", pool.slots, (B, W), torch.int32, scores)
+    _alike("pool.done", pool.done, (B,), torch.bool, scores)
     T = history.tokens.shape[0]
-    _alike("history.tokens", history.tokens, (T, B, W), torch.int32, dev)
-    _alike("history.parents", history.parents, (T, B, W), torch.int32, dev)
+    _alike("history.tokens", history.tokens, (T, B, W), torch.int32, scores)
+    _alike("history.parents", history.parents, (T, B, W), torch.int32, scores)
 
 
 def _merged(W: int, *sides):
@@ -245,12 +260,15 @@ def beam_finish(scores: torch.Tensor, pool: BeamPool, history: BeamHistory, step
     """The best ``W`` hypotheses of every request after ``step`` steps, the best first: what its pool holds and, where it is not over, its beams with
     ``scores / step ** length_penalty``.  Returns ``(tokens [B, W, step] int64, lengths [B, W] int64, scores [B, W] fp32)``; behind a sequence's
     length are ``pad_token_id``, a place without a hypothesis has the length 0 and the score ``-inf``."""
-    _need(scores.dim() == 2, f"scores: [B, W] is expected, not {tuple(scores.shape)}")
+    if scores.dim() != 2:
+        raise ValueError(f"scores: [B, W] is expected, not {tuple(scores.shape)}")
     (B, W), dev, step = scores.shape, scores.device, int(step)
-    _need(1 <= W <= MAX_BEAMS, f"between 1 and {MAX_BEAMS} beams are taken, not {W}")
-    _need(history.tokens.dim() == 3 and 1 <= step <= history.tokens.shape[0], f"{step} steps are outside a history of {tuple(history.tokens.shape)}")
-    _alike("scores", scores, (B, W), torch.float32, dev)
-    _check_books(pool, history, B, W, dev)
+    if not 1 <= W <= MAX_BEAMS:
+        raise ValueError(f"between 1 and {MAX_BEAMS} beams are taken, not {W}")
+    if not (history.tokens.dim() == 3 and 1 <= step <= history.tokens.shape[0]):
+        raise ValueError(f"{step} steps are outside a history of {tuple(history.tokens.shape)}")
+    _alike("scores", scores, (B, W), torch.float32, scores)
+    _check_books(pool, history, B, W, scores)
     eos, pad = _ids(eos_token_id, pad_token_id)
     norm = _norm(step, length_penalty)
     if not _kernel(scores):
