@@ -647,108 +647,195 @@ __global__ void __launch_bounds__(128) beam_advance_kernel(const float* __restri
     if (lane == 0) done[b] = last > -INFINITY && (early || last >= best);
 }
 
-constexpr int kTraceSteps = 16;          // steps that a warp writes at a time
+constexpr int kBatch = 8;                    // reads under way
+constexpr int kSections = 32;                // of a CTA
+constexpr int kFinishThreads = 512;
+constexpr int kFinishCluster = 8;            // CTAs of a group at most
+constexpr int kFinishBytes = 100 * 1024;     // of shared memory: a byte a step and line, and where they fit their tokens
 
-// The beams of requests that are not over join the pool, and every place's tokens are found from the last one back.  A line's history is
-// a chain of parents; a warp walks a section of it for all lines at once (lane w starts in line w at the section's end), so the
-// sections are walked side by side, joined, and walked once more for the tokens.
-__global__ void __launch_bounds__(1024) beam_finish_kernel(Books in, int W, int B, int step, float norm, long long eos, long long pad, const int* __restrict__ hist_token,
-                                   const int* __restrict__ hist_parent, long long* __restrict__ tokens, long long* __restrict__ lengths,
-                                   float* __restrict__ scores) {
-    extern __shared__ int stage[];                                       // [warps][W][kTraceSteps + 1]
+__host__ __device__ inline int token_pitch(int W) { return W | 1; }          // words a step: lanes of consecutive steps in different banks
+
+__device__ __forceinline__ void store_of_rank(unsigned char* p, int rank, int v) {          // to the same place in a CTA of the cluster
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("st.shared::cluster.u8 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+
+// The beams of requests that are not over join the pool, and every place's tokens are found from the last one back.  A line's history is a
+// chain of parents.  A cluster of CTAs has a group, each a span of its steps: the parents are brought into shared memory as bytes, with the tokens
+// on their way behind them; a section of the span is walked for all lines at once (lane w starts in line w at the section's end; a warp has as many
+// sections as it has room for lines); the sections are joined within a CTA, the spans across the cluster; then they are walked once
+// more, which leaves the line of every place at every step where the parents were.
+//   Latency bounds it, of the chain and of rows that are a few bytes each: 2000 steps of 8 lines in 64 groups 180 ms with an operation a step, 28 us with
+// one CTA a group and 32 sections.
+__global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(Books in, int W, int B, int step, int span, float norm, long long eos, long long pad,
+                                                                     const int* __restrict__ hist_token, const int* __restrict__ hist_parent,
+                                                                     long long* __restrict__ tokens, long long* __restrict__ lengths,
+                                                                     float* __restrict__ scores, unsigned char* __restrict__ scratch, int staged) {
+    extern __shared__ int finish_smem[];          // tokens [span][token_pitch] if staged, then the path [span][W] unless scratch is there
     __shared__ int enter_at[kMaxBeams], enter_slot[kMaxBeams], len[kMaxBeams], ended[kMaxBeams];
-    __shared__ unsigned char through[32][32], part[32][32], entry[32][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const long long b = blockIdx.x;
-    const int section = (step + warps - 1) / warps;
-    if (warp == 0) {
-        const bool mine = lane < W;
+    __shared__ unsigned char through[kSections][32], part[kSections][32], entry[kSections][32];
+    __shared__ unsigned char span_through[kFinishCluster][32], span_part[kFinishCluster][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nth = blockDim.x;
+    const int rank = blockIdx.x, ranks = gridDim.x;          // the cluster is a row of the grid
+    const long long b = blockIdx.y;
+    const int pitch = token_pitch(W), first = rank * span, steps = max(min(span, step - first), 0);          // t counts from `first`
+    unsigned char* path = scratch != nullptr ? scratch + (b * step + first) * W : reinterpret_cast<unsigned char*>(finish_smem + (staged ? span * pitch : 0));
+    // a line in 2^shift lanes: lane w of them has line w
+    const int shift = W <= 1 ? 0 : 32 - __clz(W - 1), wide = 1 << shift, w = lane & (wide - 1);
+    const bool used = w < W;
+    float old_score = -INFINITY, own_score = -INFINITY;
+    int old_length = 0, old_slot = 0;
+    bool over = false;
+    if (warp == 0 && lane < W) {
         const long long at = b * W + lane;
-        const float a = mine ? in.pool_score[at] : -INFINITY;
-        const float r = mine && !in.done[b] ? __fdiv_rn(in.running[at], norm) : -INFINITY;
-        const float c = r == r ? r : -INFINITY;
+        old_score = in.pool_score[at], own_score = in.running[at], old_length = in.pool_length[at], old_slot = in.pool_slot[at];
+        over = in.done[b];
+    }
+    {
+        const int apart = nth >> shift;
+        for (int t0 = tid >> shift; t0 < steps; t0 += kBatch * apart) {
+            int p[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int t = t0 + k * apart;
+                const long long at = ((long long)(first + t) * B + b) * W + w;
+                p[k] = used && t < steps ? hist_parent[at] : 0;
+                if (staged && used && t < steps)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(finish_smem + t * pitch + w)),
+                                 "l"(hist_token + at) : "memory");
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int t = t0 + k * apart;
+                if (used && t < steps) path[t * W + w] = (unsigned char)min(max(p[k], 0), W - 1);
+            }
+        }
+        fetch_commit();
+    }
+    if (warp == 0) {
+        const float r = over ? -INFINITY : __fdiv_rn(own_score, norm), c = r == r ? r : -INFINITY;
         int ra, rb;
-        merge_ranks(a, c, W, lane, ra, rb);
-        if (mine && ra < W) {
-            const int n = a > -INFINITY ? min(max(in.pool_length[at], 0), step) : 0;
-            scores[b * W + ra] = a;
+        merge_ranks(old_score, c, W, lane, ra, rb);
+        if (lane < W && ra < W) {
+            const int n = old_score > -INFINITY ? min(max(old_length, 0), step) : 0;
             len[ra] = n;
             ended[ra] = 1;
             enter_at[ra] = n - 2;            // the last token is the one that ends
-            enter_slot[ra] = min(max(in.pool_slot[at], 0), W - 1);
+            enter_slot[ra] = min(max(old_slot, 0), W - 1);
+            if (rank == 0) scores[b * W + ra] = old_score, lengths[b * W + ra] = n;
         }
-        if (mine && rb < W) {
+        if (lane < W && rb < W) {
             const int n = c > -INFINITY ? step : 0;
-            scores[b * W + rb] = c;
             len[rb] = n;
             ended[rb] = 0;
             enter_at[rb] = n - 1;
             enter_slot[rb] = lane;
+            if (rank == 0) scores[b * W + rb] = c, lengths[b * W + rb] = n;
         }
     }
     __syncthreads();
-    const int mine = min(lane, W - 1);
-    const int lo = warp * section, hi = min(step, lo + section);
-    const int t_in = enter_at[mine];
-    {
-        int line = mine, cur = enter_slot[mine];
-        for (int t1 = hi; t1 > lo; t1 -= kTraceSteps) {
-            const int t0 = max(lo, t1 - kTraceSteps);
-            int p[kTraceSteps];
+    const int sections = max(min(min(kSections, (steps + 15) / 16), (nth >> 5) << (5 - shift)), 1), section = (steps + sections - 1) / sections;
+    const int mine = used ? w : 0, sec = (warp << (5 - shift)) + (lane >> shift), t_in = enter_at[mine] - first;
+    const bool walks = warp << (5 - shift) < sections;
+    const int lo = sec * section;
+    // the parents of steps that a section has not are its lanes' own lines
+    auto fetch = [&](int (&p)[kBatch], int at) {
 #pragma unroll
-            for (int i = 0; i < kTraceSteps; ++i) p[i] = t1 - 1 - i >= t0 ? min(max(hist_parent[((long long)(t1 - 1 - i) * B + b) * W + mine], 0), W - 1) : 0;
+        for (int k = 0; k < kBatch; ++k) {
+            const int t = lo + section - 1 - at - k;
+            p[k] = used && t >= lo && t < steps ? path[t * W + w] : w;
+        }
+    };
+    if (walks) {
+        int line = w, cur = enter_slot[mine];
+        for (int at = 0; at < section; at += kBatch) {
+            int p[kBatch];
+            fetch(p, at);
 #pragma unroll
-            for (int i = 0; i < kTraceSteps; ++i) {
-                if (t1 - 1 - i < t0) break;
-                line = __shfl_sync(kFull, p[i], line);
-                const int next = __shfl_sync(kFull, p[i], cur);
-                if (t1 - 1 - i <= t_in) cur = next;
+            for (int k = 0; k < kBatch; ++k) {
+                line = __shfl_sync(kFull, p[k], line, wide);
+                const int next = __shfl_sync(kFull, p[k], cur, wide);
+                if (lo + section - 1 - at - k <= t_in) cur = next;
             }
         }
-        through[warp][lane] = (unsigned char)line;
-        part[warp][lane] = (unsigned char)cur;
+        if (sec < sections) through[sec][w] = (unsigned char)line, part[sec][w] = (unsigned char)cur;
     }
     __syncthreads();
-    if (warp == 0) {
-        int cur = enter_slot[mine];
-        for (int k = warps - 1; k >= 0; --k) {
-            entry[k][lane] = (unsigned char)cur;
-            const int k0 = k * section;
-            if (t_in >= k0 + section) cur = through[k][cur];             // entered above this section
-            else if (t_in >= k0) cur = part[k][lane];
+    // of lane w: where line w of the span's end comes from, and place w if it enters the span
+    auto join = [&](int t, int cur, bool keep) {
+        for (int k = sections - 1; k >= 0; --k) {
+            if (keep) entry[k][lane] = (unsigned char)cur;
+            if (t >= min((k + 1) * section, steps)) cur = through[k][cur];             // entered above this section
+            else if (t >= k * section) cur = part[k][lane];
+        }
+        return cur;
+    };
+    const int own_in = lane < W ? enter_at[lane] : -1;
+    int cur = lane < W ? enter_slot[lane] : 0;
+    if (ranks > 1) {
+        if (warp == 0 && lane < W) {
+            int line = lane;
+            for (int k = sections - 1; k >= 0; --k) line = through[k][line];
+            const int place = join(own_in - first, cur, false);
+            for (int r = 0; r < ranks; ++r) {
+                store_of_rank(&span_through[rank][lane], r, line);
+                store_of_rank(&span_part[rank][lane], r, place);
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (warp == 0 && lane < W) {
+            for (int r = ranks - 1; r > rank; --r) {
+                if (own_in >= (r + 1) * span) cur = span_through[r][cur];
+                else if (own_in >= r * span) cur = span_part[r][lane];
+            }
         }
     }
+    if (warp == 0 && lane < W) join(own_in - first, cur, true);
     __syncthreads();
-    int cur = entry[warp][lane];
-    int* own = stage + warp * W * (kTraceSteps + 1);
-    const int n = len[mine], ends = ended[mine];
-    for (int t1 = hi; t1 > lo; t1 -= kTraceSteps) {
-        const int t0 = max(lo, t1 - kTraceSteps), steps = t1 - t0;
-        int p[kTraceSteps], k[kTraceSteps];
+    if (walks) {
+        cur = sec < sections ? entry[sec][mine] : 0;
+        for (int at = 0; at < section; at += kBatch) {
+            int p[kBatch];
+            fetch(p, at);
 #pragma unroll
-        for (int i = 0; i < kTraceSteps; ++i) {
-            const long long at = ((long long)(t1 - 1 - i) * B + b) * W + mine;
-            p[i] = i < steps ? min(max(hist_parent[at], 0), W - 1) : 0;
-            k[i] = i < steps ? hist_token[at] : 0;
+            for (int k = 0; k < kBatch; ++k) {
+                const int t = lo + section - 1 - at - k;
+                const int next = __shfl_sync(kFull, p[k], cur, wide);
+                if (used && t >= lo && t < steps) path[t * W + w] = (unsigned char)cur;
+                if (t <= t_in) cur = next;
+            }
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kTraceSteps; ++i) {
-            if (i >= steps) break;
-            const int t = t1 - 1 - i;
-            const int token = __shfl_sync(kFull, k[i], cur), next = __shfl_sync(kFull, p[i], cur);
-            const bool inside = t <= t_in;
-            if (lane < W) own[lane * (kTraceSteps + 1) + t - t0] = inside ? token : (int)(ends && t == n - 1 ? eos : pad);
-            if (inside) cur = next;
-        }
-        __syncwarp();
-        for (int i = lane; i < W * kTraceSteps; i += 32) {
-            const int h = i / kTraceSteps, t = i % kTraceSteps;
-            if (t < steps) tokens[(b * W + h) * step + t0 + t] = own[h * (kTraceSteps + 1) + t];
-        }
-        __syncwarp();
     }
-    if (warp == 0 && lane < W) lengths[b * W + lane] = n;
+    fetch_wait<0>();
+    __syncthreads();
+    for (int t = tid; t < steps; t += nth) {
+        for (int h0 = 0; h0 < W; h0 += kBatch) {
+            int token[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                token[k] = 0;
+                if (h0 + k < W && first + t <= enter_at[h0 + k]) {
+                    const int line = path[t * W + h0 + k];
+                    token[k] = staged ? finish_smem[t * pitch + line] : hist_token[((long long)(first + t) * B + b) * W + line];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int h = h0 + k;
+                if (h < W)
+                    tokens[(b * W + h) * step + first + t] = first + t <= enter_at[h] ? (long long)token[k] : ended[h] && first + t == len[h] - 1 ? eos : pad;
+            }
+        }
+    }
+}
+
+// Steps of a CTA: a cluster of up to eight has a group, as long as two CTAs an SM are not exceeded and each has 64 steps.
+int finish_span(int B, int step, int* ranks) {
+    int r = 1;
+    while (r < kFinishCluster && (long long)B * r * 2 <= 2LL * nxd_num_sms() && step >= 128 * r) r *= 2;
+    *ranks = r;
+    return (step + r - 1) / r;
 }
 
 // How rows are split: threads and vectors a thread of a round, rounds of a CTA, CTAs of a row.
@@ -835,17 +922,39 @@ NXD_API int nxd_beam_advance(const float* cand_scores, const long long* cand_bea
     return 0;
 }
 
+// Bytes of scratch that a call needs, 0: none.
+NXD_API long long nxd_beam_finish_scratch(int B, int W, int step) {
+    int ranks;
+    return (long long)W * finish_span(B, step, &ranks) > kFinishBytes ? (long long)B * W * step : 0;
+}
+
 // The sequences of every group's best W hypotheses (the header has the arrays).
 NXD_API int nxd_beam_finish(const float* running, const float* pool_scores, const int* pool_lengths, const int* pool_slots, const unsigned char* done,
                             int B, int W, int step, float norm, long long eos, long long pad, const int* hist_tokens, const int* hist_parents,
-                            long long* tokens, long long* lengths, float* scores, void* stream) {
-    NXD_REQUIRE(W >= 1 && W <= kMaxBeams && step >= 0, "beam_finish: %d beams, %d steps", W, step);
+                            long long* tokens, long long* lengths, float* scores, void* scratch, void* stream) {
+    NXD_REQUIRE(W >= 1 && W <= kMaxBeams && step >= 1 && (long long)W * step < (1LL << 30) && B <= 65535, "beam_finish: %d requests of %d beams, %d steps", B, W, step);
     if (B == 0) return 0;
+    const bool large = nxd_beam_finish_scratch(B, W, step) > 0;
+    NXD_REQUIRE(!large || scratch != nullptr, "beam_finish: %d beams of %d steps need scratch", W, step);
+    int ranks;
+    const int span = finish_span(B, step, &ranks);
     const Books in = {running, pool_scores, pool_lengths, pool_slots, done};
-    const int warps = step <= kTraceSteps ? 1 : step >= 32 * kTraceSteps ? 32 : (step + kTraceSteps - 1) / kTraceSteps;
-    const int smem = warps * W * (kTraceSteps + 1) * 4;
-    NXD_CHECK_CUDA(nxd_allow_smem<beam_finish_kernel>(32 * kMaxBeams * (kTraceSteps + 1) * 4));
-    beam_finish_kernel<<<B, warps * 32, smem, (cudaStream_t)stream>>>(in, W, B, step, norm, eos, pad, hist_tokens, hist_parents, tokens, lengths, scores);
+    const long long token_bytes = 4LL * span * token_pitch(W), path_bytes = (long long)W * span;
+    const bool staged = !large && token_bytes + path_bytes <= kFinishBytes;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ranks, B);
+    cfg.blockDim = dim3(path_bytes >= kFinishThreads ? kFinishThreads : path_bytes <= 128 ? 128 : (unsigned)((path_bytes + 31) / 32 * 32));
+    cfg.dynamicSmemBytes = (large ? 0 : path_bytes) + (staged ? token_bytes : 0);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NXD_CHECK_CUDA(nxd_allow_smem<beam_finish_kernel>(kFinishBytes));
+    NXD_CHECK_CUDA(cudaLaunchKernelEx(&cfg, beam_finish_kernel, in, W, B, step, span, norm, eos, pad, hist_tokens, hist_parents, tokens, lengths, scores,
+                                      large ? (unsigned char*)scratch : (unsigned char*)nullptr, (int)staged));
     NXD_LAUNCH_CHECK();
     return 0;
 }

@@ -10,6 +10,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 256;          // of a launch: 2 KB of parameters
 constexpr int kMaxBeams = 32;
+constexpr int kDeep = 4;                  // units of a thread
 
 struct Tensors {
     char* base[kMaxTensors];
@@ -28,12 +29,14 @@ constexpr int kAside = -1, kMaxMoves = kMaxBeams + kMaxBeams / 2;
 struct Moves {
     signed char to[kMaxMoves], from[kMaxMoves];
     int n;
+    bool circles;
 };
 
 // By one warp, lane w for line w; from[w] = w: it stays.
 __device__ __forceinline__ void order_moves(int from, int lane, Moves& m) {
     unsigned left = __ballot_sync(0xffffffffu, from != lane);          // lines to be written
     int n = 0;
+    bool circles = false;
     while (left != 0) {
         // lines that a line still to be written reads
         const unsigned read = __reduce_or_sync(0xffffffffu, left >> lane & 1 ? 1u << from : 0u);
@@ -47,6 +50,7 @@ __device__ __forceinline__ void order_moves(int from, int lane, Moves& m) {
             n += __popc(ready);
             left &= ~ready;
         } else {          // circles only: the first one, around
+            circles = true;
             const int first = __ffs(left) - 1;
             if (lane == 0) m.to[n] = kAside, m.from[n] = (signed char)first;
             ++n;
@@ -60,16 +64,17 @@ __device__ __forceinline__ void order_moves(int from, int lane, Moves& m) {
             } while (at != first);
         }
     }
-    if (lane == 0) m.n = n;
+    if (lane == 0) m.n = n, m.circles = circles;
 }
 
-// Lines g * W + w of a group continue its lines g * W + parent[w], rows [start, end) of every head.  A thread takes one unit of all the
-// group's lines in an order that works in place, so there is no scratch and each line that is wanted is read once from memory however
-// many continue it.  Four reads are under way before the first of them is written.
-template <typename U>
-__global__ void __launch_bounds__(kThreads) reorder_lines_kernel(const __grid_constant__ Tensors t, Shape s, int W, const long long* __restrict__ parents,
-                                                                 const long long* __restrict__ start, const long long* __restrict__ end,
-                                                                 const int* __restrict__ table, int page_size, int max_pages, int num_pages) {
+// Lines g * W + w of a group continue its lines g * W + parent[w], rows [start, end) of every head.  A thread takes kDeep units, a block's width
+// apart, of all the group's lines in an order that works in place, so there is no scratch and each line that is wanted is read once from memory
+// however many continue it.  Two moves of four units are read before the first of them is written.
+//   With a table the lines are pages: PAGED.
+template <typename U, bool PAGED>
+__global__ void __launch_bounds__(kThreads, PAGED ? 3 : 4) reorder_lines_kernel(const __grid_constant__ Tensors t, Shape s, int W, const long long* __restrict__ parents,
+                                                                    const long long* __restrict__ start, const long long* __restrict__ end,
+                                                                    const int* __restrict__ table, int page_size, int max_pages, int num_pages) {
     __shared__ Moves moves;
     const int g = blockIdx.y;
     const long long line0 = (long long)g * W;
@@ -85,46 +90,79 @@ __global__ void __launch_bounds__(kThreads) reorder_lines_kernel(const __grid_co
     if (n == 0 || hi <= lo) return;
     const unsigned per_head = (unsigned)(hi - lo) * (unsigned)s.per_row, per_tensor = per_head * (unsigned)s.heads;
     const unsigned total = per_tensor * (unsigned)t.n;          // the host keeps it below 2^31
-    for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
-        const unsigned tensor = i / per_tensor, in_tensor = i - tensor * per_tensor;
-        const unsigned head = in_tensor / per_head, unit = in_tensor - head * per_head;
-        char* base = t.base[tensor] + (long long)head * s.head_stride;
-        int page = 0;
-        if (table == nullptr) {
-            base += line0 * s.line_stride + (lo * s.per_row + unit) * (long long)sizeof(U);
-        } else {
-            const unsigned r = unit / (unsigned)s.per_row, row = (unsigned)lo + r;
-            page = (int)(row / (unsigned)page_size);
-            base += ((long long)(row - (unsigned)page * (unsigned)page_size) * s.per_row + (unit - r * (unsigned)s.per_row)) * (long long)sizeof(U);
-        }
-        auto place = [&](int w) -> U* {
-            if (table == nullptr) return reinterpret_cast<U*>(base + w * s.line_stride);
-            const int p = table[(line0 + w) * max_pages + page];
-            return p < 0 || p >= num_pages ? nullptr : reinterpret_cast<U*>(base + p * s.line_stride);
-        };
-        U aside{};
-        bool has_aside = false;
-        for (int k0 = 0; k0 < n; k0 += 4) {
-            U v[4];
-            U* to[4];
+    for (unsigned i0 = blockIdx.x * (kThreads * kDeep) + threadIdx.x; i0 < total; i0 += gridDim.x * (kThreads * kDeep)) {
+        char* base[kDeep];          // of a unit in the group's first line, or in page 0
+        int page[PAGED ? kDeep : 1];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                to[k] = nullptr;
-                if (k0 + k >= n) continue;
-                const int d = moves.to[k0 + k], f = moves.from[k0 + k];
-                const U* src = f == kAside ? nullptr : place(f);
-                if (d == kAside) {
-                    has_aside = src != nullptr;
-                    if (has_aside) aside = *src;
-                } else {
-                    if (src != nullptr) v[k] = *src;
-                    else if (f == kAside) v[k] = aside;
-                    if (f == kAside ? has_aside : src != nullptr) to[k] = place(d);
+        for (int q = 0; q < kDeep; ++q) {
+            const unsigned i = min(i0 + q * kThreads, total - 1);
+            const unsigned tensor = i / per_tensor, in_tensor = i - tensor * per_tensor;
+            const unsigned head = in_tensor / per_head, unit = in_tensor - head * per_head;
+            char* at = t.base[tensor] + (long long)head * s.head_stride;
+            if constexpr (PAGED) {
+                const unsigned r = unit / (unsigned)s.per_row, row = (unsigned)lo + r;
+                page[q] = (int)(row / (unsigned)page_size);
+                at += ((long long)(row - (unsigned)page[q] * (unsigned)page_size) * s.per_row + (unit - r * (unsigned)s.per_row)) * (long long)sizeof(U);
+            } else {
+                at += line0 * s.line_stride + (lo * s.per_row + unit) * (long long)sizeof(U);
+            }
+            base[q] = at;
+        }
+        // of line w, or nothing where the table names no page
+        auto place = [&](int q, int w) -> U* {
+            if constexpr (PAGED) {
+                const int p = table[(line0 + w) * max_pages + page[q]];
+                return p < 0 || p >= num_pages ? nullptr : reinterpret_cast<U*>(base[q] + p * s.line_stride);
+            } else {
+                return reinterpret_cast<U*>(base[q] + w * s.line_stride);
+            }
+        };
+        const unsigned left = (total - i0 + kThreads - 1) / kThreads;          // units that are this thread's
+        if (moves.circles) {
+#pragma unroll
+            for (int q = 0; q < kDeep; ++q) {
+                if (q >= left) break;
+                U aside{};
+                bool held = false;
+#pragma unroll 1
+                for (int k = 0; k < n; ++k) {
+                    const int d = moves.to[k], f = moves.from[k];
+                    const U* src = f == kAside ? nullptr : place(q, f);
+                    U* dst = d == kAside ? nullptr : place(q, d);
+                    if (d == kAside) {
+                        held = src != nullptr;
+                        if (held) aside = *src;
+                    } else if (f == kAside) {
+                        if (held && dst != nullptr) *dst = aside;
+                    } else if (src != nullptr && dst != nullptr) {
+                        *dst = *src;
+                    }
+                }
+            }
+            continue;
+        }
+        for (int k0 = 0; k0 < n; k0 += 2) {
+            U v[2][kDeep];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (k0 + k < n) {
+#pragma unroll
+                    for (int q = 0; q < kDeep; ++q) {
+                        const U* src = place(q, moves.from[k0 + k]);
+                        if (q < left && (!PAGED || src != nullptr)) v[k][q] = *src;
+                    }
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (to[k] != nullptr) *to[k] = v[k];
+            for (int k = 0; k < 2; ++k) {
+                if (k0 + k < n) {
+#pragma unroll
+                    for (int q = 0; q < kDeep; ++q) {
+                        U* dst = place(q, moves.to[k0 + k]);
+                        if (q < left && (!PAGED || (dst != nullptr && place(q, moves.from[k0 + k]) != nullptr))) *dst = v[k][q];
+                    }
+                }
+            }
         }
     }
 }
@@ -139,7 +177,6 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
         const int n = rows != nullptr ? (int)min(max(rows[pair], 0LL), (long long)s.rows) : s.rows;
         const unsigned per_head = (unsigned)n * (unsigned)s.per_row, per_tensor = per_head * (unsigned)s.heads;
         const unsigned total = per_tensor * (unsigned)t.n;
-        constexpr int kDeep = 4;
         for (unsigned i0 = blockIdx.x * (kThreads * kDeep) + threadIdx.x; i0 < total; i0 += gridDim.x * (kThreads * kDeep)) {
             U v[kDeep];
             U* at[kDeep];
@@ -169,9 +206,17 @@ int unit_of(void* const* base, int n, long long row_bytes, long long line_stride
     return (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : (all & 1) == 0 ? 2 : 1;
 }
 
-// Blocks beside each other for one group or pair: what its units can use, and no more than fill the GPU.
+template <typename U>
+void launch_reorder(dim3 grid, cudaStream_t st, const Tensors& t, const Shape& s, int W, const long long* parents, const long long* start,
+                    const long long* end, const int* table, int page_size, int max_pages, int num_pages) {
+    if (table == nullptr) reorder_lines_kernel<U, false><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+    else reorder_lines_kernel<U, true><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+}
+
+// Blocks beside each other for one group or pair: what its units can use, up to four waves.  (16 layers, 32 lines of 900 rows: one wave 136 us, two 130,
+// four 124, sixteen 121; but a block without work costs its start, and the host does not know the ranges.)
 unsigned blocks_for(long long units, long long per_block, long long beside) {
-    const long long want = (units + per_block - 1) / per_block, room = (8LL * nxd_num_sms() + beside - 1) / beside;
+    const long long want = (units + per_block - 1) / per_block, room = (16LL * nxd_num_sms() + beside - 1) / beside;
     const long long least = nxd_num_sms();
     return (unsigned)(want < room ? want : room < least ? (want < least ? want : least) : room);
 }
@@ -197,12 +242,12 @@ NXD_API int nxd_reorder_lines(void* const* base, int n, int heads, long long row
         t.n = n - at < most ? n - at : most;
         for (int i = 0; i < kMaxTensors; ++i) t.base[i] = i < t.n ? (char*)base[at + i] : nullptr;
         const Shape s = {heads, (int)rows, (int)per_row, line_stride, head_stride};
-        const dim3 grid(blocks_for(per_tensor * t.n, kThreads, groups), groups);
+        const dim3 grid(blocks_for(per_tensor * t.n, kThreads * kDeep, groups), groups);
         cudaStream_t st = (cudaStream_t)stream;
-        if (unit == 16) reorder_lines_kernel<uint4><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-        else if (unit == 4) reorder_lines_kernel<uint32_t><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-        else if (unit == 2) reorder_lines_kernel<uint16_t><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-        else reorder_lines_kernel<uint8_t><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        if (unit == 16) launch_reorder<uint4>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        else if (unit == 4) launch_reorder<uint32_t>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        else if (unit == 2) launch_reorder<uint16_t>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
+        else launch_reorder<uint8_t>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
         NXD_LAUNCH_CHECK();
     }
     return 0;

@@ -125,10 +125,11 @@ int nxd_beam_advance(const float* cand_scores, const long long* cand_beams, cons
                      const unsigned char* done, float norm, long long eos, long long pad, int early_stopping, int length,
                      float* out_running, long long* out_tokens, long long* out_parents, float* out_pool_scores, int* out_pool_lengths,
                      int* out_pool_slots, unsigned char* out_done, int* hist_tokens, int* hist_parents, void* stream);
-/* the best W hypotheses of every group: tokens [B, W, step], lengths and scores [B, W]; history [>= step, B, W] */
+/* the best W hypotheses of every group: tokens [B, W, step], lengths and scores [B, W]; history [>= step, B, W].  Scratch in bytes, 0: none */
+long long nxd_beam_finish_scratch(int B, int W, int step);
 int nxd_beam_finish(const float* running, const float* pool_scores, const int* pool_lengths, const int* pool_slots, const unsigned char* done,
                     int B, int W, int step, float norm, long long eos, long long pad, const int* hist_tokens, const int* hist_parents,
-                    long long* tokens, long long* lengths, float* scores, void* stream);
+                    long long* tokens, long long* lengths, float* scores, void* scratch, void* stream);
 
 /* ---- cache lines and pages (csrc/kv_lines.cu) -------------------------------------------------------
  * n tensors of one shape at `base` (a HOST array of device addresses), strides and rows in bytes.  reorder: line g * W + w becomes what line

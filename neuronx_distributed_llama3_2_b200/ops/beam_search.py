@@ -20,7 +20,8 @@ _ARGS = {
     "nxd_beam_select_scratch": [_I] * 5,
     "nxd_beam_select": [_I, _P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
     "nxd_beam_advance": [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _F, _L, _L, _I, _I] + [_P] * 10,
-    "nxd_beam_finish": [_P, _P, _P, _P, _P, _I, _I, _I, _F, _L, _L] + [_P] * 6,
+    "nxd_beam_finish_scratch": [_I] * 3,
+    "nxd_beam_finish": [_P, _P, _P, _P, _P, _I, _I, _I, _F, _L, _L] + [_P] * 7,
 }
 
 
@@ -273,13 +274,18 @@ def beam_finish(scores: torch.Tensor, pool: BeamPool, history: BeamHistory, step
     norm = _norm(step, length_penalty)
     if not _kernel(scores):
         return _finish_ref(scores, pool, history, step, norm, eos, pad)
+    if B > 65535:
+        raise ValueError(f"{B} requests are more than 65535")
     tokens = torch.empty((B, W, step), dtype=torch.int64, device=dev)
     lengths = torch.empty((B, W), dtype=torch.int64, device=dev)
     best = torch.empty((B, W), dtype=torch.float32, device=dev)
     with _lib.on_device_of(scores):
+        scratch = None
+        if W * step > 2 ** 16:          # lines of many steps do not fit shared memory
+            scratch = torch.empty(_entry("nxd_beam_finish_scratch")(B, W, step), dtype=torch.uint8, device=dev)
         rc = _entry("nxd_beam_finish")(scores.data_ptr(), pool.scores.data_ptr(), pool.lengths.data_ptr(), pool.slots.data_ptr(),
                                        pool.done.data_ptr(), B, W, step, norm, eos, pad, history.tokens.data_ptr(), history.parents.data_ptr(),
-                                       tokens.data_ptr(), lengths.data_ptr(), best.data_ptr(), _lib.stream_ptr())
+                                       tokens.data_ptr(), lengths.data_ptr(), best.data_ptr(), 0 if scratch is None else scratch.data_ptr(), _lib.stream_ptr())
     _lib.check(rc, "nxd_beam_finish")
     return tokens, lengths, best
 

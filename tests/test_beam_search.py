@@ -306,6 +306,24 @@ def test_sequences_of_a_long_history_with_any_parents(device):
         assert lengths.tolist() == lens and tokens.tolist() == want
 
 
+# one CTA a request and clusters of them, spans whose tokens do not fit shared memory, and spans that do not fit at all
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,W,T", [(200, 3, 301), (40, 8, 1999), (1, 32, 5603), (1, 32, 27001), (3, 1, 4097), (1, 7, 127), (2, 9, 128), (1, 2, 16)])
+def test_sequences_of_many_steps(B, W, T):
+    g = torch.Generator().manual_seed(T)
+    history = bs.BeamHistory(torch.randint(3, 9999, (T, B, W), generator=g).int(), torch.randint(0, W, (T, B, W), generator=g).int())
+    held = torch.rand(B, W, generator=g).sort(1, descending=True).values < 0.5
+    held = held.flip(1)
+    scores, running = (-torch.rand(2, B, W, generator=g).sort(-1).values).unbind(0)
+    pool = bs.BeamPool(torch.where(held, scores, -INF), torch.where(held, torch.randint(1, T + 1, (B, W), generator=g), 0).int(),
+                       torch.where(held, torch.randint(0, W, (B, W), generator=g), 0).int(), torch.rand(B, generator=g) < 0.3)
+    kw = dict(eos_token_id=EOS, pad_token_id=PAD, length_penalty=0.5)
+    want = bs.beam_finish(running * T ** 0.5, pool, history, T, **kw)
+    put = lambda x: type(x)(*[t.cuda() for t in x])          # noqa: E731
+    got = bs.beam_finish((running * T ** 0.5).cuda(), put(pool), put(history), T, **kw)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
 # ---- lines and pages --------------------------------------------------------------------------------------------------
 
 def _values(shape, dtype, g, device):
