@@ -484,6 +484,63 @@ NXD_RT_API int nxd_kv_unshare(void* h, int line, int64_t pos, int* copy_src, int
     return 1;
 }
 
+// Of lines [first, first + n): the position from which on none of a line's pages is shared with another line.
+NXD_RT_API int nxd_kv_private_from(void* h, int first, int n, int64_t* out) {
+    KvPool* p = (KvPool*)h;
+    if (!p || !out || first < 0 || n < 0 || n > p->max_lines - first) return fail("kv_private_from: bad lines");
+    std::lock_guard<std::mutex> g(p->mu);
+    for (int i = 0; i < n; ++i) {
+        const std::vector<int>& pg = p->pages[first + i];
+        size_t k = pg.size();
+        while (k > 0 && p->refcnt[pg[k - 1]] <= 1) --k;
+        out[i] = (int64_t)k * p->page_size;
+    }
+    return 0;
+}
+
+// Pages in use move to the front of the pool: those with the highest numbers take the free places with the lowest.  (src[i], dst[i]) tell the caller
+// what to copy on the device, no page is in both lists.  Returns the number of pairs (at most num_pages / 2).
+NXD_RT_API int nxd_kv_compact(void* h, int* src, int* dst, int cap) {
+    KvPool* p = (KvPool*)h;
+    if (!p || !src || !dst) return fail("kv_compact: bad arguments");
+    std::lock_guard<std::mutex> g(p->mu);
+    const int used = p->num_pages - (int)p->free_list.size();
+    std::vector<int> to(p->num_pages, -1), holes;
+    for (int pg = 0; pg < used; ++pg)
+        if (p->refcnt[pg] == 0) holes.push_back(pg);
+    if ((int)holes.size() > cap) return fail("kv_compact: %d moves, room for %d", (int)holes.size(), cap);
+    int n = 0;
+    for (int pg = used; pg < p->num_pages; ++pg) {
+        if (p->refcnt[pg] == 0) continue;
+        src[n] = pg;
+        dst[n] = to[pg] = holes[n];
+        p->refcnt[holes[n]] = p->refcnt[pg];
+        p->refcnt[pg] = 0;
+        ++n;
+    }
+    for (auto& line : p->pages)
+        for (int& pg : line)
+            if (to[pg] >= 0) pg = to[pg];
+    p->free_list.clear();
+    for (int pg = p->num_pages - 1; pg >= used; --pg) p->free_list.push_back(pg);
+    return n;
+}
+
+// Another number of pages; what is behind the new end must be free.
+NXD_RT_API int nxd_kv_resize(void* h, int num_pages) {
+    KvPool* p = (KvPool*)h;
+    if (!p || num_pages <= 0) return fail("kv_resize: bad arguments");
+    std::lock_guard<std::mutex> g(p->mu);
+    for (int pg = num_pages; pg < p->num_pages; ++pg)
+        if (p->refcnt[pg] != 0) return fail("kv_resize: page %d is in use", pg);
+    p->refcnt.resize(num_pages, 0);
+    p->num_pages = num_pages;
+    p->free_list.clear();
+    for (int pg = num_pages - 1; pg >= 0; --pg)
+        if (p->refcnt[pg] == 0) p->free_list.push_back(pg);
+    return 0;
+}
+
 // Block-table row of `line` into out[max_pages]; unused slots get `fill` (a valid page id keeps kernels in bounds).
 NXD_RT_API int nxd_kv_block_row(void* h, int line, int32_t* out, int fill) {
     KvPool* p = (KvPool*)h;

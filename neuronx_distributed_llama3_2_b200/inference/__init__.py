@@ -2,7 +2,8 @@
 ``src/neuronx_distributed/trace/__init__.py:1-7`` + ``examples/inference``)."""
 from .checkpoint_sharding import _mock_parallel_state, get_sharded_checkpoint, shard_children  # noqa: F401
 from .config import InferenceConfig  # noqa: F401
-from .kv_cache import KVCache  # noqa: F401
+from .kv_cache import BeamLines, KVCache  # noqa: F401
+from .beam_search import BeamSearch  # noqa: F401
 from .model import (DbrxInferenceModel, GekazenInferenceModel, KVCacheInferenceMixin, LlamaInferenceModel,  # noqa: F401
                     MixtralInferenceModel)
 from .hybrid import (GogalixInferenceModel, MumazenInferenceModel, RasodraInferenceModel, TidavikInferenceModel,  # noqa: F401

@@ -33,12 +33,18 @@ class InferenceConfig:
     paged_kv: bool = False
     page_size: int = 128
     num_kv_pages: Optional[int] = None      # paged cache: size of the page pool (default: lines * pages per line)
+    num_beams: int = 1                      # > 1: generate() searches with that many beams (1 to 32) per sequence
+    length_penalty: float = 1.0             # beams are ranked by summed log-probability / length ** length_penalty
+    early_stopping: bool = False            # a beam search ends as soon as it has num_beams finished sequences
     pad_token_id: int = 0
     eos_token_id: Optional[int] = None
 
     def __post_init__(self):
         self.ctx_batch_size = self.ctx_batch_size or self.batch_size
-        self.tkg_batch_size = self.tkg_batch_size or self.batch_size
+        if not 1 <= self.num_beams <= 32:
+            raise ValueError(f"num_beams has to be between 1 and 32, not {self.num_beams}")
+        # token generation runs every beam of every sequence
+        self.tkg_batch_size = self.tkg_batch_size or self.batch_size * self.num_beams
         self.max_batch_size = self.max_batch_size or max(self.ctx_batch_size, self.tkg_batch_size)
         if self.max_context_length > self.seq_len:
             raise ValueError("max_context_length cannot exceed seq_len")

@@ -25,9 +25,11 @@ sequence at position 0 starts from zero by itself, so a line that is handed out 
 """
 from __future__ import annotations
 
-from typing import Dict, Iterable, List, Optional, Tuple
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 import torch
+
+from ..ops.kv_lines import CacheTensors, copy_pages_, reorder_lines_
 
 
 class KVCache:
@@ -44,6 +46,7 @@ class KVCache:
         specs = layer_specs if layer_specs is not None else [(kv_heads, head_dim, head_dim)] * num_layers
         self.paged, self.page_size = paged, page_size
         self.pool = None
+        self._laid_out: Optional[CacheTensors] = None
         if paged:
             self.max_pages = (seq_len + page_size - 1) // page_size
             if num_pages is None:
@@ -139,19 +142,85 @@ class KVCache:
         if self.pool is not None and self.pool.truncate(line, n_tokens) > 0:
             self.sync_lines([line])
 
-    def _copy_page(self, src: int, dst: int) -> None:
-        for t in self._tensors():
-            t[dst].copy_(t[src])
+    @property
+    def tensors(self) -> CacheTensors:
+        """The cache's tensors, laid out for the kernels that move lines and pages of all layers at once."""
+        if self._laid_out is None:
+            self._laid_out = CacheTensors(self._tensors(), self._state_tensors())
+        return self._laid_out
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int], rows: Optional[Sequence[int]] = None) -> None:
+        """Page ``dst[i]`` becomes page ``src[i]`` in every layer (its first ``rows[i]`` rows); no page may be in both lists."""
+        assert self.paged, "a contiguous cache has no pages"
+        if len(src):
+            copy_pages_(self.tensors, src, dst, rows=rows)
 
     def fork(self, src: int, dst: int) -> None:
         """``dst`` continues from ``src``'s content: full pages shared, the partial last page copied."""
+        self.fork_lines(src, [dst])
+
+    def fork_lines(self, src: int, dsts: Sequence[int], whole_pages: bool = True) -> None:
+        """Every line of ``dsts`` continues from ``src``'s content: full pages are shared, the partial last page is copied for all of them in one
+        launch (with ``whole_pages`` false only the rows of the reserved tokens).  If the pool has not enough pages no line is forked."""
         assert self.pool is not None, "fork needs the dynamic page pool (num_pages=...)"
-        copy = self.pool.fork(src, dst)
-        if copy is not None:
-            self._copy_page(*copy)
-        for t in self._state_tensors():
-            t[dst].copy_(t[src])
-        self.sync_lines([dst])
+        dsts, copies, forked = list(dsts), [], []
+        try:
+            for dst in dsts:
+                copy = self.pool.fork(src, dst)
+                forked.append(dst)
+                if copy is not None:
+                    copies.append(copy)
+        except MemoryError:
+            for dst in forked:
+                self.pool.free_line(dst)
+            raise
+        rows = None if whole_pages else [self.pool.line_tokens(src) % self.page_size] * len(copies)
+        self.copy_pages([a for a, _ in copies], [b for _, b in copies], rows)
+        for t in self._state_tensors() if dsts else ():
+            t[dsts] = t[src].clone()
+        self.sync_lines(dsts)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool, on the device in one launch a layer shape; the number of pages in use."""
+        assert self.pool is not None, "compact needs the dynamic page pool (num_pages=...)"
+        moves = self.pool.compact()
+        self.copy_pages([a for a, _ in moves], [b for _, b in moves])
+        self.sync_lines(range(self.lines))
+        return self.pool.num_pages - self.pool.num_free
+
+    def resize_pool(self, num_pages: int) -> None:
+        """A pool of another size: the pages in use move to the front and into new tensors, the old ones are let go.  ``MemoryError`` if more are in
+        use.  What holds the old tensors (a captured graph, ``BeamLines``) has to be made again."""
+        used = self.compact()
+        if used > num_pages or num_pages < 1:
+            raise MemoryError(f"{used} pages are in use, {num_pages} are not enough")
+        self.pool.resize(num_pages)
+        self._laid_out = None
+        for i, k in enumerate(self.k):
+            if k is None:
+                continue
+            v, columns = self.v[i], self.v[i]._base is not None
+            self.k[i] = self._resized(k, num_pages, used)
+            self.v[i] = self.k[i][..., : v.shape[-1]] if columns else self._resized(v, num_pages, used)
+
+    @staticmethod
+    def _resized(t: torch.Tensor, num_pages: int, used: int) -> torch.Tensor:
+        new = torch.zeros((num_pages,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device)
+        new[:used] = t[:used]
+        return new
+
+    def reorder_lines(self, parents: torch.Tensor, start: Optional[torch.Tensor] = None, end: Optional[torch.Tensor] = None) -> None:
+        """Line ``b * W + w`` becomes what line ``b * W + parents[b, w]`` was (``parents [B, W]``): rows ``[start[b], end[b])`` of every layer, and its
+        recurrent state.  With a dynamic pool ``end`` has to be given, within what the lines have reserved, and pages that hold these rows must not
+        be shared (``BeamLines`` sees to both)."""
+        if self.pool is not None and end is None:
+            raise ValueError("end: the rows of a dynamic pool end where the lines' reservations do")
+        reorder_lines_(self.tensors, parents, start, end, block_table=self.block_table, page_size=self.page_size if self.paged else 0)
+
+    def beams(self, lengths: Sequence[int], width: int, new_tokens: int = 0) -> "BeamLines":
+        """Lines ``b * width`` hold prompts of ``lengths[b]`` tokens: the ``width`` lines of each request continue it, with room for ``new_tokens``
+        more."""
+        return BeamLines(self, lengths, width, new_tokens)
 
     def prepare_write(self, line: int, pos: int) -> None:
         """Before writing position ``pos`` of ``line``: give the line a private copy of that page if it is shared."""
@@ -159,8 +228,52 @@ class KVCache:
             return
         copy = self.pool.unshare(line, pos)
         if copy is not None:
-            self._copy_page(*copy)
+            self.copy_pages([copy[0]], [copy[1]])
             self.sync_lines([line])
 
     def bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self._tensors() + self._state_tensors())
+
+
+class BeamLines:
+    """The cache lines of a beam search: line ``b * width + w`` is beam ``w`` of request ``b``.  A prompt is computed once, on its request's first
+    line, and spread over the others here: shared pages with a dynamic pool (the beams' own rows are private), copied rows otherwise.  ``reorder`` then
+    moves only what lies behind the prompts."""
+
+    def __init__(self, cache: KVCache, lengths: Sequence[int], width: int, new_tokens: int = 0):
+        lengths = [int(n) for n in lengths]
+        if not lengths or not 1 <= width <= 32 or len(lengths) * width > cache.lines:
+            raise ValueError(f"{len(lengths)} requests of {width} beams: between 1 and 32 beams, {cache.lines} cache lines")
+        if min(lengths) < 0 or new_tokens < 0 or max(lengths) + new_tokens > cache.seq_len:
+            raise ValueError(f"prompts of up to {max(lengths)} tokens and {new_tokens} more do not fit a cache of {cache.seq_len}")
+        self.cache, self.lengths, self.width = cache, lengths, width
+        device = next(t.device for t in cache._tensors() + cache._state_tensors())
+        self.start = torch.tensor(lengths, dtype=torch.int64, device=device)
+        self.limit = self.start + new_tokens
+        lines = range(len(lengths) * width)
+        if cache.pool is None:
+            if width > 1:
+                cache.reorder_lines(torch.zeros(len(lengths), width, dtype=torch.int64, device=device), None, self.start)
+            return
+        for b, n in enumerate(lengths):
+            if cache.pool.line_tokens(b * width) < n:
+                raise ValueError(f"line {b * width} has room for {cache.pool.line_tokens(b * width)} tokens, its prompt has {n}")
+        for line in lines:
+            if line % width:
+                cache.free(line)
+        for b, n in enumerate(lengths):
+            cache.truncate(b * width, n)
+            cache.fork_lines(b * width, range(b * width + 1, (b + 1) * width), whole_pages=False)
+        for line in lines:
+            cache.pool.reserve(line, lengths[line // width] + new_tokens)
+        cache.sync_lines(lines)
+
+    def reorder(self, parents: torch.Tensor, end: Optional[torch.Tensor] = None) -> None:
+        """Beam ``w`` of request ``b`` continues its beam ``parents[b, w]``; ``end [B]``: the rows that have been written."""
+        if self.cache.pool is not None:
+            private = self.cache.pool.private_from(0, len(self.lengths) * self.width)
+            shared = [i for i, at in enumerate(private) if at > self.lengths[i // self.width]]
+            if shared:
+                raise ValueError(f"line {shared[0]} shares pages behind its prompt with another line")
+            end = self.limit if end is None else torch.minimum(end, self.limit)          # behind it the table names other lines' pages
+        self.cache.reorder_lines(parents, self.start, end)

@@ -102,8 +102,8 @@ def medusa_generate(model, prompt: torch.Tensor, max_new_tokens: int, medusa_cho
     while len(out) < max_new_tokens:
         cands, _ = generate_candidates(heads[: depth1 - 1], base, tree_indices, retrieve, topk=topk)   # [paths, depth+1]
         cache.truncate(main, cur)                                        # the allocator's length = the accepted prefix
-        for line in scratch:                                             # every path continues from the accepted prefix
-            cache.fork(main, line)
+        cache.fork_lines(main, scratch)                                  # every path continues from the accepted prefix
+        for line in scratch:
             cache.reserve(line, cur + depth1)
         lines = torch.tensor(scratch, dtype=torch.int32, device=dev)
         ppos = (cur + torch.arange(depth1, device=dev)).unsqueeze(0).expand(n_paths, depth1).contiguous()

@@ -597,6 +597,53 @@ class KVCacheInferenceMixin:
         return res
 
 
+    def forward_logits(self, input_ids: torch.Tensor, position_ids: torch.Tensor, seq_ids: Optional[torch.Tensor] = None,
+                       last_token_index: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One graph without the sampler: the logits ``[B, V]`` that a beam search chooses from."""
+        return self.forward_infer(input_ids, position_ids, seq_ids, last_token_index, return_logits=True, sample=False)[1]
+
+    @torch.no_grad()
+    def generate_beams(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None, num_beams: int = 4,
+                       max_new_tokens: int = 16, eos_token_id: Optional[int] = None, length_penalty: float = 1.0,
+                       early_stopping: bool = False, num_return_sequences: int = 1, return_scores: bool = False):
+        """Beam search over right-padded prompts ``[B, T]``: the best ``num_return_sequences`` continuations of each, the best first,
+        ``[B * num_return_sequences, T + new]`` (and their scores).  Needs ``B * num_beams`` cache lines."""
+        from .beam_search import BeamSearch, search, sequences
+
+        ic = self.inference_config
+        B, T = input_ids.shape
+        dev = input_ids.device
+        if self.kv_cache is None:
+            self.init_kv_cache(device=dev)
+        cache, W = self.kv_cache, num_beams
+        if not 1 <= num_return_sequences <= W:
+            raise ValueError(f"{num_return_sequences} sequences of {W} beams")
+        if B * W > cache.lines:
+            raise ValueError(f"{B} sequences of {W} beams need {B * W} cache lines, the cache has {cache.lines} (max_batch_size)")
+        if attention_mask is None:
+            attention_mask = torch.ones_like(input_ids)
+        lens = attention_mask.sum(dim=1).to(torch.long)
+        lengths = lens.tolist()
+        if min(lengths) < 1 or max(T, max(lengths) + max_new_tokens - 1) > cache.seq_len:
+            raise ValueError(f"prompts of {min(lengths)} to {max(lengths)} tokens (padded to {T}) and {max_new_tokens} more do not fit a cache of "
+                             f"{cache.seq_len}")
+        found = BeamSearch(B, W, max_new_tokens, eos_token_id=eos_token_id, pad_token_id=ic.pad_token_id, length_penalty=length_penalty,
+                           early_stopping=early_stopping, device=dev)
+        ids = input_ids if T > 1 else torch.nn.functional.pad(input_ids, (0, 1), value=ic.pad_token_id)      # one token is a step of generation
+        if cache.pool is not None:
+            for line in range(B * W):
+                cache.free(line)
+            for b in range(B):
+                cache.reserve(b * W, min(ids.shape[1], cache.seq_len))
+        pos = torch.arange(ids.shape[1], device=dev).unsqueeze(0).expand(B, -1)
+        logits = self.forward_logits(ids, pos, torch.arange(0, B * W, W, dtype=torch.int32, device=dev), lens - 1)
+        rows = torch.arange(B * W, dtype=torch.int32, device=dev)
+        result = search(found, cache, lengths, logits, lambda tok, at: self.forward_logits(tok.reshape(-1, 1), at.reshape(-1, 1), rows))
+        self.check_steps()
+        out = sequences(input_ids, lengths, result, num_return_sequences, ic.pad_token_id)
+        return (out, result[2][:, :num_return_sequences].reshape(-1)) if return_scores else out
+
+
 class LlamaInferenceModel(KVCacheInferenceMixin, LlamaForCausalLM):
     def __init__(self, config: LlamaConfig, inference_config: Optional[InferenceConfig] = None, device=None):
         config.sequence_parallel_enabled = False

@@ -107,7 +107,8 @@ class InferenceRunner:
         ic = self.config
         builder = ModelBuilder(tp_degree=ic.tp_degree, checkpoint_loader=self.checkpoint_loader,
                                use_cuda_graphs=ic.use_cuda_graphs and self.device.type == "cuda")
-        inst = BaseModelInstance(self._make_module)
+        # a beam search chooses from the logits of all beams itself
+        inst = BaseModelInstance(self._make_module, forward_method="forward_logits" if ic.num_beams > 1 else None)
         dev = self.device
 
         def ex(b, t):
@@ -178,6 +179,8 @@ class InferenceRunner:
         """Right-padded prompts ``[B, T]`` (B <= compiled batch) -> ``[B, T + new]`` token ids."""
         assert self.nxd_model is not None, "call trace() first"
         ic, dev = self.config, self.device
+        if ic.num_beams > 1:
+            return self.generate_beams(input_ids, attention_mask, max_new_tokens, collectors=collectors)
         max_new = max_new_tokens or ic.max_new_tokens
         B, T = input_ids.shape
         if attention_mask is None:
@@ -230,6 +233,70 @@ class InferenceRunner:
         return res
 
     @torch.no_grad()
+    def generate_beams(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
+                       max_new_tokens: Optional[int] = None, num_return_sequences: int = 1, return_scores: bool = False,
+                       collectors: Optional[Dict[str, LatencyCollector]] = None):
+        """Beam search with the traced graphs (``InferenceConfig.num_beams`` > 1, ``length_penalty``, ``early_stopping``): the best
+        ``num_return_sequences`` continuations of every prompt, the best first, ``[B * num_return_sequences, T + new]`` (and their scores)."""
+        from .beam_search import BeamSearch, search, sequences
+
+        ic, dev = self.config, self.device
+        assert self.nxd_model is not None and ic.num_beams > 1, "trace() with InferenceConfig(num_beams=W) first"
+        max_new = max_new_tokens or ic.max_new_tokens
+        (B, T), W, Bc, Bt = input_ids.shape, ic.num_beams, ic.ctx_batch_size, ic.tkg_batch_size
+        cache = self.model.kv_cache
+        if not 1 <= num_return_sequences <= W:
+            raise ValueError(f"{num_return_sequences} sequences of {W} beams")
+        if B > Bc or Bc * W > cache.lines or B * W > Bt:
+            raise ValueError(f"{B} prompts (compiled for {Bc}) of {W} beams: token generation is compiled for {Bt} rows, the cache has {cache.lines} lines")
+        if attention_mask is None:
+            attention_mask = torch.ones_like(input_ids)
+        lens = attention_mask.sum(dim=1).to(torch.long)
+        lengths = lens.tolist()
+        Tb = self._bucket_len(T)
+        if Tb < 2 or min(lengths) < 1 or max(lengths) + max_new - 1 > ic.seq_len:
+            raise ValueError(f"prompts of {min(lengths)} to {max(lengths)} tokens (bucket {Tb}) and {max_new} more do not fit a cache of {ic.seq_len}")
+        if cache.pool is not None:
+            for line in range(cache.lines):
+                cache.free(line)
+            for b in range(Bc):
+                cache.reserve(b * W, Tb)
+            for line in range(B * W, Bt):          # of rows without a beam
+                cache.reserve(line, 1)
+        ids = torch.full((Bc, Tb), ic.pad_token_id, dtype=torch.long, device=dev)
+        ids[:B, :T] = input_ids.to(dev)
+        pos = torch.arange(Tb, device=dev).unsqueeze(0).expand(Bc, Tb).contiguous()
+        last = torch.zeros(Bc, dtype=torch.long, device=dev)
+        last[:B] = lens.to(dev) - 1
+        cte = collectors.get(CONTEXT_ENCODING_MODEL) if collectors else None
+        tkg = collectors.get(TOKEN_GENERATION_MODEL) if collectors else None
+        if cte:
+            cte.pre_hook()
+        logits = self.nxd_model(ids, pos, torch.arange(0, Bc * W, W, dtype=torch.int32, device=dev), last)
+        if cte:
+            cte.hook()
+        # rows without a beam write their key and value at position 0 of lines that no beam has
+        step_ids = torch.zeros(Bt, 1, dtype=torch.long, device=dev)
+        at = torch.zeros(Bt, 1, dtype=torch.long, device=dev)
+        seq, zero = torch.arange(Bt, dtype=torch.int32, device=dev), torch.zeros(Bt, dtype=torch.long, device=dev)
+
+        def step(tokens: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+            step_ids[:B * W, 0], at[:B * W, 0] = tokens, positions
+            if tkg:
+                tkg.pre_hook()
+            out = self.nxd_model(step_ids, at, seq, zero)
+            if tkg:
+                tkg.hook()
+            return out[:B * W]
+
+        found = BeamSearch(B, W, max_new, eos_token_id=ic.eos_token_id, pad_token_id=ic.pad_token_id, length_penalty=ic.length_penalty,
+                           early_stopping=ic.early_stopping, device=dev)
+        result = search(found, cache, lengths, logits[:B], step, check=lambda: self._check_steps(wait=False))
+        self._check_steps()
+        out = sequences(input_ids, lengths, result, num_return_sequences, ic.pad_token_id)
+        return (out, result[2][:, :num_return_sequences].reshape(-1)) if return_scores else out
+
+    @torch.no_grad()
     def generate_speculative(self, draft: "InferenceRunner", input_ids: torch.Tensor,
                              max_new_tokens: Optional[int] = None) -> torch.Tensor:
         """Assisted decoding (reference ``run_llama_speculative.py`` / ``utils/speculative_decoding.py``): ``draft`` proposes
@@ -239,6 +306,7 @@ class InferenceRunner:
 
         ic, dev = self.config, self.device
         assert ic.speculation_length > 0, "trace the target with InferenceConfig(speculation_length=k)"
+        assert ic.num_beams == 1 and draft.config.num_beams == 1, "assisted decoding has one sequence, not beams"
         assert input_ids.shape[0] == 1 and ic.tkg_batch_size == 1 and draft.config.tkg_batch_size == 1
         max_new = max_new_tokens or ic.max_new_tokens
         T = input_ids.shape[1]

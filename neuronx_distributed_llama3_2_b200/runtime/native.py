@@ -76,6 +76,9 @@ def lib() -> C.CDLL:
             L.nxd_kv_fork.argtypes = [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int)]
             L.nxd_kv_page_shared.argtypes = [C.c_void_p, C.c_int, C.c_int64]
             L.nxd_kv_unshare.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.POINTER(C.c_int), C.POINTER(C.c_int)]
+            L.nxd_kv_private_from.argtypes = [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int64)]
+            L.nxd_kv_compact.argtypes = [C.c_void_p, C.POINTER(C.c_int), C.POINTER(C.c_int), C.c_int]
+            L.nxd_kv_resize.argtypes = [C.c_void_p, C.c_int]
             L.nxd_kv_block_row.argtypes = [C.c_void_p, C.c_int, C.POINTER(C.c_int32), C.c_int]
             L.nxd_sched_create.restype = C.c_void_p
             L.nxd_sched_create.argtypes = [C.c_void_p, C.c_int]
@@ -258,6 +261,28 @@ class PagedKVPool:
         if lib().nxd_kv_unshare(self._h, line, pos, C.byref(a), C.byref(b)) < 0:
             raise MemoryError(_err())
         return (a.value, b.value) if a.value >= 0 else None
+
+    def private_from(self, first: int, n: int) -> List[int]:
+        """Of lines ``[first, first + n)``: the position from which on none of a line's pages is shared."""
+        out = (C.c_int64 * max(n, 1))()
+        if lib().nxd_kv_private_from(self._h, first, n, out) != 0:
+            raise ValueError(_err())
+        return list(out)[:n]
+
+    def compact(self) -> List[Tuple[int, int]]:
+        """Moves the pages in use to the front of the pool; ``(src, dst)`` pages to copy on the device, none of them in both places."""
+        cap = self.num_pages // 2 + 1
+        src, dst = (C.c_int * cap)(), (C.c_int * cap)()
+        n = lib().nxd_kv_compact(self._h, src, dst, cap)
+        if n < 0:
+            raise ValueError(_err())
+        return list(zip(src[:n], dst[:n]))
+
+    def resize(self, num_pages: int) -> None:
+        """Another number of pages; ``ValueError`` if one behind the new end is in use (``compact`` first)."""
+        if lib().nxd_kv_resize(self._h, num_pages) != 0:
+            raise ValueError(_err())
+        self.num_pages = num_pages
 
     def block_row(self, line: int, fill: int = 0) -> Tuple[List[int], int]:
         buf = (C.c_int32 * self.max_pages)()

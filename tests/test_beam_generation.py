@@ -1,0 +1,309 @@
+"""Beam search through the models' caches: every kind of cache against a search that computes all sequences anew with the training model, the
+cache's lines and pages, and the runner with its graphs."""
+import importlib
+import math
+
+import pytest
+import torch
+
+from neuronx_distributed_llama3_2_b200.inference import BeamLines, InferenceConfig, InferenceRunner, KVCache, LlamaInferenceModel
+from neuronx_distributed_llama3_2_b200.models import LlamaForCausalLM, tiny_llama
+from test_beam_search import DEVICES, _Request
+import test_beam_search as units
+
+INF = math.inf
+
+
+def _models(monkeypatch, **kw):
+    torch.manual_seed(0)
+    cfg = tiny_llama(sequence_parallel_enabled=False)
+    train = LlamaForCausalLM(cfg)
+    with torch.no_grad():          # peaked enough that beams differ, with an end that is met now and then
+        train.lm_head.weight.mul_(6.0)
+    inf = LlamaInferenceModel(tiny_llama(sequence_parallel_enabled=False), InferenceConfig(max_context_length=32, seq_len=64, page_size=8, **kw))
+    inf.load_state_dict(train.state_dict())
+    return cfg, train, inf
+
+
+def _searched(logits_of, prompt, W, steps, eos, penalty, early):
+    """The sequences and scores of a search that starts over for every beam and step; ``logits_of(sequences) -> [n, V]``."""
+    r = _Request(W, penalty, early)
+    for _ in range(steps):
+        if r.done:
+            break
+        live = [(i, s, h) for i, (s, h) in enumerate(r.beams) if s > -INF]
+        logp = torch.log_softmax(logits_of([prompt + h for _, _, h in live]).double(), -1)
+        cands = [(units._fp32(s + lp), i, v) for (i, s, _), row in zip(live, logp.tolist()) for v, lp in enumerate(row)]
+        cands.sort(key=lambda c: (-c[0], c[1], c[2]))
+        r.step(cands[:2 * W])
+    n = len(r.beams[0][1])
+    return r.finish(n)
+
+
+def _train_logits(train):
+    def logits_of(seqs):
+        with torch.no_grad():
+            return train(torch.tensor(seqs)).transpose(0, 1)[:, -1]
+    return logits_of
+
+
+@pytest.mark.parametrize("kind", ["contiguous", "paged", "pool", "continuous"])
+@pytest.mark.parametrize("W,steps,penalty,early", [(1, 6, 1.0, False), (3, 12, 1.0, False), (4, 10, 0.3, True), (5, 7, 2.0, False)])
+def test_beams_equal_a_search_without_a_cache(monkeypatch, kind, W, steps, penalty, early):
+    monkeypatch.setattr(units, "EOS", 17)
+    cache = {"contiguous": {}, "paged": dict(paged_kv=True), "pool": dict(paged_kv=True, num_kv_pages=60),
+             "continuous": dict(paged_kv=True, num_kv_pages=60, is_continuous_batching=True)}[kind]
+    cfg, train, inf = _models(monkeypatch, batch_size=2, max_batch_size=2 * W + 1, **cache)
+    with torch.no_grad():
+        train.lm_head.weight[17] *= 1.3
+        inf.lm_head.weight[17] *= 1.3
+    prompts = torch.randint(20, cfg.vocab_size, (2, 17))
+    mask = torch.ones_like(prompts)
+    mask[1, 8:] = 0                      # a prompt that ends with a page, one that does not
+    ended = 0
+    for again in range(2):               # lines that an earlier search has left
+        out, scores = inf.generate_beams(prompts, mask, num_beams=W, max_new_tokens=steps, eos_token_id=17, length_penalty=penalty, early_stopping=early,
+                                         num_return_sequences=W, return_scores=True)
+        for b in range(2):
+            L = int(mask[b].sum())
+            want = _searched(_train_logits(train), prompts[b, :L].tolist(), W, steps, 17, penalty, early)
+            for i, (s, h) in enumerate(want):
+                row = out[b * W + i]
+                assert row[:L].tolist() == prompts[b, :L].tolist() and row[L:L + len(h)].tolist() == h, (b, i)
+                assert int((row[L + len(h):] != 0).sum()) == 0
+                assert abs(float(scores[b * W + i]) - s) <= 1e-4 * abs(s)          # fp32 logits of two orders of summation, sums of a dozen
+                ended += h[-1] == 17
+        prompts = prompts.flip(0)
+        mask = mask.flip(0)
+    assert inf.kv_cache.pool is None or inf.kv_cache.pool.num_free > 0
+
+
+def test_one_token_prompts_and_no_end(monkeypatch):
+    monkeypatch.setattr(units, "EOS", -5)
+    cfg, train, inf = _models(monkeypatch, batch_size=1, max_batch_size=3)
+    prompt = torch.tensor([[77]])
+    out = inf.generate_beams(prompt, num_beams=3, max_new_tokens=5)
+    assert out[0].tolist() == [77] + _searched(_train_logits(train), [77], 3, 5, -5, 1.0, False)[0][1]
+    greedy = inf.generate_beams(prompt, num_beams=1, max_new_tokens=5)
+    assert torch.equal(greedy, inf.generate(prompt, max_new_tokens=5))
+
+
+def test_generation_refused(monkeypatch):
+    cfg, train, inf = _models(monkeypatch, batch_size=1, max_batch_size=4)
+    ids = torch.randint(1, 100, (2, 10))
+    for kw in (dict(num_beams=3), dict(num_beams=2, max_new_tokens=56), dict(num_beams=2, num_return_sequences=3), dict(num_beams=0),
+               dict(num_beams=2, attention_mask=torch.zeros_like(ids)), dict(num_beams=2, max_new_tokens=0)):
+        with pytest.raises(ValueError):
+            inf.generate_beams(ids, **kw)
+    with pytest.raises(ValueError):
+        InferenceConfig(num_beams=33)
+
+
+# recurrent state, short convolutions, latent columns and layers that share keys next to plain keys and values
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("family,pages", [("rasodra", None), ("rasodra", 90), ("gogalix", None), ("gogalix", 90)])
+def test_beams_of_recurrent_families(monkeypatch, family, pages, dev):
+    monkeypatch.setattr(units, "EOS", 3)
+    F = importlib.import_module(f"test_{family}")
+    W, steps, cfg = 4, 9, F.config()
+    model, sd = F.build(cfg, dev, torch.float32, lines=2 * W, paged=pages is not None, pages=pages)
+    other, _ = F.build(cfg, dev, torch.float32, lines=W, sd=sd)
+
+    def logits_of(seqs):
+        ids = torch.tensor(seqs, device=dev)
+        pos = torch.arange(ids.shape[1], device=dev).expand_as(ids)
+        return other.forward_infer(ids, pos, return_logits=True, sample=False)[1].float().cpu()
+
+    prompts = torch.tensor([F.tokens_of(cfg, 14, 1), F.tokens_of(cfg, 14, 2)], device=dev)
+    mask = torch.ones_like(prompts)
+    mask[0, 11:] = 0
+    out, scores = model.generate_beams(prompts, mask, num_beams=W, max_new_tokens=steps, eos_token_id=3, num_return_sequences=W, return_scores=True)
+    for b in range(2):
+        L = int(mask[b].sum())
+        for i, (s, h) in enumerate(_searched(logits_of, prompts[b, :L].tolist(), W, steps, 3, 1.0, False)):
+            assert out[b * W + i, L:L + len(h)].tolist() == h, (b, i)
+            assert abs(float(scores[b * W + i]) - s) <= 2e-3 * abs(s)          # the families' own bound between prompts and single tokens
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_the_runner_searches_with_its_buckets(monkeypatch, paged):
+    monkeypatch.setattr(units, "EOS", 17)
+    cfg, train, _ = _models(monkeypatch, batch_size=1)
+    with torch.no_grad():
+        train.lm_head.weight[17] *= 1.3
+    W, extra = 3, dict(paged_kv=True, page_size=8, num_kv_pages=80) if paged else {}
+    ic = InferenceConfig(batch_size=2, num_beams=W, max_context_length=16, seq_len=48, buckets=[8, 16], eos_token_id=17, length_penalty=0.8, **extra)
+    assert ic.tkg_batch_size == 6 and ic.max_batch_size == 6
+    r = InferenceRunner(tiny_llama(sequence_parallel_enabled=False), ic, checkpoint_loader=train.state_dict, device=torch.device("cpu"))
+    r.trace()
+    for B, T in ((2, 11), (1, 5), (2, 8)):
+        prompts = torch.randint(20, cfg.vocab_size, (B, T))
+        out, scores = r.generate_beams(prompts, max_new_tokens=9, num_return_sequences=2, return_scores=True)
+        assert torch.equal(r.generate(prompts, max_new_tokens=9), out[::2])
+        for b in range(B):
+            want = _searched(_train_logits(train), prompts[b].tolist(), W, 9, 17, 0.8, False)
+            for i in range(2):
+                h = want[i][1]
+                assert out[b * 2 + i, T:T + len(h)].tolist() == h and abs(float(scores[b * 2 + i]) - want[i][0]) <= 1e-4 * abs(want[i][0])
+    with pytest.raises(ValueError):
+        r.generate_beams(torch.ones(3, 8, dtype=torch.long), max_new_tokens=4)
+    with pytest.raises(ValueError):
+        r.generate_beams(torch.ones(1, 8, dtype=torch.long), max_new_tokens=42)
+
+
+# ---- lines and pages of a cache ---------------------------------------------------------------------------------------
+
+def _filled(cache, g):
+    for t in cache._tensors() + cache._state_tensors():
+        t.copy_(torch.randint(-99, 99, t.shape, generator=g).to(t))
+
+
+def _line(cache, i, line, n):
+    """Rows ``[0, n)`` of a line of layer ``i``, keys and values."""
+    out = []
+    for t in cache.layer(i):
+        if cache.paged:
+            pages = cache.block_table[line].long()
+            out.append(t[pages].permute(1, 0, 2, 3).reshape(t.shape[1], -1, t.shape[3])[:, :n].clone())
+        else:
+            out.append(t[line, :, :n].clone())
+    return out
+
+
+SPECS = [(2, 8, 8), (1, 12, 6, "columns"), None, (2, 8, 4, "heads", 3), (2, 8, 8)]
+
+
+def _cache(kind, device, lines=6, **kw):
+    paged = {"contiguous": {}, "paged": dict(paged=True, page_size=4), "pool": dict(paged=True, page_size=4, num_pages=40)}[kind]
+    return KVCache(5, lines, 0, 24, 0, dtype=torch.float32, device=device, layer_specs=SPECS, share_from={4: 0},
+                   state_specs={2: {"S": (2, 3, 4), "n": (5,)}}, **{**paged, **kw})
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["contiguous", "paged", "pool"])
+def test_lines_of_a_search(device, kind):
+    g = torch.Generator().manual_seed(3)
+    cache, W, lengths = _cache(kind, device), 3, [7, 8]
+    if kind == "pool":
+        for b in range(2):
+            cache.reserve(b * W, 12)
+    _filled(cache, g)
+    layers = [0, 1, 3, 4]
+    before = {(i, b): _line(cache, i, b * W, lengths[b]) for i in layers for b in range(2)}
+    states = {k: v.clone() for k, v in cache.state(2).items()}
+    lines = cache.beams(lengths, W, 10)
+    assert isinstance(lines, BeamLines) and lines.start.tolist() == lengths
+    for i in layers:
+        for line in range(2 * W):
+            assert all(torch.equal(a, b) for a, b in zip(_line(cache, i, line, lengths[line // W]), before[i, line // W])), (i, line)
+    for k, v in cache.state(2).items():
+        assert torch.equal(v, states[k][[0, 0, 0, 3, 3, 3]])
+    if kind == "pool":
+        assert cache.pool.private_from(0, 6) == [4, 4, 4, 8, 8, 8]          # a page of one prompt is shared, both of the other
+        assert cache.pool.num_free == 40 - (1 + 3 * 4) - (2 + 3 * 3)
+    # rows behind the prompts, a value a line
+    for t in cache._state_tensors():
+        t.copy_(torch.arange(6.0).reshape([6] + [1] * (t.dim() - 1)).expand_as(t))
+    for line in range(2 * W):
+        for pos in range(lengths[line // W], lengths[line // W] + 4):
+            for t in cache._tensors():
+                if cache.paged:
+                    t[int(cache.block_table[line, pos // 4]), :, pos % 4] = line * 100 + pos
+                else:
+                    t[line, :, pos] = line * 100 + pos
+    end = torch.tensor([n + 4 for n in lengths], device=device)
+    for parents in ([[0, 0, 2], [2, 1, 1]], [[1, 2, 0], [1, 0, 0]]):
+        had = {(i, line): _line(cache, i, line, 12) for i in layers for line in range(6)}
+        state = [t.clone() for t in cache._state_tensors()]
+        lines.reorder(torch.tensor(parents, device=device), end)
+        for line in range(6):
+            b, frm = line // W, line // W * W + parents[line // W][line % W]
+            n = lengths[b]
+            for i in layers:
+                for now, own, new in zip(_line(cache, i, line, 12), had[i, line], had[i, frm]):
+                    assert torch.equal(now[:, :n], own[:, :n]) and torch.equal(now[:, n:n + 4], new[:, n:n + 4]) and torch.equal(now[:, n + 4:], own[:, n + 4:])
+            assert all(torch.equal(t[line], s[frm]) for t, s in zip(cache._state_tensors(), state))
+    lines.reorder(torch.tensor([[0, 1, 1], [0, 1, 2]], device=device))          # as far as there is room
+    if kind == "pool":
+        cache.free(5)
+        cache.fork(4, 5)
+        with pytest.raises(ValueError):
+            lines.reorder(torch.tensor([[0, 1, 2]] * 2, device=device), end)
+        with pytest.raises(ValueError):
+            cache.reorder_lines(torch.tensor([[0, 1, 2]] * 2, device=device))
+    for args in (([7, 8, 9], 3), ([7], 0), ([], 3), ([25], 2), ([20], 2, 5), ([-1], 2)):
+        with pytest.raises(ValueError):
+            cache.beams(*args)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_pages_of_a_pool_fork_compact_and_move(device):
+    g = torch.Generator().manual_seed(4)
+    cache = _cache("pool", device, lines=8)
+    for line, n in ((0, 10), (1, 24), (2, 3), (3, 17)):
+        cache.reserve(line, n)
+    _filled(cache, g)
+    cache.fork_lines(0, [4, 5, 6])
+    held = {(i, line): _line(cache, i, line, n) for i in (0, 1, 3) for line, n in ((0, 10), (3, 17), (4, 10), (5, 10), (6, 10))}
+    for (i, line), rows in held.items():
+        if line > 3:
+            assert all(torch.equal(a, b) for a, b in zip(rows, held[i, 0]))
+    cache.free(1), cache.free(2)
+    used = 40 - cache.pool.num_free
+    assert cache.compact() == used and used == 2 + 4 + 5
+    assert max(max(cache.pool.block_row(line)[0][:cache.pool.block_row(line)[1]], default=0) for line in range(8)) == used - 1
+    for (i, line), rows in held.items():
+        assert all(torch.equal(a, b) for a, b in zip(_line(cache, i, line, rows[0].shape[1]), rows)), (i, line)
+    assert cache.compact() == used          # nothing to do
+    cache.prepare_write(0, 9)
+    cache.prepare_write(4, 0)
+    assert not cache.pool.page_shared(4, 0) and all(torch.equal(a, b) for a, b in zip(_line(cache, 0, 4, 10), held[0, 4]))
+    with pytest.raises(MemoryError):
+        cache.resize_pool(5)
+    for pages in (used + 1, 30, 50):
+        cache.resize_pool(pages)
+        assert cache.pool.num_pages == pages == cache.k[0].shape[0] and cache.pool.num_free == pages - used - 1
+        for (i, line), rows in held.items():
+            assert all(torch.equal(a, b) for a, b in zip(_line(cache, i, line, rows[0].shape[1]), rows)), (i, line)
+        assert cache.v[1].data_ptr() == cache.k[1].data_ptr()          # columns of the same rows
+    # more forks than there are pages: none of them is left half made
+    small = _cache("pool", device, lines=8, num_pages=6)
+    small.reserve(0, 15)
+    with pytest.raises(MemoryError):
+        small.fork_lines(0, [1, 2, 3])
+    assert small.pool.num_free == 2 and all(small.pool.block_row(line)[1] == 0 for line in (1, 2, 3))
+    small.fork_lines(0, [1, 2])
+    with pytest.raises(AssertionError):
+        _cache("contiguous", device).copy_pages([0], [1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("W", [2, 5])
+def test_captured_graphs_and_eager_steps_agree(paged, W):
+    """The runner with graphs and the model without: the same kernels on the same rows, hence the same sequences."""
+    torch.manual_seed(1)
+    cfg = tiny_llama(sequence_parallel_enabled=False, torch_dtype=torch.bfloat16, hidden_size=512, head_dim=64)
+    extra = dict(paged_kv=True, page_size=16, num_kv_pages=64) if paged else {}
+    ic = InferenceConfig(batch_size=2, num_beams=W, max_context_length=32, seq_len=64, buckets=[32], eos_token_id=11, **extra)
+    train = LlamaForCausalLM(cfg, device=torch.device("cuda"))
+    with torch.no_grad():
+        train.lm_head.weight.mul_(6.0)
+    sd = {k: v.clone() for k, v in train.state_dict().items()}
+    r = InferenceRunner(cfg, ic, checkpoint_loader=lambda: sd, device=torch.device("cuda"))
+    r.trace()
+    prompts = torch.randint(20, cfg.vocab_size, (2, 32), device="cuda")
+    out, scores = r.generate_beams(prompts, max_new_tokens=20, num_return_sequences=W, return_scores=True)
+    again = r.generate(prompts, max_new_tokens=20)
+    eager, eager_scores = r.model.generate_beams(prompts, num_beams=W, max_new_tokens=20, eos_token_id=11, num_return_sequences=W, return_scores=True)
+    assert torch.equal(out, eager) and torch.equal(scores, eager_scores) and torch.equal(again, out[::W])
+    assert bool((scores.view(2, W).diff(dim=1) <= 0).all())
+    # what a sequence's tokens are worth, from one pass over it: bf16 keys, values and logits, sums of 20
+    seq = out[0]
+    n = int((seq[32:] != 0).sum())
+    n = 20 if 11 not in seq[32:].tolist() else seq[32:].tolist().index(11) + 1
+    with torch.no_grad():
+        logits = train(seq[None]).transpose(0, 1)[0].float()
+    logp = torch.log_softmax(logits, -1)[31:31 + n].gather(1, seq[32:32 + n, None]).sum()
+    assert abs(float(logp) / n - float(scores[0])) <= 0.1
+    r.close()
