@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
     __shared__ unsigned long long cand[kCollect];
     extern __shared__ uint4 ring[];            // [kStages][NV][NT]
     __shared__ unsigned char looker[kWarps][32];
-    __shared__ uint32_t warp_top[kWarps], warp_kth[kWarps];
+    __shared__ uint32_t warp_top[kWarps], bound_keys[2 * kMaxN];
     __shared__ float warp_sum_of[kWarps];
     __shared__ int red[32];
     __shared__ unsigned long long best[kMaxN];
@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
     bool crowded = false;
     // the n best candidates in order; eight lanes compare one with all
     auto keep_best = [&](int count) {
-        for (int i0 = 0; i0 < count; i0 += NT / 8) {
-            const int i = i0 + tid / 8;
+        for (int i0 = warp * 4; i0 < count; i0 += NT / 8) {
+            const int i = i0 + lane / 8;
             const unsigned long long own = i < count ? cand[i] : ~0ull;
             int before = 0;
 #pragma unroll 4
@@ -329,14 +329,36 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
             sum += (f2_lo(part[0]) + f2_hi(part[0])) + (f2_lo(part[1]) + f2_hi(part[1]));
         }
         if (r == 0) {
-            // a k-th largest maximum of each warp that has values, warps * k >= n: the least of them has n values that are not below it
+            // the largest maxima of each warp that has values, 2 n of them: the n-th of those (its upper 16 bits, all that bf16 has) has n values that are
+            // not below it
             const int vecs = (V + mis - split * rounds * (NT * E) + VE - 1) / VE, filled = min(max((vecs + 31) / 32, 1), kWarps);
-            const uint32_t key = order_key(m), kth = kth_of_warp(key, (n + filled - 1) / filled, lane);
-            if (lane == 0) warp_kth[warp] = kth;
+            const int per = min((2 * n + filled - 1) / filled, min(2 * kMaxN / filled, 32)), keys = filled * per;
+            uint32_t key = order_key(m);
+            for (int i = 0; i < per; ++i) {
+                const uint32_t v = __reduce_max_sync(kFull, key);
+                if (lane == __ffs(__ballot_sync(kFull, key == v)) - 1) key = 0;
+                if (lane == 0 && warp < filled) bound_keys[warp * per + i] = v;
+            }
             __syncthreads();
-            uint32_t least = warp_kth[0];
+            uint32_t least = 0;
+            if (keys <= 32) {
+                const uint32_t own = lane < keys ? bound_keys[lane] : 0;
+                for (int bit = 31; bit >= 16; --bit) {
+                    const uint32_t c = least | 1u << bit;
+                    if (__popc(__ballot_sync(kFull, own >= c)) >= n) least = c;
+                }
+            } else {
+                uint32_t own[2 * kMaxN / 32];
 #pragma unroll
-            for (int i = 1; i < kWarps; ++i) least = i < filled ? min(least, warp_kth[i]) : least;
+                for (int q = 0; q < 2 * kMaxN / 32; ++q) own[q] = q * 32 + lane < keys ? bound_keys[q * 32 + lane] : 0;
+                for (int bit = 31; bit >= 16; --bit) {
+                    const uint32_t c = least | 1u << bit;
+                    int mine = 0;
+#pragma unroll
+                    for (int q = 0; q < 2 * kMaxN / 32; ++q) mine += own[q] >= c;
+                    if (__reduce_add_sync(kFull, mine) >= n) least = c;
+                }
+            }
             // the number below that bound (below zero one that is not equal to it), so that what is above it is looked at in every round
             least = max(least, kLowestKey) - 1;
             floor = key_value(least == 0x7fffffffu ? least - 1 : least);
@@ -476,9 +498,9 @@ __global__ void __launch_bounds__(1024, 1) beam_join_kernel(const float* __restr
         if ((uint32_t)(head[l] >> 32) >= floor) list_of[atomicAdd(&s_heads, 1)] = l;
     __syncthreads();
     const int heads = s_heads;
-    // what these lists hold bounds the n-th score once more
+    // what these lists hold, around the warps again, bounds the n-th score once more
     own = 0;
-    for (int e = tid; e < heads * n; e += nth) {
+    for (int e = lane * warps + warp; e < heads * n; e += nth) {
         const int l = list_of[e / n];
         own = max(own, (uint32_t)(score_of(in.entry[(l0 + l) * n + e % n], l / splits) >> 32));
     }
@@ -496,7 +518,7 @@ __global__ void __launch_bounds__(1024, 1) beam_join_kernel(const float* __restr
             }
         }
     };
-    for (int e = tid; e < heads * n; e += nth) take(list_of[e / n], e % n, (unsigned long long)floor << 32);
+    for (int e = lane * warps + warp; e < heads * n; e += nth) take(list_of[e / n], e % n, (unsigned long long)floor << 32);
     __syncthreads();
     int count = s_count;
     if (count > room) {

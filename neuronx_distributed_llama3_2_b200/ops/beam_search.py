@@ -103,18 +103,18 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
     scores = scores.contiguous()
     code, device = _DTYPES[logits.dtype], logits.device
     out = torch.empty((2, B, n), dtype=torch.int64, device=device)
-    best = torch.empty((B, n), dtype=torch.float32, device=device)
+    best = scores.new_empty((B, n))
     if B:
         with _lib.on_device_of(logits):
             size = _scratch_bytes(code, B, W, V, n)
             if size <= 0:
                 raise ValueError(f"{W} beams of {V} tokens are more than one call takes")
-            scratch = torch.empty(size, dtype=torch.uint8, device=device)          # the call's own
+            scratch = scores.new_empty((size + 3) // 4)          # the call's own
             at = out.data_ptr()
             rc = _entry("nxd_beam_select")(code, logits.data_ptr(), stride, scores.data_ptr(), B, W, V, n, scratch.data_ptr(), best.data_ptr(), at,
                                            at + 8 * B * n, _lib.stream_ptr())
         _lib.check(rc, "nxd_beam_select")
-    return (best, *out.unbind(0))
+    return best, out[0], out[1]          # an index costs a third of unbind()
 
 
 @functools.lru_cache(maxsize=1024)
@@ -166,13 +166,8 @@ def beam_advance(candidates: Tuple[torch.Tensor, torch.Tensor, torch.Tensor], sc
     norm = _norm(step + 1, length_penalty)
     if not _kernel(scores):
         return _advance_ref(cand_scores, cand_beams, cand_tokens, scores, pool, history, step, norm, eos, pad, early_stopping)
-    wide = torch.empty((2, B, W), dtype=torch.int64, device=dev)
-    floats = torch.empty((2, B, W), dtype=torch.float32, device=dev)
-    ints = torch.empty((2, B, W), dtype=torch.int32, device=dev)
-    done = torch.empty(B, dtype=torch.bool, device=dev)
-    tokens, parents = wide.unbind(0)
-    running, pool_scores = floats.unbind(0)
-    lengths, slots = ints.unbind(0)
+    running, tokens, parents = torch.empty_like(scores), cand_tokens.new_empty((B, W)), cand_beams.new_empty((B, W))
+    pool_scores, lengths, slots, done = (torch.empty_like(t) for t in pool)
     row = 4 * step * B * W
     with _lib.on_device_of(scores):
         rc = _entry("nxd_beam_advance")(cand_scores.data_ptr(), cand_beams.data_ptr(), cand_tokens.data_ptr(), B, W, N, scores.data_ptr(),
@@ -278,7 +273,7 @@ def beam_finish(scores: torch.Tensor, pool: BeamPool, history: BeamHistory, step
         raise ValueError(f"{B} requests are more than 65535")
     tokens = torch.empty((B, W, step), dtype=torch.int64, device=dev)
     lengths = torch.empty((B, W), dtype=torch.int64, device=dev)
-    best = torch.empty((B, W), dtype=torch.float32, device=dev)
+    best = torch.empty_like(scores)
     with _lib.on_device_of(scores):
         scratch = None
         if W * step > 2 ** 16:          # lines of many steps do not fit shared memory

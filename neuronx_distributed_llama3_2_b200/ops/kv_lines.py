@@ -28,15 +28,12 @@ class _Alike:
     """Tensors of one shape: their addresses for a launch."""
 
     def __init__(self, key: tuple):
-        self.key, self.tensors = key, []
-
-    def table(self) -> None:
-        self.at = [t.data_ptr() for t in self.tensors]
-        self.base = (_c.c_void_p * len(self.at))(*self.at)
+        self.key, self.tensors, self.at = key, [], []
 
     def addresses(self):
-        if [t.data_ptr() for t in self.tensors] != self.at:          # ``t.data = ...`` moves a tensor
-            self.table()
+        at = [f() for f in self.where]
+        if at != self.at:          # ``t.data = ...`` moves a tensor
+            self.at, self.base = at, (_c.c_void_p * len(at))(*at)
         return self.base
 
 
@@ -74,11 +71,11 @@ class CacheTensors:
             kinds[1].setdefault(key, _Alike(key)).tensors.append(t)
         self.kinds, self.state_kinds = list(kinds[0].values()), list(kinds[1].values())
         for kind in self.kinds + self.state_kinds:
-            kind.table()
-
-    @property
-    def lines(self) -> int:
-        return min(t.shape[0] for t in self.cache + self.states)
+            kind.where = [t.data_ptr for t in kind.tensors]
+        # how many lines there are with and without a block table
+        self.lines = min(t.shape[0] for t in self.cache + self.states)
+        self.state_lines = min((t.shape[0] for t in self.states), default=None)
+        self.cuda = self.device.type == "cuda"
 
 
 def _laid_out(cache: Union[CacheTensors, Sequence[torch.Tensor]], states: Sequence[torch.Tensor] = ()) -> CacheTensors:
@@ -90,7 +87,7 @@ def _laid_out(cache: Union[CacheTensors, Sequence[torch.Tensor]], states: Sequen
 
 
 def _index(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> torch.Tensor:
-    if tuple(t.shape) != shape or t.dtype not in (torch.int64, torch.int32) or t.device != device:
+    if t.shape != shape or t.dtype not in (torch.int64, torch.int32) or t.device != device:
         raise ValueError(f"{name}: an int64 or int32 tensor {shape} on {device} is expected, not {t.dtype} {tuple(t.shape)} on {t.device}")
     return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
@@ -116,10 +113,10 @@ def reorder_lines_(cache: Union[CacheTensors, Sequence[torch.Tensor]], parents: 
         if page_size < 1 or any(k.key[2] != page_size for k in c.kinds):
             raise ValueError(f"page_size {page_size} is not that of the cache's pages")
         table = block_table
-    short = [k.key[0] for k in (c.state_kinds if table is not None else c.kinds + c.state_kinds)] + ([table.shape[0]] if table is not None else [])
-    if short and min(short) < B * W:
-        raise ValueError(f"{B} groups of {W} lines are more than the {min(short)} that there are")
-    if not c.device.type == "cuda" or not _lib.available():
+    lines = c.lines if table is None else table.shape[0] if c.state_lines is None else min(table.shape[0], c.state_lines)
+    if lines < B * W:
+        raise ValueError(f"{B} groups of {W} lines are more than the {lines} that there are")
+    if not c.cuda or not _lib.available():
         return _reorder_ref(c, parents, start, end, table, page_size)
     if B > 65535:
         raise ValueError(f"{B} groups are more than 65535")
@@ -175,29 +172,14 @@ def copy_pages_(cache: Union[CacheTensors, Sequence[torch.Tensor]], src: Union[t
     c = _laid_out(cache)
     if not c.cache:
         return
-    pages = min(k.key[0] for k in c.kinds)
-    lists = [None if x is None or isinstance(x, torch.Tensor) else [int(i) for i in x] for x in (src, dst)]
-    n = len(src)
-    if len(dst) != n or (rows is not None and len(rows) != n):
-        raise ValueError(f"{n} pages to copy, {len(dst)} to copy to" + ("" if rows is None else f", rows of {len(rows)}"))
-    for name, x in zip(("src", "dst"), lists):
-        if x is not None and any(not 0 <= i < pages for i in x):
-            raise ValueError(f"{name}: page {next(i for i in x if not 0 <= i < pages)} is not one of the {pages} that there are")
-    if lists[1] is not None:
-        if len(set(lists[1])) != n:
-            raise ValueError("dst: a page is written twice")
-        if lists[0] is not None and set(lists[0]) & set(lists[1]):
-            raise ValueError(f"page {min(set(lists[0]) & set(lists[1]))} is both read and written")
-    if n == 0:
-        return
-    host = [x if x is not None and not isinstance(x, torch.Tensor) else None for x in (src, dst, rows)]
-    if any(x is not None for x in host):          # one copy for what comes as lists
-        packed = torch.tensor([[int(i) for i in x] for x in host if x is not None], dtype=torch.int64).to(c.device)
-        packed = iter(packed.unbind(0))
-        src, dst, rows = (next(packed) if h is not None else x for h, x in zip(host, (src, dst, rows)))
+    if not (isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and (rows is None or isinstance(rows, torch.Tensor))):
+        src, dst, rows = _from_lists(c, src, dst, rows)
+    n = src.shape[0] if src.dim() else -1
     src, dst = _index("src", src, (n,), c.device), _index("dst", dst, (n,), c.device)
     rows = None if rows is None else _index("rows", rows, (n,), c.device)
-    if not c.device.type == "cuda" or not _lib.available():
+    if n == 0:
+        return
+    if not c.cuda or not _lib.available():
         return _copy_ref(c, src, dst, rows)
     fn = _entry("nxd_copy_pages")
     with _lib.on_device_of(src):
@@ -206,6 +188,24 @@ def copy_pages_(cache: Union[CacheTensors, Sequence[torch.Tensor]], src: Union[t
             rc = fn(k.addresses(), len(k.at), lead, heads, page, row, line, head, n, src.data_ptr(), dst.data_ptr(),
                     0 if rows is None else rows.data_ptr(), _lib.stream_ptr())
             _lib.check(rc, "nxd_copy_pages")
+
+
+def _from_lists(c: CacheTensors, src, dst, rows):
+    """What comes as lists is checked here and brought to the device, in one copy."""
+    pages = min(k.key[0] for k in c.kinds)
+    lists = [None if x is None or isinstance(x, torch.Tensor) else [int(i) for i in x] for x in (src, dst, rows)]
+    if len(dst) != len(src) or (rows is not None and len(rows) != len(src)):
+        raise ValueError(f"{len(src)} pages to copy, {len(dst)} to copy to" + ("" if rows is None else f", rows of {len(rows)}"))
+    for name, x in zip(("src", "dst"), lists):
+        if x is not None and any(not 0 <= i < pages for i in x):
+            raise ValueError(f"{name}: page {next(i for i in x if not 0 <= i < pages)} is not one of the {pages} that there are")
+    if lists[1] is not None:
+        if len(set(lists[1])) != len(lists[1]):
+            raise ValueError("dst: a page is written twice")
+        if lists[0] is not None and set(lists[0]) & set(lists[1]):
+            raise ValueError(f"page {min(set(lists[0]) & set(lists[1]))} is both read and written")
+    packed = iter(torch.tensor([x for x in lists if x is not None], dtype=torch.int64).to(c.device, non_blocking=True))
+    return tuple(next(packed) if x is not None else given for x, given in zip(lists, (src, dst, rows)))
 
 
 def _copy_ref(c: CacheTensors, src, dst, rows) -> None:
