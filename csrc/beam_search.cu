@@ -1,13 +1,17 @@
 // Beam search for sm_100a: the choice of a step's candidates, the books of the beams, and the sequences at the end.
 //
 // Choice.  Of group b's beams w with running scores s[w] and logits x[w, v] the n best of s[w] + x[w, v] - log sum_u exp x[w, u], of equal
-// ones the lowest w * V + v.  One pass over the logits: a CTA takes a chunk of one row into registers (256 threads x E values), has its
-// maximum and its sum of exponentials, and the chunk's n best in order.  A second kernel joins the chunks of a group's rows.
-//   The n best of a chunk: the n-th largest of the 256 threads' maxima bounds the n-th largest value from below, so what is not below it is
-// collected (little more than n values as a rule) and ranked by counting.  Equal values in numbers (masked ones) do not fit the buffer: the exact
-// n-th key is then found bit by bit and its ties are taken in the order of their indices.
+// ones the lowest w * V + v.  One pass over the logits: a CTA goes through a chunk of one row in rounds (512 threads x 4 vectors, 256 x 2 where
+// rows are few), with its running maximum and sum of exponentials, and ends with the chunk's n best in order.  A second kernel joins the
+// chunks of a group's rows.
+//   The n best of a chunk: the n-th largest of a few maxima of every warp bounds the n-th largest value from below, so what is not below it is
+// collected (about 1.3 n values of a round as a rule) and ranked by counting; later rounds look only at what is above the n-th so far.  Equal values in
+// numbers (masked ones) do not fit the buffer: the exact n-th key of every round is then found bit by bit and its ties are taken in the order of
+// their indices.
 //   Scores are compared in 64 bits: sums of near size decide between rows.  Within a row the logits decide.
-// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.
+// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 26 us for the rows and 6 for the
+// join.  Instructions bound the rows (a conversion, the difference, its scaling, an exponential and two sums per value, about 300 instructions
+// for the 1024 values of a warp's round with everything else), and 256 rows on 148 SMs; one request of 4 rows takes 4.7 and 5.4 us of latency.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -688,8 +692,8 @@ __device__ __forceinline__ void store_of_rank(unsigned char* p, int rank, int v)
 // on their way behind them; a section of the span is walked for all lines at once (lane w starts in line w at the section's end; a warp has as many
 // sections as it has room for lines); the sections are joined within a CTA, the spans across the cluster; then they are walked once
 // more, which leaves the line of every place at every step where the parents were.
-//   Latency bounds it, of the chain and of rows that are a few bytes each: 2000 steps of 8 lines in 64 groups 180 ms with an operation a step, 28 us with
-// one CTA a group and 32 sections.
+//   Latency bounds it, of the chain and of rows that are a few bytes each: 2000 steps of 8 lines in 64 groups 181 ms with an operation a step, 21 us with
+// one CTA a group, 12 us with four (16 MB: 2.5 us at 6555 GB/s).
 __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(Books in, int W, int B, int step, int span, float norm, long long eos, long long pad,
                                                                      const int* __restrict__ hist_token, const int* __restrict__ hist_parent,
                                                                      long long* __restrict__ tokens, long long* __restrict__ lengths,
@@ -865,8 +869,9 @@ struct Split {
     int threads, vecs, rounds, splits;
 };
 
-// Rounds of 512 threads x 4 vectors where that leaves no SM without a CTA, as many of them per CTA as leave one wave (two CTAs an SM); rounds of 256 x 2
-// where rows are few.
+// Rounds of 512 threads x 4 vectors where that leaves no SM without a CTA, as many of them per CTA as leave one wave (two CTAs an SM): every CTA pays
+// for its first bound and for putting candidates in order (256 rows of 128256: one CTA a row 29 us, two 31 to 36, four 33, eight 38).  Rounds of 256 x 2
+// where rows are few (4 rows: 4.7 us, with 256 x 4 5.0).
 Split split_of(long long rows, int W, int V, int elem) {
     const int per_vec = 16 / elem;
     const long long sms = nxd_num_sms(), span = V + per_vec - 1, large = 512LL * 4 * per_vec;
@@ -928,7 +933,7 @@ NXD_API int nxd_beam_select(int dtype, const void* logits, long long stride, con
     return 0;
 }
 
-// One step of the books (the header has the arrays).
+// One step of the books (the header has the arrays).  3 us, latency: a warp a group.
 NXD_API int nxd_beam_advance(const float* cand_scores, const long long* cand_beams, const long long* cand_tokens, int B, int W, int N,
                              const float* running, const float* pool_scores, const int* pool_lengths, const int* pool_slots,
                              const unsigned char* done, float norm, long long eos, long long pad, int early_stopping, int length,

@@ -19,6 +19,7 @@
 #include <deque>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -504,26 +505,32 @@ NXD_RT_API int nxd_kv_compact(void* h, int* src, int* dst, int cap) {
     KvPool* p = (KvPool*)h;
     if (!p || !src || !dst) return fail("kv_compact: bad arguments");
     std::lock_guard<std::mutex> g(p->mu);
-    const int used = p->num_pages - (int)p->free_list.size();
-    std::vector<int> to(p->num_pages, -1), holes;
-    for (int pg = 0; pg < used; ++pg)
-        if (p->refcnt[pg] == 0) holes.push_back(pg);
-    if ((int)holes.size() > cap) return fail("kv_compact: %d moves, room for %d", (int)holes.size(), cap);
-    int n = 0;
-    for (int pg = used; pg < p->num_pages; ++pg) {
-        if (p->refcnt[pg] == 0) continue;
-        src[n] = pg;
-        dst[n] = to[pg] = holes[n];
-        p->refcnt[holes[n]] = p->refcnt[pg];
-        p->refcnt[pg] = 0;
-        ++n;
+    try {
+        const int used = p->num_pages - (int)p->free_list.size();
+        std::vector<int> to(p->num_pages, -1), holes, free_list;          // all memory before the first change
+        holes.reserve(used);
+        free_list.reserve(p->num_pages);
+        for (int pg = 0; pg < used; ++pg)
+            if (p->refcnt[pg] == 0) holes.push_back(pg);
+        if ((int)holes.size() > cap) return fail("kv_compact: %d moves, room for %d", (int)holes.size(), cap);
+        int n = 0;
+        for (int pg = used; pg < p->num_pages; ++pg) {
+            if (p->refcnt[pg] == 0) continue;
+            src[n] = pg;
+            dst[n] = to[pg] = holes[n];
+            p->refcnt[holes[n]] = p->refcnt[pg];
+            p->refcnt[pg] = 0;
+            ++n;
+        }
+        for (auto& line : p->pages)
+            for (int& pg : line)
+                if (to[pg] >= 0) pg = to[pg];
+        for (int pg = p->num_pages - 1; pg >= used; --pg) free_list.push_back(pg);
+        p->free_list.swap(free_list);
+        return n;
+    } catch (const std::bad_alloc&) {
+        return fail("kv_compact: out of host memory");
     }
-    for (auto& line : p->pages)
-        for (int& pg : line)
-            if (to[pg] >= 0) pg = to[pg];
-    p->free_list.clear();
-    for (int pg = p->num_pages - 1; pg >= used; --pg) p->free_list.push_back(pg);
-    return n;
 }
 
 // Another number of pages; what is behind the new end must be free.
@@ -533,12 +540,20 @@ NXD_RT_API int nxd_kv_resize(void* h, int num_pages) {
     std::lock_guard<std::mutex> g(p->mu);
     for (int pg = num_pages; pg < p->num_pages; ++pg)
         if (p->refcnt[pg] != 0) return fail("kv_resize: page %d is in use", pg);
-    p->refcnt.resize(num_pages, 0);
-    p->num_pages = num_pages;
-    p->free_list.clear();
-    for (int pg = num_pages - 1; pg >= 0; --pg)
-        if (p->refcnt[pg] == 0) p->free_list.push_back(pg);
-    return 0;
+    try {
+        std::vector<int> free_list, refcnt(num_pages, 0);
+        free_list.reserve(num_pages);
+        for (int pg = num_pages - 1; pg >= 0; --pg) {
+            if (pg < p->num_pages) refcnt[pg] = p->refcnt[pg];
+            if (refcnt[pg] == 0) free_list.push_back(pg);
+        }
+        p->refcnt.swap(refcnt);
+        p->free_list.swap(free_list);
+        p->num_pages = num_pages;
+        return 0;
+    } catch (const std::bad_alloc&) {
+        return fail("kv_resize: out of host memory");
+    }
 }
 
 // Block-table row of `line` into out[max_pages]; unused slots get `fill` (a valid page id keeps kernels in bounds).

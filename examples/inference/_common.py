@@ -37,6 +37,8 @@ def common_parser(presets: Dict[str, Callable], default_model: str) -> argparse.
     ap.add_argument("--layers", type=int, default=0, help="truncate the model to this many layers (smoke runs)")
     ap.add_argument("--no_cuda_graphs", action="store_true")
     ap.add_argument("--paged_kv", action="store_true")
+    ap.add_argument("--num_beams", type=int, default=1, help="beam search with that many beams per prompt")
+    ap.add_argument("--length_penalty", type=float, default=1.0)
     return ap
 
 
@@ -57,7 +59,7 @@ def inference_config(args, **extra) -> InferenceConfig:
     kw = dict(tp_degree=args.tp_degree, batch_size=args.batch_size, max_context_length=args.max_context_length,
               seq_len=args.seq_len, max_new_tokens=args.max_new_tokens, top_k=args.top_k, top_p=args.top_p,
               temperature=args.temperature, do_sample=args.top_k > 1, use_cuda_graphs=not args.no_cuda_graphs,
-              paged_kv=args.paged_kv)
+              paged_kv=args.paged_kv, num_beams=args.num_beams, length_penalty=args.length_penalty)
     kw.update(extra)
     return InferenceConfig(**kw)
 

@@ -41,6 +41,8 @@ class ContinuousBatcher:
         self.cache = model.kv_cache
         assert self.cache.pool is not None, "continuous batching needs InferenceConfig(paged_kv=True, num_kv_pages=N)"
         ic = model.inference_config
+        if ic.num_beams > 1:
+            raise ValueError("continuous batching serves one sequence per request, not beams")
         self.max_running = max_running or self.cache.lines
         self.sched = NativeScheduler(self.cache.pool, self.max_running)
         self.eos = eos_token_id if eos_token_id is not None else ic.eos_token_id

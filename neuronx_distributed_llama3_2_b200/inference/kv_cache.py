@@ -47,6 +47,7 @@ class KVCache:
         self.paged, self.page_size = paged, page_size
         self.pool = None
         self._laid_out: Optional[CacheTensors] = None
+        self._held: tuple = ()
         if paged:
             self.max_pages = (seq_len + page_size - 1) // page_size
             if num_pages is None:
@@ -145,8 +146,9 @@ class KVCache:
     @property
     def tensors(self) -> CacheTensors:
         """The cache's tensors, laid out for the kernels that move lines and pages of all layers at once."""
-        if self._laid_out is None:
-            self._laid_out = CacheTensors(self._tensors(), self._state_tensors())
+        held = (*self.k, *self.v, *self._state_tensors())
+        if self._laid_out is None or len(held) != len(self._held) or any(a is not b for a, b in zip(held, self._held)):
+            self._laid_out, self._held = CacheTensors(self._tensors(), self._state_tensors()), held
         return self._laid_out
 
     def copy_pages(self, src: Sequence[int], dst: Sequence[int], rows: Optional[Sequence[int]] = None) -> None:

@@ -125,7 +125,7 @@ def _scratch_bytes(code: int, B: int, W: int, V: int, n: int) -> int:
 def beam_select_ref(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The same in torch operations, in 64 bits."""
     (B, W), V = scores.shape, logits.shape[-1]
-    x = logits.reshape(B, W, V).double()
+    x, scores = logits.detach().reshape(B, W, V).double(), scores.detach()
     total = scores.double()[..., None] + (x - torch.logsumexp(x, -1, keepdim=True))
     total = torch.where(x.isinf() | total.isnan(), -float("inf"), total).reshape(B, W * V)
     best, at = torch.sort(total, dim=1, descending=True, stable=True)

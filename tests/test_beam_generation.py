@@ -8,6 +8,7 @@ import torch
 
 from neuronx_distributed_llama3_2_b200.inference import BeamLines, InferenceConfig, InferenceRunner, KVCache, LlamaInferenceModel
 from neuronx_distributed_llama3_2_b200.models import LlamaForCausalLM, tiny_llama
+from conftest import run_distributed
 from test_beam_search import DEVICES, _Request
 import test_beam_search as units
 
@@ -149,6 +150,65 @@ def test_the_runner_searches_with_its_buckets(monkeypatch, paged):
         r.generate_beams(torch.ones(3, 8, dtype=torch.long), max_new_tokens=4)
     with pytest.raises(ValueError):
         r.generate_beams(torch.ones(1, 8, dtype=torch.long), max_new_tokens=42)
+
+
+@pytest.mark.parametrize("W,penalty", [(2, 1.0), (4, 0.0), (4, 0.6)])
+def test_sequences_equal_those_of_transformers(W, penalty):
+    transformers = pytest.importorskip("transformers")
+    from neuronx_distributed_llama3_2_b200.inference import BeamSearch
+
+    torch.manual_seed(0)
+    model = transformers.LlamaForCausalLM(transformers.LlamaConfig(
+        vocab_size=60, hidden_size=32, intermediate_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, eos_token_id=5,
+        pad_token_id=0, bos_token_id=1)).eval().double()
+    with torch.no_grad():
+        model.lm_head.weight.mul_(40.0)
+        model.lm_head.weight[5] *= 1.1
+        for seed in range(6):
+            ids = torch.randint(6, 60, (1, 7), generator=torch.Generator().manual_seed(seed))
+            ref = model.generate(ids, num_beams=W, max_new_tokens=14, do_sample=False, length_penalty=penalty, early_stopping=False,
+                                 num_return_sequences=W)[:, 7:].tolist()
+            ref = [r[:r.index(5) + 1] if 5 in r else r for r in ref]
+            s = BeamSearch(1, W, 14, eos_token_id=5, length_penalty=penalty)
+            hist = [ids[0].tolist()] * W
+            for t in range(14):
+                if s.finished():
+                    break
+                tokens, parents = s.advance(model(torch.tensor(hist if t else hist[:1])).logits[:, -1].float())
+                hist = [hist[p] + [v] for v, p in zip(tokens[0].tolist(), parents[0].tolist())]
+            tokens, lengths, _ = s.finish()
+            assert [tokens[0, i, :n].tolist() for i, n in enumerate(lengths[0].tolist())] == ref, seed
+
+
+def _tp_worker(rank, world):
+    from neuronx_distributed_llama3_2_b200.inference import _mock_parallel_state
+    from neuronx_distributed_llama3_2_b200.parallel import parallel_state as ps
+
+    kw = dict(max_context_length=16, seq_len=48, buckets=[16], num_beams=3, eos_token_id=17, use_cuda_graphs=False)
+    with _mock_parallel_state(1, 0):          # one process, before the groups exist
+        torch.manual_seed(0)
+        train = LlamaForCausalLM(tiny_llama(sequence_parallel_enabled=False))
+        with torch.no_grad():
+            train.lm_head.weight.mul_(6.0)
+        sd = {k: v.clone() for k, v in train.state_dict().items()}
+        prompts = torch.randint(20, 512, (2, 13), generator=torch.Generator().manual_seed(5))
+        ref = LlamaInferenceModel(tiny_llama(sequence_parallel_enabled=False), InferenceConfig(batch_size=2, **kw))
+        ref.load_state_dict(sd)
+        want, want_scores = ref.generate_beams(prompts, num_beams=3, max_new_tokens=12, eos_token_id=17, num_return_sequences=3, return_scores=True)
+        ps.set_tensor_model_parallel_size(None)
+        ps.set_tensor_model_parallel_rank(None)
+    ps.initialize_model_parallel(tensor_model_parallel_size=2)
+    for extra in ({}, dict(paged_kv=True, page_size=8, num_kv_pages=40)):
+        r = InferenceRunner(tiny_llama(sequence_parallel_enabled=False), InferenceConfig(batch_size=2, tp_degree=2, **kw, **extra),
+                            checkpoint_loader=lambda: sd, device=torch.device("cpu"))
+        r.trace()
+        got, scores = r.generate_beams(prompts, max_new_tokens=12, num_return_sequences=3, return_scores=True)
+        assert torch.equal(got, want), (rank, got, want)
+        assert bool(((scores - want_scores).abs() <= 1e-4 * want_scores.abs()).all())
+
+
+def test_two_ranks_search_like_one():
+    run_distributed(_tp_worker, 2)
 
 
 # ---- lines and pages of a cache ---------------------------------------------------------------------------------------
