@@ -5,9 +5,9 @@
 // rows are few), with its running maximum and sum of exponentials, and ends with the chunk's n best in order.  A second kernel joins the
 // chunks of a group's rows.
 //   The n best of a chunk: the n-th largest of a few maxima of every warp bounds the n-th largest value from below, so what is not below it is
-// collected (about 1.3 n values of a round as a rule) and ranked by counting; later rounds look only at what is above the n-th so far.  Equal values in
-// numbers (masked ones) do not fit the buffer: the exact n-th key of every round is then found bit by bit and its ties are taken in the order of
-// their indices.
+// collected (about 1.3 n values of a round as a rule) and ranked by counting; later rounds look only at what is above the n-th so far.  Where that
+// is too much (equal values in numbers, values that rise along the row, masks that leave a stretch of it) the rounds are gone through once more with
+// the n-th largest of the threads' best, ties by their indices.
 //   Scores are compared in 64 bits: sums of near size decide between rows.  Within a row the logits decide.
 // Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 26 us for the rows and 6 for the
 // join.  Instructions bound the rows (a conversion, the difference, its scaling, an exponential and two sums per value, about 300 instructions
@@ -23,8 +23,9 @@ namespace {
 constexpr int kMaxN = 64;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 4096;          // chunks of a group
-constexpr int kStages = 3;               // rounds under way
-constexpr int kCollect = 512;            // candidates that a CTA holds
+constexpr int kStages = 2;               // rounds under way
+constexpr int kEasy = 512;               // candidates that are ranked without more ado
+constexpr int kCollect = kMaxN + kMaxN * 32;          // that a CTA holds: those it keeps, and all values of n threads
 constexpr unsigned kFull = 0xffffffffu;
 
 // order-preserving keys; -0 and +0 are one value (the caller adds 0)
@@ -57,17 +58,6 @@ template <typename T> __device__ __forceinline__ float to_float(T x);
 template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ float to_float<bf16>(bf16 x) { return __bfloat162float(x); }
 template <> __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
-
-// Sum over the block's threads; red: 32 ints.
-__device__ __forceinline__ int block_count(int v, int* red) {
-    v = __reduce_add_sync(kFull, v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    int t = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
-    return t;
-}
 
 // What a call leaves for the second kernel: per chunk its maximum, the sum of exponentials behind it, and n entries in order, 0 behind the last.
 struct Lists {
@@ -153,6 +143,17 @@ __device__ __forceinline__ void unpack_vec(const uint4& raw, float* f) {
     unpack_word<T>(raw.w, f + 3 * per);
 }
 
+// What a word's values are above `base`: one instruction a 16-bit value, conversion and difference.
+template <typename T>
+__device__ __forceinline__ void above_word(uint32_t w, float base, float* d) {
+    if constexpr (sizeof(T) == 4)
+        d[0] = __uint_as_float(w) - base;
+    else if constexpr (std::is_same_v<T, bf16>)
+        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tsub.f32.bf16 %0, lo, %3;\n\tsub.f32.bf16 %1, hi, %3;}" : "=f"(d[0]), "=f"(d[1]) : "r"(w), "f"(base));
+    else
+        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tsub.f32.f16 %0, lo, %3;\n\tsub.f32.f16 %1, hi, %3;}" : "=f"(d[0]), "=f"(d[1]) : "r"(w), "f"(base));
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -183,75 +184,47 @@ __device__ __forceinline__ uint32_t kth_of_warp(uint32_t key, int k, int lane) {
     return v;
 }
 
-// Many values, equal ones as a rule: the n-th key of a round bit by bit, then what is above it, then its ties in the order of their indices, behind
-// the `have` candidates that there are.  Reads the round's values once more, so that they hold no registers meanwhile.
+// A round that has more values above the bound than are ranked easily: equal ones, or many in few threads.  The n-th largest of the threads' best
+// entries, found bit by bit (entries differ, so it is one thread's), has n entries that are not below it, all of them in n threads: what is collected
+// behind the `have` candidates fits.  Reads the round's values once more.
 template <typename T, int NT, int NV>
-__device__ __noinline__ int collect_exactly(const T* row, int first, int V, int n, int have, unsigned long long* cand, int* s_count, int* red) {
-    constexpr int VE = Vec<T>::n, kWarps = NT / 32;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __noinline__ int collect_carefully(const T* row, int first, int V, int n, int have, float floor, unsigned long long* cand, int* s_count) {
+    constexpr int VE = Vec<T>::n;
     uint4 raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw[i] = load_vec<T>(row, first + i * NT * VE, V);
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = t | (1u << bit);
-        int mine = 0;
+    unsigned long long best = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[VE];
+        unpack_vec<T>(raw[i], f);
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+            if (f[j] > floor) best = max(best, entry_key(f[j], first + i * NT * VE + j));
+    }
+    if (threadIdx.x == 0) *s_count = have;
+    unsigned long long least = 0;
+    int count = __syncthreads_count(best > 0);
+    for (int bit = 63; bit >= 0 && count > n; --bit) {
+        const unsigned long long c = least | 1ull << bit;
+        const int above = __syncthreads_count(best >= c);
+        if (above >= n) least = c, count = above;
+    }
+    least = max(least, 1ull);
+    if (best >= least) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float f[VE];
             unpack_vec<T>(raw[i], f);
 #pragma unroll
-            for (int j = 0; j < VE; ++j) mine += f[j] == f[j] && order_key(f[j] + 0.f) >= c;
-        }
-        if (block_count(mine, red) >= n) t = c;
-    }
-    const float tie = key_value(max(t, kLowestKey));          // fewer than n finite ones: all of them
-    if (tid == 0) *s_count = have;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float f[VE];
-        unpack_vec<T>(raw[i], f);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            if (f[j] > tie) {                // fewer than n
-                cand[atomicAdd(s_count, 1)] = entry_key(f[j], first + i * NT * VE + j);
+            for (int j = 0; j < VE; ++j) {
+                const unsigned long long e = entry_key(f[j], first + i * NT * VE + j);
+                if (f[j] > floor && e >= least) cand[atomicAdd(s_count, 1)] = e;
             }
         }
     }
     __syncthreads();
-    int filled = *s_count;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float f[VE];
-        unpack_vec<T>(raw[i], f);
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) mine += f[j] == tie;
-        int before = mine;               // of this thread and the ones before it
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(kFull, before, o);
-            if (lane >= o) before += x;
-        }
-        __syncthreads();
-        if (lane == 31) red[warp] = before;
-        __syncthreads();
-        int at = filled + before - mine;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) at += red[w];
-            filled += red[w];
-        }
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            if (f[j] == tie) {
-                if (at < have + n) cand[at] = entry_key(tie, first + i * NT * VE + j);
-                ++at;
-            }
-        }
-    }
-    __syncthreads();
-    return min(filled, have + n);
+    return *s_count;
 }
 
 // A CTA takes `rounds` rounds of 256 threads x NV vectors of one row.  Between rounds it keeps candidates, at least the n best so far; only values above
@@ -265,7 +238,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
     __shared__ unsigned char looker[kWarps][32];
     __shared__ uint32_t warp_top[kWarps], bound_keys[2 * kMaxN];
     __shared__ float warp_sum_of[kWarps];
-    __shared__ int red[32];
     __shared__ unsigned long long best[kMaxN];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -278,14 +250,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
 
     if (tid == 0) s_count = 0;
 #pragma unroll
-    for (int q = 0; q < kStages; ++q) {
+    for (int q = 0; q < kStages - 1; ++q) {
         if (q < rounds) fetch_round<T, NT, NV>(ring + q * (NV * NT), row, first + q * (NT * E), V);
         fetch_commit();
     }
     float top = -INFINITY, sum = 0.f;          // this thread's
     float floor = -INFINITY;                   // only what is above it counts
     int until = 1;                             // the next round that puts the candidates in order
-    bool crowded = false;
+    int since = 0, kept = 0;                   // the first round since, and what was kept then
+    float kept_floor = -INFINITY;
     // the n best candidates in order; eight lanes compare one with all
     auto keep_best = [&](int count) {
         for (int i0 = warp * 4; i0 < count; i0 += NT / 8) {
@@ -304,37 +277,46 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
         if (tid < count) cand[tid] = best[tid];
         if (tid == 0) s_count = count;
         __syncthreads();
-        floor = count == n ? key_value((uint32_t)(best[n - 1] >> 32)) : -INFINITY;
+        kept = count;
+        floor = kept_floor = count == n ? key_value((uint32_t)(best[n - 1] >> 32)) : -INFINITY;
     };
     for (int r = 0; r < rounds; ++r) {
         uint4* stage = ring + r % kStages * (NV * NT);
-        fetch_wait<kStages - 1>();
+        fetch_wait<kStages - 2>();
         uint4 raw[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) raw[i] = stage[i * NT + tid];
+        // into the round before, which the warp is done with; not with the first ones, which would arrive later for it
+        if (r + kStages - 1 < rounds)
+            fetch_round<T, NT, NV>(ring + (r + kStages - 1) % kStages * (NV * NT), row, first + (kStages - 1) * (NT * E), V);
+        fetch_commit();
         float m = max_of<T, NV>(raw) + 0.f;          // no -0; passes NaN by
         {
             // the differences first: a product of the maximum would lose their last bits.  A NaN, or an infinity, makes the sum NaN
             const float big = fmaxf(top, m), base = big == -INFINITY ? 0.f : big;
             if (top != -INFINITY) sum *= exp2_approx((top - base) * kLog2e);
             top = big;
-            const uint64_t away = f2_pack(-base, -base), one = f2_pack(1.f, 1.f), log2e = f2_pack(kLog2e, kLog2e);
+            const uint64_t one = f2_pack(1.f, 1.f), log2e = f2_pack(kLog2e, kLog2e);
             uint64_t part[2] = {0, 0};
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
+                constexpr int per = VE / 4;
                 float f[VE];
-                unpack_vec<T>(raw[i], f);
+                above_word<T>(raw[i].x, base, f);
+                above_word<T>(raw[i].y, base, f + per);
+                above_word<T>(raw[i].z, base, f + 2 * per);
+                above_word<T>(raw[i].w, base, f + 3 * per);
 #pragma unroll
                 for (int j = 0; j < VE; j += 2) {
-                    const uint64_t d = f2_mul(f2_fma(f2_pack(f[j], f[j + 1]), one, away), log2e);
+                    const uint64_t d = f2_mul(f2_pack(f[j], f[j + 1]), log2e);
                     part[j / 2 % 2] = f2_fma(f2_pack(exp2_approx(f2_lo(d)), exp2_approx(f2_hi(d))), one, part[j / 2 % 2]);
                 }
             }
             sum += (f2_lo(part[0]) + f2_hi(part[0])) + (f2_lo(part[1]) + f2_hi(part[1]));
         }
         if (r == 0) {
-            // the largest maxima of each warp that has values, 2 n of them: the n-th of those (its upper 16 bits, all that bf16 has) has n values that are
-            // not below it
+            // the largest maxima of each warp that has values, 2 n of them: the n-th of those (of more than 32 its upper 16 bits) has n values that are not
+            // below it
             const int vecs = (V + mis - split * rounds * (NT * E) + VE - 1) / VE, filled = min(max((vecs + 31) / 32, 1), kWarps);
             const int per = min((2 * n + filled - 1) / filled, min(2 * kMaxN / filled, 32)), keys = filled * per;
             uint32_t key = order_key(m);
@@ -347,10 +329,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
             uint32_t least = 0;
             if (keys <= 32) {
                 const uint32_t own = lane < keys ? bound_keys[lane] : 0;
-                for (int bit = 31; bit >= 16; --bit) {
-                    const uint32_t c = least | 1u << bit;
-                    if (__popc(__ballot_sync(kFull, own >= c)) >= n) least = c;
-                }
+                int before = 0;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) before += __shfl_sync(kFull, own, j) > own;
+                least = __reduce_min_sync(kFull, before < n ? own : kFull);
             } else {
                 uint32_t own[2 * kMaxN / 32];
 #pragma unroll
@@ -383,32 +365,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
             }
             __syncwarp();
         }
-        if (r + kStages < rounds) fetch_round<T, NT, NV>(stage, row, first + kStages * (NT * E), V);          // the warp is done with its part
-        fetch_commit();
         if (r == until || r + 1 == rounds) {
             __syncthreads();
             const int count = s_count;
-            if (count > kCollect) {
-                crowded = true;                  // more than there is room for: the rest only adds up
-                floor = INFINITY;
-                until = rounds;
-            } else if (!crowded) {
+            if (count <= kEasy) {
                 keep_best(count);
-                until = 4 * r + 2;          // 1, 6, 26: few pass the bound between these
+            } else {          // the rounds since the last time once more, one by one
+                __syncthreads();
+                floor = kept_floor;
+                for (int q = since; q <= r; ++q) keep_best(collect_carefully<T, NT, NV>(row, first - (r - q) * (NT * E), V, n, kept, floor, cand, &s_count));
             }
+            since = r + 1;
+            until = 4 * r + 3;          // 1, 7, 31: at most 3 n or so pass the bound between these
         }
         first += NT * E;
     }
     pdl_trigger();
-    if (crowded) {
-        int count = 0;
-        for (int q = 0; q < rounds; ++q) {
-            __syncthreads();
-            count = collect_exactly<T, NT, NV>(row, split * rounds * (NT * E) + q * (NT * E) + tid * VE - mis, V, n, count, cand, &s_count, red);
-            keep_best(count);
-            count = min(count, n);
-        }
-    }
     const uint32_t block_key = __reduce_max_sync(kFull, order_key(top));
     if (lane == 0) warp_top[warp] = block_key;
     __syncthreads();
