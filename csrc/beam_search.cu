@@ -9,9 +9,9 @@
 // is too much (equal values in numbers, values that rise along the row, masks that leave a stretch of it) the rounds are gone through once more with
 // the n-th largest of the threads' best, ties by their indices.
 //   Scores are compared in 64 bits: sums of near size decide between rows.  Within a row the logits decide.
-// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 26 us for the rows and 6 for the
-// join.  Instructions bound the rows (a conversion, the difference, its scaling, an exponential and two sums per value, about 300 instructions
-// for the 1024 values of a warp's round with everything else), and 256 rows on 148 SMs; one request of 4 rows takes 4.7 and 5.4 us of latency.
+// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 21 us for the rows and 6 for the
+// join (rows in rising order, every round of which has too many: 170).  Instructions bound the rows (a difference with its conversion, its
+// scaling, an exponential and two sums per value), and 256 rows on 148 SMs; one request of 4 rows takes 4.4 and 4.9 us of latency.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -23,7 +23,7 @@ namespace {
 constexpr int kMaxN = 64;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 4096;          // chunks of a group
-constexpr int kStages = 2;               // rounds under way
+constexpr int kStages = 2;               // rounds under way (3: 22.7 instead of 21.6 us, 4 leave one CTA an SM)
 constexpr int kEasy = 512;               // candidates that are ranked without more ado
 constexpr int kCollect = kMaxN + kMaxN * 32;          // that a CTA holds: those it keeps, and all values of n threads
 constexpr unsigned kFull = 0xffffffffu;
@@ -842,7 +842,7 @@ struct Split {
 };
 
 // Rounds of 512 threads x 4 vectors where that leaves no SM without a CTA, as many of them per CTA as leave one wave (two CTAs an SM): every CTA pays
-// for its first bound and for putting candidates in order (256 rows of 128256: one CTA a row 29 us, two 31 to 36, four 33, eight 38).  Rounds of 256 x 2
+// for its first bound and for putting candidates in order (256 rows of 128256: one CTA a row 22 us, two of 256 threads 25).  Rounds of 256 x 2
 // where rows are few (4 rows: 4.7 us, with 256 x 4 5.0).
 Split split_of(long long rows, int W, int V, int elem) {
     const int per_vec = 16 / elem;
