@@ -76,17 +76,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
     ``-inf`` and beams with the score ``-inf`` are left out, and so is a beam whose logits hold NaN or ``+inf``, or nothing finite; where fewer
     than ``n`` candidates are left the rest have the score ``-inf``, from the lowest ``w * V + v`` on.  Scores are compared in 64 bits; tokens of one
     beam by their logits.  Returns ``(scores [B, n] fp32, beams [B, n] int64, tokens [B, n] int64)``; not differentiable."""
-    if scores.dim() != 2 or scores.dtype is not torch.float32:
-        raise ValueError(f"scores: an fp32 tensor [B, W] is expected, not {scores.dtype} {tuple(scores.shape)}")
-    B, W = scores.shape
-    if logits.dim() not in (2, 3) or logits.shape[:-1] != ((B, W) if logits.dim() == 3 else (B * W,)):
-        raise ValueError(f"logits {tuple(logits.shape)} do not go with scores of {B} x {W} beams")
+    shape, sizes = scores.shape, logits.shape
+    if len(shape) != 2 or scores.dtype is not torch.float32:
+        raise ValueError(f"scores: an fp32 tensor [B, W] is expected, not {scores.dtype} {tuple(shape)}")
+    B, W = shape
+    if not (len(sizes) == 3 and sizes[0] == B and sizes[1] == W or len(sizes) == 2 and sizes[0] == B * W):
+        raise ValueError(f"logits {tuple(sizes)} do not go with scores of {B} x {W} beams")
     if not logits.is_floating_point():
         raise ValueError(f"logits of {logits.dtype} are no floating-point numbers")
     if logits.get_device() != scores.get_device():
         raise ValueError(f"logits on {logits.device}, scores on {scores.device}")
-    V = logits.shape[-1]
-    n = int(n)
+    V, n = sizes[-1], int(n)
     if not 1 <= n <= MAX_CANDIDATES:
         raise ValueError(f"between 1 and {MAX_CANDIDATES} candidates are taken, not {n}")
     if not 1 <= W <= MAX_BEAMS:
@@ -95,26 +95,27 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
         raise ValueError(f"{n} candidates are more than {W} beams of {V} tokens have")
     if not _kernel(logits):
         return beam_select_ref(logits, scores, n)
-    if logits.dtype not in _DTYPES:
+    code = _DTYPES.get(logits.dtype)
+    if code is None:
         raise ValueError(f"logits of {logits.dtype} are not taken on the GPU: fp32, bf16 or fp16")
-    if logits.dim() == 3 and not (W == 1 or B == 1 or logits.stride(0) == W * logits.stride(1)) or (logits.stride(-1) != 1 and V != 1):
+    strides = logits.stride()
+    if (strides[-1] != 1 and V != 1) or len(sizes) == 3 and W > 1 and B > 1 and strides[0] != W * strides[1]:
         logits = logits.contiguous()
-    stride = (logits.stride(1) if W > 1 else logits.stride(0)) if logits.dim() == 3 else logits.stride(0)
-    scores = scores.contiguous()
-    code, device = _DTYPES[logits.dtype], logits.device
-    out = torch.empty((2, B, n), dtype=torch.int64, device=device)
-    best = scores.new_empty((B, n))
+        strides = logits.stride()
+    if not scores.is_contiguous():
+        scores = scores.contiguous()
+    tokens = torch.empty((B, n), dtype=torch.int64, device=logits.device)
+    beams, best = torch.empty_like(tokens), scores.new_empty((B, n))
     if B:
         with _lib.on_device_of(logits):
             size = _scratch_bytes(code, B, W, V, n)
             if size <= 0:
                 raise ValueError(f"{W} beams of {V} tokens are more than one call takes")
             scratch = scores.new_empty((size + 3) // 4)          # the call's own
-            at = out.data_ptr()
-            rc = _entry("nxd_beam_select")(code, logits.data_ptr(), stride, scores.data_ptr(), B, W, V, n, scratch.data_ptr(), best.data_ptr(), at,
-                                           at + 8 * B * n, _lib.stream_ptr())
+            rc = _entry("nxd_beam_select")(code, logits.data_ptr(), strides[1] if len(sizes) == 3 and W > 1 else strides[0], scores.data_ptr(), B, W, V, n,
+                                           scratch.data_ptr(), best.data_ptr(), beams.data_ptr(), tokens.data_ptr(), _lib.stream_ptr())
         _lib.check(rc, "nxd_beam_select")
-    return best, out[0], out[1]          # an index costs a third of unbind()
+    return best, beams, tokens
 
 
 @functools.lru_cache(maxsize=1024)
@@ -272,7 +273,7 @@ def beam_finish(scores: torch.Tensor, pool: BeamPool, history: BeamHistory, step
     if B > 65535:
         raise ValueError(f"{B} requests are more than 65535")
     tokens = torch.empty((B, W, step), dtype=torch.int64, device=dev)
-    lengths = torch.empty((B, W), dtype=torch.int64, device=dev)
+    lengths = tokens.new_empty((B, W))
     best = torch.empty_like(scores)
     with _lib.on_device_of(scores):
         scratch = None
