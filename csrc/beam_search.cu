@@ -227,8 +227,8 @@ __device__ __noinline__ int collect_carefully(const T* row, int first, int V, in
     return *s_count;
 }
 
-// A CTA takes `rounds` rounds of 256 threads x NV vectors of one row.  Between rounds it keeps candidates, at least the n best so far; only values above
-// the n-th of those are looked at further.
+// A CTA takes `rounds` rounds of NT threads x NV vectors of one row.  It keeps candidates, at least the n best so far; only values above the n-th of
+// those, when they were last put in order, are looked at further.
 template <typename T, int NT, int NV>
 __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __restrict__ logits, int V, long long stride, int splits, int rounds, int n,
                                                                    Lists out) {
