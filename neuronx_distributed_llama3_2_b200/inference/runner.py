@@ -257,7 +257,7 @@ class InferenceRunner:
         if Tb < 2 or min(lengths) < 1 or max(lengths) + max_new - 1 > ic.seq_len:
             raise ValueError(f"prompts of {min(lengths)} to {max(lengths)} tokens (bucket {Tb}) and {max_new} more do not fit a cache of {ic.seq_len}")
         if cache.pool is not None:
-            for line in range(cache.lines):
+            for line in range(max(Bc * W, Bt)):
                 cache.free(line)
             for b in range(Bc):
                 cache.reserve(b * W, Tb)

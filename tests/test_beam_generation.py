@@ -207,6 +207,23 @@ def _tp_worker(rank, world):
         assert bool(((scores - want_scores).abs() <= 1e-4 * want_scores.abs()).all())
 
 
+def test_lines_that_no_beam_has_keep_their_pages():
+    torch.manual_seed(0)
+    train = LlamaForCausalLM(tiny_llama(sequence_parallel_enabled=False))
+    ic = InferenceConfig(batch_size=2, num_beams=2, max_batch_size=6, max_context_length=16, seq_len=32, buckets=[16], paged_kv=True, page_size=8, num_kv_pages=40)
+    r = InferenceRunner(tiny_llama(sequence_parallel_enabled=False), ic, checkpoint_loader=train.state_dict, device=torch.device("cpu"))
+    r.trace()
+    cache = r.model.kv_cache
+    cache.reserve(5, 11)
+    pages = cache.pool.block_row(5)[0][:2]
+    for t in cache._tensors():
+        t[pages] = 3.0
+    for B in (2, 1):
+        r.generate_beams(torch.randint(1, 500, (B, 9)), max_new_tokens=6)
+    assert cache.pool.line_tokens(5) == 11 and cache.pool.block_row(5)[0][:2] == pages
+    assert all(bool((t[pages] == 3.0).all()) for t in cache._tensors())
+
+
 def test_two_ranks_search_like_one():
     run_distributed(_tp_worker, 2)
 
