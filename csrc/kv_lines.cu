@@ -1,14 +1,16 @@
 // Whole lines and pages of a key/value cache, in every layer at once: lines that continue other lines (beam search), and pages that are copied
 // (a line forks, a shared page is about to be written, a pool is compacted).
 //
-// Both only move bytes, so HBM bounds them: 699 MB (16 layers, 32 lines of up to 900 rows, recurrent states) are 107 us at 6555 GB/s and take 124; 1007 MB of
+// Both only move bytes, so HBM bounds them: 699 MB (16 layers, 32 lines of up to 900 rows, recurrent states) are 107 us at 6555 GB/s and take 120; 1007 MB of
 // pages are 154 us and take 156.  All tensors of one shape share a launch; their addresses travel as kernel parameters.
 #include "common.cuh"
+#include "nxd_b200.h"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTensors = 256;          // of a launch: 2 KB of parameters
+constexpr int kMaxTensors = 256;          // of a launch of page copies: 2 KB of parameters
+constexpr int kJobTensors = 128;          // of one of the two shapes of a launch of lines
 constexpr int kMaxBeams = 32;
 constexpr int kDeep = 4;                  // units of a thread
 
@@ -71,13 +73,29 @@ __device__ __forceinline__ void order_moves(int from, int lane, Moves& m) {
 // apart, of all the group's lines in an order that works in place, so there is no scratch and each line that is wanted is read once from memory
 // however many continue it.  Two moves of four units are read before the first of them is written (one unit: 147 us instead of 111 for the layers of the
 // case above).  Circles go one unit at a time, at 0.7 of that rate; no step of a search makes one.
-//   With a table the lines are pages: PAGED.
+//   With a table the lines are pages: PAGED.  Two shapes share a launch (keys and values, and a recurrent state): the first blocks are one's, the
+// others the other's (the case above: 120 us instead of 124).
+struct Job {
+    char* base[kJobTensors];
+    int n, num_pages;
+    bool whole;                           // all rows, whatever start and end are
+    unsigned first, blocks;
+    Shape s;
+};
+struct Jobs {
+    Job job[2];
+};
+
 template <typename U, bool PAGED>
-__global__ void __launch_bounds__(kThreads, PAGED ? 3 : 4) reorder_lines_kernel(const __grid_constant__ Tensors t, Shape s, int W, const long long* __restrict__ parents,
-                                                                    const long long* __restrict__ start, const long long* __restrict__ end,
-                                                                    const int* __restrict__ table, int page_size, int max_pages, int num_pages) {
+__global__ void __launch_bounds__(kThreads, PAGED ? 3 : 4) reorder_lines_kernel(const __grid_constant__ Jobs jobs, int W, const long long* __restrict__ parents,
+                                                                                const long long* __restrict__ start, const long long* __restrict__ end,
+                                                                                const int* __restrict__ table, int page_size, int max_pages) {
     __shared__ Moves moves;
     const int g = blockIdx.y;
+    const Job& t = jobs.job[blockIdx.x >= jobs.job[1].first];
+    const Shape s = t.s;
+    const unsigned block = blockIdx.x - t.first;
+    const int num_pages = t.num_pages;
     const long long line0 = (long long)g * W;
     if (threadIdx.x < 32) {
         const int w = threadIdx.x;
@@ -87,11 +105,11 @@ __global__ void __launch_bounds__(kThreads, PAGED ? 3 : 4) reorder_lines_kernel(
     }
     __syncthreads();
     const int n = moves.n;
-    const long long lo = start != nullptr ? max(start[g], 0LL) : 0, hi = end != nullptr ? min(end[g], (long long)s.rows) : s.rows;
+    const long long lo = !t.whole && start != nullptr ? max(start[g], 0LL) : 0, hi = !t.whole && end != nullptr ? min(end[g], (long long)s.rows) : s.rows;
     if (n == 0 || hi <= lo) return;
     const unsigned per_head = (unsigned)(hi - lo) * (unsigned)s.per_row, per_tensor = per_head * (unsigned)s.heads;
     const unsigned total = per_tensor * (unsigned)t.n;          // the host keeps it below 2^31
-    for (unsigned i0 = blockIdx.x * (kThreads * kDeep) + threadIdx.x; i0 < total; i0 += gridDim.x * (kThreads * kDeep)) {
+    for (unsigned i0 = block * (kThreads * kDeep) + threadIdx.x; i0 < total; i0 += t.blocks * (kThreads * kDeep)) {
         char* base[kDeep];          // of a unit in the group's first line, or in page 0
         int page[PAGED ? kDeep : 1];
 #pragma unroll
@@ -207,13 +225,6 @@ int unit_of(void* const* base, int n, long long row_bytes, long long line_stride
     return (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : (all & 1) == 0 ? 2 : 1;
 }
 
-template <typename U>
-void launch_reorder(dim3 grid, cudaStream_t st, const Tensors& t, const Shape& s, int W, const long long* parents, const long long* start,
-                    const long long* end, const int* table, int page_size, int max_pages, int num_pages) {
-    if (table == nullptr) reorder_lines_kernel<U, false><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-    else reorder_lines_kernel<U, true><<<grid, kThreads, 0, st>>>(t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-}
-
 // Blocks beside each other for one group or pair: what its units can use, up to four waves.  (16 layers, 32 lines of 900 rows: one wave 136 us, two 130,
 // four 124, sixteen 121; but a block without work costs its start, and the host does not know the ranges.)
 unsigned blocks_for(long long units, long long per_block, long long beside) {
@@ -226,31 +237,55 @@ constexpr long long kMaxUnits = (1LL << 31) - (1LL << 22);          // of a grou
 
 }  // namespace
 
-// n tensors of one shape at `base` (host array of device addresses): [lines, heads, rows, row_bytes] or, with a block table
-// [lines, max_pages], pages [num_pages, heads, page_size, row_bytes]; strides in bytes, rows side by side.
-NXD_API int nxd_reorder_lines(void* const* base, int n, int heads, long long rows, long long row_bytes, long long line_stride, long long head_stride,
-                              int groups, int W, const long long* parents, const long long* start, const long long* end, const int* table,
-                              int page_size, int max_pages, int num_pages, void* stream) {
+// The header has the arrays.  Shapes whose widest unit is the same go two to a launch.
+NXD_API int nxd_reorder_lines(const nxd_lines* kinds, int n_kinds, int groups, int W, const long long* parents, const long long* start, const long long* end,
+                              const int* table, int page_size, int max_pages, void* stream) {
     NXD_REQUIRE(W >= 1 && W <= kMaxBeams, "reorder_lines: %d lines of a group are not between 1 and %d", W, kMaxBeams);
     NXD_REQUIRE(groups >= 0 && groups <= 65535, "reorder_lines: %d groups are more than 65535", groups);
-    if (n == 0 || groups == 0 || rows == 0 || row_bytes == 0 || heads == 0) return 0;
-    const int unit = unit_of(base, n, row_bytes, line_stride, head_stride);
-    const long long per_row = row_bytes / unit, per_tensor = rows * per_row * heads;
-    NXD_REQUIRE(per_tensor <= kMaxUnits, "reorder_lines: a line of %lld rows of %lld bytes in %d heads is too long", rows, row_bytes, heads);
-    const int most = (int)(kMaxUnits / per_tensor < kMaxTensors ? kMaxUnits / per_tensor : kMaxTensors);
-    for (int at = 0; at < n; at += most) {
-        Tensors t;
-        t.n = n - at < most ? n - at : most;
-        for (int i = 0; i < kMaxTensors; ++i) t.base[i] = i < t.n ? (char*)base[at + i] : nullptr;
-        const Shape s = {heads, (int)rows, (int)per_row, line_stride, head_stride};
-        const dim3 grid(blocks_for(per_tensor * t.n, kThreads * kDeep, groups), groups);
-        cudaStream_t st = (cudaStream_t)stream;
-        if (unit == 16) launch_reorder<uint4>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-        else if (unit == 4) launch_reorder<uint32_t>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-        else if (unit == 2) launch_reorder<uint16_t>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-        else launch_reorder<uint8_t>(grid, st, t, s, W, parents, start, end, table, page_size, max_pages, num_pages);
-        NXD_LAUNCH_CHECK();
+    if (groups == 0) return 0;
+    Jobs jobs;
+    int held = 0, held_unit = 0;
+    bool held_paged = false;
+    cudaStream_t st = (cudaStream_t)stream;
+    auto launch = [&]() -> cudaError_t {
+        if (held == 0) return cudaSuccess;
+        jobs.job[0].first = 0;
+        jobs.job[1].first = jobs.job[0].blocks;          // of one job: behind the last block
+        const dim3 grid(jobs.job[0].blocks + (held > 1 ? jobs.job[1].blocks : 0), groups);
+        held = 0;
+#define NXD_REORDER(U)                                                                                                                          \
+    (held_paged ? reorder_lines_kernel<U, true><<<grid, kThreads, 0, st>>>(jobs, W, parents, start, end, table, page_size, max_pages)           \
+                : reorder_lines_kernel<U, false><<<grid, kThreads, 0, st>>>(jobs, W, parents, start, end, nullptr, 0, 0))
+        if (held_unit == 16) NXD_REORDER(uint4);
+        else if (held_unit == 4) NXD_REORDER(uint32_t);
+        else if (held_unit == 2) NXD_REORDER(uint16_t);
+        else NXD_REORDER(uint8_t);
+#undef NXD_REORDER
+        nxd_count_launches(1);
+        return cudaGetLastError();
+    };
+    for (int k = 0; k < n_kinds; ++k) {
+        const nxd_lines& d = kinds[k];
+        const bool paged = table != nullptr && !d.whole;
+        const long long rows = paged ? (long long)page_size * max_pages : d.rows;
+        if (d.n == 0 || rows == 0 || d.row_bytes == 0 || d.heads == 0) continue;
+        const int unit = unit_of(d.base, d.n, d.row_bytes, d.line_stride, d.head_stride);
+        const long long per_row = d.row_bytes / unit, per_tensor = rows * per_row * d.heads;
+        NXD_REQUIRE(per_tensor <= kMaxUnits, "reorder_lines: a line of %lld rows of %lld bytes in %d heads is too long", rows, d.row_bytes, d.heads);
+        const int most = (int)(kMaxUnits / per_tensor < kJobTensors ? kMaxUnits / per_tensor : kJobTensors);
+        for (int at = 0; at < d.n; at += most) {
+            if (held == 2 || (held == 1 && (held_unit != unit || held_paged != paged))) NXD_CHECK_CUDA(launch());
+            Job& j = jobs.job[held++];
+            held_unit = unit, held_paged = paged;
+            j.n = d.n - at < most ? d.n - at : most;
+            for (int i = 0; i < j.n; ++i) j.base[i] = (char*)d.base[at + i];
+            j.num_pages = d.pages;
+            j.whole = d.whole != 0;
+            j.s = {d.heads, (int)rows, (int)per_row, d.line_stride, d.head_stride};
+            j.blocks = blocks_for(per_tensor * j.n, kThreads * kDeep, groups);
+        }
     }
+    NXD_CHECK_CUDA(launch());
     return 0;
 }
 

@@ -132,12 +132,18 @@ int nxd_beam_finish(const float* running, const float* pool_scores, const int* p
                     long long* tokens, long long* lengths, float* scores, void* scratch, void* stream);
 
 /* ---- cache lines and pages (csrc/kv_lines.cu) -------------------------------------------------------
- * n tensors of one shape at `base` (a HOST array of device addresses), strides and rows in bytes.  reorder: line g * W + w becomes what line
- * g * W + parents[g, w] was, rows [start[g], end[g]) (NULL: all), in place; with a block table [lines, max_pages] the tensors are pages.
- * copy: page dst[i] becomes page src[i], its first used[i] rows of every head (NULL: all). */
-int nxd_reorder_lines(void* const* base, int n, int heads, long long rows, long long row_bytes, long long line_stride, long long head_stride,
-                      int groups, int W, const long long* parents, const long long* start, const long long* end, const int* table,
-                      int page_size, int max_pages, int num_pages, void* stream);
+ * n tensors of one shape at `base` (a HOST array of device addresses), strides and rows in bytes.  reorder: line g * W + w of every shape becomes
+ * what line g * W + parents[g, w] was, rows [start[g], end[g]) (NULL: all; `whole`: all anyway), in place; with a block table [lines, max_pages] the
+ * tensors that are not whole are `pages` pages of page_size rows.  copy: page dst[i] becomes page src[i], its first used[i] rows of every head
+ * (NULL: all). */
+typedef struct {
+    void* const* base;
+    int n, heads;
+    long long rows, row_bytes, line_stride, head_stride;
+    int pages, whole;
+} nxd_lines;
+int nxd_reorder_lines(const nxd_lines* kinds, int n_kinds, int groups, int W, const long long* parents, const long long* start, const long long* end,
+                      const int* table, int page_size, int max_pages, void* stream);
 int nxd_copy_pages(void* const* base, int n, int pages, int heads, long long rows, long long row_bytes, long long page_stride,
                    long long head_stride, int pairs, const long long* src, const long long* dst, const long long* used, void* stream);
 

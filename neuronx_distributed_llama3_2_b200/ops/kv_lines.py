@@ -12,7 +12,7 @@ from . import _lib
 MAX_BEAMS = 32
 _P, _I, _L = _c.c_void_p, _c.c_int, _c.c_longlong
 _ARGS = {
-    "nxd_reorder_lines": [_P, _I, _I, _L, _L, _L, _L, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P],
+    "nxd_reorder_lines": [_P, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P],
     "nxd_copy_pages": [_P, _I, _I, _I, _L, _L, _L, _L, _I, _P, _P, _P, _P],
 }
 
@@ -24,11 +24,16 @@ def _entry(name: str):
     return fn
 
 
-class _Alike:
-    """Tensors of one shape: their addresses for a launch."""
+class _Kind(_c.Structure):          # nxd_lines
+    _fields_ = [("base", _P), ("n", _I), ("heads", _I), ("rows", _L), ("row_bytes", _L), ("line_stride", _L), ("head_stride", _L), ("pages", _I),
+                ("whole", _I)]
 
-    def __init__(self, key: tuple):
-        self.key, self.tensors, self.at = key, [], []
+
+class _Alike:
+    """Tensors of one shape: ``key`` is lines or pages, heads, rows, bytes of a row, strides of lines and heads in bytes."""
+
+    def __init__(self, key: tuple, whole: bool):
+        self.key, self.whole, self.tensors, self.at = key, whole, [], []
 
     def addresses(self):
         at = [f() for f in self.where]
@@ -59,7 +64,7 @@ class CacheTensors:
                 raise ValueError(f"cache tensors on {self.device} and on {t.device}")
             size = t.element_size()
             key = (t.shape[0], t.shape[1], t.shape[2], t.shape[3] * size, t.stride(0) * size, t.stride(1) * size)
-            kinds[0].setdefault(key, _Alike(key)).tensors.append(t)
+            kinds[0].setdefault(key, _Alike(key, False)).tensors.append(t)
         for t in self.states:
             if t.dim() < 1 or (t.shape[0] and not t[0].is_contiguous()):
                 raise ValueError(f"a state [lines, ...] with a line's values side by side is expected, not {tuple(t.shape)} with strides {t.stride()}")
@@ -68,7 +73,7 @@ class CacheTensors:
             size = t.element_size()
             line = t[0].numel() * size if t.shape[0] else 0
             key = (t.shape[0], 1, 1, line, t.stride(0) * size, line)
-            kinds[1].setdefault(key, _Alike(key)).tensors.append(t)
+            kinds[1].setdefault(key, _Alike(key, True)).tensors.append(t)
         self.kinds, self.state_kinds = list(kinds[0].values()), list(kinds[1].values())
         for kind in self.kinds + self.state_kinds:
             kind.where = [t.data_ptr for t in kind.tensors]
@@ -76,6 +81,9 @@ class CacheTensors:
         self.lines = min(t.shape[0] for t in self.cache + self.states)
         self.state_lines = min((t.shape[0] for t in self.states), default=None)
         self.cuda = self.device.type == "cuda"
+        self.every = self.kinds + self.state_kinds
+        self.table = (_Kind * len(self.every))(*[_Kind(0, len(k.tensors), k.key[1], k.key[2], k.key[3], k.key[4], k.key[5], k.key[0], k.whole)
+                                                 for k in self.every])
 
 
 def _laid_out(cache: Union[CacheTensors, Sequence[torch.Tensor]], states: Sequence[torch.Tensor] = ()) -> CacheTensors:
@@ -120,21 +128,13 @@ def reorder_lines_(cache: Union[CacheTensors, Sequence[torch.Tensor]], parents: 
         return _reorder_ref(c, parents, start, end, table, page_size)
     if B > 65535:
         raise ValueError(f"{B} groups are more than 65535")
-    fn = _entry("nxd_reorder_lines")
+    for kind, entry in zip(c.every, c.table):
+        entry.base = _c.addressof(kind.addresses())
     with _lib.on_device_of(parents):
-        stream = _lib.stream_ptr()
-        s, e = 0 if start is None else start.data_ptr(), 0 if end is None else end.data_ptr()
-        for k in c.kinds:
-            lead, heads, rows, row, line, head = k.key
-            if table is None:
-                rc = fn(k.addresses(), len(k.at), heads, rows, row, line, head, B, W, parents.data_ptr(), s, e, 0, 0, 0, 0, stream)
-            else:
-                rc = fn(k.addresses(), len(k.at), heads, table.shape[1] * page_size, row, line, head, B, W, parents.data_ptr(), s, e,
-                        table.data_ptr(), page_size, table.shape[1], lead, stream)
-            _lib.check(rc, "nxd_reorder_lines")
-        for k in c.state_kinds:
-            rc = fn(k.addresses(), len(k.at), 1, 1, k.key[3], k.key[4], k.key[5], B, W, parents.data_ptr(), 0, 0, 0, 0, 0, 0, stream)
-            _lib.check(rc, "nxd_reorder_lines")
+        rc = _entry("nxd_reorder_lines")(c.table, len(c.every), B, W, parents.data_ptr(), 0 if start is None else start.data_ptr(),
+                                         0 if end is None else end.data_ptr(), 0 if table is None else table.data_ptr(), page_size,
+                                         0 if table is None else table.shape[1], _lib.stream_ptr())
+    _lib.check(rc, "nxd_reorder_lines")
 
 
 def _reorder_ref(c: CacheTensors, parents, start, end, table, page_size) -> None:
