@@ -24,6 +24,7 @@ constexpr int kMaxN = 64;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 4096;          // chunks of a group
 constexpr int kStages = 2;               // rounds under way (3: 22.7 instead of 21.6 us, 4 leave one CTA an SM)
+constexpr int kMany = 384;               // candidates that are all compared with each other (2048 rows of 500, 64 of them wanted: 189 us, with the search 116)
 constexpr int kEasy = 512;               // candidates that are ranked without more ado
 constexpr int kCollect = kMaxN + kMaxN * 32;          // that a CTA holds: those it keeps, and all values of n threads
 constexpr unsigned kFull = 0xffffffffu;
@@ -259,8 +260,28 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
     int until = 1;                             // the next round that puts the candidates in order
     int since = 0, kept = 0;                   // the first round since, and what was kept then
     float kept_floor = -INFINITY;
-    // the n best candidates in order; eight lanes compare one with all
+    // the n best candidates in order; eight lanes compare one with all, of many only the n best, found bit by bit
     auto keep_best = [&](int count) {
+        if (count > kMany && count > 2 * n) {
+            unsigned long long least = 0;
+            int above = count;
+            for (int bit = 63; bit >= 0 && above > n; --bit) {
+                const unsigned long long c = least | 1ull << bit;
+                int now = 0;
+                for (int i = tid; i - tid < count; i += NT) now += __syncthreads_count(i < count && cand[i] >= c);
+                if (now >= n) least = c, above = now;
+            }
+            if (tid == 0) s_count = 0;
+            __syncthreads();
+            for (int i = tid; i < count; i += NT) {
+                const unsigned long long e = cand[i];
+                if (e >= least) best[atomicAdd(&s_count, 1)] = e;
+            }
+            __syncthreads();
+            if (tid < n) cand[tid] = best[tid];
+            count = n;
+            __syncthreads();
+        }
         for (int i0 = warp * 4; i0 < count; i0 += NT / 8) {
             const int i = i0 + lane / 8;
             const unsigned long long own = i < count ? cand[i] : ~0ull;
@@ -843,12 +864,13 @@ struct Split {
 
 // Rounds of 512 threads x 4 vectors where that leaves no SM without a CTA, as many of them per CTA as leave one wave (two CTAs an SM): every CTA pays
 // for its first bound and for putting candidates in order (256 rows of 128256: one CTA a row 22 us, two of 256 threads 25).  Rounds of 256 x 2
-// where rows are few (4 rows: 4.7 us, with 256 x 4 5.0).
+// where rows are few (4 rows: 4.7 us, with 256 x 4 5.0) or no longer than two of them (512 rows of 2000: 12 us instead of 23, of 5000 14 instead of 22; of
+// 16000 16 instead of 17, and 256 rows of 16000 14 instead of 12).
 Split split_of(long long rows, int W, int V, int elem) {
     const int per_vec = 16 / elem;
     const long long sms = nxd_num_sms(), span = V + per_vec - 1, large = 512LL * 4 * per_vec;
     Split s;
-    const bool few = rows * ((span + large - 1) / large) < sms;
+    const bool few = rows * ((span + large - 1) / large) < sms || span <= 2 * 512LL * per_vec;
     s.threads = few ? 256 : 512;
     s.vecs = few ? 2 : 4;
     const long long round = (long long)s.threads * s.vecs * per_vec, chunks = (span + round - 1) / round;
