@@ -9,7 +9,7 @@
 // is too much (equal values in numbers, values that rise along the row, masks that leave a stretch of it) the rounds are gone through once more with
 // the n-th largest of the threads' best, ties by their indices.
 //   Scores are compared in 64 bits: sums of near size decide between rows.  Within a row the logits decide.
-// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 21 us for the rows and 6 for the
+// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 21 us for the rows and 4 for the
 // join (rows in rising order, every round of which has too many: 170).  Instructions bound the rows (a difference with its conversion, its
 // scaling, an exponential and two sums per value), and 256 rows on 148 SMs; one request of 4 rows takes 4.4 and 4.9 us of latency.
 #include <cuda_fp16.h>
@@ -23,6 +23,8 @@ namespace {
 constexpr int kMaxN = 64;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 4096;          // chunks of a group
+constexpr int kOwn = 2;                  // entries of a thread of the join where that is all (32 groups of 8 lists of 16: 4.4 us, by their heads 5.9; with four
+                                         // entries, one group of 128 lists of 8: 5.6, by their heads 4.9)
 constexpr int kStages = 2;               // rounds under way (3: 22.7 instead of 21.6 us, 4 leave one CTA an SM)
 constexpr int kMany = 384;               // candidates that are all compared with each other (2048 rows of 500, 64 of them wanted: 189 us, with the search 116)
 constexpr int kEasy = 512;               // candidates that are ranked without more ado
@@ -433,8 +435,8 @@ __device__ __forceinline__ int rank_by_eight(const unsigned long long* score, co
     return before;
 }
 
-// One CTA joins the lists of one group's rows.  Every list is in order, so its head is its best: the n lists with the best heads hold
-// the n best values, and none of those is below the n-th head.
+// One CTA joins the lists of one group's rows: up to two entries a thread are all looked at.  Of more, every list being in order, its head is
+// its best: the n lists with the best heads hold the n best values, and none of those is below the n-th head.
 __global__ void __launch_bounds__(1024, 1) beam_join_kernel(const float* __restrict__ scores, int W, int V, int splits, int n, int room, Lists in,
                                                             float* __restrict__ out_scores, long long* __restrict__ out_beams,
                                                             long long* __restrict__ out_tokens) {
@@ -454,7 +456,15 @@ __global__ void __launch_bounds__(1024, 1) beam_join_kernel(const float* __restr
     if (tid == 0) s_count = s_heads = 0;
     if (tid < 2 * kMaxN) used[tid] = 0;
     pdl_wait();
-    const unsigned long long first = lane * warps + warp < lists ? in.entry[(l0 + lane * warps + warp) * n] : 0;          // of this thread's first list
+    // what a thread reads first: up to kOwn entries around the warps if that is all of them, else the head of its first list
+    const bool all = lists * n <= kOwn * nth;
+    auto place = [&](int q) { return q * nth + lane * warps + (warp + lane & warps - 1); };          // every warp has heads of lists
+    unsigned long long first[kOwn];
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+        const int e = all ? place(q) : lane * warps + warp;
+        first[q] = all ? (e < lists * n ? in.entry[l0 * n + e] : 0) : q == 0 && e < lists ? in.entry[(l0 + e) * n] : 0;
+    }
     for (int w = warp; w < W; w += warps) {
         const float2* part = in.sum + l0 + (long long)w * splits;
         const float own = scores[g * W + w];
@@ -478,65 +488,89 @@ __global__ void __launch_bounds__(1024, 1) beam_join_kernel(const float* __restr
     auto score_of = [&](unsigned long long entry, int w) -> unsigned long long {          // as a key, that of -inf where there is none
         return order_key(entry != 0 && so_far[w] > -INFINITY ? so_far[w] + ((double)key_value((uint32_t)(entry >> 32)) - lse[w]) : -INFINITY);
     };
-    // lists go around the warps; of the best heads of its threads each warp has a k-th largest, warps * k >= n
+    // of its threads' best each warp has a k-th largest, warps * k >= n: the least of those has n scores that are not below it
     const int k = (n + warps - 1) / warps;
-    uint32_t own = 0;
-    for (int l = lane * warps + warp; l < lists; l += nth) {
-        const unsigned long long h = score_of(l < nth ? first : in.entry[(l0 + l) * n], l / splits);
-        head[l] = h;
-        own = max(own, (uint32_t)(h >> 32));
-    }
-    uint32_t kth = kth_of_warp(own, k, lane);
-    if (lane == 0) kth_of[0][warp] = kth;
-    __syncthreads();
-    uint32_t floor = __reduce_min_sync(kFull, lane < warps ? kth_of[0][lane] : kFull);
-    floor = max(floor, kLowestKeyHi);
-    for (int l = tid; l < lists; l += nth)
-        if ((uint32_t)(head[l] >> 32) >= floor) list_of[atomicAdd(&s_heads, 1)] = l;
-    __syncthreads();
-    const int heads = s_heads;
-    // what these lists hold, around the warps again, bounds the n-th score once more
-    own = 0;
-    for (int e = lane * warps + warp; e < heads * n; e += nth) {
-        const int l = list_of[e / n];
-        own = max(own, (uint32_t)(score_of(in.entry[(l0 + l) * n + e % n], l / splits) >> 32));
-    }
-    kth = kth_of_warp(own, k, lane);
-    if (lane == 0) kth_of[1][warp] = kth;
-    __syncthreads();
-    floor = max(floor, __reduce_min_sync(kFull, lane < warps ? kth_of[1][lane] : kFull));
-    auto take = [&](int l, int e, unsigned long long least) {
-        const unsigned long long entry = in.entry[(l0 + l) * n + e], s = score_of(entry, l / splits);
-        if (s >= least) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < room) {
-                cand[at] = s;
-                cand_i[at] = l / splits * V + (int)~(uint32_t)entry;
+    auto bound = [&](uint32_t own, uint32_t* kth_of) {
+        const uint32_t kth = kth_of_warp(own, k, lane);
+        if (lane == 0) kth_of[warp] = kth;
+        __syncthreads();
+        return max(__reduce_min_sync(kFull, lane < warps ? kth_of[lane] : kFull), kLowestKeyHi);
+    };
+    int count;
+    if (all) {
+        uint32_t own = 0;
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q) {
+            const int e = place(q);
+            if (e < lists * n) own = max(own, (uint32_t)(score_of(first[q], e / n / splits) >> 32));
+        }
+        const uint32_t floor = bound(own, kth_of[0]);
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q) {
+            const int e = place(q);
+            if (e < lists * n) {
+                const unsigned long long s = score_of(first[q], e / n / splits);
+                if ((uint32_t)(s >> 32) >= floor) {
+                    const int at = atomicAdd(&s_count, 1);
+                    cand[at] = s;
+                    cand_i[at] = e / n / splits * V + (int)~(uint32_t)first[q];
+                }
             }
         }
-    };
-    for (int e = lane * warps + warp; e < heads * n; e += nth) take(list_of[e / n], e % n, (unsigned long long)floor << 32);
-    __syncthreads();
-    int count = s_count;
-    if (count > room) {
-        // equal scores in numbers: of the lists only the n with the best heads (those of a row are in the order of the lists), and nothing below
-        // the n-th head
-        for (int i0 = 0; i0 < heads; i0 += nth) {
-            if (i0 + tid < heads) cand[i0 + tid] = head[list_of[i0 + tid]];
-        }
-        __syncthreads();
-        for (int i0 = 0; i0 < heads; i0 += nth / 8) {
-            const int i = i0 + tid / 8;
-            const int r = rank_by_eight(cand, list_of, heads, i < heads ? cand[i] : 0, i < heads ? list_of[i] : 0);
-            if (i < heads && r < n && tid % 8 == 0) sel[r] = list_of[i];
-        }
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-        const int picked = min(heads, n);
-        const unsigned long long least = max(heads >= n ? head[sel[n - 1]] : 0ull, (unsigned long long)kLowestKeyHi << 32);
-        for (int e = tid; e < picked * n; e += nth) take(sel[e / n], e % n, least);
         __syncthreads();
         count = s_count;
+    } else {
+        uint32_t own = 0;
+        for (int l = lane * warps + warp; l < lists; l += nth) {
+            const unsigned long long h = score_of(l < nth ? first[0] : in.entry[(l0 + l) * n], l / splits);
+            head[l] = h;
+            own = max(own, (uint32_t)(h >> 32));
+        }
+        uint32_t floor = bound(own, kth_of[0]);
+        for (int l = tid; l < lists; l += nth)
+            if ((uint32_t)(head[l] >> 32) >= floor) list_of[atomicAdd(&s_heads, 1)] = l;
+        __syncthreads();
+        const int heads = s_heads;
+        // what these lists hold, around the warps again, bounds the n-th score once more
+        own = 0;
+        for (int e = lane * warps + warp; e < heads * n; e += nth) {
+            const int l = list_of[e / n];
+            own = max(own, (uint32_t)(score_of(in.entry[(l0 + l) * n + e % n], l / splits) >> 32));
+        }
+        floor = max(floor, bound(own, kth_of[1]));
+        auto take = [&](int l, int e, unsigned long long least) {
+            const unsigned long long entry = in.entry[(l0 + l) * n + e], s = score_of(entry, l / splits);
+            if (s >= least) {
+                const int at = atomicAdd(&s_count, 1);
+                if (at < room) {
+                    cand[at] = s;
+                    cand_i[at] = l / splits * V + (int)~(uint32_t)entry;
+                }
+            }
+        };
+        for (int e = lane * warps + warp; e < heads * n; e += nth) take(list_of[e / n], e % n, (unsigned long long)floor << 32);
+        __syncthreads();
+        count = s_count;
+        if (count > room) {
+            // equal scores in numbers: of the lists only the n with the best heads (those of a row are in the order of the lists), and nothing below
+            // the n-th head
+            for (int i0 = 0; i0 < heads; i0 += nth) {
+                if (i0 + tid < heads) cand[i0 + tid] = head[list_of[i0 + tid]];
+            }
+            __syncthreads();
+            for (int i0 = 0; i0 < heads; i0 += nth / 8) {
+                const int i = i0 + tid / 8;
+                const int r = rank_by_eight(cand, list_of, heads, i < heads ? cand[i] : 0, i < heads ? list_of[i] : 0);
+                if (i < heads && r < n && tid % 8 == 0) sel[r] = list_of[i];
+            }
+            if (tid == 0) s_count = 0;
+            __syncthreads();
+            const int picked = min(heads, n);
+            const unsigned long long least = max(heads >= n ? head[sel[n - 1]] : 0ull, (unsigned long long)kLowestKeyHi << 32);
+            for (int e = tid; e < picked * n; e += nth) take(sel[e / n], e % n, least);
+            __syncthreads();
+            count = s_count;
+        }
     }
     for (int i0 = 0; i0 < count; i0 += nth / 8) {
         const int i = i0 + tid / 8;
@@ -919,8 +953,8 @@ NXD_API int nxd_beam_select(int dtype, const void* logits, long long stride, con
     else if (dtype == 1) NXD_CHECK_CUDA(launch_rows<bf16>(p, rows * splits, s, logits, V, stride, n, l));
     else NXD_CHECK_CUDA(launch_rows<__half>(p, rows * splits, s, logits, V, stride, n, l));
     NXD_LAUNCH_CHECK();
-    const int room = lists > n * (n < lists ? n : lists) ? lists : n * (n < lists ? n : lists);
-    const int smem = (lists + room) * 12, threads = lists > 256 || n > 16 ? 1024 : 256;
+    const int threads = lists * n > 1024 ? 1024 : 256, picked = n * (n < lists ? n : lists);
+    const int room = lists * n <= kOwn * threads ? lists * n : lists > picked ? lists : picked, smem = (lists + room) * 12;
     NXD_CHECK_CUDA(nxd_allow_smem<beam_join_kernel>(kMaxLists * 24));
     NXD_CHECK_CUDA(nxd_launch_pdl(beam_join_kernel, dim3(B), dim3(threads), smem, s, scores, W, V, splits, n, room, l, out_scores, out_beams, out_tokens));
     NXD_LAUNCH_CHECK();
