@@ -80,11 +80,11 @@ def search(search_: BeamSearch, cache: KVCache, lengths: List[int], prompt_logit
 
 def sequences(input_ids: torch.Tensor, lengths: List[int], found: Tuple[torch.Tensor, torch.Tensor, torch.Tensor], n: int,
               pad_token_id: int) -> torch.Tensor:
-    """Prompts with their best ``n`` continuations behind them, ``[B * n, T + steps]``."""
-    tokens = found[0]
+    """Prompts with their best ``n`` continuations behind them, ``[B * n, T + the longest's tokens]``."""
+    tokens = found[0][:, :n, : int(found[1][:, :n].max())]
     B, T = input_ids.shape
     out = torch.full((B, n, T + tokens.shape[2]), pad_token_id, dtype=input_ids.dtype, device=tokens.device)
     for b, length in enumerate(lengths):
         out[b, :, :length] = input_ids[b, :length].to(tokens.device)
-        out[b, :, length:length + tokens.shape[2]] = tokens[b, :n].to(out.dtype)
+        out[b, :, length:length + tokens.shape[2]] = tokens[b].to(out.dtype)
     return out.reshape(B * n, -1)
