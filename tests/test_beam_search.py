@@ -118,6 +118,47 @@ def test_candidates_of_strided_and_misaligned_logits(device):
         _check_select(wide.view(2, 3, -1), scores.t().contiguous().t(), 6)
 
 
+# rows whose first round tells nothing about the others, and rounds with more values than are ranked easily; several rounds a row, one or many
+# chunks of it, few and many entries to join
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,W,V,n", [(2, 4, 40000, 8), (1, 32, 70001, 64), (300, 1, 17001, 3), (150, 2, 60003, 48), (3, 8, 131000, 16), (200, 4, 9001, 8)])
+@pytest.mark.parametrize("kind", ["rising", "falling", "few values", "equal", "a stretch is masked", "a stretch is lowest", "few are allowed", "a plateau"])
+def test_candidates_of_rows_unlike_a_sample(B, W, V, n, kind):
+    g = torch.Generator(device="cuda").manual_seed(V + n)
+    dtype = [torch.bfloat16, torch.float32, torch.float16][(V + n) % 3]
+    low = torch.finfo(dtype).min
+    x = torch.randn(B * W, V, generator=g, device="cuda") * 3
+    lo, hi = V // 5, V - V // 9
+    if kind in ("rising", "falling"):
+        x = x.sort(1, descending=kind == "falling").values
+    elif kind == "few values":
+        x = torch.randint(0, 5, x.shape, generator=g, device="cuda").float()
+    elif kind == "equal":
+        x.zero_()
+    x = x.to(dtype)
+    if kind == "a stretch is masked":
+        x[:, lo:hi] = -INF
+        x[::3, :hi] = -INF
+    elif kind == "a stretch is lowest":
+        x[:, :hi] = low
+    elif kind == "few are allowed":
+        x.masked_fill_(torch.rand(x.shape, generator=g, device="cuda") > 5 / V, low)
+    elif kind == "a plateau":
+        x[:, lo:hi] = 9.0
+    scores = -torch.rand(B, W, generator=g, device="cuda") * 4
+    x = x.view(B, W, V)
+    total = scores.double()[..., None] + (x.double() - torch.logsumexp(x.double(), -1, keepdim=True))
+    want, at = torch.sort(total.flatten(1), dim=1, descending=True, stable=True)
+    got, beams, tokens = bs.beam_select(x, scores, n)
+    # where scores of two beams are nearer than log-sum-exp is good to (2^-20 as above), either may be first
+    far = (want[:, :n] - total.flatten(1).gather(1, beams * V + tokens)).abs() > 2.0 ** -20 + 2.0 ** -50 * want[:, :n].abs()
+    assert not bool((far & (want[:, :n] > -INF)).any())
+    assert bool((at[:, :n] == beams * V + tokens).float().mean() > 0.99) and all(len(set(r)) == n for r in (beams * V + tokens).tolist())
+    fine = want[:, :n].float() > -INF
+    assert torch.equal(fine, got > -INF)
+    assert bool(((got.double() - want[:, :n]).abs() <= 2.0 ** -20 + 2.0 ** -24 * want[:, :n].abs())[fine].all())
+
+
 def test_candidates_refused():
     x, s = torch.randn(2, 3, 50), torch.zeros(2, 3)
     for logits, scores, n in ((x, s, 0), (x, s, 65), (x, s, 151), (x, s.double(), 4), (x, s[0], 4), (x[:, :2], s, 4), (x.reshape(-1), s, 4), (x.long(), s, 4),
