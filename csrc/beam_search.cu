@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
         }
         if (r == 0) {
             // the largest maxima of each warp that has values, 2 n of them: the n-th of those (of more than 32 its upper 16 bits) has n values that are not
-            // below it
+            // below it.  One warp has 32 at most: where more candidates are wanted nothing is known
             const int vecs = (V + mis - split * rounds * (NT * E) + VE - 1) / VE, filled = min(max((vecs + 31) / 32, 1), kWarps);
             const int per = min((2 * n + filled - 1) / filled, min(2 * kMaxN / filled, 32)), keys = filled * per;
             uint32_t key = order_key(m);
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
                 int before = 0;
 #pragma unroll
                 for (int j = 0; j < 32; ++j) before += __shfl_sync(kFull, own, j) > own;
-                least = __reduce_min_sync(kFull, before < n ? own : kFull);
+                if (n <= keys) least = __reduce_min_sync(kFull, before < n ? own : kFull);
             } else {
                 uint32_t own[2 * kMaxN / 32];
 #pragma unroll

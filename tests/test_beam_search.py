@@ -118,6 +118,32 @@ def test_candidates_of_strided_and_misaligned_logits(device):
         _check_select(wide.view(2, 3, -1), scores.t().contiguous().t(), 6)
 
 
+# pieces of a row with a value a thread in one warp and nothing behind it, and more candidates wanted than that warp has threads
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [33, 48, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_more_candidates_than_the_threads_of_a_short_piece(device, dtype, n):
+    g = torch.Generator().manual_seed(n)
+    per = 16 // dtype.itemsize                # values of 16 bytes
+    short = [32 * per - i for i in (0, 1, per - 1)]
+    for V in (*short, 31 * per, 33 * per, 512 * per + 32 * per, 12 * 512 * per + 32 * per):
+        lo = V - min(V, 32 * per)             # all that is allowed lies in the last piece
+        wide = torch.randn(3, V + per, generator=g).to(dtype)
+        wide[:, :lo] = -INF
+        wide[1, lo:] = 0.0                    # one high value in 16 bytes
+        wide[1, lo::per] = 10.0
+        for at in range(per if V in short else 1):
+            x = wide[:, at:at + V].to(device)
+            _check_select(x, torch.zeros(3, 1, device=device), n)
+    for W in (17, 32):                        # a first step with rows for all beams
+        x = (torch.randn(2, W, 32 * per, generator=g) * 3).to(dtype)
+        x[:, 0] = 0.0
+        x[:, 0, per - 1::per] = 5.0
+        scores = torch.full((2, W), -INF)
+        scores[:, 0] = 0.0
+        _check_select(x.to(device), scores.to(device), n)
+
+
 # rows whose first round tells nothing about the others, and rounds with more values than are ranked easily; several rounds a row, one or many
 # chunks of it, few and many entries to join
 @pytest.mark.gpu
