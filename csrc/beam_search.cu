@@ -708,6 +708,9 @@ constexpr int kFinishBytes = 100 * 1024;     // of shared memory: a byte a step 
 
 __host__ __device__ inline int token_pitch(int W) { return W | 1; }          // words a step: lanes of consecutive steps in different banks
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 __device__ __forceinline__ void store_of_rank(unsigned char* p, int rank, int v) {          // to the same place in a CTA of the cluster
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
@@ -731,6 +734,8 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(Books in, i
     __shared__ unsigned char span_through[kFinishCluster][32], span_part[kFinishCluster][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nth = blockDim.x;
     const int rank = blockIdx.x, ranks = gridDim.x;          // the cluster is a row of the grid
+    // here a CTA says that it runs; the wait for the others' word stands before the first store into their shared memory
+    if (ranks > 1) cluster_arrive();
     const long long b = blockIdx.y;
     const int pitch = token_pitch(W), first = rank * span, steps = max(min(span, step - first), 0);          // t counts from `first`
     unsigned char* path = scratch != nullptr ? scratch + (b * step + first) * W : reinterpret_cast<unsigned char*>(finish_smem + (staged ? span * pitch : 0));
@@ -827,6 +832,7 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(Books in, i
     const int own_in = lane < W ? enter_at[lane] : -1;
     int cur = lane < W ? enter_slot[lane] : 0;
     if (ranks > 1) {
+        cluster_wait();
         if (warp == 0 && lane < W) {
             int line = lane;
             for (int k = sections - 1; k >= 0; --k) line = through[k][line];
@@ -836,7 +842,9 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(Books in, i
                 store_of_rank(&span_part[rank][lane], r, place);
             }
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
         if (warp == 0 && lane < W) {
             for (int r = ranks - 1; r > rank; --r) {
                 if (own_in >= (r + 1) * span) cur = span_through[r][cur];

@@ -3,6 +3,7 @@ GPU (kernels), and what they refuse."""
 import itertools
 import math
 import random
+from pathlib import Path
 
 import pytest
 import torch
@@ -389,6 +390,29 @@ def test_sequences_of_many_steps(B, W, T):
     put = lambda x: type(x)(*[t.cuda() for t in x])          # noqa: E731
     got = bs.beam_finish((running * T ** 0.5).cuda(), put(pool), put(history), T, **kw)
     assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
+def test_a_cluster_waits_for_its_blocks_before_it_stores_into_them():
+    """Another block's shared memory may be written once that block is known to run."""
+    source = (Path(bs.__file__).parents[2] / "csrc" / "beam_search.cu").read_text()
+    body = source[source.index("beam_finish_kernel("):source.index("finish_span(")]
+    arrive, wait, store = (body.index(s) for s in ("cluster_arrive()", "cluster_wait()", "store_of_rank("))
+    assert arrive < body.index("hist_parent[at]") < wait < store          # said at the start, waited for where it is needed
+    assert body.rindex("cluster_arrive()") > body.rindex("store_of_rank(")
+
+
+# clusters of two, four and eight blocks whose last has the fewest steps, launches behind each other
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,W,T", [(148, 3, 129), (74, 5, 257), (37, 8, 513), (1, 32, 1025), (5, 1, 1031), (20, 4, 700)])
+def test_sequences_of_uneven_spans(B, W, T):
+    g = torch.Generator().manual_seed(T)
+    history = bs.BeamHistory(torch.randint(3, 9999, (T, B, W), generator=g).int(), torch.randint(0, W, (T, B, W), generator=g).int())
+    pool, running = bs.new_beam_pool(B, W), -torch.rand(B, W, generator=g).sort(-1).values
+    want = bs.beam_finish(running, pool, history, T, length_penalty=0.0)
+    put = lambda x: type(x)(*[t.cuda() for t in x])          # noqa: E731
+    args = running.cuda(), put(pool), put(history), T
+    for got in [bs.beam_finish(*args, length_penalty=0.0) for _ in range(20)]:
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
 
 
 # ---- lines and pages --------------------------------------------------------------------------------------------------
