@@ -85,7 +85,8 @@ template <typename T>
 __device__ __forceinline__ uint4 load_vec(const T* row, int at, int V) {
     if (at >= 0 && at + Vec<T>::n <= V) return __ldg(reinterpret_cast<const uint4*>(row + at));
     // over an end of the row: its elements one by one, -inf outside
-    constexpr uint32_t kOut = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, bf16> ? 0xff80u : 0xfc00u;
+    constexpr uint32_t kOut = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, bf16> ? 0xff80u : 0xfc00u, kAll = sizeof(T) == 4 ? kOut : kOut << 16 | kOut;
+    if (at >= V) return make_uint4(kAll, kAll, kAll, kAll);
     constexpr int kBits = 8 * sizeof(T);
     unsigned long long lo = 0, hi = 0;
 #pragma unroll 1
@@ -97,26 +98,57 @@ __device__ __forceinline__ uint4 load_vec(const T* row, int at, int V) {
     return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
+// Rows start anywhere, threads have the same elements of every row all the same, so that equal rows come to equal sums.  In memory a thread's vector
+// then lies in two of the 16-byte ones, `mis` elements behind the start of the first.
+template <typename T>
+__device__ __forceinline__ uint4 join_vecs(const uint4& a, const uint4& b, int mis) {
+    const int bytes = mis * (int)sizeof(T), bits = bytes % 4 * 8;          // the same for the whole block
+    switch (bytes / 4) {
+        case 0: return make_uint4(__funnelshift_r(a.x, a.y, bits), __funnelshift_r(a.y, a.z, bits), __funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits));
+        case 1: return make_uint4(__funnelshift_r(a.y, a.z, bits), __funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits));
+        case 2: return make_uint4(__funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits), __funnelshift_r(b.y, b.z, bits));
+        default: return make_uint4(__funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits), __funnelshift_r(b.y, b.z, bits), __funnelshift_r(b.z, b.w, bits));
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 load_elements(const T* row, int at, int V, int mis) {
+    const uint4 a = load_vec<T>(row, at - mis, V);
+    return mis == 0 ? a : join_vecs<T>(a, load_vec<T>(row, at - mis + Vec<T>::n, V), mis);
+}
+
 __device__ __forceinline__ void fetch_vec(uint4* to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
-// A thread's vectors of a round on their way into shared memory (one group of copies; the ends of a row are stored at once).  Whether a round
-// lies inside the row the block decides at once.
+// A round in shared memory: 33 vectors a warp and vector of its threads, of which the last is the next warp's first.
+constexpr int kStagePitch = 33;
+
+// A thread's vectors of a round on their way there (one group of copies; the ends of a row are stored at once).  Whether a round lies
+// inside the row the block decides at once.  Of a row that starts on 16 bytes nobody reads the 33rd ones.
 template <typename T, int NT, int NV>
-__device__ __forceinline__ void fetch_round(uint4* stage, const T* row, int first, int V) {
-    constexpr int VE = Vec<T>::n;
+__device__ __forceinline__ void fetch_round(uint4* stage, const T* row, int first, int V, int mis) {
+    constexpr int VE = Vec<T>::n, kWarps = NT / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, more = mis != 0 ? VE : 0;
+    stage += warp * kStagePitch + lane;
+    first -= mis;
     const int begin = first - (int)threadIdx.x * VE;
-    if (begin >= 0 && begin + NT * NV * VE <= V) {
+    if (begin >= 0 && begin + NT * NV * VE + more <= V) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) fetch_vec(stage + i * NT + threadIdx.x, row + first + i * NT * VE);
+        for (int i = 0; i < NV; ++i) fetch_vec(stage + i * kWarps * kStagePitch, row + first + i * NT * VE);
+        if (mis != 0 && lane == 31) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) fetch_vec(stage + i * kWarps * kStagePitch + 1, row + first + i * NT * VE + VE);
+        }
         return;
     }
+    auto fetch = [&](uint4* to, int at) {
+        if (at >= 0 && at + VE <= V) fetch_vec(to, row + at);
+        else *to = load_vec<T>(row, at, V);
+    };
 #pragma unroll 1
-    for (int i = 0; i < NV; ++i) {
-        const int at = first + i * NT * VE;
-        if (at >= 0 && at + VE <= V) fetch_vec(stage + i * NT + threadIdx.x, row + at);
-        else stage[i * NT + threadIdx.x] = load_vec<T>(row, at, V);
+    for (int i = 0; i < NV; ++i, first += NT * VE, stage += kWarps * kStagePitch) {
+        fetch(stage, first);
+        if (mis != 0 && lane == 31) fetch(stage + 1, first + VE);
     }
 }
 __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -191,11 +223,11 @@ __device__ __forceinline__ uint32_t kth_of_warp(uint32_t key, int k, int lane) {
 // entries, found bit by bit (entries differ, so it is one thread's), has n entries that are not below it, all of them in n threads: what is collected
 // behind the `have` candidates fits.  Reads the round's values once more.
 template <typename T, int NT, int NV>
-__device__ __noinline__ int collect_carefully(const T* row, int first, int V, int n, int have, float floor, unsigned long long* cand, int* s_count) {
+__device__ __noinline__ int collect_carefully(const T* row, int first, int V, int mis, int n, int have, float floor, unsigned long long* cand, int* s_count) {
     constexpr int VE = Vec<T>::n;
     uint4 raw[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i] = load_vec<T>(row, first + i * NT * VE, V);
+    for (int i = 0; i < NV; ++i) raw[i] = load_elements<T>(row, first + i * NT * VE, V, mis);
     unsigned long long best = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -237,7 +269,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
                                                                    Lists out) {
     constexpr int VE = Vec<T>::n, E = NV * VE, kWarps = NT / 32;
     __shared__ unsigned long long cand[kCollect];
-    extern __shared__ uint4 ring[];            // [kStages][NV][NT]
+    constexpr int kStage = NV * kWarps * kStagePitch;
+    extern __shared__ uint4 ring[];            // [kStages][NV][kWarps][kStagePitch]
     __shared__ unsigned char looker[kWarps][32];
     __shared__ uint32_t warp_top[kWarps], bound_keys[2 * kMaxN];
     __shared__ float warp_sum_of[kWarps];
@@ -247,14 +280,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
     const long long list = blockIdx.x;
     const int split = (int)(list % splits);
     const T* row = logits + (list / splits) * stride;
-    // vectors start on 16 bytes: the row's first element is element `mis` of the first one
+    // loads start on 16 bytes: the row's first element is element `mis` of the first vector
     const int mis = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % VE);
-    int first = split * rounds * (NT * E) + tid * VE - mis;          // index of this thread's first element of the round
+    int first = split * rounds * (NT * E) + tid * VE;          // index of this thread's first element of the round
 
     if (tid == 0) s_count = 0;
 #pragma unroll
     for (int q = 0; q < kStages - 1; ++q) {
-        if (q < rounds) fetch_round<T, NT, NV>(ring + q * (NV * NT), row, first + q * (NT * E), V);
+        if (q < rounds) fetch_round<T, NT, NV>(ring + q * kStage, row, first + q * (NT * E), V, mis);
         fetch_commit();
     }
     float top = -INFINITY, sum = 0.f;          // this thread's
@@ -304,14 +337,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
         floor = kept_floor = count == n ? key_value((uint32_t)(best[n - 1] >> 32)) : -INFINITY;
     };
     for (int r = 0; r < rounds; ++r) {
-        uint4* stage = ring + r % kStages * (NV * NT);
+        const uint4* stage = ring + r % kStages * kStage + warp * kStagePitch;          // this warp's
         fetch_wait<kStages - 2>();
         uint4 raw[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) raw[i] = stage[i * NT + tid];
+        for (int i = 0; i < NV; ++i) raw[i] = stage[i * kWarps * kStagePitch + lane];
+        if (mis != 0) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) raw[i] = join_vecs<T>(raw[i], stage[i * kWarps * kStagePitch + lane + 1], mis);
+        }
         // into the round before, which the warp is done with; not with the first ones, which would arrive later for it
         if (r + kStages - 1 < rounds)
-            fetch_round<T, NT, NV>(ring + (r + kStages - 1) % kStages * (NV * NT), row, first + (kStages - 1) * (NT * E), V);
+            fetch_round<T, NT, NV>(ring + (r + kStages - 1) % kStages * kStage, row, first + (kStages - 1) * (NT * E), V, mis);
         fetch_commit();
         float m = max_of<T, NV>(raw) + 0.f;          // no -0; passes NaN by
         {
@@ -340,7 +378,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
         if (r == 0) {
             // the largest maxima of each warp that has values, 2 n of them: the n-th of those (of more than 32 its upper 16 bits) has n values that are not
             // below it.  One warp has 32 at most: where more candidates are wanted nothing is known
-            const int vecs = (V + mis - split * rounds * (NT * E) + VE - 1) / VE, filled = min(max((vecs + 31) / 32, 1), kWarps);
+            const int vecs = (V - split * rounds * (NT * E) + VE - 1) / VE, filled = min(max((vecs + 31) / 32, 1), kWarps);
             const int per = min((2 * n + filled - 1) / filled, min(2 * kMaxN / filled, 32)), keys = filled * per;
             uint32_t key = order_key(m);
             for (int i = 0; i < per; ++i) {
@@ -380,7 +418,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
             __syncwarp();
             for (int e = lane; e < __popc(lookers) * E; e += 32) {
                 const int who = looker[warp][e / E], i = e % E / VE, j = e % VE;
-                const float f = to_float<T>(reinterpret_cast<const T*>(stage + i * NT + warp * 32 + who)[j]);
+                const float f = to_float<T>(reinterpret_cast<const T*>(stage + i * kWarps * kStagePitch + who)[mis + j]);
                 if (f > floor) {
                     const int to = atomicAdd(&s_count, 1);
                     if (to < kCollect) cand[to] = entry_key(f, first + (who - lane) * VE + i * NT * VE + j);
@@ -396,7 +434,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const T* __res
             } else {          // the rounds since the last time once more, one by one
                 __syncthreads();
                 floor = kept_floor;
-                for (int q = since; q <= r; ++q) keep_best(collect_carefully<T, NT, NV>(row, first - (r - q) * (NT * E), V, n, kept, floor, cand, &s_count));
+                for (int q = since; q <= r; ++q) keep_best(collect_carefully<T, NT, NV>(row, first - (r - q) * (NT * E), V, mis, n, kept, floor, cand, &s_count));
             }
             since = r + 1;
             until = 4 * r + 3;          // 1, 7, 31: at most 3 n or so pass the bound between these
@@ -910,7 +948,7 @@ struct Split {
 // 16000 16 instead of 17, and 256 rows of 16000 14 instead of 12).
 Split split_of(long long rows, int W, int V, int elem) {
     const int per_vec = 16 / elem;
-    const long long sms = nxd_num_sms(), span = V + per_vec - 1, large = 512LL * 4 * per_vec;
+    const long long sms = nxd_num_sms(), span = V, large = 512LL * 4 * per_vec;
     Split s;
     const bool few = rows * ((span + large - 1) / large) < sms || span <= 2 * 512LL * per_vec;
     s.threads = few ? 256 : 512;
@@ -926,11 +964,11 @@ Split split_of(long long rows, int W, int V, int elem) {
 
 template <typename T>
 cudaError_t launch_rows(const Split& p, long long ctas, cudaStream_t s, const void* logits, int V, long long stride, int n, Lists out) {
-    const int smem = (p.rounds < kStages ? p.rounds : kStages) * p.vecs * p.threads * 16;
+    const int smem = (p.rounds < kStages ? p.rounds : kStages) * p.vecs * (p.threads / 32) * kStagePitch * 16;
     if (p.threads == 256) {
         beam_rows_kernel<T, 256, 2><<<(unsigned)ctas, 256, smem, s>>>((const T*)logits, V, stride, p.splits, p.rounds, n, out);
     } else {
-        const cudaError_t e = nxd_allow_smem<beam_rows_kernel<T, 512, 4>>(kStages * 4 * 512 * 16);
+        const cudaError_t e = nxd_allow_smem<beam_rows_kernel<T, 512, 4>>(kStages * 4 * 16 * kStagePitch * 16);
         if (e != cudaSuccess) return e;
         beam_rows_kernel<T, 512, 4><<<(unsigned)ctas, 512, smem, s>>>((const T*)logits, V, stride, p.splits, p.rounds, n, out);
     }

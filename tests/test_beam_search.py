@@ -95,6 +95,34 @@ def test_candidates_of_equal_beams_and_equal_logits(device):
     _check_select(x.to(device), torch.tensor([[-1.5, -1.5, -2.0, -1.5]] * 2, device=device), 64)
 
 
+# rows that start at different places of 16 bytes: what they add up to does not depend on it
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,n", [(301, 8), (5003, 8), (5003, 64), (30522, 10), (128257, 16)])
+def test_candidates_of_equal_beams_at_any_alignment(device, dtype, V, n):
+    g = torch.Generator().manual_seed(V)
+    B, W = (24, 8) if device == "cuda" else (2, 8)
+    for pitch in (V, V + 1, V + 3):
+        row = (torch.randn(B, 1, V, generator=g) * 2.5).to(dtype)
+        wide = torch.randn(B, W, pitch, generator=g).to(dtype)
+        wide[:, :, pitch - V:] = row
+        x = wide.to(device)[:, :, pitch - V:]
+        scores, beams, tokens = (t.cpu() for t in bs.beam_select(x, torch.full((B, W), -1.5, device=device), n))
+        # the first token of all beams from the lowest on, then the second
+        order = torch.sort(row[:, 0].float(), dim=1, descending=True, stable=True)
+        for b in range(B):
+            values, at = order.values[b].tolist(), order.indices[b].tolist()
+            want, i = [], 0
+            while len(want) < n:               # tokens of one logit: beam by beam, the lower tokens first
+                j = i
+                while j < V and values[j] == values[i]:
+                    j += 1
+                want += [(w, v) for w in range(W) for v in at[i:j]]
+                i = j
+            assert list(zip(beams[b].tolist(), tokens[b].tolist())) == want[:n], b
+            assert len(set(scores[b, :W].tolist())) == 1
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_candidates_of_rising_and_large_logits(device):
     x = torch.arange(5000, dtype=torch.float32).flip(0).repeat(1, 2, 1) * 1e-3
