@@ -197,13 +197,13 @@ class KVCache:
         if used > num_pages or num_pages < 1:
             raise MemoryError(f"{used} pages are in use, {num_pages} are not enough")
         self.pool.resize(num_pages)
-        self._laid_out = None
-        for i, k in enumerate(self.k):
-            if k is None:
+        self._laid_out, self._held = None, ()          # they hold the old tensors
+        for i in range(self.num_layers):
+            if self.k[i] is None:
                 continue
-            v, columns = self.v[i], self.v[i]._base is not None
-            self.k[i] = self._resized(k, num_pages, used)
-            self.v[i] = self.k[i][..., : v.shape[-1]] if columns else self._resized(v, num_pages, used)
+            dim, columns = self.v[i].shape[-1], self.v[i]._base is not None
+            self.k[i] = self._resized(self.k[i], num_pages, used)
+            self.v[i] = self.k[i][..., :dim] if columns else self._resized(self.v[i], num_pages, used)
 
     @staticmethod
     def _resized(t: torch.Tensor, num_pages: int, used: int) -> torch.Tensor:

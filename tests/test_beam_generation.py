@@ -2,6 +2,7 @@
 cache's lines and pages, and the runner with its graphs."""
 import importlib
 import math
+import weakref
 
 import pytest
 import torch
@@ -352,6 +353,27 @@ def test_pages_of_a_pool_fork_compact_and_move(device):
     small.fork_lines(0, [1, 2])
     with pytest.raises(AssertionError):
         _cache("contiguous", device).copy_pages([0], [1])
+
+
+@pytest.mark.parametrize("pages", [12, 40, 60])
+def test_a_resized_pool_lets_the_old_tensors_go(monkeypatch, pages):
+    cache = _cache("pool", None)
+    cache.reserve(0, 10)
+    cache.fork_lines(0, [1, 2])
+    held = [weakref.ref(t) for t in cache._tensors()]
+    alive, resized = [], KVCache._resized
+
+    def counted(t, num_pages, used):
+        new = resized(t, num_pages, used)
+        alive.append(sum(r() is not None for r in held))
+        return new
+
+    monkeypatch.setattr(KVCache, "_resized", staticmethod(counted))
+    cache.resize_pool(pages)
+    assert not any(r() is not None for r in held)
+    assert alive == list(range(len(held), 0, -1))          # one after the other
+    cache.fork_lines(0, [3])
+    assert cache.tensors.cache[0].shape[0] == pages
 
 
 @pytest.mark.gpu
