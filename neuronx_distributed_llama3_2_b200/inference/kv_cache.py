@@ -192,11 +192,15 @@ class KVCache:
 
     def resize_pool(self, num_pages: int) -> None:
         """A pool of another size: the pages in use move to the front and into new tensors, the old ones are let go.  ``MemoryError`` if more are in
-        use.  What holds the old tensors (a captured graph, ``BeamLines``) has to be made again."""
+        use; where a new tensor cannot be had the cache keeps working and may be resized again.  What holds the old tensors (a captured graph,
+        ``BeamLines``) has to be made again."""
         used = self.compact()
         if used > num_pages or num_pages < 1:
             raise MemoryError(f"{used} pages are in use, {num_pages} are not enough")
-        self.pool.resize(num_pages)
+        # where memory runs out on the way, the allocator names no page that a tensor has not
+        shrinks = num_pages < self.pool.num_pages
+        if shrinks:
+            self.pool.resize(num_pages)
         self._laid_out, self._held = None, ()          # they hold the old tensors
         for i in range(self.num_layers):
             if self.k[i] is None:
@@ -204,6 +208,8 @@ class KVCache:
             dim, columns = self.v[i].shape[-1], self.v[i]._base is not None
             self.k[i] = self._resized(self.k[i], num_pages, used)
             self.v[i] = self.k[i][..., :dim] if columns else self._resized(self.v[i], num_pages, used)
+        if not shrinks:
+            self.pool.resize(num_pages)
 
     @staticmethod
     def _resized(t: torch.Tensor, num_pages: int, used: int) -> torch.Tensor:

@@ -376,6 +376,43 @@ def test_a_resized_pool_lets_the_old_tensors_go(monkeypatch, pages):
     assert cache.tensors.cache[0].shape[0] == pages
 
 
+@pytest.mark.parametrize("pages", [12, 60])
+@pytest.mark.parametrize("at", range(5))
+def test_a_pool_that_could_not_be_resized_names_no_page_that_is_not_there(monkeypatch, pages, at):
+    cache = _cache("pool", None)
+    cache.reserve(1, 3), cache.reserve(0, 10), cache.free(1)
+    _filled(cache, torch.Generator().manual_seed(2))
+    layers = (0, 1, 3, 4)
+    held = {i: _line(cache, i, 0, 10) for i in layers}
+    calls, resized = [], KVCache._resized
+
+    def failing(t, num_pages, used):
+        calls.append(t)
+        if len(calls) == at + 1:
+            raise torch.OutOfMemoryError("no room")
+        return resized(t, num_pages, used)
+
+    def check():
+        assert cache.pool.num_pages <= min(t.shape[0] for t in cache._tensors())
+        assert cache.pool.num_free == cache.pool.num_pages - 3
+        for i in layers:
+            assert all(torch.equal(a, b) for a, b in zip(_line(cache, i, 0, 10), held[i]))
+            k, v = cache.layer(i)
+            assert (v._base is None) == (i != 1) and k.shape[0] >= cache.pool.num_pages <= v.shape[0]
+
+    monkeypatch.setattr(KVCache, "_resized", staticmethod(failing))
+    with pytest.raises(torch.OutOfMemoryError):
+        cache.resize_pool(pages)
+    check()
+    cache.reserve(2, 24)
+    cache.fork_lines(0, [3])          # the kernels' layout copes with pools of two sizes
+    cache.free(2), cache.free(3)
+    monkeypatch.setattr(KVCache, "_resized", staticmethod(resized))
+    cache.resize_pool(pages)
+    check()
+    assert cache.pool.num_pages == pages == max(t.shape[0] for t in cache._tensors())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("paged", [False, True])
 @pytest.mark.parametrize("W", [2, 5])
