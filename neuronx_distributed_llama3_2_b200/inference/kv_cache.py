@@ -271,6 +271,8 @@ class BeamLines:
                 cache.free(line)
         for b, n in enumerate(lengths):
             cache.truncate(b * width, n)
+            if n % cache.page_size:
+                cache.prepare_write(b * width, n)          # a prompt may end in a page that it shares
             cache.fork_lines(b * width, range(b * width + 1, (b + 1) * width), whole_pages=False)
         for line in lines:
             cache.pool.reserve(line, lengths[line // width] + new_tokens)

@@ -315,6 +315,32 @@ def test_lines_of_a_search(device, kind):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_a_prompt_that_ends_in_a_page_of_another_line(device):
+    cache = _cache("pool", device, lines=6)
+    cache.reserve(0, 8)
+    cache.reserve(2, 8)
+    cache.fork_lines(0, [4])
+    _filled(cache, torch.Generator().manual_seed(6))
+    other = {i: _line(cache, i, 4, 8) for i in (0, 1, 3)}
+    lines = cache.beams([6, 8], 2, 4)          # rows 6 and 7 are written again
+    assert all(at <= n for at, n in zip(cache.pool.private_from(0, 4), (6, 6, 8, 8)))
+    for line in range(4):
+        for i in (0, 1, 3):
+            assert all(torch.equal(a, b[:, :6]) for a, b in zip(_line(cache, i, line, 6), other[i])) or line > 1
+        for pos in range(6 if line < 2 else 8, 10):
+            for t in cache._tensors():
+                t[int(cache.block_table[line, pos // 4]), :, pos % 4] = 100 * line + pos
+    lines.reorder(torch.tensor([[1, 1], [0, 0]], device=device), torch.tensor([10, 10], device=device))
+    for i in (0, 1, 3):
+        assert all(torch.equal(a, b) for a, b in zip(_line(cache, i, 4, 8), other[i]))
+        for line in range(4):
+            for now, had in zip(_line(cache, i, line, 10), other[i]):
+                first, frm = (6, 1) if line < 2 else (8, 2)
+                assert torch.equal(now[:, first:], (100.0 * frm + torch.arange(first, 10, device=device))[None, :, None].expand_as(now[:, first:]))
+                assert line > 1 or torch.equal(now[:, :6], had[:, :6])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_pages_of_a_pool_fork_compact_and_move(device):
     g = torch.Generator().manual_seed(4)
     cache = _cache("pool", device, lines=8)
