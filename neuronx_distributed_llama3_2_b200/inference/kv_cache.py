@@ -246,7 +246,7 @@ class KVCache:
 class BeamLines:
     """The cache lines of a beam search: line ``b * width + w`` is beam ``w`` of request ``b``.  A prompt is computed once, on its request's first
     line, and spread over the others here: shared pages with a dynamic pool (the beams' own rows are private), copied rows otherwise.  ``reorder`` then
-    moves only what lies behind the prompts."""
+    moves only what lies behind the prompts.  Where a pool has not enough pages (``MemoryError``) the prompts stay and the other lines are free."""
 
     def __init__(self, cache: KVCache, lengths: Sequence[int], width: int, new_tokens: int = 0):
         lengths = [int(n) for n in lengths]
@@ -269,13 +269,21 @@ class BeamLines:
         for line in lines:
             if line % width:
                 cache.free(line)
-        for b, n in enumerate(lengths):
-            cache.truncate(b * width, n)
-            if n % cache.page_size:
-                cache.prepare_write(b * width, n)          # a prompt may end in a page that it shares
-            cache.fork_lines(b * width, range(b * width + 1, (b + 1) * width), whole_pages=False)
-        for line in lines:
-            cache.pool.reserve(line, lengths[line // width] + new_tokens)
+        try:
+            for b, n in enumerate(lengths):
+                cache.truncate(b * width, n)
+                if n % cache.page_size:
+                    cache.prepare_write(b * width, n)          # a prompt may end in a page that it shares
+                cache.fork_lines(b * width, range(b * width + 1, (b + 1) * width), whole_pages=False)
+            for line in lines:
+                cache.pool.reserve(line, lengths[line // width] + new_tokens)
+        except MemoryError:
+            for line in lines:
+                if line % width:
+                    cache.free(line)
+                else:
+                    cache.truncate(line, lengths[line // width])
+            raise
         cache.sync_lines(lines)
 
     def reorder(self, parents: torch.Tensor, end: Optional[torch.Tensor] = None) -> None:

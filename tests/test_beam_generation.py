@@ -340,6 +340,20 @@ def test_a_prompt_that_ends_in_a_page_of_another_line(device):
                 assert line > 1 or torch.equal(now[:, :6], had[:, :6])
 
 
+@pytest.mark.parametrize("pages", [6, 7, 9, 11, 13])
+def test_beams_that_a_pool_has_no_pages_for_leave_the_prompts_alone(pages):
+    cache = _cache("pool", None, num_pages=pages)
+    cache.reserve(0, 7)
+    cache.reserve(3, 8)
+    _filled(cache, torch.Generator().manual_seed(8))
+    had = [_line(cache, 0, line, n) for line, n in ((0, 7), (3, 8))]
+    with pytest.raises(MemoryError):
+        cache.beams([7, 8], 3, 12)
+    assert cache.pool.num_free == pages - 4 and [cache.pool.line_tokens(line) for line in range(6)] == [7, 0, 0, 8, 0, 0]
+    for rows, (line, n) in zip(had, ((0, 7), (3, 8))):
+        assert all(torch.equal(a, b) for a, b in zip(_line(cache, 0, line, n), rows))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_pages_of_a_pool_fork_compact_and_move(device):
     g = torch.Generator().manual_seed(4)
