@@ -46,6 +46,8 @@ class InferenceConfig:
         # token generation runs every beam of every sequence
         self.tkg_batch_size = self.tkg_batch_size or self.batch_size * self.num_beams
         self.max_batch_size = self.max_batch_size or max(self.ctx_batch_size, self.tkg_batch_size)
+        if self.num_beams > 1 and self.max_batch_size < self.tkg_batch_size:
+            raise ValueError(f"{self.tkg_batch_size} rows of beams need as many cache lines, not {self.max_batch_size} (max_batch_size)")
         if self.max_context_length > self.seq_len:
             raise ValueError("max_context_length cannot exceed seq_len")
 

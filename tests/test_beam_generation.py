@@ -101,6 +101,13 @@ def test_generation_refused(monkeypatch):
         InferenceConfig(num_beams=33)
 
 
+def test_rows_of_beams_need_cache_lines():
+    for kw in (dict(batch_size=2, max_batch_size=2), dict(batch_size=1, tkg_batch_size=8, max_batch_size=4), dict(batch_size=1, max_batch_size=3)):
+        with pytest.raises(ValueError):
+            InferenceConfig(num_beams=4, **kw)          # the graph of a step would write behind the cache
+    assert InferenceConfig(num_beams=4, batch_size=2, max_batch_size=8).tkg_batch_size == 8
+
+
 # recurrent state, short convolutions, latent columns and layers that share keys next to plain keys and values
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("family,pages", [("rasodra", None), ("rasodra", 90), ("gogalix", None), ("gogalix", 90)])
