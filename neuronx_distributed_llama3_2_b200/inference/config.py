@@ -43,6 +43,8 @@ class InferenceConfig:
         self.ctx_batch_size = self.ctx_batch_size or self.batch_size
         if not 1 <= self.num_beams <= 32:
             raise ValueError(f"num_beams has to be between 1 and 32, not {self.num_beams}")
+        if self.num_beams > 1 and self.do_sample:
+            raise ValueError("a beam search takes the best continuations and does not sample")
         # token generation runs every beam of every sequence
         self.tkg_batch_size = self.tkg_batch_size or self.batch_size * self.num_beams
         self.max_batch_size = self.max_batch_size or max(self.ctx_batch_size, self.tkg_batch_size)

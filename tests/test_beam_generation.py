@@ -108,6 +108,12 @@ def test_rows_of_beams_need_cache_lines():
     assert InferenceConfig(num_beams=4, batch_size=2, max_batch_size=8).tkg_batch_size == 8
 
 
+def test_a_search_does_not_sample():
+    with pytest.raises(ValueError):
+        InferenceConfig(num_beams=2, do_sample=True, top_k=5)
+    assert InferenceConfig(num_beams=1, do_sample=True, top_k=5).do_sample
+
+
 # recurrent state, short convolutions, latent columns and layers that share keys next to plain keys and values
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("family,pages", [("rasodra", None), ("rasodra", 90), ("gogalix", None), ("gogalix", 90)])
