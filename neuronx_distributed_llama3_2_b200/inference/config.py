@@ -33,11 +33,11 @@ class InferenceConfig:
     paged_kv: bool = False
     page_size: int = 128
     num_kv_pages: Optional[int] = None      # paged cache: size of the page pool (default: lines * pages per line)
+    pad_token_id: int = 0
+    eos_token_id: Optional[int] = None
     num_beams: int = 1                      # > 1: generate() searches with that many beams (1 to 32) per sequence
     length_penalty: float = 1.0             # beams are ranked by summed log-probability / length ** length_penalty
     early_stopping: bool = False            # a beam search ends as soon as it has num_beams finished sequences
-    pad_token_id: int = 0
-    eos_token_id: Optional[int] = None
 
     def __post_init__(self):
         self.ctx_batch_size = self.ctx_batch_size or self.batch_size

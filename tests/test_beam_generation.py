@@ -1,5 +1,6 @@
 """Beam search through the models' caches: every kind of cache against a search that computes all sequences anew with the training model, the
 cache's lines and pages, and the runner with its graphs."""
+import dataclasses
 import importlib
 import math
 import weakref
@@ -112,6 +113,11 @@ def test_a_search_does_not_sample():
     with pytest.raises(ValueError):
         InferenceConfig(num_beams=2, do_sample=True, top_k=5)
     assert InferenceConfig(num_beams=1, do_sample=True, top_k=5).do_sample
+
+
+def test_the_search_has_the_last_fields_of_a_configuration():
+    names = [f.name for f in dataclasses.fields(InferenceConfig)]
+    assert names[-5:] == ["pad_token_id", "eos_token_id", "num_beams", "length_penalty", "early_stopping"]
 
 
 # recurrent state, short convolutions, latent columns and layers that share keys next to plain keys and values
