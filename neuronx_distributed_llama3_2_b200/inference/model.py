@@ -624,7 +624,7 @@ class KVCacheInferenceMixin:
             attention_mask = torch.ones_like(input_ids)
         lens = attention_mask.sum(dim=1).to(torch.long)
         lengths = lens.tolist()
-        if min(lengths) < 1 or max(T, max(lengths) + max_new_tokens - 1) > cache.seq_len:
+        if min(lengths) < 1 or max(T, 2, max(lengths) + max_new_tokens - 1) > cache.seq_len:          # one token is computed as two
             raise ValueError(f"prompts of {min(lengths)} to {max(lengths)} tokens (padded to {T}) and {max_new_tokens} more do not fit a cache of "
                              f"{cache.seq_len}")
         found = BeamSearch(B, W, max_new_tokens, eos_token_id=eos_token_id, pad_token_id=ic.pad_token_id, length_penalty=length_penalty,

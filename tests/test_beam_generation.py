@@ -120,6 +120,14 @@ def test_the_search_has_the_last_fields_of_a_configuration():
     assert names[-5:] == ["pad_token_id", "eos_token_id", "num_beams", "length_penalty", "early_stopping"]
 
 
+@pytest.mark.parametrize("cache", [{}, dict(paged_kv=True), dict(paged_kv=True, num_kv_pages=8)])
+def test_a_cache_of_one_token_is_refused(cache):
+    # a prompt of one token is computed as two, the second of which has no row there
+    model = LlamaInferenceModel(tiny_llama(sequence_parallel_enabled=False), InferenceConfig(max_context_length=1, seq_len=1, max_batch_size=3, page_size=1, **cache))
+    with pytest.raises(ValueError):
+        model.generate_beams(torch.tensor([[5]]), num_beams=3, max_new_tokens=1)
+
+
 # recurrent state, short convolutions, latent columns and layers that share keys next to plain keys and values
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("family,pages", [("rasodra", None), ("rasodra", 90), ("gogalix", None), ("gogalix", 90)])
