@@ -214,6 +214,28 @@ def test_candidates_of_rows_unlike_a_sample(B, W, V, n, kind):
     assert bool(((got.double() - want[:, :n]).abs() <= 2.0 ** -20 + 2.0 ** -24 * want[:, :n].abs())[fine].all())
 
 
+# one beam: its logits decide, so every place is known
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,V,n", [(2, 40000, 8), (300, 17001, 64), (1, 262147, 64), (200, 9001, 16), (900, 1003, 33)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_candidates_of_one_beam_unlike_a_sample(B, V, n, dtype):
+    g = torch.Generator(device="cuda").manual_seed(V + n)
+    low, lo, hi = torch.finfo(dtype).min, V // 5, V - V // 9
+    x = torch.randn(B, V, generator=g, device="cuda") * 3
+    rows = {"rising": x.sort(1).values, "falling": x.sort(1, descending=True).values, "few values": torch.randint(0, 5, x.shape, generator=g, device="cuda").float(),
+            "equal": torch.zeros_like(x), "a plateau": x.clone(), "masked": x.clone(), "lowest": x.clone(), "few": x.clone()}
+    rows["a plateau"][:, lo:hi] = 9.0
+    rows = {k: v.to(dtype) for k, v in rows.items()}
+    rows["masked"][:, lo:hi] = -INF
+    rows["masked"][::3, :hi] = -INF
+    rows["lowest"][:, :hi] = low
+    rows["few"].masked_fill_(torch.rand(x.shape, generator=g, device="cuda") > 5 / V, low)
+    for kind, logits in rows.items():
+        got, beams, tokens = bs.beam_select(logits, torch.full((B, 1), -2.0, device="cuda"), n)
+        assert torch.equal(tokens, torch.sort(logits.float(), dim=1, descending=True, stable=True).indices[:, :n]) and not bool(beams.any()), kind
+        assert not bool((got == -INF).any()) or kind in ("lowest", "few", "masked"), kind
+
+
 def test_candidates_refused():
     x, s = torch.randn(2, 3, 50), torch.zeros(2, 3)
     for logits, scores, n in ((x, s, 0), (x, s, 65), (x, s, 151), (x, s.double(), 4), (x, s[0], 4), (x[:, :2], s, 4), (x.reshape(-1), s, 4), (x.long(), s, 4),
