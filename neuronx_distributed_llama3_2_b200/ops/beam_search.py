@@ -75,7 +75,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
     ``logits``: ``[B, W, V]`` or ``[B * W, V]``, fp32, bf16 or fp16, unit stride along the tokens; ``scores``: ``[B, W]`` fp32.  Tokens with the logit
     ``-inf`` and beams with the score ``-inf`` are left out, and so is a beam whose logits hold NaN or ``+inf``, or nothing finite; where fewer
     than ``n`` candidates are left the rest have the score ``-inf``, from the lowest ``w * V + v`` on.  Tokens of one beam are compared by their logits,
-    those of different beams by their scores in 64 bits, in which a beam's log-sum-exp is good to about 2^-22 (equal rows have equal ones).  Returns ``(scores [B, n] fp32, beams [B, n] int64, tokens [B, n] int64)``; not differentiable."""
+    those of different beams by their scores in 64 bits, in which a beam's log-sum-exp is good to 2^-20 with up to 2^18 tokens and to 2^-19 with 2^20 (equal
+    rows have equal ones).  Returns ``(scores [B, n] fp32, beams [B, n] int64, tokens [B, n] int64)``; not differentiable."""
     shape, sizes = scores.shape, logits.shape
     if len(shape) != 2 or scores.dtype is not torch.float32:
         raise ValueError(f"scores: an fp32 tensor [B, W] is expected, not {scores.dtype} {tuple(shape)}")

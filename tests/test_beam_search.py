@@ -236,6 +236,28 @@ def test_candidates_of_one_beam_unlike_a_sample(B, V, n, dtype):
         assert not bool((got == -INF).any()) or kind in ("lowest", "few", "masked"), kind
 
 
+# The scores are such that the results are near zero: what is left is the error of log-sum-exp.  Exponentials are good to 2^-22; the argument of one d below
+# the maximum to half a step of d log2(e), which is 2^-20.5 at 12 and counts by the weight of such terms, at most a half beside the maximum's own (hence
+# 2^-21.5); forty additions with the signs of chance to 2^-22.  Together less than 2^-20.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [500, 5003, 30522, 128256, 262144])
+def test_log_sum_exp_of_a_beam(V, dtype):
+    g = torch.Generator(device="cuda").manual_seed(V)
+    B = min(256, 2 ** 25 // V)
+    rows = [torch.randn(B, V, generator=g, device="cuda") * s for s in (0.1, 1.0, 2.5, 6.0)]
+    for f in (0.25, 1.0, 4.0):                 # one high value, the others together a part of its weight
+        x = (-math.log(V * f) - torch.rand(B, 1, generator=g, device="cuda")).repeat(1, V)
+        x[:, V // 3] = 0.0
+        rows.append(x)
+    for x in rows:
+        x = x.to(dtype)
+        lse, top = torch.logsumexp(x.double(), -1), x.amax(-1).double()
+        scores = (lse - top).float()
+        got = bs.beam_select(x, scores[:, None], 1)[0].double()[:, 0]
+        assert bool(((got - (scores.double() + (top - lse))).abs() <= 2.0 ** -20).all())
+
+
 def test_candidates_refused():
     x, s = torch.randn(2, 3, 50), torch.zeros(2, 3)
     for logits, scores, n in ((x, s, 0), (x, s, 65), (x, s, 151), (x, s.double(), 4), (x, s[0], 4), (x[:, :2], s, 4), (x.reshape(-1), s, 4), (x.long(), s, 4),
