@@ -8,10 +8,13 @@
 // collected (about 1.3 n values of a round as a rule) and ranked by counting; later rounds look only at what is above the n-th so far.  Where that
 // is too much (equal values in numbers, values that rise along the row, masks that leave a stretch of it) the rounds are gone through once more with
 // the n-th largest of the threads' best, ties by their indices.
-//   Scores are compared in 64 bits: sums of near size decide between rows.  Within a row the logits decide.
-// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 21 us for the rows and 4 for the
-// join (rows in rising order, every round of which has too many: 170).  Instructions bound the rows (a difference with its conversion, its
-// scaling, an exponential and two sums per value), and 256 rows on 148 SMs; one request of 4 rows takes 4.4 and 4.9 us of latency.
+//   Scores are compared in 64 bits: sums of near size decide between rows.  Within a row the logits decide.  Threads have the same elements of every
+// row, wherever it starts, so equal rows have equal sums and the lower of two equal beams comes first.
+// Floor: the logits are read once, 65.7 MB (32 requests of 8 beams, 128256 tokens, bf16) are 10.0 us at 6555 GB/s.  Measured: 20.6 us for the rows and 4.1 for
+// the join (rows of 128257, which start anywhere: 4 us more; rows in rising order, every round of which has too many: 181 in all).  Nothing is
+// saturated in the rows: instructions are issued in 60 % of the cycles, DRAM stands at 35 %.  A warp waits 10.7 cycles an instruction: 2.1 for fixed
+// latencies, 2.0 for shared memory, 1.7 at barriers (all CTAs put their candidates in order in the same rounds), 1.4 for its turn, 0.9 for memory; and 256
+// rows on 148 SMs leave 14 % of them idle.  One request of 4 rows takes 3.8 and 5.0 us of latency.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -25,8 +28,8 @@ constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 4096;          // chunks of a group
 constexpr int kOwn = 2;                  // entries of a thread of the join where that is all (32 groups of 8 lists of 16: 4.4 us, by their heads 5.9; with four
                                          // entries, one group of 128 lists of 8: 5.6, by their heads 4.9)
-constexpr int kStages = 2;               // rounds under way (3: 22.7 instead of 21.6 us, 4 leave one CTA an SM)
-constexpr int kMany = 384;               // candidates that are all compared with each other (2048 rows of 500, 64 of them wanted: 189 us, with the search 116)
+constexpr int kStages = 2;               // rounds under way (3 leave one CTA an SM: 29 instead of 23 us for 256 rows of 128256 in all)
+constexpr int kMany = 384;               // candidates that are all compared with each other (2048 rows of 500, 64 of them wanted: 158 us, with the search 84)
 constexpr int kEasy = 512;               // candidates that are ranked without more ado
 constexpr int kCollect = kMaxN + kMaxN * 32;          // that a CTA holds: those it keeps, and all values of n threads
 constexpr unsigned kFull = 0xffffffffu;
@@ -943,9 +946,9 @@ struct Split {
 };
 
 // Rounds of 512 threads x 4 vectors where that leaves no SM without a CTA, as many of them per CTA as leave one wave (two CTAs an SM): every CTA pays
-// for its first bound and for putting candidates in order (256 rows of 128256: one CTA a row 22 us, two of 256 threads 25).  Rounds of 256 x 2
-// where rows are few (4 rows: 4.7 us, with 256 x 4 5.0) or no longer than two of them (512 rows of 2000: 12 us instead of 23, of 5000 14 instead of 22; of
-// 16000 16 instead of 17, and 256 rows of 16000 14 instead of 12).
+// for its first bound and for putting candidates in order (256 rows of 128256, rows and join: 23 us, by 256 threads x 2 vectors 29).  Rounds of 256 x 2
+// where rows are few (one row of 128256 6.6 us instead of 7.0, though four 8.0 instead of 7.4) or no longer than two of them (512 rows of 2000: 9 us
+// instead of 16, of 5000 10 instead of 16; of 16000, which are longer, 15 instead of 16, but 256 rows of 16000 12 instead of 10).
 Split split_of(long long rows, int W, int V, int elem) {
     const int per_vec = 16 / elem;
     const long long sms = nxd_num_sms(), span = V, large = 512LL * 4 * per_vec;

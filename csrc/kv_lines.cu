@@ -1,8 +1,8 @@
 // Whole lines and pages of a key/value cache, in every layer at once: lines that continue other lines (beam search), and pages that are copied
 // (a line forks, a shared page is about to be written, a pool is compacted).
 //
-// Both only move bytes, so HBM bounds them: 699 MB (16 layers, 32 lines of up to 900 rows, recurrent states) are 107 us at 6555 GB/s and take 120; 1007 MB of
-// pages are 154 us and take 156.  All tensors of one shape share a launch; their addresses travel as kernel parameters.
+// Both only move bytes, so HBM bounds them: 699 MB (16 layers, 32 lines of up to 900 rows, recurrent states) are 107 us at 6555 GB/s and take 119, through a
+// block table 139 (its entries are read for every unit and move); 1007 MB of pages are 154 us and take 156.  All tensors of one shape share a launch; their addresses travel as kernel parameters.
 #include "common.cuh"
 #include "nxd_b200.h"
 
@@ -71,10 +71,10 @@ __device__ __forceinline__ void order_moves(int from, int lane, Moves& m) {
 
 // Lines g * W + w of a group continue its lines g * W + parent[w], rows [start, end) of every head.  A thread takes kDeep units, a block's width
 // apart, of all the group's lines in an order that works in place, so there is no scratch and each line that is wanted is read once from memory
-// however many continue it.  Two moves of four units are read before the first of them is written (one unit: 147 us instead of 111 for the layers of the
-// case above).  Circles go one unit at a time, at 0.7 of that rate; no step of a search makes one.
+// however many continue it.  Two moves of four units are read before the first of them is written (one unit: 147 us instead of 111 for the case
+// above without its states, 98 of bytes).  Circles go one unit at a time, at 0.7 of that rate; no step of a search makes one.
 //   With a table the lines are pages: PAGED.  Two shapes share a launch (keys and values, and a recurrent state): the first blocks are one's, the
-// others the other's (the case above: 120 us instead of 124).
+// others the other's (the case above: 119 us instead of 124).
 struct Job {
     char* base[kJobTensors];
     int n, num_pages;
