@@ -35,7 +35,7 @@ class InferenceConfig:
     num_kv_pages: Optional[int] = None      # paged cache: size of the page pool (default: lines * pages per line)
     pad_token_id: int = 0
     eos_token_id: Optional[int] = None
-    num_beams: int = 1                      # > 1: generate() searches with that many beams (1 to 32) per sequence
+    num_beams: int = 1                      # > 1: generate() searches with that many beams (1 to 32) per sequence; not with do_sample
     length_penalty: float = 1.0             # beams are ranked by summed log-probability / length ** length_penalty
     early_stopping: bool = False            # a beam search ends as soon as it has num_beams finished sequences
 
